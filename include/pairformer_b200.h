@@ -117,6 +117,18 @@ PF_API int pf_selftest_bounded_wait(int64_t limit_ns, void* stream);
 PF_API int pf_layernorm_fwd(const void* x, void* y, const float* gamma, const float* beta,
                      int64_t rows, int32_t c, float eps, int32_t dtype, void* stream);
 
+/* The backward pass of pf_layernorm_fwd (the reference's layer_norm_cuda_kernel.cu:413-840): with
+ * xh = (x - mean) / sqrt(var + eps) and g = gamma * dy,
+ *   dx = (g - mean(g) - xh mean(g xh)) / sqrt(var + eps),
+ *   dgamma = sum over rows of dy xh,  dbeta = sum over rows of dy   (fp32, overwritten).
+ * Mean and variance are recomputed from x. x, dy and dx are [rows, c] contiguous in `dtype`; dx may
+ * be x or dy. dx, dgamma and dbeta may each be NULL (not computed); gamma NULL is a scale of one.
+ * The sums over rows have a fixed order (no atomics). */
+PF_API int pf_layernorm_bwd_workspace_size(int64_t rows, int32_t c, int32_t dtype, size_t* bytes);
+PF_API int pf_layernorm_bwd(const void* x, const void* dy, const float* gamma, void* dx, float* dgamma,
+                     float* dbeta, int64_t rows, int32_t c, float eps, int32_t dtype, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 /* ---- Triangle multiplicative update -----------------------------------------------------
  * Replaces TriangleMultiplicativeUpdate.forward (opendde/model/triangular/triangular.py:458-567,
  * _combine_projections :112-139) and its Fold-CP adapter
@@ -473,6 +485,70 @@ PF_API int pf_copy_regions(const pf_copy_region* regions, int32_t n_regions, voi
 /* The same copies by the GPU's copy engines (any number of regions; one 2-D or 3-D copy per
  * region, no SMs), so a band copied on a side stream overlaps kernels on another stream. */
 PF_API int pf_copy_regions_dma(const pf_copy_region* regions, int32_t n_regions, void* stream);
+
+/* ---- Attention with a learned bias, forward and backward -------------------------------------
+ * The core of AttentionPairBias (opendde/model/modules/transformer.py:39-671: one sequence, a bias
+ * per head) and of triangle attention (opendde/model/triangular/layers.py:325-494: the rows of the
+ * pair tensor as a batch that shares one bias) with its gradients:
+ *   t = scale q.k + bias,  p = softmax over the visible keys of t,  o = p v
+ *   D = sum_e do o,  ds = p (do.v - D)
+ *   dq = scale ds k,  dk = scale ds^T q,  dv = p^T do,  dbias = ds
+ * dk and dv add the query heads that share a key head; dbias adds the batch where it is shared. The
+ * backward recomputes p from the row statistics that the forward kept. A query that sees no key has
+ * o = 0 and gradients 0; keys the mask drops are not read. */
+typedef struct {
+  int64_t batch, n_q, n_k;
+  int32_t heads, kv_heads, head_dim; /* kv_heads divides heads; head_dim in [1, 128]   */
+  float scale;
+  int32_t dtype;                     /* q, k, v, o and their gradients                  */
+  int32_t bias_dtype;                /* bias and dbias                                  */
+} pf_attention_shape;
+
+/* Element (b, n, h, e) at ptr + b*batch_stride + n*seq_stride + h*head_stride + e. */
+typedef struct {
+  void* ptr;
+  int64_t batch_stride, seq_stride, head_stride;
+} pf_head_view;
+
+/* Element (b, h, i, j) at ptr + b*batch_stride + h*head_stride + i*row_stride + j; batch_stride 0: one
+ * plane per head, shared by the batch. ptr NULL: no bias. */
+typedef struct {
+  void* ptr;
+  int64_t batch_stride, head_stride, row_stride;
+} pf_bias_view;
+
+/* mask(b, j) != 0: key j of batch entry b is visible (mask.ptr NULL: all are).
+ * stats (fp32 [2][batch][heads][n_q]: the rows' maximum and sum) and, in bf16, o_lo (16 bits per
+ * element, [batch][n_q][heads][head_dim] contiguous: what the rounding of o dropped) are kept for the
+ * backward; both may be NULL where none follows. */
+PF_API int pf_attention_fwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
+                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, float* stats, void* o_lo,
+                     void* stream);
+PF_API int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* bytes);
+/* dq.ptr, dbias.ptr, and dk.ptr together with dv.ptr, may be NULL (not computed). Gradients are
+ * overwritten; none may overlap an input. */
+PF_API int pf_attention_bwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
+                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, const float* stats, const void* o_lo,
+                     pf_head_view d_o, pf_head_view dq, pf_head_view dk, pf_head_view dv, pf_bias_view dbias,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Relative-position bias -----------------------------------------------------------------
+ * The relative-position features of pf_trunk_init_fwd (RelativePositionEncoding,
+ * opendde/model/modules/embedders.py:124-302) as a bias of attention heads, and the gradient of
+ * their table W [heads, 4 r_max + 2 s_max + 7], for rows [row0, row0 + n_rows) x cols
+ * [col0, col0 + n_cols):
+ *   out[h, i, j] = W[h, residue offset] + W[h, token offset] + W[h, copy offset] + [same entity] W[h, entity]
+ *   dW[h, f]     = sum over the pairs with feature f of dout[h, i, j]   (fp32, overwritten, fixed order)
+ * The planes are addressed as [h*head_stride + i*row_stride + j]. At most 2048 features. */
+PF_API int pf_relpos_bias_fwd(const void* w, int32_t w_dtype, pf_token_ids ids, void* out, int64_t head_stride,
+                     int64_t row_stride, int32_t dtype, int64_t n_token, int64_t row0, int64_t n_rows,
+                     int64_t col0, int64_t n_cols, int32_t heads, int32_t r_max, int32_t s_max, void* stream);
+PF_API int pf_relpos_bias_bwd_workspace_size(int64_t n_rows, int64_t n_cols, int32_t heads, int32_t r_max,
+                     int32_t s_max, size_t* bytes);
+PF_API int pf_relpos_bias_bwd(const void* dout, int64_t head_stride, int64_t row_stride, int32_t dtype,
+                     pf_token_ids ids, float* dw, int64_t n_token, int64_t row0, int64_t n_rows, int64_t col0,
+                     int64_t n_cols, int32_t heads, int32_t r_max, int32_t s_max, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -58,6 +58,9 @@ EXPORTED = (
     "pf_pair_head_workspace_size", "pf_pair_head_fwd",
     "pf_confidence_pair_init_workspace_size", "pf_confidence_pair_init_fwd",
     "pf_diffusion_pair_cond_workspace_size", "pf_diffusion_pair_cond_fwd",
+    "pf_layernorm_bwd_workspace_size", "pf_layernorm_bwd",
+    "pf_attention_fwd", "pf_attention_bwd_workspace_size", "pf_attention_bwd",
+    "pf_relpos_bias_fwd", "pf_relpos_bias_bwd_workspace_size", "pf_relpos_bias_bwd",
 )
 
 # pf_pair_head_fwd forms (include/pairformer_b200.h)
@@ -134,6 +137,19 @@ class ConfidenceInitParams(Structure):
 class DiffusionPairParams(Structure):
     _fields_ = [(n, c_void_p) for n in ("ln_zt_w", "w_zt", "w_relp", "ln_z_w", "w_z")] + [
         ("t1", TransitionParams), ("t2", TransitionParams)]
+
+
+class AttentionShape(Structure):
+    _fields_ = [("batch", c_int64), ("n_q", c_int64), ("n_k", c_int64), ("heads", c_int32), ("kv_heads", c_int32),
+                ("head_dim", c_int32), ("scale", c_float), ("dtype", c_int32), ("bias_dtype", c_int32)]
+
+
+class HeadView(Structure):
+    _fields_ = [("ptr", c_void_p), ("batch_stride", c_int64), ("seq_stride", c_int64), ("head_stride", c_int64)]
+
+
+class BiasView(Structure):
+    _fields_ = [("ptr", c_void_p), ("batch_stride", c_int64), ("head_stride", c_int64), ("row_stride", c_int64)]
 
 
 _lib = None
@@ -226,6 +242,20 @@ def load(path: str = LIB_PATH):
         "pf_opm_fwd": ([POINTER(OpmParams), PairView, MaskView, PairView, c_int64, c_int64, c_int64, c_int64, c_int64,
                         c_int64, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p, c_size_t, c_void_p],
                        c_int),
+        "pf_layernorm_bwd_workspace_size": ([c_int64, c_int32, c_int32, sz], c_int),
+        "pf_layernorm_bwd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float,
+                              c_int32, c_void_p, c_size_t, c_void_p], c_int),
+        "pf_attention_fwd": ([POINTER(AttentionShape), HeadView, HeadView, HeadView, BiasView, MaskView, HeadView,
+                              c_void_p, c_void_p, c_void_p], c_int),
+        "pf_attention_bwd_workspace_size": ([POINTER(AttentionShape), sz], c_int),
+        "pf_attention_bwd": ([POINTER(AttentionShape), HeadView, HeadView, HeadView, BiasView, MaskView, HeadView,
+                              c_void_p, c_void_p, HeadView, HeadView, HeadView, HeadView, BiasView, c_void_p,
+                              c_size_t, c_void_p], c_int),
+        "pf_relpos_bias_fwd": ([c_void_p, c_int32, TokenIds, c_void_p, c_int64, c_int64, c_int32, c_int64, c_int64,
+                                c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p], c_int),
+        "pf_relpos_bias_bwd_workspace_size": ([c_int64, c_int64, c_int32, c_int32, c_int32, sz], c_int),
+        "pf_relpos_bias_bwd": ([c_void_p, c_int64, c_int64, c_int32, TokenIds, c_void_p, c_int64, c_int64, c_int64,
+                                c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_size_t, c_void_p], c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -14,6 +14,7 @@
 #include "pf_simt.h"
 #include "pf_tc.h"
 #include "pf_tmap.h"
+#include "pf_train.h"
 
 namespace pf {
 
@@ -90,6 +91,33 @@ int pf_layernorm_fwd(const void* x, void* y, const float* gamma, const float* be
   // the scalar warp-per-row kernel when rows are not whole 16-byte vectors.
   set_path("simt");
   return simt::layernorm(x, y, gamma, beta, rows, c, eps, dtype, (cudaStream_t)stream);
+}
+
+int pf_layernorm_bwd_workspace_size(int64_t rows, int32_t c, int32_t dtype, size_t* bytes) {
+  PF_TRY(check_dtype(dtype));
+  if (!bytes) return fail(PF_EINVAL_ARG, "bytes is NULL");
+  if (rows < 0 || c <= 0 || c > 1024)
+    return fail(PF_EINVAL_SHAPE, "layernorm backward: rows=%lld c=%d", (long long)rows, c);
+  *bytes = rows == 0 ? 0 : train::layernorm_bwd_ws_bytes(rows, c, dtype);
+  return PF_OK;
+}
+
+int pf_layernorm_bwd(const void* x, const void* dy, const float* gamma, void* dx, float* dgamma, float* dbeta,
+                     int64_t rows, int32_t c, float eps, int32_t dtype, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  size_t need;
+  PF_TRY(pf_layernorm_bwd_workspace_size(rows, c, dtype, &need));
+  if (rows > 0 && (!x || !dy)) return fail(PF_EINVAL_ARG, "layernorm backward: null input");
+  cudaStream_t st = (cudaStream_t)stream;
+  set_path("simt");
+  if (rows == 0) {  // a sum over no rows
+    if (dgamma) PF_CUDA_TRY(cudaMemsetAsync(dgamma, 0, (size_t)c * sizeof(float), st));
+    if (dbeta) PF_CUDA_TRY(cudaMemsetAsync(dbeta, 0, (size_t)c * sizeof(float), st));
+    return PF_OK;
+  }
+  if (!dx && !dgamma && !dbeta) return PF_OK;
+  PF_TRY(check_ws(workspace, workspace_bytes, need, "layernorm backward"));
+  return train::layernorm_bwd(x, dy, gamma, dx, dgamma, dbeta, rows, c, eps, dtype, workspace, workspace_bytes, st);
 }
 
 // ------------------------------------------------------------------ triangle multiplication
@@ -772,6 +800,162 @@ int pf_diffusion_pair_cond_fwd(const pf_diffusion_pair_params* w, pf_pair_view z
                           workspace, workspace_bytes, (cudaStream_t)stream));
   set_path(dtype == PF_BF16 && !force_simt() ? "tc.rows" : "simt");
   return PF_OK;
+}
+
+// ------------------------------------------------------------------ attention with a learned bias
+static int check_attention(const pf_attention_shape* s) {
+  if (!s) return fail(PF_EINVAL_ARG, "attention: null shape");
+  PF_TRY(check_dtype(s->dtype));
+  PF_TRY(check_dtype(s->bias_dtype));
+  const int64_t lim = 1ll << 31;
+  if (s->batch < 0 || s->n_q < 0 || s->n_k < 0 || s->batch >= lim || s->n_q >= lim || s->n_k >= lim)
+    return fail(PF_EINVAL_SHAPE, "attention: batch=%lld n_q=%lld n_k=%lld", (long long)s->batch, (long long)s->n_q,
+                (long long)s->n_k);
+  if (s->heads <= 0 || s->kv_heads <= 0 || s->heads % s->kv_heads != 0)
+    return fail(PF_EINVAL_SHAPE, "attention: %d heads over %d key heads", s->heads, s->kv_heads);
+  if (s->head_dim <= 0) return fail(PF_EINVAL_SHAPE, "attention: head_dim=%d", s->head_dim);
+  if (s->head_dim > 128) return fail(PF_EUNSUPPORTED, "attention: head_dim %d is above 128", s->head_dim);
+  return PF_OK;
+}
+
+// a view of n > 0 elements; alignment to the element size is what every load needs
+static bool heads_ok(const pf_head_view& v, int dtype) {
+  return v.ptr != nullptr && v.batch_stride >= 0 && v.seq_stride >= 0 && v.head_stride >= 0 &&
+         (uintptr_t)v.ptr % (dtype == PF_F32 ? 4 : 2) == 0;
+}
+static bool bias_ok(const pf_bias_view& v, int dtype) {
+  return v.batch_stride >= 0 && v.head_stride >= 0 && v.row_stride >= 0 &&
+         (uintptr_t)v.ptr % (dtype == PF_F32 ? 4 : 2) == 0;
+}
+// an output view whose elements are distinct
+static bool heads_out_ok(const pf_head_view& v, int64_t batch, int64_t n, int heads, int d, int dtype) {
+  return heads_ok(v, dtype) && (batch == 1 || v.batch_stride >= d) && (n == 1 || v.seq_stride >= d) &&
+         (heads == 1 || v.head_stride >= d);
+}
+
+int pf_attention_fwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
+                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, float* stats, void* o_lo, void* stream) {
+  PF_TRY(check_attention(shape));
+  const pf_attention_shape& s = *shape;
+  set_path("attention");
+  if (s.batch == 0 || s.n_q == 0) return PF_OK;
+  if (!heads_ok(q, s.dtype) || !heads_out_ok(o, s.batch, s.n_q, s.heads, s.head_dim, s.dtype))
+    return fail(PF_EINVAL_ARG, "attention: bad view of q or o");
+  if (s.n_k > 0 && (!heads_ok(k, s.dtype) || !heads_ok(v, s.dtype)))
+    return fail(PF_EINVAL_ARG, "attention: bad view of k or v");
+  if (bias.ptr && !bias_ok(bias, s.bias_dtype)) return fail(PF_EINVAL_ARG, "attention: bad bias view");
+  if (mask.ptr && (mask.row_stride < 0 || mask.col_stride < 0))
+    return fail(PF_EINVAL_ARG, "attention: bad mask view");
+  return train::attention_fwd(s, q, k, v, bias, mask, o, stats, (int16_t*)o_lo, (cudaStream_t)stream);
+}
+
+int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* bytes) {
+  PF_TRY(check_attention(shape));
+  if (!bytes) return fail(PF_EINVAL_ARG, "bytes is NULL");
+  *bytes = train::attention_bwd_ws_bytes(*shape);
+  return PF_OK;
+}
+
+int pf_attention_bwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
+                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, const float* stats, const void* o_lo,
+                     pf_head_view d_o, pf_head_view dq, pf_head_view dk, pf_head_view dv, pf_bias_view dbias,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need;
+  PF_TRY(pf_attention_bwd_workspace_size(shape, &need));
+  const pf_attention_shape& s = *shape;
+  set_path("attention");
+  if ((dk.ptr == nullptr) != (dv.ptr == nullptr))
+    return fail(PF_EINVAL_ARG, "attention backward: dk and dv are computed together");
+  if (dbias.ptr && !bias.ptr) return fail(PF_EINVAL_ARG, "attention backward: dbias without a bias");
+  const bool rows = s.batch > 0 && s.n_q > 0, keys = s.batch > 0 && s.n_k > 0;
+  if (rows && (!heads_ok(q, s.dtype) || !heads_ok(o, s.dtype) || !heads_ok(d_o, s.dtype) || !stats))
+    return fail(PF_EINVAL_ARG, "attention backward: bad view of q, o or do, or no row statistics");
+  if (rows && s.dtype == PF_BF16 && !o_lo)
+    return fail(PF_EINVAL_ARG, "attention backward: bf16 needs the o_lo of the forward pass");
+  if (keys && (!heads_ok(k, s.dtype) || !heads_ok(v, s.dtype)))
+    return fail(PF_EINVAL_ARG, "attention backward: bad view of k or v");
+  if (bias.ptr && !bias_ok(bias, s.bias_dtype)) return fail(PF_EINVAL_ARG, "attention backward: bad bias view");
+  if (mask.ptr && (mask.row_stride < 0 || mask.col_stride < 0))
+    return fail(PF_EINVAL_ARG, "attention backward: bad mask view");
+  if ((dq.ptr && rows && !heads_out_ok(dq, s.batch, s.n_q, s.heads, s.head_dim, s.dtype)) ||
+      (dk.ptr && keys && (!heads_out_ok(dk, s.batch, s.n_k, s.kv_heads, s.head_dim, s.dtype) ||
+                          !heads_out_ok(dv, s.batch, s.n_k, s.kv_heads, s.head_dim, s.dtype))))
+    return fail(PF_EINVAL_ARG, "attention backward: bad view of a gradient");
+  if (dbias.ptr) {
+    if (!bias_ok(dbias, s.bias_dtype) || (s.n_q > 1 && dbias.row_stride < s.n_k) ||
+        (s.heads > 1 && dbias.head_stride < s.n_k))
+      return fail(PF_EINVAL_ARG, "attention backward: bad dbias view");
+    if (s.batch > 1 && (bias.batch_stride == 0) != (dbias.batch_stride == 0))
+      return fail(PF_EINVAL_ARG, "attention backward: dbias is shared by the batch exactly where the bias is");
+  }
+  if (dbias.ptr && s.batch == 0)
+    return fail(PF_EINVAL_SHAPE, "attention backward: dbias of an empty batch");
+  if (!rows && !keys) return PF_OK;
+  PF_TRY(check_ws(workspace, workspace_bytes, need, "attention backward"));
+  return train::attention_bwd(s, q, k, v, bias, mask, o, stats, (const int16_t*)o_lo, d_o, dq, dk, dv, dbias,
+                              workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+// ------------------------------------------------------------------ relative-position bias
+static int check_relpos(int64_t n_token, int64_t row0, int64_t n_rows, int64_t col0, int64_t n_cols, int heads,
+                        int r_max, int s_max) {
+  if (n_rows < 0 || n_cols < 0 || row0 < 0 || col0 < 0 || row0 > n_token - n_rows || col0 > n_token - n_cols ||
+      heads <= 0 || r_max < 0 || s_max < 0)
+    return fail(PF_EINVAL_SHAPE, "relative-position bias: rows [%lld, +%lld) x cols [%lld, +%lld) of %lld tokens, "
+                "heads=%d r_max=%d s_max=%d", (long long)row0, (long long)n_rows, (long long)col0, (long long)n_cols,
+                (long long)n_token, heads, r_max, s_max);
+  if (r_max > 2048 || s_max > 2048 || 4 * r_max + 2 * s_max + 7 > 2048)
+    return fail(PF_EUNSUPPORTED, "relative-position bias: more than 2048 features (r_max=%d s_max=%d)", r_max, s_max);
+  return PF_OK;
+}
+static bool ids_ok(const pf_token_ids& t) {
+  return t.asym_id && t.residue_index && t.entity_id && t.token_index && t.sym_id;
+}
+
+int pf_relpos_bias_fwd(const void* w, int32_t w_dtype, pf_token_ids ids, void* out, int64_t head_stride,
+                       int64_t row_stride, int32_t dtype, int64_t n_token, int64_t row0, int64_t n_rows, int64_t col0,
+                       int64_t n_cols, int32_t heads, int32_t r_max, int32_t s_max, void* stream) {
+  PF_TRY(check_dtype(dtype));
+  PF_TRY(check_dtype(w_dtype));
+  PF_TRY(check_relpos(n_token, row0, n_rows, col0, n_cols, heads, r_max, s_max));
+  set_path("simt");
+  if (n_rows == 0 || n_cols == 0) return PF_OK;
+  if (!w || !out || !ids_ok(ids)) return fail(PF_EINVAL_ARG, "relative-position bias: null pointer");
+  if ((n_rows > 1 && row_stride < n_cols) || (heads > 1 && head_stride < n_cols))
+    return fail(PF_EINVAL_ARG, "relative-position bias: overlapping rows of the output");
+  return train::relpos_bias(w, w_dtype, ids, out, head_stride, row_stride, dtype, row0, n_rows, col0, n_cols, heads,
+                            r_max, s_max, (cudaStream_t)stream);
+}
+
+int pf_relpos_bias_bwd_workspace_size(int64_t n_rows, int64_t n_cols, int32_t heads, int32_t r_max, int32_t s_max,
+                                      size_t* bytes) {
+  if (!bytes) return fail(PF_EINVAL_ARG, "bytes is NULL");
+  const int64_t n = n_rows > n_cols ? n_rows : n_cols;
+  PF_TRY(check_relpos(n, 0, n_rows, 0, n_cols, heads, r_max, s_max));
+  *bytes = train::relpos_bias_bwd_ws_bytes(n_rows, n_cols, heads, r_max, s_max);
+  return PF_OK;
+}
+
+int pf_relpos_bias_bwd(const void* dout, int64_t head_stride, int64_t row_stride, int32_t dtype, pf_token_ids ids,
+                       float* dw, int64_t n_token, int64_t row0, int64_t n_rows, int64_t col0, int64_t n_cols,
+                       int32_t heads, int32_t r_max, int32_t s_max, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  PF_TRY(check_dtype(dtype));
+  PF_TRY(check_relpos(n_token, row0, n_rows, col0, n_cols, heads, r_max, s_max));
+  set_path("simt");
+  if (!dw) return fail(PF_EINVAL_ARG, "relative-position bias: null gradient");
+  cudaStream_t st = (cudaStream_t)stream;
+  if (n_rows == 0 || n_cols == 0) {  // a sum over no pairs
+    PF_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)heads * (4 * r_max + 2 * s_max + 7) * sizeof(float), st));
+    return PF_OK;
+  }
+  if (!dout || !ids_ok(ids)) return fail(PF_EINVAL_ARG, "relative-position bias: null pointer");
+  if (head_stride < 0 || row_stride < 0) return fail(PF_EINVAL_ARG, "relative-position bias: negative stride");
+  size_t need;
+  PF_TRY(pf_relpos_bias_bwd_workspace_size(n_rows, n_cols, heads, r_max, s_max, &need));
+  PF_TRY(check_ws(workspace, workspace_bytes, need, "relative-position bias"));
+  return train::relpos_bias_bwd(dout, head_stride, row_stride, dtype, ids, dw, row0, n_rows, col0, n_cols, heads,
+                                r_max, s_max, workspace, workspace_bytes, st);
 }
 
 }  // extern "C"

@@ -9,7 +9,8 @@ bfloat16 -> PF_BF16 (tcgen05 tensor cores where the shape is covered).
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional
+import math
+from typing import Dict, NamedTuple, Optional
 
 import torch
 
@@ -406,3 +407,241 @@ def diffusion_pair_cond(pack: WeightPack, z_trunk: torch.Tensor, ids, z_out: tor
     check(_abi.load().pf_diffusion_pair_cond_fwd(ctypes.byref(pack.struct), pair_view(z_trunk), tid,
                                                  pair_view(z_out), n_token, row0, n_rows, col0, n_cols, c_z, c_zd,
                                                  r_max, s_max, code, ws.data_ptr(), ws.numel(), stream_ptr()))
+
+
+# ------------------------------------------------------------------------------ training operators
+# Each call launches on the current stream of its tensors' device, whichever device is current, and
+# can be captured into a CUDA graph (its workspace then lies in the graph's own pool).
+
+def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    require_cuda(*ts)
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"tensors lie on different devices: {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _float_param(p: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if p is None else p.detach().float().contiguous()
+
+
+def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-5,
+                  need=(True, True, True)):
+    """(dx, dweight, dbias) of :func:`layernorm` for the output's gradient ``dy`` (see
+    pf_layernorm_bwd): dx in x's shape and dtype, the other two float32 [c] sums over all rows. ``need``
+    drops the ones not wanted (None in their place)."""
+    dev = _same_device(x, dy, weight)
+    code = dtype_code(x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy {tuple(dy.shape)} {dy.dtype} is not like x {tuple(x.shape)} {x.dtype}")
+    c = x.shape[-1]
+    if weight is not None and tuple(weight.shape) != (c,):
+        raise ValueError(f"weight {tuple(weight.shape)} does not match {c} channels")
+    with torch.cuda.device(dev):
+        x, dy, w = x.detach().contiguous(), dy.detach().contiguous(), _float_param(weight)
+        dx = torch.empty_like(x) if need[0] else None
+        dw = torch.empty(c, device=dev, dtype=torch.float32) if need[1] else None
+        db = torch.empty(c, device=dev, dtype=torch.float32) if need[2] else None
+        rows = x.numel() // c
+        nbytes = _abi.workspace_bytes("pf_layernorm_bwd_workspace_size", rows, c, code)
+        ws = workspace(nbytes, dev)
+        check(_abi.load().pf_layernorm_bwd(x.data_ptr(), dy.data_ptr(), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db), rows, c,
+                                           eps, code, ws.data_ptr(), ws.numel(), stream_ptr()))
+    return dx, dw, db
+
+
+class AttentionSaved(NamedTuple):
+    """What :func:`attention` keeps for :func:`attention_bwd`: the rows' maximum and sum (float32
+    [2, B, H, n_q]) and, for bfloat16, the 16 bits of the output that its rounding dropped."""
+    stats: torch.Tensor
+    o_lo: Optional[torch.Tensor]
+
+
+def _head_view(t: Optional[torch.Tensor]) -> _abi.HeadView:
+    if t is None:
+        return _abi.HeadView(None, 0, 0, 0)
+    return _abi.HeadView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _bias_view(t: Optional[torch.Tensor]) -> _abi.BiasView:
+    if t is None:
+        return _abi.BiasView(None, 0, 0, 0)
+    return _abi.BiasView(t.data_ptr(), 0 if t.shape[0] == 1 else t.stride(0), t.stride(1), t.stride(2))
+
+
+def _batched_heads(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dim() not in (3, 4):
+        raise ValueError(f"{name} must be [B, N, H, d] or [N, H, d], got shape {tuple(t.shape)}")
+    t = t.detach()
+    t = t[None] if t.dim() == 3 else t
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        raise ValueError(f"{name} must have contiguous channels")
+    return t
+
+
+def _attention_args(q, k, v, bias, mask, scale):
+    """Checked [B, N, H, d] views, the [1 or B, H, n_q, n_k] bias, the float32 mask and the shape."""
+    dev = _same_device(q, k, v, bias, mask)
+    code = dtype_code(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must share the dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if not q.dim() == k.dim() == v.dim():
+        raise ValueError("q, k and v must all be batched or all be unbatched")
+    q, k, v = _batched_heads(q, "q"), _batched_heads(k, "k"), _batched_heads(v, "v")
+    b, n_q, heads, d = q.shape
+    n_k, kv_heads = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"attention shapes disagree: q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    if bias is not None:
+        if bias.dim() not in (3, 4):
+            raise ValueError(f"bias must be [H, n_q, n_k] or [B, H, n_q, n_k], got shape {tuple(bias.shape)}")
+        bias = bias.detach()
+        bias = bias[None] if bias.dim() == 3 else bias
+        if bias.shape[0] not in (1, b) or tuple(bias.shape[1:]) != (heads, n_q, n_k):
+            raise ValueError(f"bias {tuple(bias.shape)} is not [1 or {b}, {heads}, {n_q}, {n_k}]")
+        if bias.stride(3) != 1 and n_k > 1:
+            raise ValueError("bias must have contiguous keys")
+        if bias.shape[0] > 1 and bias.stride(0) == 0:
+            bias = bias[:1]
+    mv = _abi.MaskView(None, 0, 0)
+    if mask is not None:
+        if tuple(mask.shape) not in ((n_k,), (b, n_k)):
+            raise ValueError(f"mask {tuple(mask.shape)} is not [{n_k}] or [{b}, {n_k}]")
+        mask = mask.detach()
+        if mask.dtype != torch.float32:
+            if mask.dtype not in (torch.bool, torch.bfloat16, torch.float16, torch.uint8, torch.int32, torch.int64):
+                raise TypeError(f"mask must be boolean or float32 like the pair masks, got {mask.dtype}")
+            mask = (mask != 0).to(torch.float32)
+        mask = mask[None].expand(b, n_k) if mask.dim() == 1 else mask
+        mv = mask_view(mask)
+    if scale is None:
+        scale = 1.0 / math.sqrt(d) if d else 1.0
+    shape = _abi.AttentionShape(b, n_q, n_k, heads, kv_heads, d, float(scale), code,
+                                _abi.PF_F32 if bias is None else dtype_code(bias))
+    return dev, q, k, v, bias, mask, mv, shape
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[torch.Tensor] = None,
+              mask: Optional[torch.Tensor] = None, scale: Optional[float] = None, save: bool = False):
+    """softmax(scale q k^T + bias) v over the visible keys (see pf_attention_fwd).
+
+    q [B, n_q, H, d], k and v [B, n_k, H_kv, d] (H_kv divides H; or all three without the batch
+    dimension), any strides with contiguous channels, float32 or bfloat16, d <= 128. ``bias``
+    [1 or B, H, n_q, n_k] or [H, n_q, n_k], float32 or bfloat16 whatever q is. ``mask`` [B, n_k] or
+    [n_k]: non-zero where a key is visible; a query that sees none gets 0. ``scale`` defaults to
+    1 / sqrt(d). Returns the contiguous output in q's shape; with ``save`` also what
+    :func:`attention_bwd` needs."""
+    dev, q4, k4, v4, bias, mask, mv, shape = _attention_args(q, k, v, bias, mask, scale)
+    with torch.cuda.device(dev):
+        o = torch.empty(q4.shape, device=dev, dtype=q.dtype)
+        stats = o_lo = None
+        if save:
+            stats = torch.empty((2, shape.batch, shape.heads, shape.n_q), device=dev, dtype=torch.float32)
+            if shape.dtype == _abi.PF_BF16:
+                o_lo = torch.empty(q4.shape, device=dev, dtype=torch.int16)
+        check(_abi.load().pf_attention_fwd(ctypes.byref(shape), _head_view(q4), _head_view(k4), _head_view(v4),
+                                           _bias_view(bias), mv, _head_view(o), _ptr(stats), _ptr(o_lo),
+                                           stream_ptr()))
+    o = o.view(q.shape)
+    return (o, AttentionSaved(stats, o_lo)) if save else o
+
+
+def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                  saved: AttentionSaved, bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                  scale: Optional[float] = None, need=(True, True, True, True)):
+    """(dq, dk, dv, dbias) of :func:`attention` for the output's gradient ``do`` (see pf_attention_bwd);
+    the other arguments are the forward's. dbias has bias's shape and dtype (summed over the batch where
+    bias is shared by it) and is None without one. ``need`` drops the ones not wanted (None in their
+    place)."""
+    n_batch = None if bias is None else (1 if bias.dim() == 3 else bias.shape[0])
+    dbias_shape = None if bias is None else bias.shape
+    dev, q4, k4, v4, bias, mask, mv, shape = _attention_args(q, k, v, bias, mask, scale)
+    if _same_device(do, o, saved.stats, q) != dev or (saved.o_lo is not None and saved.o_lo.device != dev):
+        raise ValueError("do, o and the saved tensors must lie on q's device")
+    for t, name in ((do, "do"), (o, "o")):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} is not like q {tuple(q.shape)} {q.dtype}")
+    if (tuple(saved.stats.shape) != (2, shape.batch, shape.heads, shape.n_q) or not saved.stats.is_contiguous()
+            or saved.stats.dtype != torch.float32):
+        raise ValueError("saved does not come from a forward of these shapes")
+    if shape.dtype == _abi.PF_BF16 and (saved.o_lo is None or saved.o_lo.shape != q4.shape
+                                        or saved.o_lo.dtype != torch.int16 or not saved.o_lo.is_contiguous()):
+        raise ValueError("saved does not come from a bfloat16 forward of these shapes")
+    do4, o4 = _batched_heads(do, "do"), _batched_heads(o, "o")
+    with torch.cuda.device(dev):
+        dq = torch.empty(q4.shape, device=dev, dtype=q.dtype) if need[0] else None
+        dk = dv = dbias = dbias_v = None
+        if need[1] or need[2]:
+            dk = torch.empty(k4.shape, device=dev, dtype=q.dtype)
+            dv = torch.empty(v4.shape, device=dev, dtype=q.dtype)
+        if bias is not None and need[3]:
+            if shape.batch == 0:
+                dbias = torch.zeros(dbias_shape, device=dev, dtype=bias.dtype)
+            elif bias.shape[0] == n_batch:
+                dbias = torch.empty(bias.shape, device=dev, dtype=bias.dtype)
+                dbias_v = dbias
+            else:  # one plane expanded over the batch: every entry has a gradient of its own
+                dbias = torch.empty((n_batch,) + tuple(bias.shape[1:]), device=dev, dtype=bias.dtype)
+                dbias_v = dbias
+                bias = bias.expand(dbias.shape).contiguous()
+        nbytes = _abi.workspace_bytes("pf_attention_bwd_workspace_size", ctypes.byref(shape))
+        ws = workspace(nbytes, dev)
+        check(_abi.load().pf_attention_bwd(
+            ctypes.byref(shape), _head_view(q4), _head_view(k4), _head_view(v4), _bias_view(bias), mv, _head_view(o4),
+            saved.stats.data_ptr(), _ptr(saved.o_lo), _head_view(do4), _head_view(dq), _head_view(dk),
+            _head_view(dv), _bias_view(dbias_v), ws.data_ptr(), ws.numel(), stream_ptr()))
+    return (None if dq is None else dq.view(q.shape), dk.view(k.shape) if need[1] else None,
+            dv.view(v.shape) if need[2] else None, None if dbias is None else dbias.view(dbias_shape))
+
+
+def _check_ids(ids, dev) -> int:
+    n_token = None
+    for t in ids:
+        if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError("token ids must be contiguous int32 [N_token] vectors")
+        if t.device != dev or (n_token is not None and t.shape[0] != n_token):
+            raise ValueError("token ids must lie on one device and have one length")
+        n_token = t.shape[0]
+    if len(ids) != 5:
+        raise ValueError("five id vectors: asym_id, residue_index, entity_id, token_index, sym_id")
+    return n_token
+
+
+def _plane(t: torch.Tensor, name: str) -> None:
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise ValueError(f"{name} must be [H, R, C] with contiguous columns, got shape {tuple(t.shape)}")
+
+
+def relpos_bias(weight: torch.Tensor, ids, out: torch.Tensor, row0: int, col0: int, r_max: int, s_max: int) -> None:
+    """out [H, R, C] = the relative-position bias of rows [row0, row0 + R) x cols [col0, col0 + C) from
+    the table ``weight`` [H, 4 r_max + 2 s_max + 7] (see pf_relpos_bias_fwd). ``ids``: int32 CUDA tensors
+    asym_id, residue_index, entity_id, token_index, sym_id."""
+    dev = _same_device(weight, out, *ids)
+    code, n_token = dtype_code(out), _check_ids(ids, dev)
+    _plane(out, "out")
+    if tuple(weight.shape) != (out.shape[0], 4 * r_max + 2 * s_max + 7):
+        raise ValueError(f"weight {tuple(weight.shape)} is not [{out.shape[0]}, {4 * r_max + 2 * s_max + 7}]")
+    w = weight.detach().contiguous()
+    with torch.cuda.device(dev):
+        check(_abi.load().pf_relpos_bias_fwd(w.data_ptr(), dtype_code(w), _abi.TokenIds(*[t.data_ptr() for t in ids]),
+                                             out.data_ptr(), out.stride(0), out.stride(1), code, n_token, row0,
+                                             out.shape[1], col0, out.shape[2], out.shape[0], r_max, s_max,
+                                             stream_ptr()))
+
+
+def relpos_bias_bwd(dout: torch.Tensor, ids, row0: int, col0: int, r_max: int, s_max: int) -> torch.Tensor:
+    """The float32 [H, 4 r_max + 2 s_max + 7] gradient of :func:`relpos_bias`'s table for the plane's
+    gradient ``dout`` [H, R, C] (see pf_relpos_bias_bwd)."""
+    dev = _same_device(dout, *ids)
+    code, n_token = dtype_code(dout), _check_ids(ids, dev)
+    _plane(dout, "dout")
+    heads, rows, cols = dout.shape
+    with torch.cuda.device(dev):
+        nbytes = _abi.workspace_bytes("pf_relpos_bias_bwd_workspace_size", rows, cols, heads, r_max, s_max)
+        ws = workspace(nbytes, dev)
+        dw = torch.empty((heads, 4 * r_max + 2 * s_max + 7), device=dev, dtype=torch.float32)
+        check(_abi.load().pf_relpos_bias_bwd(dout.data_ptr(), dout.stride(0), dout.stride(1), code,
+                                             _abi.TokenIds(*[t.data_ptr() for t in ids]), dw.data_ptr(), n_token,
+                                             row0, rows, col0, cols, heads, r_max, s_max, ws.data_ptr(), ws.numel(),
+                                             stream_ptr()))
+    return dw
