@@ -8,8 +8,9 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
-from .. import kernels
+from .. import autograd, kernels
 from .._abi import ApbParams
 from .primitives import Linear, LinearNoBias
 from .triangular import LayerNorm
@@ -112,3 +113,24 @@ class AttentionPairBias(nn.Module):
             bias = (bias + (e if e.dim() == 3 else e[None])).contiguous()
         out = torch.empty_like(a)
         return self.apply_(a, z if bias is None else None, out, accumulate=False, bias=bias)
+
+    def differentiable(self, a: torch.Tensor, z: torch.Tensor,
+                       extra_attn_bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``forward(a, None, z)`` of one [N, c_a] single and [N, N, c_z] pair representation with gradients of a, z,
+        ``extra_attn_bias`` and the parameters: layer norms and attention are this package's kernels, the
+        projections are library products. The bias is float32 whatever a is, as in ``forward``."""
+        kernels.require_cuda(a, z, extra_attn_bias)
+        if a.dim() != 2 or z.dim() != 3:
+            raise ValueError("differentiable takes one [N, c_a] and one [N, N, c_z] tensor")
+        att, y = self.attention, self.layernorm_a.differentiable(a)
+        heads = (a.shape[0], self.n_heads, att.c_hidden)
+        b_q = att.linear_q.bias
+        q = F.linear(y, att.linear_q.weight.to(y.dtype), None if b_q is None else b_q.to(y.dtype))
+        k, v, g = (F.linear(y, m.weight.to(y.dtype)) for m in (att.linear_k, att.linear_v, att.linear_g))
+        w_z = self.linear_nobias_z.weight.to(z.dtype)
+        bias = F.linear(self.layernorm_z.differentiable(z), w_z).permute(2, 0, 1).to(torch.float32)
+        if extra_attn_bias is not None:
+            e = extra_attn_bias.to(device=a.device, dtype=torch.float32)
+            bias = bias + (e if e.dim() == 3 else e[None])
+        o = autograd.attention(q.view(heads), k.view(heads), v.view(heads), bias)
+        return F.linear(o.flatten(1) * torch.sigmoid(g), att.linear_o.weight.to(y.dtype))

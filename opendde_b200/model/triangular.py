@@ -16,8 +16,9 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
-from .. import kernels
+from .. import autograd, kernels
 from .._abi import TriattParams, TrimulParams
 
 _TRIMUL_CHOICES = {"torch", "cuequivariance"}
@@ -89,6 +90,10 @@ class LayerNorm(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return kernels.layernorm(x, self.weight, self.bias, self.eps)
+
+    def differentiable(self, x: torch.Tensor) -> torch.Tensor:
+        """``forward`` with gradients of x and of the parameters."""
+        return autograd.layer_norm(x, self.weight, self.bias, self.eps)
 
 
 class Attention(nn.Module):
@@ -263,3 +268,24 @@ class TriangleAttention(nn.Module):
             return self.apply_(zz, mm, out, accumulate=False)
 
         return _batched(one, x, mask)
+
+    def differentiable(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The update of one [N, N, c_in] pair tensor with gradients of x and of the parameters: the layer norm and
+        the attention over rows (which share the triangle bias) are this package's kernels, the projections are
+        library products. A non-zero ``mask`` entry is a visible key; a row without any attends to all of its keys
+        (a constant added to every logit changes nothing)."""
+        kernels.require_cuda(x, mask)
+        if x.dim() != 3 or x.shape[0] != x.shape[1]:
+            raise ValueError("differentiable takes one [N, N, c_in] pair tensor")
+        seen = None if mask is None else mask != 0
+        if not self.starting:
+            x, seen = x.transpose(0, 1), None if seen is None else seen.t()
+        if seen is not None:
+            seen = (seen | ~seen.any(-1, keepdim=True)).to(device=x.device, dtype=torch.float32)
+        y = self.layer_norm.differentiable(x)
+        heads = (*y.shape[:2], self.no_heads, self.c_hidden)
+        q, k, v, g, bias = (F.linear(y, m.weight.to(y.dtype)) for m in (
+            self.mha.linear_q, self.mha.linear_k, self.mha.linear_v, self.mha.linear_g, self.linear))
+        o = autograd.attention(q.view(heads), k.view(heads), v.view(heads), bias.permute(2, 0, 1), seen)
+        out = F.linear(o.flatten(2) * torch.sigmoid(g), self.mha.linear_o.weight.to(y.dtype))
+        return out if self.starting else out.transpose(0, 1)

@@ -16,7 +16,7 @@ from typing import Any, Dict, Optional
 import torch
 import torch.nn as nn
 
-from .. import kernels
+from .. import autograd, kernels
 from .._abi import PairLinearParams, TrunkInitParams
 from .primitives import LinearNoBias
 
@@ -79,6 +79,17 @@ class RelativePositionEncoding(nn.Module):
         input_feature_dict["relp"] = LazyRelativePositionEncodingFeatures(
             *[input_feature_dict[k] for k in _ID_KEYS], r_max=self.r_max, s_max=self.s_max)
         return input_feature_dict
+
+    def head_bias(self, relp_feature, tile=None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The encoding as a bias of attention heads (``c_z`` of them), [c_z, N, N], with the gradient of its
+        weight: what :func:`autograd.attention` takes as ``bias`` or
+        :meth:`AttentionPairBias.differentiable` as ``extra_attn_bias``. ``tile`` = (row0, R, col0, C) selects a
+        part of the plane (the tile of a mesh position)."""
+        w = self.linear_no_bias.weight
+        feats = _relp_features(relp_feature)
+        if (int(feats.r_max), int(feats.s_max)) != (self.r_max, self.s_max):
+            raise ValueError("the features were made for another r_max or s_max")
+        return autograd.relative_position_bias(w, feats.ids(w.device), self.r_max, self.s_max, tile, dtype)
 
 
 def _relp_features(relp_feature) -> LazyRelativePositionEncodingFeatures:
