@@ -1,15 +1,1197 @@
-// pf_attention_bf16.cu -- the bf16 kernels of pf_attention.cuh.
+// pf_attention_bf16.cu -- the bf16 kernels of pf_attention.cuh on warp-level tensor-core products.
+//
+// Work of one warp: 16 MT query rows against groups of 16 keys (forward, dq, dbias), or 16 KM keys
+// against groups of 16 queries (dk, dv); four warps to a block, streamed tiles of 64 rows
+// double-buffered by cp.async. For the heads of 24 and 32 channels of this package a 16 x 16 block of
+// scores costs two to four products of depth 32 next to 256 exponentials, so the kernels are bound by
+// the issue of products, exponentials and the arithmetic around them, not by memory: two row blocks
+// per warp (MT = 2, KM = 2) use every streamed fragment twice.
+//
+// Columns of a group of 16 keys are permuted so that a lane's four columns are four neighbouring keys
+// (lane t of a quad: keys 4t..4t+3 in place of 2t, 2t+1, 2t+8, 2t+9): a bias row is then read, and a
+// dbias row written, 8 (bf16) or 16 (fp32) bytes at a time in full 32-byte sectors. The permutation is
+// in the row addresses of ldmatrix alone. Shared rows are whole (no padding) with their 16-byte chunks
+// XOR-swizzled so that natural and permuted row sets are both free of bank conflicts.
+//
+// dk and dv need the transposed p and ds as left operands; the scores are computed with queries down
+// the rows all the same (the bias is read along its rows) and each 8 x 8 block is transposed in
+// registers by movmatrix.
+
 #include "pf_attention.cuh"
 
 namespace pf {
 namespace train {
 namespace attn {
-int launch_bf16(Kind kind, const Args& a, int64_t blocks, double flops, cudaStream_t st) {
-  return launch_dim<__nv_bfloat16>(kind, a, blocks, flops, st);
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 64;  // rows of a streamed tile
+
+// ---------------------------------------------------------------- shared tiles
+
+template <int DP>
+struct Tile {
+  static constexpr int RB = DP == 96 ? 256 : DP * 2;  // bytes of a row
+  static constexpr int CH = DP / 8;                   // 16-byte chunks in use
+  static __device__ __forceinline__ int swz(int row) {
+    return DP == 32 ? ((row >> 1) & 3) ^ ((row >> 3) & 1) : (row & 7) ^ (((row >> 3) & 1) << 1);
+  }
+  static __device__ __forceinline__ uint32_t off(int row, int ch) { return row * RB + ((ch ^ swz(row)) << 4); }
+};
+
+// A lane's row address inside a block of 16 rows for one ldmatrix.x4 pattern.
+template <int DP>
+struct LaneAddr {
+  uint32_t rb, v;
+  __device__ __forceinline__ LaneAddr(int row, int ch) : rb(row * Tile<DP>::RB), v(ch ^ Tile<DP>::swz(row)) {}
+  // rows 16 blk.. of the tile at `base`, chunks 2 pair, 2 pair + 1
+  __device__ __forceinline__ uint32_t at(uint32_t base, int blk, int pair) const {
+    return base + blk * 16 * Tile<DP>::RB + rb + (((uint32_t)(2 * pair) ^ v) << 4);
+  }
+};
+__device__ __forceinline__ int perm_row(int r, int half) { return 4 * (r >> 1) + (r & 1) + 2 * half; }
+// left operand, natural rows
+template <int DP>
+__device__ __forceinline__ LaneAddr<DP> lane_a() {
+  const int l = threadIdx.x & 31;
+  return LaneAddr<DP>(l & 15, l >> 4);
 }
+// right operand with the depth along the row (keys are its columns, permuted)
+template <int DP>
+__device__ __forceinline__ LaneAddr<DP> lane_b() {
+  const int l = threadIdx.x & 31;
+  return LaneAddr<DP>(perm_row(l & 7, l >> 4), (l >> 3) & 1);
+}
+// right operand with the depth down the rows (transposing load): permuted keys, or natural rows
+template <int DP>
+__device__ __forceinline__ LaneAddr<DP> lane_bt() {
+  const int l = threadIdx.x & 31;
+  return LaneAddr<DP>(perm_row(l & 7, (l >> 3) & 1), l >> 4);
+}
+template <int DP>
+__device__ __forceinline__ LaneAddr<DP> lane_bn() {
+  const int l = threadIdx.x & 31;
+  return LaneAddr<DP>(l & 15, l >> 4);
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Rows [r0, r0 + ROWS) of (b, h), zero past n and d and where `live` has no bit for a row (tiles of 64).
+template <int DP, int ROWS>
+__device__ __forceinline__ void load_rows(uint32_t sm, const bf16* base, int64_t ns, int vec, int64_t r0, int64_t n,
+                                          int d, uint64_t live) {
+  constexpr int CH = Tile<DP>::CH;
+  if (vec) {
+#pragma unroll
+    for (int i = threadIdx.x; i < ROWS * CH; i += kThreads) {
+      const int r = i / CH, c = i - r * CH;
+      const bool ok = r0 + r < n && c * 8 < d && ((live >> (r & 63)) & 1);
+      cp_async16(sm + Tile<DP>::off(r, c), ok ? base + (r0 + r) * ns + c * 8 : base, ok);
+    }
+  } else {
+    for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
+      const int r = i / DP, c = i - r * DP;
+      const bool ok = r0 + r < n && c < d && ((live >> (r & 63)) & 1);
+      const bf16 x = ok ? base[(r0 + r) * ns + c] : from_f<bf16>(0.f);
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(sm + Tile<DP>::off(r, c >> 3) + (c & 7) * 2),
+                   "h"(*reinterpret_cast<const unsigned short*>(&x))
+                   : "memory");
+    }
+  }
+}
+__device__ __forceinline__ const bf16* head_base(const Heads& s, int64_t b, int h) {
+  return (const bf16*)s.p + b * s.bs + (int64_t)h * s.hs;
+}
+
+// ---------------------------------------------------------------- visible keys
+
+// Mask values of keys j0 + lane and j0 + 32 + lane (0 past the end), read a tile ahead of their use.
+__device__ __forceinline__ float2 seen_raw(const Args& a, int64_t b, int64_t j0) {
+  const int64_t j = j0 + (threadIdx.x & 31);
+  float2 r;
+  if (a.mask) {
+    const float* m = a.mask + b * a.m_bs;
+    r.x = j < a.nk ? m[j * a.m_ks] : 0.f;
+    r.y = j + 32 < a.nk ? m[(j + 32) * a.m_ks] : 0.f;
+  } else {
+    r.x = j < a.nk ? 1.f : 0.f;
+    r.y = j + 32 < a.nk ? 1.f : 0.f;
+  }
+  return r;
+}
+__device__ __forceinline__ uint64_t seen_ballot(float2 r) {
+  return (uint64_t)__ballot_sync(0xffffffffu, r.x != 0.f) |
+         ((uint64_t)__ballot_sync(0xffffffffu, r.y != 0.f) << 32);
+}
+
+// ---------------------------------------------------------------- bias fragments
+// BT: 0 no bias, 1 bf16, 2 fp32. Four neighbouring keys of one row.
+
+template <int BT>
+struct Bias4 {
+  uint32_t w[BT == 2 ? 4 : (BT == 1 ? 2 : 1)];
+};
+template <int BT>
+__device__ __forceinline__ const char* bias_row(const Args& a, int64_t b, int h, int64_t i) {
+  if (BT == 0) return nullptr;
+  return (const char*)a.bias + (b * a.b_bs + (int64_t)h * a.b_hs + i * a.b_rs) * (BT == 2 ? 4 : 2);
+}
+// keys j .. j + 3 of the row at p; `fast`: all exist and are aligned together
+template <int BT>
+__device__ __forceinline__ void bias_load(Bias4<BT>& r, const char* p, int64_t j, int64_t nk, bool fast) {
+  if (BT == 1) {
+    if (fast) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + j * 2);
+      r.w[0] = v.x, r.w[1] = v.y;
+    } else {
+      const unsigned short* q = (const unsigned short*)p + j;
+      uint32_t e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = j + i < nk ? q[i] : 0;
+      r.w[0] = e[0] | (e[1] << 16), r.w[1] = e[2] | (e[3] << 16);
+    }
+  } else if (BT == 2) {
+    if (fast) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + j * 4);
+      r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    } else {
+      const uint32_t* q = (const uint32_t*)p + j;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = j + i < nk ? q[i] : 0;
+    }
+  }
+}
+template <int BT>
+__device__ __forceinline__ float bias_val(const Bias4<BT>& r, int i) {
+  if (BT == 1) return (i & 1) ? hi_f(r.w[i >> 1]) : lo_f(r.w[i >> 1]);
+  if (BT == 2) return __uint_as_float(r.w[i]);
+  return 0.f;
+}
+// scale * s + bias, s in natural units (next to a bias of the type's lowest value a factor log2(e) overflows)
+template <int BT>
+__device__ __forceinline__ float score(float s, float scale, const Bias4<BT>& r, int i) {
+  return BT == 0 ? s * scale : fmaf(s, scale, bias_val<BT>(r, i));
+}
+
+// one row's four columns of a group as stored by the products: x[0][2r..] then x[1][2r..]
+template <int BT>
+__device__ __forceinline__ void store_bias4(const Args& a, char* p, int64_t j, bool fast, float v0, float v1, float v2,
+                                            float v3) {
+  if (BT == 2) {
+    float* q = (float*)p + j;
+    if (fast) {
+      *reinterpret_cast<float4*>(q) = make_float4(v0, v1, v2, v3);
+    } else {
+      if (j < a.nk) q[0] = v0;
+      if (j + 1 < a.nk) q[1] = v1;
+      if (j + 2 < a.nk) q[2] = v2;
+      if (j + 3 < a.nk) q[3] = v3;
+    }
+  } else {
+    bf16* q = (bf16*)p + j;
+    if (fast) {
+      *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf16(v0, v1), pack_bf16(v2, v3));
+    } else {
+      if (j < a.nk) q[0] = __float2bfloat16_rn(v0);
+      if (j + 1 < a.nk) q[1] = __float2bfloat16_rn(v1);
+      if (j + 2 < a.nk) q[2] = __float2bfloat16_rn(v2);
+      if (j + 3 < a.nk) q[3] = __float2bfloat16_rn(v3);
+    }
+  }
+}
+
+// 8 consecutive accumulator columns of a row, two per lane
+__device__ __forceinline__ void store_pair(bf16* p, int col, int d, bool vec, float v0, float v1) {
+  if (vec) {
+    if (col < d) *reinterpret_cast<uint32_t*>(p + col) = pack_bf16(v0, v1);
+  } else {
+    if (col < d) p[col] = __float2bfloat16_rn(v0);
+    if (col + 1 < d) p[col + 1] = __float2bfloat16_rn(v1);
+  }
+}
+__device__ __forceinline__ bool pair_ok(const void* p, int64_t bs, int64_t ns, int64_t hs, int d) {
+  return ((uintptr_t)p & 3) == 0 && ((bs | ns | hs | d) & 1) == 0;
+}
+
+// ---------------------------------------------------------------- forward
+
+template <int DP, int BT, int MT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
+  using S = Tile<DP>;
+  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sq = smem_addr(raw), sk = sq + QR * S::RB, sv = sk + 2 * kTile * S::RB;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV);
+  const int64_t b = id / a.H;
+  const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT;
+  const int nt = (int)((a.nk + kTile - 1) / kTile);
+  const bf16 *bk = head_base(a.k, b, kh), *bv = head_base(a.v, b, kh);
+  load_rows<DP, QR>(sq, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+  auto issue = [&](int kt, uint64_t live) {
+    const uint32_t s = (kt & 1) * kTile * S::RB;
+    load_rows<DP, kTile>(sk + s, bk, a.k.ns, a.vec_k, (int64_t)kt * kTile, a.nk, a.d, live);
+    load_rows<DP, kTile>(sv + s, bv, a.v.ns, a.vec_v, (int64_t)kt * kTile, a.nk, a.d, live);
+    cp_commit();
+  };
+  const char* brow[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + m * 16 + r * 8 + g;
+      brow[m][r] = bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1);  // rows past the end are not stored
+    }
+  Bias4<BT> ring[2][MT][2];
+  auto fetch_bias = [&](int slot, int64_t j0) {  // keys j0 .. j0 + 15
+    if (BT == 0 || j0 >= a.nk) return;
+    const bool fast = a.bias_vec && j0 + 16 <= a.nk;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][m][r], brow[m][r], j0 + 4 * t, a.nk, fast);
+  };
+  float acc[MT][NB][4], mx[MT][2], sum[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+    mx[m][0] = mx[m][1] = -INFINITY;
+    sum[m][0] = sum[m][1] = 0.f;
+  }
+  uint32_t fq[MT][KS][4];
+  float2 rawm = seen_raw(a, b, 0);
+  uint64_t bits = seen_ballot(rawm);
+  if (nt > 0) issue(0, bits);
+  rawm = seen_raw(a, b, kTile);
+  fetch_bias(0, 0);
+  fetch_bias(1, 16);
+  for (int kt = 0; kt < nt; ++kt) {
+    const uint64_t next = seen_ballot(rawm);
+    cp_wait<0>();
+    __syncthreads();
+    if (kt == 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
+    }
+    if (kt + 1 < nt) issue(kt + 1, next);
+    rawm = seen_raw(a, b, (int64_t)(kt + 2) * kTile);
+    const int64_t j0 = (int64_t)kt * kTile;
+    if (bits == 0) {  // no visible key: the same for the whole block
+      fetch_bias(0, j0 + 64);
+      fetch_bias(1, j0 + 80);
+      bits = next;
+      continue;
+    }
+    const uint32_t tk = sk + (kt & 1) * kTile * S::RB, tv = sv + (kt & 1) * kTile * S::RB;
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb) {  // 32 keys
+      float x[MT][4][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[m][n][e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t r[4];
+          ldsm4(r, lb.at(tk, hb * 2 + q, k));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma(x[m][2 * q], fq[m][k], r[0], r[1]);
+            mma(x[m][2 * q + 1], fq[m][k], r[2], r[3]);
+          }
+        }
+      const uint32_t hbits = (uint32_t)(bits >> (32 * hb));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[m][2 * q + n][e] = score<BT>(x[m][2 * q + n][e], a.scale, ring[q][m][e >> 1], 2 * n + (e & 1));
+        fetch_bias(q, j0 + hb * 32 + q * 16 + 32);
+      }
+      if (hbits != 0xffffffffu) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t mine = hbits >> (16 * q + 4 * t);
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!((mine >> (2 * n + e)) & 1))
+#pragma unroll
+                for (int m = 0; m < MT; ++m) x[m][2 * q + n][e] = x[m][2 * q + n][2 + e] = -INFINITY;
+        }
+      }
+      bool grew = false;
+      float nm[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float v = mx[m][r];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) v = fmaxf(v, fmaxf(x[m][n][2 * r], x[m][n][2 * r + 1]));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          nm[m][r] = v;
+          grew |= v != mx[m][r];
+        }
+      if (__any_sync(0xffffffffu, grew)) {  // rare after the first tiles
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float corr = nm[m][r] == mx[m][r] ? 1.f : ex2((mx[m][r] - nm[m][r]) * kLog2e);
+            mx[m][r] = nm[m][r];
+            sum[m][r] *= corr;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              acc[m][n][2 * r] *= corr;
+              acc[m][n][2 * r + 1] *= corr;
+            }
+          }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float base = mx[m][r] == -INFINITY ? 0.f : mx[m][r];  // nothing seen yet: every p is 0
+          float s = 0.f;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float p = ex2((x[m][n][2 * r + e] - base) * kLog2e);
+              x[m][n][2 * r + e] = p;
+              s += p;
+            }
+          sum[m][r] += s;
+        }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t f[NB / 2][4];
+#pragma unroll
+        for (int c = 0; c < NB / 2; ++c) ldsm4_t(f[c], lt.at(tv, hb * 2 + q, c));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          // p as the sum of bf16 values (see the head of pf_attention.cuh)
+          for (int term = 0; term < a.p_terms; ++term) {
+            uint32_t pa[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float* v = &x[m][2 * q + (i >> 1)][2 * (i & 1)];
+              pa[i] = pack_bf16(v[0], v[1]);
+              v[0] -= lo_f(pa[i]);
+              v[1] -= hi_f(pa[i]);
+            }
+#pragma unroll
+            for (int c = 0; c < NB / 2; ++c) {
+              mma(acc[m][2 * c], pa, f[c][0], f[c][1]);
+              mma(acc[m][2 * c + 1], pa, f[c][2], f[c][3]);
+            }
+          }
+        }
+      }
+    }
+    bits = next;
+  }
+  cp_commit();
+  cp_wait<0>();
+  const bool vec = pair_ok(a.o, a.o_bs, a.o_ns, a.o_hs, a.d);
+  const bool lo_vec = (a.d & 1) == 0;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float l = sum[m][r];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t i = w0 + m * 16 + r * 8 + g;
+      if (i >= a.nq) continue;
+      if (a.stats && t == 0) {
+        const int64_t at = (b * a.H + h) * a.nq + i;
+        a.stats[at] = mx[m][r];
+        a.stats[a.rows_plane + at] = l;
+      }
+      bf16* o = (bf16*)a.o + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
+      int16_t* lo = a.o_lo ? a.o_lo + ((b * a.nq + i) * a.H + h) * a.d : nullptr;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int col = n * 8 + 2 * t;
+        const float v0 = acc[m][n][2 * r] * inv, v1 = acc[m][n][2 * r + 1] * inv;
+        store_pair(o, col, a.d, vec, v0, v1);
+        if (lo) {
+          // fp32 bits of o less those of its bf16 rounding: o is their sum again (a tie that rounds down
+          // would need one more than 16 bits hold and loses the last bit; NaN keeps none)
+          const uint32_t w = pack_bf16(v0, v1);
+          const int d0 = min((int)(__float_as_uint(v0) - (w << 16)), 32767);
+          const int d1 = min((int)(__float_as_uint(v1) - (w & 0xffff0000u)), 32767);
+          const int16_t l0 = v0 == v0 ? (int16_t)d0 : (int16_t)0, l1 = v1 == v1 ? (int16_t)d1 : (int16_t)0;
+          if (lo_vec) {
+            if (col < a.d) *reinterpret_cast<short2*>(lo + col) = make_short2(l0, l1);
+          } else {
+            if (col < a.d) lo[col] = l0;
+            if (col + 1 < a.d) lo[col + 1] = l1;
+          }
+        }
+      }
+    }
+}
+
+// ---------------------------------------------------------------- row constants
+
+// Eight lanes per row (b, i, h): D, and {m, -log2 l, peak, -D}; peak = 1 where one key has all of the
+// row's weight in fp32 (l = 1).
+__global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ stats, Heads o,
+                                              const int16_t* __restrict__ lo, float4* __restrict__ rows) {
+  const int sub = threadIdx.x & 7;
+  const int64_t r = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const bool live = r < a.rows_plane;
+  const int64_t rr = live ? r : 0;
+  const int h = (int)(rr % a.H);
+  const int64_t bi = rr / a.H, b = bi / a.nq, i = bi - b * a.nq;
+  const bf16* po = head_base(o, b, h) + i * o.ns;
+  const bf16* pg = head_base(a.g, b, h) + i * a.g.ns;
+  float s = 0.f;
+  if (live)
+    for (int e = sub; e < a.d; e += 8) {
+      float v = to_f(po[e]);
+      if (v == v) v = __uint_as_float(__float_as_uint(v) + (int)lo[rr * a.d + e]);
+      s += v * to_f(pg[e]);
+    }
+  s += __shfl_xor_sync(0xffffffffu, s, 1);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  s += __shfl_xor_sync(0xffffffffu, s, 4);
+  if (!live || sub) return;
+  const int64_t at = (b * a.H + h) * a.nq + i;
+  const float m = stats[at], l = stats[a.rows_plane + at];
+  const bool none = l == 0.f;
+  rows[at] = make_float4(none ? INFINITY : m, none ? 0.f : -log2f(l), l == 1.f ? 1.f : 0.f, none ? 0.f : -s);
+}
+
+// ---------------------------------------------------------------- dq (and dbias of one batch entry)
+
+template <int DP, int BT, int MT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
+  using S = Tile<DP>;
+  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sq = smem_addr(raw), sg = sq + QR * S::RB, sk = sg + QR * S::RB, sv = sk + 2 * kTile * S::RB;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV);
+  const int64_t b = id / a.H;
+  const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT;
+  const int nt = (int)((a.nk + kTile - 1) / kTile);
+  const bf16 *bk = head_base(a.k, b, kh), *bv = head_base(a.v, b, kh);
+  load_rows<DP, QR>(sq, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+  load_rows<DP, QR>(sg, head_base(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+  auto issue = [&](int kt, uint64_t live) {
+    const uint32_t s = (kt & 1) * kTile * S::RB;
+    load_rows<DP, kTile>(sk + s, bk, a.k.ns, a.vec_k, (int64_t)kt * kTile, a.nk, a.d, live);
+    load_rows<DP, kTile>(sv + s, bv, a.v.ns, a.vec_v, (int64_t)kt * kTile, a.nk, a.d, live);
+    cp_commit();
+  };
+  const char* brow[MT][2];
+  char* drow[MT][2];
+  float4 rc[MT][2];
+  const int bsz = BT == 2 ? 4 : 2;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + m * 16 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
+      brow[m][r] = bias_row<BT>(a, b, h, ic);
+      drow[m][r] = (BT && a.dbias && i < a.nq)
+                       ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs) * bsz
+                       : nullptr;
+      rc[m][r] = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
+    }
+  bool peaked = false;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) peaked |= rc[m][0].z != 0.f || rc[m][1].z != 0.f;
+  peaked = __any_sync(0xffffffffu, peaked);
+  Bias4<BT> ring[2][MT][2];
+  auto fetch_bias = [&](int slot, int64_t j0) {
+    if (BT == 0 || j0 >= a.nk) return;
+    const bool fast = a.bias_vec && j0 + 16 <= a.nk;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][m][r], brow[m][r], j0 + 4 * t, a.nk, fast);
+  };
+  float acc[MT][NB][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+  uint32_t fq[MT][KS][4], fg[MT][KS][4];
+  float2 rawm = seen_raw(a, b, 0);
+  uint64_t bits = seen_ballot(rawm);
+  if (nt > 0) issue(0, bits);
+  rawm = seen_raw(a, b, kTile);
+  fetch_bias(0, 0);
+  fetch_bias(1, 16);
+  for (int kt = 0; kt < nt; ++kt) {
+    const uint64_t next = seen_ballot(rawm);
+    cp_wait<0>();
+    __syncthreads();
+    if (kt == 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
+          ldsm4(fg[m][k], la.at(sg, warp * MT + m, k));
+        }
+    }
+    if (kt + 1 < nt) issue(kt + 1, next);
+    rawm = seen_raw(a, b, (int64_t)(kt + 2) * kTile);
+    const int64_t j0 = (int64_t)kt * kTile;
+    const uint32_t tk = sk + (kt & 1) * kTile * S::RB, tv = sv + (kt & 1) * kTile * S::RB;
+    if (bits == 0 && !(BT && a.dbias)) {
+      fetch_bias(0, j0 + 64);
+      fetch_bias(1, j0 + 80);
+      bits = next;
+      continue;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // 16 keys
+      float x[MT][2][4], y[MT][2][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[m][n][e] = y[m][n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t r[4], u[4];
+        ldsm4(r, lb.at(tk, q, k));
+        ldsm4(u, lb.at(tv, q, k));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma(x[m][0], fq[m][k], r[0], r[1]);
+          mma(x[m][1], fq[m][k], r[2], r[3]);
+          mma(y[m][0], fg[m][k], u[0], u[1]);
+          mma(y[m][1], fg[m][k], u[2], u[3]);
+        }
+      }
+      const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[m][n][e] = score<BT>(x[m][n][e], a.scale, ring[q & 1][m][e >> 1], 2 * n + (e & 1));
+      fetch_bias(q & 1, j0 + q * 16 + 32);
+      if (qbits != 0xffffu) {
+        const uint32_t mine = qbits >> (4 * t);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!((mine >> (2 * n + e)) & 1))
+#pragma unroll
+              for (int m = 0; m < MT; ++m) x[m][n][e] = x[m][n][2 + e] = -INFINITY;
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 c = rc[m][e >> 1];
+            const float p = ex2(fmaf(x[m][n][e] - c.x, kLog2e, c.y));
+            x[m][n][e] = p;
+            y[m][n][e] = p * (y[m][n][e] + c.w);
+          }
+      if (peaked) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (x[m][n][e] == 1.f) y[m][n][e] = 0.f;
+      }
+      if (BT && a.dbias) {
+        const int64_t j = j0 + q * 16 + 4 * t;
+        const bool fast = a.db_vec && j0 + q * 16 + 16 <= a.nk;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (drow[m][r])
+              store_bias4<BT>(a, drow[m][r], j, fast, y[m][0][2 * r], y[m][0][2 * r + 1], y[m][1][2 * r],
+                              y[m][1][2 * r + 1]);
+      }
+      uint32_t da[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) da[m][i] = pack_bf16(y[m][i >> 1][2 * (i & 1)], y[m][i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+      for (int c = 0; c < NB / 2; ++c) {
+        uint32_t f[4];
+        ldsm4_t(f, lt.at(tk, q, c));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma(acc[m][2 * c], da[m], f[0], f[1]);
+          mma(acc[m][2 * c + 1], da[m], f[2], f[3]);
+        }
+      }
+    }
+    bits = next;
+  }
+  cp_commit();
+  cp_wait<0>();
+  if (!a.dq) return;
+  const bool vec = pair_ok(a.dq, a.o_bs, a.o_ns, a.o_hs, a.d);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + m * 16 + r * 8 + g;
+      if (i >= a.nq) continue;
+      bf16* o = (bf16*)a.dq + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        store_pair(o, n * 8 + 2 * t, a.d, vec, acc[m][n][2 * r] * a.scale, acc[m][n][2 * r + 1] * a.scale);
+    }
+}
+
+// ---------------------------------------------------------------- dk, dv
+
+// 16 KM keys per warp; HOLD: their fragments stay in registers.
+template <int DP, int BT, int KM>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
+  using S = Tile<DP>;
+  constexpr int KR = 64 * KM, KS = DP / 16, NB = DP / 8;
+  constexpr bool HOLD = DP <= 64;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sk = smem_addr(raw), sv = sk + KR * S::RB, sq = sv + KR * S::RB, sg = sq + 2 * kTile * S::RB,
+                 sc = sg + 2 * kTile * S::RB;
+  const float4* cst = (const float4*)(raw + (sc - sk));  // [2][64]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), ln = lane_bn<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int kh = id % a.KV, group = a.H / a.KV;
+  const int64_t b = id / a.KV;
+  const int64_t j0 = (int64_t)tile * KR, w0 = j0 + warp * 16 * KM;
+  const int per = (int)((a.nq + kTile - 1) / kTile);
+  uint64_t live[KM];  // visible keys of the block, 64 at a time
+#pragma unroll
+  for (int i = 0; i < KM; ++i) live[i] = seen_ballot(seen_raw(a, b, j0 + 64 * i));
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < KM; ++i) {
+    any |= live[i] != 0;
+    load_rows<DP, 64>(sk + i * 64 * S::RB, head_base(a.k, b, kh), a.k.ns, a.vec_k, j0 + 64 * i, a.nk, a.d, live[i]);
+    load_rows<DP, 64>(sv + i * 64 * S::RB, head_base(a.v, b, kh), a.v.ns, a.vec_v, j0 + 64 * i, a.nk, a.d, live[i]);
+  }
+  // the warp's keys, 16 KM bits
+  const uint32_t mine = (uint32_t)(live[(warp * 16 * KM) / 64] >> ((warp * 16 * KM) & 63)) &
+                        (KM == 2 ? 0xffffffffu : 0xffffu);
+  const bool full = mine == (KM == 2 ? 0xffffffffu : 0xffffu);
+  const bool bfast = a.bias_vec && w0 + 16 * KM <= a.nk;
+  // head and query tile of the step being loaded
+  int lh = 0, lt = 0, stage = 0;
+  auto issue = [&]() {
+    const int h = kh * group + lh;
+    const int64_t i0 = (int64_t)lt * kTile;
+    const uint32_t s = stage * kTile * S::RB;
+    load_rows<DP, kTile>(sq + s, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+    load_rows<DP, kTile>(sg + s, head_base(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+    if (threadIdx.x < kTile) {
+      const int64_t i = i0 + threadIdx.x;
+      const float4* p = (const float4*)a.rows + (b * a.H + h) * a.nq;
+      cp_async16(sc + (stage * kTile + threadIdx.x) * 16, i < a.nq ? p + i : p, i < a.nq);
+    }
+    cp_commit();
+    stage ^= 1;
+    if (++lt == per) lt = 0, ++lh;
+  };
+  float dk[KM][NB][4], dv[KM][NB][4];
+#pragma unroll
+  for (int m = 0; m < KM; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dk[m][n][e] = dv[m][n][e] = 0.f;
+  uint32_t fk[HOLD ? KM : 1][HOLD ? KS : 1][4], fv[HOLD ? KM : 1][HOLD ? KS : 1][4];
+  Bias4<BT> ring[2][KM][2];
+  if (any && per > 0) {
+    issue();
+    for (int hh = 0; hh < group; ++hh) {
+      const int h = kh * group + hh;
+      // rows i0 + 16 blk + g (+ 8) of this head into a slot; 0 past the end
+      auto fetch_bias = [&](int slot, int64_t i0) {
+        if (BT == 0) return;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int64_t i = i0 + 8 * r + g;
+          if (i < a.nq) {
+            const char* p = bias_row<BT>(a, b, h, i);
+#pragma unroll
+            for (int m = 0; m < KM; ++m) bias_load<BT>(ring[slot][m][r], p, w0 + 16 * m + 4 * t, a.nk, bfast);
+          } else {
+#pragma unroll
+            for (int m = 0; m < KM; ++m)
+#pragma unroll
+              for (int w = 0; w < (BT == 2 ? 4 : 2); ++w)
+                if (BT) ring[slot][m][r].w[w] = 0;
+          }
+        }
+      };
+      fetch_bias(0, 0);
+      fetch_bias(1, 16);
+      for (int qt = 0; qt < per; ++qt) {
+        const int s = (hh * per + qt) & 1;
+        cp_wait<0>();
+        __syncthreads();
+        if (HOLD && hh == 0 && qt == 0) {
+#pragma unroll
+          for (int m = 0; m < (HOLD ? KM : 0); ++m)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              ldsm4(fk[m][k], lb.at(sk, warp * KM + m, k));
+              ldsm4(fv[m][k], lb.at(sv, warp * KM + m, k));
+            }
+        }
+        if (lh < group) issue();
+        const uint32_t tq = sq + s * kTile * S::RB, tg = sg + s * kTile * S::RB;
+        const int64_t i0 = (int64_t)qt * kTile;
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {  // 16 queries
+          float x[KM][2][4], y[KM][2][4];
+#pragma unroll
+          for (int m = 0; m < KM; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[m][n][e] = y[m][n][e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            uint32_t fq[4], fg[4];
+            ldsm4(fq, la.at(tq, blk, k));
+            ldsm4(fg, la.at(tg, blk, k));
+#pragma unroll
+            for (int m = 0; m < KM; ++m) {
+              uint32_t rk[4], rv[4];
+              if (HOLD) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rk[i] = fk[m][k][i], rv[i] = fv[m][k][i];
+              } else {
+                ldsm4(rk, lb.at(sk, warp * KM + m, k));
+                ldsm4(rv, lb.at(sv, warp * KM + m, k));
+              }
+              mma(x[m][0], fq, rk[0], rk[1]);
+              mma(x[m][1], fq, rk[2], rk[3]);
+              mma(y[m][0], fg, rv[0], rv[1]);
+              mma(y[m][1], fg, rv[2], rv[3]);
+            }
+          }
+          const float4 c[2] = {cst[s * kTile + blk * 16 + g], cst[s * kTile + blk * 16 + 8 + g]};
+#pragma unroll
+          for (int m = 0; m < KM; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[m][n][e] = score<BT>(x[m][n][e], a.scale, ring[blk & 1][m][e >> 1], 2 * n + (e & 1));
+          fetch_bias(blk & 1, i0 + blk * 16 + 32);
+          if (!full) {
+#pragma unroll
+            for (int m = 0; m < KM; ++m)
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (!((mine >> (16 * m + 4 * t + 2 * n + e)) & 1)) x[m][n][e] = x[m][n][2 + e] = -INFINITY;
+          }
+          const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
+          uint32_t pa[KM][4], da[KM][4];
+#pragma unroll
+          for (int m = 0; m < KM; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                float p[2], ds[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  p[e] = ex2(fmaf(x[m][n][2 * r + e] - c[r].x, kLog2e, c[r].y));
+                  ds[e] = p[e] * (y[m][n][2 * r + e] + c[r].w);
+                  if (peaked && p[e] == 1.f) ds[e] = 0.f;
+                }
+                pa[m][2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
+                da[m][2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
+              }
+#pragma unroll
+          for (int n = 0; n < NB / 2; ++n) {
+            uint32_t fg[4], fq[4];
+            ldsm4_t(fg, ln.at(tg, blk, n));
+            ldsm4_t(fq, ln.at(tq, blk, n));
+#pragma unroll
+            for (int m = 0; m < KM; ++m) {
+              mma(dv[m][2 * n], pa[m], fg[0], fg[1]);
+              mma(dv[m][2 * n + 1], pa[m], fg[2], fg[3]);
+              mma(dk[m][2 * n], da[m], fq[0], fq[1]);
+              mma(dk[m][2 * n + 1], da[m], fq[2], fq[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+  cp_commit();
+  cp_wait<0>();
+  const bool vk = pair_ok(a.dk, a.dk_bs, a.dk_ns, a.dk_hs, a.d), vv = pair_ok(a.dv, a.dv_bs, a.dv_ns, a.dv_hs, a.d);
+#pragma unroll
+  for (int m = 0; m < KM; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t j = w0 + 16 * m + perm_row(g, r);  // row g + 8 r of the block holds this key
+      if (j >= a.nk) continue;
+      bf16* ok = (bf16*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j * a.dk_ns;
+      bf16* ov = (bf16*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j * a.dv_ns;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        store_pair(ok, n * 8 + 2 * t, a.d, vk, dk[m][n][2 * r] * a.scale, dk[m][n][2 * r + 1] * a.scale);
+        store_pair(ov, n * 8 + 2 * t, a.d, vv, dv[m][n][2 * r], dv[m][n][2 * r + 1]);
+      }
+    }
+}
+
+// ---------------------------------------------------------------- dbias shared by the batch
+
+// A 128 x 64 tile of one head's plane, summed over the batch entries of a part; with one part the
+// result is written, else an fp32 partial plane [part][H][n_q][n_k] that k_sum_planes adds up.
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, float* part, int parts) {
+  using S = Tile<DP>;
+  constexpr int MT = 2, QR = 128, KS = DP / 16;
+  constexpr bool HOLD = DP == 32;
+  extern __shared__ __align__(128) unsigned char raw[];
+  constexpr int kStage = (2 * QR + 2 * kTile) * S::RB + QR * 16;
+  const uint32_t s0 = smem_addr(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned nkt = (unsigned)((a.nk + kTile - 1) / kTile);
+  const unsigned kt = id % nkt;
+  id /= nkt;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV);
+  const int p = id / a.H;
+  const int64_t b0 = a.B * p / parts, b1 = a.B * (p + 1) / parts;
+  const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT, j0 = (int64_t)kt * kTile;
+  auto issue = [&](int64_t b, uint64_t live) {
+    const uint32_t q = s0 + (int)(b & 1) * kStage, gr = q + QR * S::RB, k = gr + QR * S::RB, v = k + kTile * S::RB,
+                   c = v + kTile * S::RB;
+    load_rows<DP, QR>(q, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+    load_rows<DP, QR>(gr, head_base(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+    load_rows<DP, kTile>(k, head_base(a.k, b, kh), a.k.ns, a.vec_k, j0, a.nk, a.d, live);
+    load_rows<DP, kTile>(v, head_base(a.v, b, kh), a.v.ns, a.vec_v, j0, a.nk, a.d, live);
+    const int64_t i = i0 + threadIdx.x;  // kThreads == QR
+    const float4* pr = (const float4*)a.rows + (b * a.H + h) * a.nq;
+    cp_async16(c + threadIdx.x * 16, i < a.nq ? pr + i : pr, i < a.nq);
+    cp_commit();
+  };
+  const char* brow[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + m * 16 + r * 8 + g;
+      brow[m][r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1);
+    }
+  const bool fast = a.bias_vec && j0 + kTile <= a.nk;
+  float acc[MT][8][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+  uint64_t bits = b0 < b1 ? seen_ballot(seen_raw(a, b0, j0)) : 0;
+  if (b0 < b1) issue(b0, bits);
+  float2 rawm = b0 + 1 < b1 ? seen_raw(a, b0 + 1, j0) : make_float2(0.f, 0.f);
+  for (int64_t b = b0; b < b1; ++b) {
+    const uint64_t next = seen_ballot(rawm);
+    cp_wait<0>();
+    __syncthreads();
+    if (b + 1 < b1) issue(b + 1, next);
+    rawm = b + 2 < b1 ? seen_raw(a, b + 2, j0) : make_float2(0.f, 0.f);
+    if (bits == 0) {
+      bits = next;
+      continue;
+    }
+    const uint32_t tq = s0 + (int)(b & 1) * kStage, tg = tq + QR * S::RB, tk = tg + QR * S::RB,
+                   tv = tk + kTile * S::RB;
+    const float4* cst = (const float4*)(raw + (int)(b & 1) * kStage + (2 * QR + 2 * kTile) * S::RB);
+    uint32_t fq[HOLD ? MT : 1][HOLD ? KS : 1][4], fg[HOLD ? MT : 1][HOLD ? KS : 1][4];
+    if (HOLD) {
+#pragma unroll
+      for (int m = 0; m < (HOLD ? MT : 0); ++m)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          ldsm4(fq[m][k], la.at(tq, warp * MT + m, k));
+          ldsm4(fg[m][k], la.at(tg, warp * MT + m, k));
+        }
+    }
+    float4 rc[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) rc[m][r] = cst[warp * 16 * MT + m * 16 + r * 8 + g];
+    bool peaked = false;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) peaked |= rc[m][0].z != 0.f || rc[m][1].z != 0.f;
+    peaked = __any_sync(0xffffffffu, peaked);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      Bias4<BT> br[MT][2];  // the same every batch entry: from L1
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) bias_load<BT>(br[m][r], brow[m][r], j0 + q * 16 + 4 * t, a.nk, fast);
+      float x[MT][2][4], y[MT][2][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[m][n][e] = y[m][n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t r[4], u[4];
+        ldsm4(r, lb.at(tk, q, k));
+        ldsm4(u, lb.at(tv, q, k));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint32_t rq[4], rg[4];
+          if (HOLD) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rq[i] = fq[m][k][i], rg[i] = fg[m][k][i];
+          } else {
+            ldsm4(rq, la.at(tq, warp * MT + m, k));
+            ldsm4(rg, la.at(tg, warp * MT + m, k));
+          }
+          mma(x[m][0], rq, r[0], r[1]);
+          mma(x[m][1], rq, r[2], r[3]);
+          mma(y[m][0], rg, u[0], u[1]);
+          mma(y[m][1], rg, u[2], u[3]);
+        }
+      }
+      const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = score<BT>(x[m][n][e], a.scale, br[m][e >> 1], 2 * n + (e & 1));
+            if (qbits != 0xffffu && !((qbits >> (4 * t + 2 * n + (e & 1))) & 1)) v = -INFINITY;
+            const float4 c = rc[m][e >> 1];
+            const float pr = ex2(fmaf(v - c.x, kLog2e, c.y));
+            const float dl = (peaked && pr == 1.f) ? 0.f : y[m][n][e] + c.w;
+            acc[m][2 * q + n][e] = fmaf(pr, dl, acc[m][2 * q + n][e]);
+          }
+    }
+    bits = next;
+  }
+  cp_commit();
+  cp_wait<0>();
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + m * 16 + r * 8 + g;
+      if (i >= a.nq) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t j = j0 + q * 16 + 4 * t;
+        const float v0 = acc[m][2 * q][2 * r], v1 = acc[m][2 * q][2 * r + 1], v2 = acc[m][2 * q + 1][2 * r],
+                    v3 = acc[m][2 * q + 1][2 * r + 1];
+        if (parts == 1)
+          store_bias4<BT>(a, (char*)a.dbias + ((int64_t)h * a.db_hs + i * a.db_rs) * (BT == 2 ? 4 : 2), j,
+                          a.db_vec && j0 + q * 16 + 16 <= a.nk, v0, v1, v2, v3);
+        else
+          store_bias4<2>(a, (char*)(part + (((int64_t)p * a.H + h) * a.nq + i) * a.nk), j,
+                         (a.nk & 3) == 0 && j0 + q * 16 + 16 <= a.nk, v0, v1, v2, v3);
+      }
+    }
+}
+
+template <int BT>
+__global__ void __launch_bounds__(256) k_sum_planes(Args a, const float* __restrict__ part, int parts) {
+  const int64_t n = (int64_t)a.H * a.nq * a.nk;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p) s += part[p * n + i];
+    const int64_t j = i % a.nk, hi = i / a.nk, h = hi / a.nq, q = hi - h * a.nq;
+    const int64_t off = h * a.db_hs + q * a.db_rs + j;
+    if (BT == 2)
+      ((float*)a.dbias)[off] = s;
+    else
+      ((bf16*)a.dbias)[off] = __float2bfloat16_rn(s);
+  }
+}
+
+// ---------------------------------------------------------------- launches
+
+template <class F, class... X>
+int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cudaStream_t st, X... x) {
+  if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
+  if (smem > 40 * 1024)
+    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  {
+    PF_LAUNCH_SCOPE_WORK(st, name, flops, 'f');
+    kern<<<(unsigned)blocks, kThreads, smem, st>>>(x...);
+  }
+  PF_CHECK_LAUNCH();
+  return PF_OK;
+}
+
+template <int DP, int BT>
+int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
+  constexpr size_t RB = Tile<DP>::RB;
+  // two row blocks per warp where the accumulators leave room for them and there are blocks enough
+  const int64_t rows = kind == kDkv ? a.nk : a.nq, heads = (kind == kDkv ? a.KV : a.H) * a.B;
+  const int64_t t1 = (rows + 63) / 64, t2 = (rows + 127) / 128;
+  const bool two = DP == 32 && t2 * heads >= 3 * 148;
+  a.tiles = two ? t2 : t1;
+  const int64_t blocks = a.tiles * heads;
+  if (blocks == 0) return PF_OK;
+  switch (kind) {
+    case kFwd:
+      if constexpr (DP == 32)
+        if (two) return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
+      return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
+    case kDq:
+      if constexpr (DP == 32)
+        if (two) return go(k_dq<DP, BT, 2>, (256 + 4 * kTile) * RB, blocks, "k_attn_dq", flops, st, a);
+      return go(k_dq<DP, BT, 1>, (128 + 4 * kTile) * RB, blocks, "k_attn_dq", flops, st, a);
+    default:
+      if constexpr (DP == 32)
+        if (two) return go(k_dkv<DP, BT, 2>, (256 + 4 * kTile) * RB + 2048, blocks, "k_attn_dkv", flops, st, a);
+      return go(k_dkv<DP, BT, 1>, (128 + 4 * kTile) * RB + 2048, blocks, "k_attn_dkv", flops, st, a);
+  }
+}
+
+template <int DP, int BT>
+int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
+  constexpr size_t smem = 2 * ((size_t)(256 + 128) * Tile<DP>::RB + 2048);
+  a.tiles = (a.nq + 127) / 128;
+  PF_TRY(go(k_dbias<DP, BT>, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, "k_attn_dbias", flops, st, a, part,
+            parts));
+  if (parts == 1) return PF_OK;
+  const int64_t n = (int64_t)a.H * a.nq * a.nk, want = (n + 255) / 256;
+  {
+    PF_LAUNCH_SCOPE_WORK(st, "k_attn_sum_planes", 4.0 * n * (parts + 1), 'b');
+    k_sum_planes<BT><<<(unsigned)(want < 148 * 8 ? want : 148 * 8), 256, 0, st>>>(a, part, parts);
+  }
+  PF_CHECK_LAUNCH();
+  return PF_OK;
+}
+
+}  // namespace
+
+#define PF_ATT_DIM(FN, BT, ...)                    \
+  do {                                             \
+    if (a.d <= 32) return FN<32, BT>(__VA_ARGS__); \
+    if (a.d <= 64) return FN<64, BT>(__VA_ARGS__); \
+    if (a.d <= 96) return FN<96, BT>(__VA_ARGS__); \
+    return FN<128, BT>(__VA_ARGS__);               \
+  } while (0)
+
+int launch_bf16(Kind kind, const Args& a, double flops, cudaStream_t st) {
+  if (!a.bias) PF_ATT_DIM(launch_t, 0, kind, a, flops, st);
+  if (a.bias_f32) PF_ATT_DIM(launch_t, 2, kind, a, flops, st);
+  PF_ATT_DIM(launch_t, 1, kind, a, flops, st);
+}
+
+// Parts of the batch: about three blocks per SM.
+int dbias_parts_bf16(int64_t B, int64_t nq, int64_t nk, int H) {
+  const int64_t blocks = ((nq + 127) / 128) * ((nk + 63) / 64) * H;
+  if (blocks <= 0) return 1;
+  int64_t p = (3 * 148 + blocks - 1) / blocks;
+  if (p > B / 4) p = B / 4;
+  return p < 1 ? 1 : (int)p;
+}
+int dbias_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
+  if (a.bias_f32) PF_ATT_DIM(launch_db, 2, a, part, parts, flops, st);
+  PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);
+}
+
 int rows_bf16(const Args& a, const float* stats, Heads o, const int16_t* lo, float* rows, cudaStream_t st) {
-  return launch_rows<__nv_bfloat16>(a, stats, o, lo, rows, st);
+  const int64_t blocks = (a.rows_plane + 31) / 32;
+  if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: too many rows");
+  {
+    PF_LAUNCH_SCOPE_WORK(st, "k_attn_rows", (6.0 * a.d + 24.0) * (double)a.rows_plane, 'b');
+    k_rows<<<(unsigned)blocks, 256, 0, st>>>(a, stats, o, lo, (float4*)rows);
+  }
+  PF_CHECK_LAUNCH();
+  return PF_OK;
 }
+
 }  // namespace attn
 }  // namespace train
 }  // namespace pf
