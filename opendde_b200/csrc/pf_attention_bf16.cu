@@ -78,20 +78,48 @@ __device__ __forceinline__ LaneAddr<DP> lane_bn() {
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the first product of a sum
+__device__ __forceinline__ void mma0(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Two fp32 values side by side: one instruction for both (half the issue slots of scalar arithmetic).
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit F2(float a) : F2(a, a) {}
+  __device__ __forceinline__ void get(float& a, float& b) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -196,10 +224,25 @@ __device__ __forceinline__ float bias_val(const Bias4<BT>& r, int i) {
   if (BT == 2) return __uint_as_float(r.w[i]);
   return 0.f;
 }
-// scale * s + bias, s in natural units (next to a bias of the type's lowest value a factor log2(e) overflows)
+// Scores of two neighbouring columns, scale * s + bias, s in natural units (next to a bias of the type's lowest
+// value a factor log2(e) would overflow).
 template <int BT>
-__device__ __forceinline__ float score(float s, float scale, const Bias4<BT>& r, int i) {
-  return BT == 0 ? s * scale : fmaf(s, scale, bias_val<BT>(r, i));
+__device__ __forceinline__ void score2(float* x, F2 scale, const Bias4<BT>& r, int n) {
+  const F2 s = F2(x[0], x[1]);
+  const F2 y = BT == 0 ? mul2(s, scale) : fma2(s, scale, F2(bias_val<BT>(r, 2 * n), bias_val<BT>(r, 2 * n + 1)));
+  y.get(x[0], x[1]);
+}
+// p of two neighbouring columns from their scores: exp(t - m) / l with nm = -m, c = -log2 l
+__device__ __forceinline__ F2 prob2(const float* x, F2 nm, F2 c) {
+  const F2 y = fma2(add2(F2(x[0], x[1]), nm), F2(kLog2e), c);
+  float p0, p1;
+  y.get(p0, p1);
+  return F2(ex2(p0), ex2(p1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // one row's four columns of a group as stored by the products: x[0][2r..] then x[1][2r..]
@@ -248,6 +291,7 @@ template <int DP, int BT, int MT>
 __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
   using S = Tile<DP>;
   constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8;
+  constexpr int TERMS = BT == 2 ? 3 : 2;  // bf16 values that p is split into (see the head of pf_attention.cuh)
   extern __shared__ __align__(128) unsigned char raw[];
   const uint32_t sq = smem_addr(raw), sk = sq + QR * S::RB, sv = sk + 2 * kTile * S::RB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -284,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][m][r], brow[m][r], j0 + 4 * t, a.nk, fast);
   };
+  const F2 scale(a.scale);
   float acc[MT][NB][4], mx[MT][2], sum[MT][2];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -325,12 +370,6 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
     for (int hb = 0; hb < 2; ++hb) {  // 32 keys
       float x[MT][4][4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[m][n][e] = 0.f;
-#pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
@@ -338,8 +377,13 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
           ldsm4(r, lb.at(tk, hb * 2 + q, k));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            mma(x[m][2 * q], fq[m][k], r[0], r[1]);
-            mma(x[m][2 * q + 1], fq[m][k], r[2], r[3]);
+            if (k == 0) {
+              mma0(x[m][2 * q], fq[m][k], r[0], r[1]);
+              mma0(x[m][2 * q + 1], fq[m][k], r[2], r[3]);
+            } else {
+              mma(x[m][2 * q], fq[m][k], r[0], r[1]);
+              mma(x[m][2 * q + 1], fq[m][k], r[2], r[3]);
+            }
           }
         }
       const uint32_t hbits = (uint32_t)(bits >> (32 * hb));
@@ -350,8 +394,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[m][2 * q + n][e] = score<BT>(x[m][2 * q + n][e], a.scale, ring[q][m][e >> 1], 2 * n + (e & 1));
+            for (int r = 0; r < 2; ++r) score2<BT>(&x[m][2 * q + n][2 * r], scale, ring[q][m][r], n);
         fetch_bias(q, j0 + hb * 32 + q * 16 + 32);
       }
       if (hbits != 0xffffffffu) {
@@ -375,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
         for (int r = 0; r < 2; ++r) {
           float v = mx[m][r];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) v = fmaxf(v, fmaxf(x[m][n][2 * r], x[m][n][2 * r + 1]));
+          for (int n = 0; n < 4; ++n) v = max3(v, x[m][n][2 * r], x[m][n][2 * r + 1]);
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
           nm[m][r] = v;
@@ -400,16 +443,17 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float base = mx[m][r] == -INFINITY ? 0.f : mx[m][r];  // nothing seen yet: every p is 0
-          float s = 0.f;
+          const F2 nm(mx[m][r] == -INFINITY ? 0.f : -mx[m][r]);  // nothing seen yet: every p is 0
+          F2 s2;
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float p = ex2((x[m][n][2 * r + e] - base) * kLog2e);
-              x[m][n][2 * r + e] = p;
-              s += p;
-            }
+          for (int n = 0; n < 4; ++n) {
+            const F2 p = prob2(&x[m][n][2 * r], nm, F2(0.f));
+            p.get(x[m][n][2 * r], x[m][n][2 * r + 1]);
+            s2 = n == 0 ? p : add2(s2, p);
+          }
+          float s, s1;
+          s2.get(s, s1);
+          s += s1;
           sum[m][r] += s;
         }
 #pragma unroll
@@ -419,15 +463,14 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
         for (int c = 0; c < NB / 2; ++c) ldsm4_t(f[c], lt.at(tv, hb * 2 + q, c));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          // p as the sum of bf16 values (see the head of pf_attention.cuh)
-          for (int term = 0; term < a.p_terms; ++term) {
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
             uint32_t pa[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float* v = &x[m][2 * q + (i >> 1)][2 * (i & 1)];
               pa[i] = pack_bf16(v[0], v[1]);
-              v[0] -= lo_f(pa[i]);
-              v[1] -= hi_f(pa[i]);
+              if (term + 1 < TERMS) add2(F2(v[0], v[1]), F2(-lo_f(pa[i]), -hi_f(pa[i]))).get(v[0], v[1]);
             }
 #pragma unroll
             for (int c = 0; c < NB / 2; ++c) {
@@ -543,7 +586,9 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
   };
   const char* brow[MT][2];
   char* drow[MT][2];
-  float4 rc[MT][2];
+  F2 nmx[MT][2], lg[MT][2], nd[MT][2];
+  const F2 scale(a.scale);
+  bool peaked = false;
   const int bsz = BT == 2 ? 4 : 2;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -554,11 +599,10 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
       drow[m][r] = (BT && a.dbias && i < a.nq)
                        ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs) * bsz
                        : nullptr;
-      rc[m][r] = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
+      const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
+      nmx[m][r] = F2(-c.x), lg[m][r] = F2(c.y), nd[m][r] = F2(c.w);
+      peaked |= c.z != 0.f;
     }
-  bool peaked = false;
-#pragma unroll
-  for (int m = 0; m < MT; ++m) peaked |= rc[m][0].z != 0.f || rc[m][1].z != 0.f;
   peaked = __any_sync(0xffffffffu, peaked);
   Bias4<BT> ring[2][MT][2];
   auto fetch_bias = [&](int slot, int64_t j0) {
@@ -606,15 +650,9 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
       bits = next;
       continue;
     }
-#pragma unroll
+#pragma unroll 2
     for (int q = 0; q < 4; ++q) {  // 16 keys
       float x[MT][2][4], y[MT][2][4];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[m][n][e] = y[m][n][e] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t r[4], u[4];
@@ -622,10 +660,17 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
         ldsm4(u, lb.at(tv, q, k));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          mma(x[m][0], fq[m][k], r[0], r[1]);
-          mma(x[m][1], fq[m][k], r[2], r[3]);
-          mma(y[m][0], fg[m][k], u[0], u[1]);
-          mma(y[m][1], fg[m][k], u[2], u[3]);
+          if (k == 0) {
+            mma0(x[m][0], fq[m][k], r[0], r[1]);
+            mma0(x[m][1], fq[m][k], r[2], r[3]);
+            mma0(y[m][0], fg[m][k], u[0], u[1]);
+            mma0(y[m][1], fg[m][k], u[2], u[3]);
+          } else {
+            mma(x[m][0], fq[m][k], r[0], r[1]);
+            mma(x[m][1], fq[m][k], r[2], r[3]);
+            mma(y[m][0], fg[m][k], u[0], u[1]);
+            mma(y[m][1], fg[m][k], u[2], u[3]);
+          }
         }
       }
       const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
@@ -634,8 +679,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[m][n][e] = score<BT>(x[m][n][e], a.scale, ring[q & 1][m][e >> 1], 2 * n + (e & 1));
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[q & 1][m][r], n);
       fetch_bias(q & 1, j0 + q * 16 + 32);
       if (qbits != 0xffffu) {
         const uint32_t mine = qbits >> (4 * t);
@@ -652,11 +696,10 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 c = rc[m][e >> 1];
-            const float p = ex2(fmaf(x[m][n][e] - c.x, kLog2e, c.y));
-            x[m][n][e] = p;
-            y[m][n][e] = p * (y[m][n][e] + c.w);
+          for (int r = 0; r < 2; ++r) {
+            const F2 p = prob2(&x[m][n][2 * r], nmx[m][r], lg[m][r]);
+            p.get(x[m][n][2 * r], x[m][n][2 * r + 1]);
+            mul2(p, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[m][r])).get(y[m][n][2 * r], y[m][n][2 * r + 1]);
           }
       if (peaked) {
 #pragma unroll
@@ -766,6 +809,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
     stage ^= 1;
     if (++lt == per) lt = 0, ++lh;
   };
+  const F2 scale(a.scale);
   float dk[KM][NB][4], dv[KM][NB][4];
 #pragma unroll
   for (int m = 0; m < KM; ++m)
@@ -816,15 +860,9 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
         if (lh < group) issue();
         const uint32_t tq = sq + s * kTile * S::RB, tg = sg + s * kTile * S::RB;
         const int64_t i0 = (int64_t)qt * kTile;
-#pragma unroll
+#pragma unroll 2
         for (int blk = 0; blk < 4; ++blk) {  // 16 queries
           float x[KM][2][4], y[KM][2][4];
-#pragma unroll
-          for (int m = 0; m < KM; ++m)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[m][n][e] = y[m][n][e] = 0.f;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             uint32_t fq[4], fg[4];
@@ -840,20 +878,28 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
                 ldsm4(rk, lb.at(sk, warp * KM + m, k));
                 ldsm4(rv, lb.at(sv, warp * KM + m, k));
               }
-              mma(x[m][0], fq, rk[0], rk[1]);
-              mma(x[m][1], fq, rk[2], rk[3]);
-              mma(y[m][0], fg, rv[0], rv[1]);
-              mma(y[m][1], fg, rv[2], rv[3]);
+              if (k == 0) {
+                mma0(x[m][0], fq, rk[0], rk[1]);
+                mma0(x[m][1], fq, rk[2], rk[3]);
+                mma0(y[m][0], fg, rv[0], rv[1]);
+                mma0(y[m][1], fg, rv[2], rv[3]);
+              } else {
+                mma(x[m][0], fq, rk[0], rk[1]);
+                mma(x[m][1], fq, rk[2], rk[3]);
+                mma(y[m][0], fg, rv[0], rv[1]);
+                mma(y[m][1], fg, rv[2], rv[3]);
+              }
             }
           }
           const float4 c[2] = {cst[s * kTile + blk * 16 + g], cst[s * kTile + blk * 16 + 8 + g]};
+          const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)},
+                   nd[2] = {F2(c[0].w), F2(c[1].w)};
 #pragma unroll
           for (int m = 0; m < KM; ++m)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[m][n][e] = score<BT>(x[m][n][e], a.scale, ring[blk & 1][m][e >> 1], 2 * n + (e & 1));
+              for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[blk & 1][m][r], n);
           fetch_bias(blk & 1, i0 + blk * 16 + 32);
           if (!full) {
 #pragma unroll
@@ -873,11 +919,12 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 float p[2], ds[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  p[e] = ex2(fmaf(x[m][n][2 * r + e] - c[r].x, kLog2e, c[r].y));
-                  ds[e] = p[e] * (y[m][n][2 * r + e] + c[r].w);
-                  if (peaked && p[e] == 1.f) ds[e] = 0.f;
+                const F2 p2 = prob2(&x[m][n][2 * r], nmx[r], lg[r]);
+                p2.get(p[0], p[1]);
+                mul2(p2, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
+                if (peaked) {
+                  if (p[0] == 1.f) ds[0] = 0.f;
+                  if (p[1] == 1.f) ds[1] = 0.f;
                 }
                 pa[m][2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
                 da[m][2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
@@ -963,6 +1010,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
       brow[m][r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1);
     }
   const bool fast = a.bias_vec && j0 + kTile <= a.nk;
+  const F2 scale(a.scale);
   float acc[MT][8][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -996,14 +1044,16 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
           ldsm4(fg[m][k], la.at(tg, warp * MT + m, k));
         }
     }
-    float4 rc[MT][2];
+    F2 nmx[MT][2], lg[MT][2], nd[MT][2];
+    bool peaked = false;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) rc[m][r] = cst[warp * 16 * MT + m * 16 + r * 8 + g];
-    bool peaked = false;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) peaked |= rc[m][0].z != 0.f || rc[m][1].z != 0.f;
+      for (int r = 0; r < 2; ++r) {
+        const float4 c = cst[warp * 16 * MT + m * 16 + r * 8 + g];
+        nmx[m][r] = F2(-c.x), lg[m][r] = F2(c.y), nd[m][r] = F2(c.w);
+        peaked |= c.z != 0.f;
+      }
     peaked = __any_sync(0xffffffffu, peaked);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -1013,12 +1063,6 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
 #pragma unroll
         for (int r = 0; r < 2; ++r) bias_load<BT>(br[m][r], brow[m][r], j0 + q * 16 + 4 * t, a.nk, fast);
       float x[MT][2][4], y[MT][2][4];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[m][n][e] = y[m][n][e] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t r[4], u[4];
@@ -1034,10 +1078,17 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
             ldsm4(rq, la.at(tq, warp * MT + m, k));
             ldsm4(rg, la.at(tg, warp * MT + m, k));
           }
-          mma(x[m][0], rq, r[0], r[1]);
-          mma(x[m][1], rq, r[2], r[3]);
-          mma(y[m][0], rg, u[0], u[1]);
-          mma(y[m][1], rg, u[2], u[3]);
+          if (k == 0) {
+            mma0(x[m][0], rq, r[0], r[1]);
+            mma0(x[m][1], rq, r[2], r[3]);
+            mma0(y[m][0], rg, u[0], u[1]);
+            mma0(y[m][1], rg, u[2], u[3]);
+          } else {
+            mma(x[m][0], rq, r[0], r[1]);
+            mma(x[m][1], rq, r[2], r[3]);
+            mma(y[m][0], rg, u[0], u[1]);
+            mma(y[m][1], rg, u[2], u[3]);
+          }
         }
       }
       const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
@@ -1046,13 +1097,23 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = score<BT>(x[m][n][e], a.scale, br[m][e >> 1], 2 * n + (e & 1));
-            if (qbits != 0xffffu && !((qbits >> (4 * t + 2 * n + (e & 1))) & 1)) v = -INFINITY;
-            const float4 c = rc[m][e >> 1];
-            const float pr = ex2(fmaf(v - c.x, kLog2e, c.y));
-            const float dl = (peaked && pr == 1.f) ? 0.f : y[m][n][e] + c.w;
-            acc[m][2 * q + n][e] = fmaf(pr, dl, acc[m][2 * q + n][e]);
+          for (int r = 0; r < 2; ++r) {
+            float* v = &x[m][n][2 * r];
+            float* d = &acc[m][2 * q + n][2 * r];
+            score2<BT>(v, scale, br[m][r], n);
+            if (qbits != 0xffffu) {
+              if (!((qbits >> (4 * t + 2 * n)) & 1)) v[0] = -INFINITY;
+              if (!((qbits >> (4 * t + 2 * n + 1)) & 1)) v[1] = -INFINITY;
+            }
+            const F2 p = prob2(v, nmx[m][r], lg[m][r]);
+            F2 dl = add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[m][r]);
+            if (peaked) {
+              float p0, p1, d0, d1;
+              p.get(p0, p1);
+              dl.get(d0, d1);
+              dl = F2(p0 == 1.f ? 0.f : d0, p1 == 1.f ? 0.f : d1);
+            }
+            fma2(p, dl, F2(d[0], d[1])).get(d[0], d[1]);
           }
     }
     bits = next;
