@@ -517,20 +517,27 @@ typedef struct {
   int64_t batch_stride, head_stride, row_stride;
 } pf_bias_view;
 
-/* mask(b, j) != 0: key j of batch entry b is visible (mask.ptr NULL: all are).
+/* The operands of one call. mask(b, j) != 0: key j of batch entry b is visible (mask.ptr NULL: all are).
  * stats (fp32 [2][batch][heads][n_q]: the rows' maximum and sum) and, in bf16, o_lo (16 bits per
- * element, [batch][n_q][heads][head_dim] contiguous: what the rounding of o dropped) are kept for the
- * backward; both may be NULL where none follows. */
-PF_API int pf_attention_fwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
-                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, float* stats, void* o_lo,
-                     void* stream);
+ * element, [batch][n_q][heads][head_dim] contiguous: what the rounding of o dropped) are written by the
+ * forward for the backward; both may be NULL where none follows. The fields from d_o on are the
+ * backward's: dq.ptr, dbias.ptr, and dk.ptr together with dv.ptr, may be NULL (not computed). Outputs
+ * are overwritten and may not overlap an input. */
+typedef struct {
+  pf_attention_shape shape;
+  pf_head_view q, k, v;
+  pf_bias_view bias;
+  pf_mask_view mask;
+  pf_head_view o;
+  float* stats;
+  void* o_lo;
+  pf_head_view d_o, dq, dk, dv;
+  pf_bias_view dbias;
+} pf_attention_call;
+
+PF_API int pf_attention_fwd(const pf_attention_call* call, void* stream);
 PF_API int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* bytes);
-/* dq.ptr, dbias.ptr, and dk.ptr together with dv.ptr, may be NULL (not computed). Gradients are
- * overwritten; none may overlap an input. */
-PF_API int pf_attention_bwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
-                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, const float* stats, const void* o_lo,
-                     pf_head_view d_o, pf_head_view dq, pf_head_view dk, pf_head_view dv, pf_bias_view dbias,
-                     void* workspace, size_t workspace_bytes, void* stream);
+PF_API int pf_attention_bwd(const pf_attention_call* call, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Relative-position bias -----------------------------------------------------------------
  * The relative-position features of pf_trunk_init_fwd (RelativePositionEncoding,

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -152,6 +153,19 @@ class BiasView(Structure):
     _fields_ = [("ptr", c_void_p), ("batch_stride", c_int64), ("head_stride", c_int64), ("row_stride", c_int64)]
 
 
+class AttentionCall(Structure):
+    _fields_ = [("shape", AttentionShape), ("q", HeadView), ("k", HeadView), ("v", HeadView), ("bias", BiasView),
+                ("mask", MaskView), ("o", HeadView), ("stats", c_void_p), ("o_lo", c_void_p), ("d_o", HeadView),
+                ("dq", HeadView), ("dk", HeadView), ("dv", HeadView), ("dbias", BiasView)]
+
+
+# The same bytes from plain numbers (shape; q, k, v; bias; mask; o; stats, o_lo; d_o, dq, dk, dv; dbias): filling the
+# nested structures one by one would cost more than a small launch.
+ATTENTION_SHAPE = struct.Struct("@3q3if2i")
+ATTENTION_CALL = struct.Struct("@3q3if2i" + "P3q" * 3 + "P3q" + "P2q" + "P3q" + "2P" + "P3q" * 4 + "P3q")
+assert ATTENTION_SHAPE.size == ctypes.sizeof(AttentionShape) and ATTENTION_CALL.size == ctypes.sizeof(AttentionCall)
+
+
 _lib = None
 
 
@@ -245,12 +259,10 @@ def load(path: str = LIB_PATH):
         "pf_layernorm_bwd_workspace_size": ([c_int64, c_int32, c_int32, sz], c_int),
         "pf_layernorm_bwd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float,
                               c_int32, c_void_p, c_size_t, c_void_p], c_int),
-        "pf_attention_fwd": ([POINTER(AttentionShape), HeadView, HeadView, HeadView, BiasView, MaskView, HeadView,
-                              c_void_p, c_void_p, c_void_p], c_int),
-        "pf_attention_bwd_workspace_size": ([POINTER(AttentionShape), sz], c_int),
-        "pf_attention_bwd": ([POINTER(AttentionShape), HeadView, HeadView, HeadView, BiasView, MaskView, HeadView,
-                              c_void_p, c_void_p, HeadView, HeadView, HeadView, HeadView, BiasView, c_void_p,
-                              c_size_t, c_void_p], c_int),
+        # the call and the shape as packed bytes (ATTENTION_CALL, ATTENTION_SHAPE) or structures
+        "pf_attention_fwd": ([c_void_p, c_void_p], c_int),
+        "pf_attention_bwd_workspace_size": ([c_void_p, sz], c_int),
+        "pf_attention_bwd": ([c_void_p, c_void_p, c_size_t, c_void_p], c_int),
         "pf_relpos_bias_fwd": ([c_void_p, c_int32, TokenIds, c_void_p, c_int64, c_int64, c_int32, c_int64, c_int64,
                                 c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p], c_int),
         "pf_relpos_bias_bwd_workspace_size": ([c_int64, c_int64, c_int32, c_int32, c_int32, sz], c_int),

@@ -833,20 +833,28 @@ static bool heads_out_ok(const pf_head_view& v, int64_t batch, int64_t n, int he
          (heads == 1 || v.head_stride >= d);
 }
 
-int pf_attention_fwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
-                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, float* stats, void* o_lo, void* stream) {
-  PF_TRY(check_attention(shape));
-  const pf_attention_shape& s = *shape;
+// what both directions read beside q
+static int check_keys(const pf_attention_call& c) {
+  const pf_attention_shape& s = c.shape;
+  if (s.batch > 0 && s.n_k > 0 && (!heads_ok(c.k, s.dtype) || !heads_ok(c.v, s.dtype)))
+    return fail(PF_EINVAL_ARG, "attention: bad view of k or v");
+  if (c.bias.ptr && !bias_ok(c.bias, s.bias_dtype)) return fail(PF_EINVAL_ARG, "attention: bad bias view");
+  if (c.mask.ptr && (c.mask.row_stride < 0 || c.mask.col_stride < 0))
+    return fail(PF_EINVAL_ARG, "attention: bad mask view");
+  return PF_OK;
+}
+
+int pf_attention_fwd(const pf_attention_call* call, void* stream) {
+  if (!call) return fail(PF_EINVAL_ARG, "attention: null call");
+  const pf_attention_call& c = *call;
+  const pf_attention_shape& s = c.shape;
+  PF_TRY(check_attention(&s));
   set_path("attention");
   if (s.batch == 0 || s.n_q == 0) return PF_OK;
-  if (!heads_ok(q, s.dtype) || !heads_out_ok(o, s.batch, s.n_q, s.heads, s.head_dim, s.dtype))
+  if (!heads_ok(c.q, s.dtype) || !heads_out_ok(c.o, s.batch, s.n_q, s.heads, s.head_dim, s.dtype))
     return fail(PF_EINVAL_ARG, "attention: bad view of q or o");
-  if (s.n_k > 0 && (!heads_ok(k, s.dtype) || !heads_ok(v, s.dtype)))
-    return fail(PF_EINVAL_ARG, "attention: bad view of k or v");
-  if (bias.ptr && !bias_ok(bias, s.bias_dtype)) return fail(PF_EINVAL_ARG, "attention: bad bias view");
-  if (mask.ptr && (mask.row_stride < 0 || mask.col_stride < 0))
-    return fail(PF_EINVAL_ARG, "attention: bad mask view");
-  return train::attention_fwd(s, q, k, v, bias, mask, o, stats, (int16_t*)o_lo, (cudaStream_t)stream);
+  PF_TRY(check_keys(c));
+  return train::attention_fwd(c, (cudaStream_t)stream);
 }
 
 int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* bytes) {
@@ -856,44 +864,37 @@ int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* byt
   return PF_OK;
 }
 
-int pf_attention_bwd(const pf_attention_shape* shape, pf_head_view q, pf_head_view k, pf_head_view v,
-                     pf_bias_view bias, pf_mask_view mask, pf_head_view o, const float* stats, const void* o_lo,
-                     pf_head_view d_o, pf_head_view dq, pf_head_view dk, pf_head_view dv, pf_bias_view dbias,
-                     void* workspace, size_t workspace_bytes, void* stream) {
+int pf_attention_bwd(const pf_attention_call* call, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!call) return fail(PF_EINVAL_ARG, "attention backward: null call");
+  const pf_attention_call& c = *call;
+  const pf_attention_shape& s = c.shape;
   size_t need;
-  PF_TRY(pf_attention_bwd_workspace_size(shape, &need));
-  const pf_attention_shape& s = *shape;
+  PF_TRY(pf_attention_bwd_workspace_size(&s, &need));
   set_path("attention");
-  if ((dk.ptr == nullptr) != (dv.ptr == nullptr))
+  if ((c.dk.ptr == nullptr) != (c.dv.ptr == nullptr))
     return fail(PF_EINVAL_ARG, "attention backward: dk and dv are computed together");
-  if (dbias.ptr && !bias.ptr) return fail(PF_EINVAL_ARG, "attention backward: dbias without a bias");
+  if (c.dbias.ptr && !c.bias.ptr) return fail(PF_EINVAL_ARG, "attention backward: dbias without a bias");
   const bool rows = s.batch > 0 && s.n_q > 0, keys = s.batch > 0 && s.n_k > 0;
-  if (rows && (!heads_ok(q, s.dtype) || !heads_ok(o, s.dtype) || !heads_ok(d_o, s.dtype) || !stats))
+  if (rows && (!heads_ok(c.q, s.dtype) || !heads_ok(c.o, s.dtype) || !heads_ok(c.d_o, s.dtype) || !c.stats))
     return fail(PF_EINVAL_ARG, "attention backward: bad view of q, o or do, or no row statistics");
-  if (rows && s.dtype == PF_BF16 && !o_lo)
+  if (rows && s.dtype == PF_BF16 && !c.o_lo)
     return fail(PF_EINVAL_ARG, "attention backward: bf16 needs the o_lo of the forward pass");
-  if (keys && (!heads_ok(k, s.dtype) || !heads_ok(v, s.dtype)))
-    return fail(PF_EINVAL_ARG, "attention backward: bad view of k or v");
-  if (bias.ptr && !bias_ok(bias, s.bias_dtype)) return fail(PF_EINVAL_ARG, "attention backward: bad bias view");
-  if (mask.ptr && (mask.row_stride < 0 || mask.col_stride < 0))
-    return fail(PF_EINVAL_ARG, "attention backward: bad mask view");
-  if ((dq.ptr && rows && !heads_out_ok(dq, s.batch, s.n_q, s.heads, s.head_dim, s.dtype)) ||
-      (dk.ptr && keys && (!heads_out_ok(dk, s.batch, s.n_k, s.kv_heads, s.head_dim, s.dtype) ||
-                          !heads_out_ok(dv, s.batch, s.n_k, s.kv_heads, s.head_dim, s.dtype))))
+  PF_TRY(check_keys(c));
+  if ((c.dq.ptr && rows && !heads_out_ok(c.dq, s.batch, s.n_q, s.heads, s.head_dim, s.dtype)) ||
+      (c.dk.ptr && keys && (!heads_out_ok(c.dk, s.batch, s.n_k, s.kv_heads, s.head_dim, s.dtype) ||
+                            !heads_out_ok(c.dv, s.batch, s.n_k, s.kv_heads, s.head_dim, s.dtype))))
     return fail(PF_EINVAL_ARG, "attention backward: bad view of a gradient");
-  if (dbias.ptr) {
-    if (!bias_ok(dbias, s.bias_dtype) || (s.n_q > 1 && dbias.row_stride < s.n_k) ||
-        (s.heads > 1 && dbias.head_stride < s.n_k))
+  if (c.dbias.ptr) {
+    if (!bias_ok(c.dbias, s.bias_dtype) || (s.n_q > 1 && c.dbias.row_stride < s.n_k) ||
+        (s.heads > 1 && c.dbias.head_stride < s.n_k))
       return fail(PF_EINVAL_ARG, "attention backward: bad dbias view");
-    if (s.batch > 1 && (bias.batch_stride == 0) != (dbias.batch_stride == 0))
+    if (s.batch > 1 && (c.bias.batch_stride == 0) != (c.dbias.batch_stride == 0))
       return fail(PF_EINVAL_ARG, "attention backward: dbias is shared by the batch exactly where the bias is");
+    if (s.batch == 0) return fail(PF_EINVAL_SHAPE, "attention backward: dbias of an empty batch");
   }
-  if (dbias.ptr && s.batch == 0)
-    return fail(PF_EINVAL_SHAPE, "attention backward: dbias of an empty batch");
   if (!rows && !keys) return PF_OK;
   PF_TRY(check_ws(workspace, workspace_bytes, need, "attention backward"));
-  return train::attention_bwd(s, q, k, v, bias, mask, o, stats, (const int16_t*)o_lo, d_o, dq, dk, dv, dbias,
-                              workspace, workspace_bytes, (cudaStream_t)stream);
+  return train::attention_bwd(c, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 // ------------------------------------------------------------------ relative-position bias

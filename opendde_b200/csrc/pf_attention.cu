@@ -12,6 +12,46 @@ int launch(int dtype, attn::Kind kind, const Args& a, double flops, cudaStream_t
   return dtype == PF_BF16 ? attn::launch_bf16(kind, a, flops, st) : attn::launch_f32(kind, a, flops, st);
 }
 
+template <int BT>
+__global__ void __launch_bounds__(256) k_sum_planes(Args a, const float* __restrict__ part, int parts) {
+  const int64_t n = (int64_t)a.H * a.nq * a.nk;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p) s += part[p * n + i];
+    const int64_t j = i % a.nk, hi = i / a.nk, h = hi / a.nq, q = hi - h * a.nq;
+    const int64_t off = h * a.db_hs + q * a.db_rs + j;
+    if (BT == 2)
+      ((float*)a.dbias)[off] = s;
+    else
+      ((__nv_bfloat16*)a.dbias)[off] = __float2bfloat16_rn(s);
+  }
+}
+
+int sum_planes(const Args& a, const float* part, int parts, cudaStream_t st) {
+  const int64_t n = (int64_t)a.H * a.nq * a.nk, want = (n + 255) / 256;
+  const unsigned blocks = (unsigned)(want < 148 * 8 ? want : 148 * 8);
+  {
+    PF_LAUNCH_SCOPE_WORK(st, "k_attn_sum_planes", 4.0 * n * (parts + 1), 'b');
+    if (a.bias_f32)
+      k_sum_planes<2><<<blocks, 256, 0, st>>>(a, part, parts);
+    else
+      k_sum_planes<1><<<blocks, 256, 0, st>>>(a, part, parts);
+  }
+  PF_CHECK_LAUNCH();
+  return PF_OK;
+}
+
+// Parts of the batch for the gradient of a shared bias: about three blocks per SM, and at least four
+// entries each (a part costs a plane written and read).
+int dbias_parts(const pf_attention_shape& s) {
+  const int64_t rows = s.dtype == PF_BF16 ? 128 : 64, keys = s.dtype == PF_BF16 ? 64 : 32;
+  const int64_t blocks = ((s.n_q + rows - 1) / rows) * ((s.n_k + keys - 1) / keys) * s.heads;
+  if (blocks == 0) return 1;
+  int64_t p = (3 * 148 + blocks - 1) / blocks;
+  if (p > s.batch / 4) p = s.batch / 4;
+  return p < 1 ? 1 : (int)p;
+}
+
 Heads heads(const pf_head_view& v) { return Heads{v.ptr, v.batch_stride, v.seq_stride, v.head_stride}; }
 
 // 16-byte accesses: the base, every stride and the channels are whole 16-byte units
@@ -27,8 +67,11 @@ int whole_quads(const pf_bias_view& v, int dtype) {
          v.row_stride % 4 == 0;
 }
 
-Args make_args(const pf_attention_shape& s, pf_head_view q, pf_head_view k, pf_head_view v, pf_bias_view bias,
-               pf_mask_view mask) {
+Args make_args(const pf_attention_call& c) {
+  const pf_attention_shape& s = c.shape;
+  const pf_head_view &q = c.q, &k = c.k, &v = c.v;
+  const pf_bias_view& bias = c.bias;
+  const pf_mask_view& mask = c.mask;
   Args a{};
   a.q = heads(q);
   a.k = heads(k);
@@ -58,18 +101,16 @@ Args make_args(const pf_attention_shape& s, pf_head_view q, pf_head_view k, pf_h
 
 }  // namespace
 
-int attention_fwd(const pf_attention_shape& s, pf_head_view q, pf_head_view k, pf_head_view v, pf_bias_view bias,
-                  pf_mask_view mask, pf_head_view o, float* stats, int16_t* o_lo, cudaStream_t st) {
-  Args a = make_args(s, q, k, v, bias, mask);
-  a.o = o.ptr;
-  a.o_bs = o.batch_stride;
-  a.o_ns = o.seq_stride;
-  a.o_hs = o.head_stride;
-  a.stats = stats;
-  a.o_lo = o_lo;
-  a.p_terms = bias.ptr && s.bias_dtype == PF_F32 ? 3 : 2;
-  const double pair = 2.0 * s.batch * s.heads * s.n_q * s.n_k * s.head_dim;
-  return launch(s.dtype, attn::kFwd, a, 2 * pair, st);
+int attention_fwd(const pf_attention_call& c, cudaStream_t st) {
+  const pf_attention_shape& s = c.shape;
+  Args a = make_args(c);
+  a.o = c.o.ptr;
+  a.o_bs = c.o.batch_stride;
+  a.o_ns = c.o.seq_stride;
+  a.o_hs = c.o.head_stride;
+  a.stats = c.stats;
+  a.o_lo = (int16_t*)c.o_lo;
+  return launch(s.dtype, attn::kFwd, a, 4.0 * s.batch * s.heads * s.n_q * s.n_k * s.head_dim, st);
 }
 
 // The row constants (16 bytes per row), then the partial planes of a shared bias's gradient. Sized as if
@@ -77,27 +118,27 @@ int attention_fwd(const pf_attention_shape& s, pf_head_view q, pf_head_view k, p
 size_t attention_bwd_ws_bytes(const pf_attention_shape& s) {
   Arena ar(nullptr, 0);
   ar.take<float>((size_t)4 * s.batch * s.heads * s.n_q);
-  if (s.dtype == PF_BF16 && s.batch > 1) {
-    const int parts = attn::dbias_parts_bf16(s.batch, s.n_q, s.n_k, s.heads);
+  if (s.batch > 1) {
+    const int parts = dbias_parts(s);
     if (parts > 1) ar.take<float>((size_t)parts * s.heads * s.n_q * s.n_k);
   }
   return ar.used;
 }
 
-int attention_bwd(const pf_attention_shape& s, pf_head_view q, pf_head_view k, pf_head_view v, pf_bias_view bias,
-                  pf_mask_view mask, pf_head_view o, const float* stats, const int16_t* o_lo, pf_head_view d_o,
-                  pf_head_view dq, pf_head_view dk, pf_head_view dv, pf_bias_view dbias, void* ws,
-                  size_t ws_bytes, cudaStream_t st) {
-  Args a = make_args(s, q, k, v, bias, mask);
-  a.g = heads(d_o);
-  a.vec_g = whole16(d_o, s);
+int attention_bwd(const pf_attention_call& c, void* ws, size_t ws_bytes, cudaStream_t st) {
+  const pf_attention_shape& s = c.shape;
+  const pf_head_view &dq = c.dq, &dk = c.dk, &dv = c.dv;
+  const pf_bias_view& dbias = c.dbias;
+  Args a = make_args(c);
+  a.g = heads(c.d_o);
+  a.vec_g = whole16(c.d_o, s);
   Arena ar(ws, ws_bytes);
   float* rows = ar.take<float>((size_t)4 * a.rows_plane);
   a.rows = rows;
   const double pair = 2.0 * s.batch * s.heads * s.n_q * s.n_k * s.head_dim;
   if (a.rows_plane > 0)
-    PF_TRY(s.dtype == PF_BF16 ? attn::rows_bf16(a, stats, heads(o), o_lo, rows, st)
-                              : attn::rows_f32(a, stats, heads(o), rows, st));
+    PF_TRY(s.dtype == PF_BF16 ? attn::rows_bf16(a, c.stats, heads(c.o), (const int16_t*)c.o_lo, rows, st)
+                              : attn::rows_f32(a, c.stats, heads(c.o), rows, st));
   const bool shared = dbias.ptr && s.batch > 1 && dbias.batch_stride == 0;
   if (dbias.ptr) {
     a.db_bs = dbias.batch_stride;
@@ -126,11 +167,12 @@ int attention_bwd(const pf_attention_shape& s, pf_head_view q, pf_head_view k, p
   }
   if (shared && s.n_q > 0 && s.n_k > 0) {
     a.dbias = dbias.ptr;
-    if (s.dtype == PF_F32) return attn::dbias_f32(a, 2 * pair, st);
-    const int parts = attn::dbias_parts_bf16(s.batch, s.n_q, s.n_k, s.heads);
+    const int parts = dbias_parts(s);
     float* part = parts > 1 ? ar.take<float>((size_t)parts * s.heads * s.n_q * s.n_k) : nullptr;
     if (!ar.ok()) return fail(PF_EWORKSPACE, "attention backward: workspace too small");
-    return attn::dbias_bf16(a, part, parts, 2 * pair, st);
+    PF_TRY(s.dtype == PF_BF16 ? attn::dbias_bf16(a, part, parts, 2 * pair, st)
+                              : attn::dbias_f32(a, part, parts, 2 * pair, st));
+    if (parts > 1) return sum_planes(a, part, parts, st);
   }
   return PF_OK;
 }

@@ -64,7 +64,6 @@ struct Args {
   int H, KV, d;
   float scale;
   int vec_q, vec_k, vec_v, vec_g;  // 16-byte accesses allowed
-  int p_terms;                     // forward, bf16: bf16 values that p is split into
   int64_t tiles;                   // tiles along the split axis of this launch
 };
 
@@ -92,9 +91,8 @@ enum Kind { kFwd, kDq, kDkv };
 // planes [parts][H][n_q][n_k] in `part` where parts > 1; rows_*: the row constants, 16 bytes per row.
 int launch_bf16(Kind kind, const Args& a, double flops, cudaStream_t st);
 int launch_f32(Kind kind, const Args& a, double flops, cudaStream_t st);
-int dbias_parts_bf16(int64_t B, int64_t nq, int64_t nk, int H);
 int dbias_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st);
-int dbias_f32(const Args& a, double flops, cudaStream_t st);
+int dbias_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st);
 int rows_bf16(const Args& a, const float* stats, Heads o, const int16_t* lo, float* rows, cudaStream_t st);
 int rows_f32(const Args& a, const float* stats, Heads o, float* rows, cudaStream_t st);
 

@@ -18,6 +18,7 @@
 // registers by movmatrix.
 
 #include "pf_attention.cuh"
+#include "pf_f32x2.cuh"
 
 namespace pf {
 namespace train {
@@ -95,31 +96,6 @@ __device__ __forceinline__ void mma0(float* c, const uint32_t* a, uint32_t b0, u
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-// Two fp32 values side by side: one instruction for both (half the issue slots of scalar arithmetic).
-struct F2 {
-  unsigned long long v;
-  __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ explicit F2(float a) : F2(a, a) {}
-  __device__ __forceinline__ void get(float& a, float& b) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  }
-};
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -359,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
     if (kt + 1 < nt) issue(kt + 1, next);
     rawm = seen_raw(a, b, (int64_t)(kt + 2) * kTile);
     const int64_t j0 = (int64_t)kt * kTile;
-    if (bits == 0) {  // no visible key: the same for the whole block
+    if (bits == 0 || w0 >= a.nq) {  // no visible key, or a warp past the end
       fetch_bias(0, j0 + 64);
       fetch_bias(1, j0 + 80);
       bits = next;
@@ -644,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
     rawm = seen_raw(a, b, (int64_t)(kt + 2) * kTile);
     const int64_t j0 = (int64_t)kt * kTile;
     const uint32_t tk = sk + (kt & 1) * kTile * S::RB, tv = sv + (kt & 1) * kTile * S::RB;
-    if (bits == 0 && !(BT && a.dbias)) {
+    if (w0 >= a.nq || (bits == 0 && !(BT && a.dbias))) {
       fetch_bias(0, j0 + 64);
       fetch_bias(1, j0 + 80);
       bits = next;
@@ -837,8 +813,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
 #pragma unroll
             for (int m = 0; m < KM; ++m)
 #pragma unroll
-              for (int w = 0; w < (BT == 2 ? 4 : 2); ++w)
-                if (BT) ring[slot][m][r].w[w] = 0;
+              for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][m][r].w[w] = 0;
           }
         }
       };
@@ -850,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
         __syncthreads();
         if (HOLD && hh == 0 && qt == 0) {
 #pragma unroll
-          for (int m = 0; m < (HOLD ? KM : 0); ++m)
+          for (int m = 0; m < (HOLD ? KM : 1); ++m)
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
               ldsm4(fk[m][k], lb.at(sk, warp * KM + m, k));
@@ -858,6 +833,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
             }
         }
         if (lh < group) issue();
+        if (mine == 0) continue;  // none of the warp's keys is visible
         const uint32_t tq = sq + s * kTile * S::RB, tg = sg + s * kTile * S::RB;
         const int64_t i0 = (int64_t)qt * kTile;
 #pragma unroll 2
@@ -1027,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
     __syncthreads();
     if (b + 1 < b1) issue(b + 1, next);
     rawm = b + 2 < b1 ? seen_raw(a, b + 2, j0) : make_float2(0.f, 0.f);
-    if (bits == 0) {
+    if (bits == 0 || w0 >= a.nq) {
       bits = next;
       continue;
     }
@@ -1037,7 +1013,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
     uint32_t fq[HOLD ? MT : 1][HOLD ? KS : 1][4], fg[HOLD ? MT : 1][HOLD ? KS : 1][4];
     if (HOLD) {
 #pragma unroll
-      for (int m = 0; m < (HOLD ? MT : 0); ++m)
+      for (int m = 0; m < (HOLD ? MT : 1); ++m)
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           ldsm4(fq[m][k], la.at(tq, warp * MT + m, k));
@@ -1141,21 +1117,6 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
     }
 }
 
-template <int BT>
-__global__ void __launch_bounds__(256) k_sum_planes(Args a, const float* __restrict__ part, int parts) {
-  const int64_t n = (int64_t)a.H * a.nq * a.nk;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (int p = 0; p < parts; ++p) s += part[p * n + i];
-    const int64_t j = i % a.nk, hi = i / a.nk, h = hi / a.nq, q = hi - h * a.nq;
-    const int64_t off = h * a.db_hs + q * a.db_rs + j;
-    if (BT == 2)
-      ((float*)a.dbias)[off] = s;
-    else
-      ((bf16*)a.dbias)[off] = __float2bfloat16_rn(s);
-  }
-}
-
 // ---------------------------------------------------------------- launches
 
 template <class F, class... X>
@@ -1201,16 +1162,8 @@ template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
   constexpr size_t smem = 2 * ((size_t)(256 + 128) * Tile<DP>::RB + 2048);
   a.tiles = (a.nq + 127) / 128;
-  PF_TRY(go(k_dbias<DP, BT>, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, "k_attn_dbias", flops, st, a, part,
-            parts));
-  if (parts == 1) return PF_OK;
-  const int64_t n = (int64_t)a.H * a.nq * a.nk, want = (n + 255) / 256;
-  {
-    PF_LAUNCH_SCOPE_WORK(st, "k_attn_sum_planes", 4.0 * n * (parts + 1), 'b');
-    k_sum_planes<BT><<<(unsigned)(want < 148 * 8 ? want : 148 * 8), 256, 0, st>>>(a, part, parts);
-  }
-  PF_CHECK_LAUNCH();
-  return PF_OK;
+  return go(k_dbias<DP, BT>, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, "k_attn_dbias", flops, st, a, part,
+            parts);
 }
 
 }  // namespace
@@ -1229,14 +1182,6 @@ int launch_bf16(Kind kind, const Args& a, double flops, cudaStream_t st) {
   PF_ATT_DIM(launch_t, 1, kind, a, flops, st);
 }
 
-// Parts of the batch: about three blocks per SM.
-int dbias_parts_bf16(int64_t B, int64_t nq, int64_t nk, int H) {
-  const int64_t blocks = ((nq + 127) / 128) * ((nk + 63) / 64) * H;
-  if (blocks <= 0) return 1;
-  int64_t p = (3 * 148 + blocks - 1) / blocks;
-  if (p > B / 4) p = B / 4;
-  return p < 1 ? 1 : (int)p;
-}
 int dbias_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
   if (a.bias_f32) PF_ATT_DIM(launch_db, 2, a, part, parts, flops, st);
   PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);

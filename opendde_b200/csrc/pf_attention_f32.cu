@@ -2,6 +2,7 @@
 // against streamed tiles of BN rows that cp.async double-buffers in shared memory, with FFMA.
 
 #include "pf_attention.cuh"
+#include "pf_f32x2.cuh"
 
 namespace pf {
 namespace train {
@@ -72,26 +73,36 @@ __device__ __forceinline__ bool all_seen(uint64_t bits) {
 template <int DP, int BN>
 struct Prod {
   static constexpr int P = Pitch<DP>::value;
+  // c = a b^T; pairs hold the sums over even and odd depths
   static __device__ void nt(float (&c)[BN / 8][4], const float* a, const float* b) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    F2 s[BN / 8][4];
 #pragma unroll
-    for (int n = 0; n < BN / 8; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+    for (int n = 0; n < BN / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = F2(0.f);
 #pragma unroll 4
     for (int k = 0; k < DP; k += 4) {
       const float4 a0 = *reinterpret_cast<const float4*>(a + g * P + k);
       const float4 a1 = *reinterpret_cast<const float4*>(a + (g + 8) * P + k);
+      const F2 a0l(a0.x, a0.y), a0h(a0.z, a0.w), a1l(a1.x, a1.y), a1h(a1.z, a1.w);
 #pragma unroll
       for (int n = 0; n < BN / 8; ++n) {
         const float4 b0 = *reinterpret_cast<const float4*>(b + (n * 8 + 2 * t) * P + k);
         const float4 b1 = *reinterpret_cast<const float4*>(b + (n * 8 + 2 * t + 1) * P + k);
-        c[n][0] += a0.x * b0.x + a0.y * b0.y + a0.z * b0.z + a0.w * b0.w;
-        c[n][1] += a0.x * b1.x + a0.y * b1.y + a0.z * b1.z + a0.w * b1.w;
-        c[n][2] += a1.x * b0.x + a1.y * b0.y + a1.z * b0.z + a1.w * b0.w;
-        c[n][3] += a1.x * b1.x + a1.y * b1.y + a1.z * b1.z + a1.w * b1.w;
+        const F2 b0l(b0.x, b0.y), b0h(b0.z, b0.w), b1l(b1.x, b1.y), b1h(b1.z, b1.w);
+        s[n][0] = fma2(a0h, b0h, fma2(a0l, b0l, s[n][0]));
+        s[n][1] = fma2(a0h, b1h, fma2(a0l, b1l, s[n][1]));
+        s[n][2] = fma2(a1h, b0h, fma2(a1l, b0l, s[n][2]));
+        s[n][3] = fma2(a1h, b1h, fma2(a1l, b1l, s[n][3]));
       }
     }
+#pragma unroll
+    for (int n = 0; n < BN / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[n][e] = s[n][e].sum();
   }
-  // p goes through the warp's scratch rows [16][BN + 4]
+  // acc += p b; p goes through the warp's scratch rows [16][BN + 4]
   static __device__ void nn(float (&acc)[DP / 8][4], const float (&p)[BN / 8][4], float* sc, const float* b) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     constexpr int Q = BN + 4;
@@ -102,21 +113,32 @@ struct Prod {
       *reinterpret_cast<float2*>(sc + (g + 8) * Q + n * 8 + 2 * t) = make_float2(p[n][2], p[n][3]);
     }
     __syncwarp();
+    F2 s[DP / 8][2];
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      s[n][0] = F2(acc[n][0], acc[n][1]);
+      s[n][1] = F2(acc[n][2], acc[n][3]);
+    }
 #pragma unroll 2
     for (int k = 0; k < BN; k += 4) {
       const float4 a0 = *reinterpret_cast<const float4*>(sc + g * Q + k);
       const float4 a1 = *reinterpret_cast<const float4*>(sc + (g + 8) * Q + k);
       const float x0[4] = {a0.x, a0.y, a0.z, a0.w}, x1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 4; ++u) {
+        const F2 y0(x0[u]), y1(x1[u]);
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n) {
           const float2 v = *reinterpret_cast<const float2*>(b + (k + u) * P + n * 8 + 2 * t);
-          acc[n][0] += x0[u] * v.x;
-          acc[n][1] += x0[u] * v.y;
-          acc[n][2] += x1[u] * v.x;
-          acc[n][3] += x1[u] * v.y;
+          s[n][0] = fma2(y0, F2(v.x, v.y), s[n][0]);
+          s[n][1] = fma2(y1, F2(v.x, v.y), s[n][1]);
         }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      s[n][0].get(acc[n][0], acc[n][1]);
+      s[n][1].get(acc[n][2], acc[n][3]);
     }
   }
 };
@@ -264,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_fwd(Args a) {
     cp_wait<0>();
     __syncthreads();
     if (kt + 1 < nt) issue(kt + 1);
-    if (bits == 0) continue;  // the same for the whole block
+    if (bits == 0 || w0 >= a.nq) continue;  // nothing to see, or a warp past the end
     const int s = (int)(kt & 1);
     float x[BN / 8][4];
     M::nt(x, sq + warp * 16 * S::P, sk + s * S::kStream);
@@ -442,6 +464,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(Args a) {
     if (kt + 1 < nt) issue(kt + 1);
     const int s = (int)(kt & 1);
     float x[BN / 8][4], y[BN / 8][4];
+    if (w0 >= a.nq) continue;  // a warp past the end
     if (bits == 0) {
 #pragma unroll
       for (int n = 0; n < BN / 8; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
@@ -514,6 +537,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dkv(Args a) {
       cp_wait<0>();
       __syncthreads();
       if (it + 1 < nt) issue(it + 1);
+      if (w0 >= a.nk) continue;  // a warp past the end
       float x[BN / 8][4], y[BN / 8][4];
       M::nt(x, sk + warp * 16 * S::P, sq + s * S::kStream);
       M::nt(y, sv + warp * 16 * S::P, sg + s * S::kStream);
@@ -544,9 +568,10 @@ __global__ void __launch_bounds__(kThreads) k_attn_dkv(Args a) {
   store_rows<DP>(a.dv, b * a.dv_bs + (int64_t)kh * a.dv_hs, a.dv_ns, w0, a.nk, a.d, dv, 1.f, 1.f);
 }
 
-// dbias of one 64 x BN tile of the plane of head h, summed over the batch.
+// dbias of one 64 x BN tile of the plane of head h, summed over a part of the batch: the result where there
+// is one part, else an fp32 partial plane.
 template <int DP, int BN>
-__global__ void __launch_bounds__(kThreads) k_attn_dbias(Args a) {
+__global__ void __launch_bounds__(kThreads) k_attn_dbias(Args a, float* part, int parts) {
   using M = Prod<DP, BN>;
   using S = Smem<DP, BN>;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -557,7 +582,9 @@ __global__ void __launch_bounds__(kThreads) k_attn_dbias(Args a) {
   const int64_t kt = id % nkt;
   id /= nkt;
   const int64_t tile = id % a.tiles;
-  const int h = (int)(id / a.tiles), kh = h / (a.H / a.KV);
+  id /= a.tiles;
+  const int h = (int)(id % a.H), kh = h / (a.H / a.KV), pt = (int)(id / a.H);
+  const int64_t b0 = a.B * pt / parts, b1 = a.B * (pt + 1) / parts;
   const int64_t i0 = tile * BM, w0 = i0 + warp * 16, j0 = kt * BN;
   auto issue = [&](int64_t b) {
     float* p = sm[b & 1];
@@ -570,13 +597,13 @@ __global__ void __launch_bounds__(kThreads) k_attn_dbias(Args a) {
   float acc[BN / 8][4];
 #pragma unroll
   for (int n = 0; n < BN / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  issue(0);
-  for (int64_t b = 0; b < a.B; ++b) {
+  if (b0 < b1) issue(b0);
+  for (int64_t b = b0; b < b1; ++b) {
     const uint64_t bits = seen_bits<BN>(a, b, j0);
     cp_wait<0>();
     __syncthreads();
-    if (b + 1 < a.B) issue(b + 1);
-    if (bits == 0) continue;
+    if (b + 1 < b1) issue(b + 1);
+    if (bits == 0 || w0 >= a.nq) continue;
     const float* p = sm[b & 1];
     const RowConst rc = row_const(a, b, h, w0);
     float x[BN / 8][4], y[BN / 8][4];
@@ -590,21 +617,33 @@ __global__ void __launch_bounds__(kThreads) k_attn_dbias(Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[n][e] += y[n][e];
   }
+  cp_commit();
   cp_wait<0>();
-  store_dbias<BN>(a, 0, h, w0, j0, acc);
+  if (parts == 1) {
+    store_dbias<BN>(a, 0, h, w0, j0, acc);
+  } else {
+    Args w = a;  // the part's plane in dbias's place
+    w.dbias = part;
+    w.bias_f32 = 1;
+    w.db_vec = (a.nk & 3) == 0;
+    w.db_rs = a.nk;
+    w.db_hs = a.nq * a.nk;
+    w.db_bs = a.H * a.nq * a.nk;
+    store_dbias<BN>(w, pt, h, w0, j0, acc);
+  }
 }
 
 // ---------------------------------------------------------------- launches
 
-int go(void (*kern)(Args), const Args& a, size_t smem, int64_t blocks, const char* name, double flops,
-       cudaStream_t st) {
+template <class F, class... X>
+int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cudaStream_t st, X... x) {
   if (blocks == 0) return PF_OK;
   if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
   if (smem > 40 * 1024)
     PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   {
     PF_LAUNCH_SCOPE_WORK(st, name, flops, 'f');
-    kern<<<(unsigned)blocks, kThreads, smem, st>>>(a);
+    kern<<<(unsigned)blocks, kThreads, smem, st>>>(x...);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;
@@ -616,16 +655,16 @@ int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   using S = Smem<DP, BN>;
   a.tiles = ((kind == kDkv ? a.nk : a.nq) + BM - 1) / BM;
   const int64_t blocks = a.tiles * (kind == kDkv ? a.KV : a.H) * a.B;
-  if (kind == kFwd) return go(k_attn_fwd<DP, BN>, a, S::bytes(1, 2), blocks, "k_attn_fwd", flops, st);
-  if (kind == kDq) return go(k_attn_dq<DP, BN>, a, S::bytes(2, 2), blocks, "k_attn_dq", flops, st);
-  return go(k_attn_dkv<DP, BN>, a, S::bytes(2, 2), blocks, "k_attn_dkv", flops, st);
+  if (kind == kFwd) return go(k_attn_fwd<DP, BN>, S::bytes(1, 2), blocks, "k_attn_fwd", flops, st, a);
+  if (kind == kDq) return go(k_attn_dq<DP, BN>, S::bytes(2, 2), blocks, "k_attn_dq", flops, st, a);
+  return go(k_attn_dkv<DP, BN>, S::bytes(2, 2), blocks, "k_attn_dkv", flops, st, a);
 }
 template <int DP>
-int launch_db(Args a, double flops, cudaStream_t st) {
+int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
   constexpr int BN = 32;
   a.tiles = (a.nq + BM - 1) / BM;
-  return go(k_attn_dbias<DP, BN>, a, Smem<DP, BN>::bytes(4, 2), a.tiles * ((a.nk + BN - 1) / BN) * a.H,
-            "k_attn_dbias", flops, st);
+  return go(k_attn_dbias<DP, BN>, Smem<DP, BN>::bytes(4, 2), a.tiles * ((a.nk + BN - 1) / BN) * a.H * parts,
+            "k_attn_dbias", flops, st, a, part, parts);
 }
 
 }  // namespace
@@ -636,11 +675,11 @@ int launch_f32(Kind kind, const Args& a, double flops, cudaStream_t st) {
   if (a.d <= 96) return launch_t<96>(kind, a, flops, st);
   return launch_t<128>(kind, a, flops, st);
 }
-int dbias_f32(const Args& a, double flops, cudaStream_t st) {
-  if (a.d <= 32) return launch_db<32>(a, flops, st);
-  if (a.d <= 64) return launch_db<64>(a, flops, st);
-  if (a.d <= 96) return launch_db<96>(a, flops, st);
-  return launch_db<128>(a, flops, st);
+int dbias_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
+  if (a.d <= 32) return launch_db<32>(a, part, parts, flops, st);
+  if (a.d <= 64) return launch_db<64>(a, part, parts, flops, st);
+  if (a.d <= 96) return launch_db<96>(a, part, parts, flops, st);
+  return launch_db<128>(a, part, parts, flops, st);
 }
 int rows_f32(const Args& a, const float* stats, Heads o, float* rows, cudaStream_t st) {
   const int64_t blocks = (a.rows_plane + 31) / 32;

@@ -13,6 +13,7 @@
 // rows in a fixed order (no atomics: equal inputs give equal bits). One block writes the result itself.
 
 #include "pf_common.cuh"
+#include "pf_f32x2.cuh"
 #include "pf_prof.h"
 #include "pf_train.h"
 
@@ -75,26 +76,28 @@ __device__ __forceinline__ float group_sum(float v) {
 
 constexpr int kWarps = 8;
 
-// L lanes per row, V chunks of E channels per lane, U rows of a lane in flight.
-template <class T, int E, int L, int V, int U>
+// L lanes per row, V chunks of E channels per lane, U rows of a lane in flight; FULL: c = L V E.
+template <class T, int E, int L, int V, int U, bool FULL>
 __global__ void __launch_bounds__(kWarps * 32) k_layernorm_bwd(const T* x, const T* dy,
                                                                const float* __restrict__ gamma, T* dx, float* dg_out,
-                                                               float* db_out, int64_t rows, int c, float eps) {
+                                                               float* db_out, int64_t part, int64_t rows, int c,
+                                                               float eps) {
   constexpr int R = 32 / L;  // rows of a warp side by side
+  constexpr int N = V * E / 2;  // channel pairs of a lane
   extern __shared__ float sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane & (L - 1), grp = lane / L;
   const int nv = c / E;
   const float inv_c = 1.f / (float)c;
-  float gw[V * E], ag[V * E], ab[V * E];
+  auto in = [&](int i) { return FULL || sub + (i / E) * L < nv; };       // element i of the lane exists
+  auto channel = [&](int i) { return (sub + (i / E) * L) * E + i % E; };  // its channel
+  F2 gw[N], ag[N], ab[N];
 #pragma unroll
-  for (int t = 0; t < V; ++t)
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int v = sub + t * L;
-      gw[t * E + e] = v < nv ? (gamma ? gamma[v * E + e] : 1.f) : 0.f;
-      ag[t * E + e] = ab[t * E + e] = 0.f;
-    }
+  for (int i = 0; i < N; ++i) {
+    gw[i] = F2(in(2 * i) ? (gamma ? gamma[channel(2 * i)] : 1.f) : 0.f,
+               in(2 * i + 1) ? (gamma ? gamma[channel(2 * i + 1)] : 1.f) : 0.f);
+    ag[i] = ab[i] = F2(0.f);
+  }
   const int64_t step = (int64_t)gridDim.x * kWarps * R * U;
   for (int64_t base = ((int64_t)blockIdx.x * kWarps + warp) * R * U; base < rows; base += step) {
     Chunk<T, E> xr[U][V], gr[U][V];
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_layernorm_bwd(const T* x, const
 #pragma unroll
       for (int t = 0; t < V; ++t) {
         const int v = sub + t * L;
-        if (row < rows && v < nv) {
+        if (row < rows && (FULL || v < nv)) {
           xr[u][t].load(x + row * c + (int64_t)v * E);
           gr[u][t].load(dy + row * c + (int64_t)v * E);
         } else {
@@ -116,103 +119,111 @@ __global__ void __launch_bounds__(kWarps * 32) k_layernorm_bwd(const T* x, const
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + (int64_t)u * R + grp;
-      float s0 = 0.f;
+      float f[V * E], g[V * E];
 #pragma unroll
       for (int t = 0; t < V; ++t) {
-        float f[E];
-        xr[u][t].get(f);
-#pragma unroll
-        for (int e = 0; e < E; ++e) s0 += f[e];
+        xr[u][t].get(f + t * E);
+        gr[u][t].get(g + t * E);
       }
-      const float mean = group_sum<L>(s0) * inv_c;
-      float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      F2 s0 = F2(f[0], f[1]);
 #pragma unroll
-      for (int t = 0; t < V; ++t) {
-        float f[E], g[E];
-        xr[u][t].get(f);
-        gr[u][t].get(g);
-        const bool in = sub + t * L < nv;
+      for (int i = 1; i < N; ++i) s0 = add2(s0, F2(f[2 * i], f[2 * i + 1]));
+      const float mean = group_sum<L>(s0.sum()) * inv_c;
+      const F2 nmean(-mean);
+      F2 s1(0.f), s2(0.f), s3(0.f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float d = in ? f[e] - mean : 0.f, gg = g[e] * gw[t * E + e];
-          s1 += d * d;
-          s2 += gg;
-          s3 += gg * d;
+      for (int i = 0; i < N; ++i) {
+        F2 d = add2(F2(f[2 * i], f[2 * i + 1]), nmean);
+        d.get(f[2 * i], f[2 * i + 1]);
+        if (!FULL) {
+          if (!in(2 * i)) f[2 * i] = 0.f;
+          if (!in(2 * i + 1)) f[2 * i + 1] = 0.f;
+          d = F2(f[2 * i], f[2 * i + 1]);
         }
+        const F2 gg = mul2(F2(g[2 * i], g[2 * i + 1]), gw[i]);
+        s1 = fma2(d, d, s1);
+        s2 = add2(s2, gg);
+        s3 = fma2(gg, d, s3);
       }
-      s1 = group_sum<L>(s1);
-      s2 = group_sum<L>(s2);
-      s3 = group_sum<L>(s3);
+      const float q1 = group_sum<L>(s1.sum()), q2 = group_sum<L>(s2.sum()), q3 = group_sum<L>(s3.sum());
       // rows past the end are zero and add nothing, whatever eps is
-      const float rstd = row < rows ? rsqrtf(s1 * inv_c + eps) : 0.f;
-      const float m1 = s2 * inv_c, m2 = s3 * inv_c * rstd * rstd;
+      const float rstd = row < rows ? rsqrtf(q1 * inv_c + eps) : 0.f;
+      // dx = rstd (g - mean(g)) - d rstd^3 mean(g d)
+      const F2 r2(rstd), m1(-q2 * inv_c * rstd), m2(-q3 * inv_c * rstd * rstd * rstd);
 #pragma unroll
-      for (int t = 0; t < V; ++t) {
-        float f[E], g[E], o[E];
-        xr[u][t].get(f);
-        gr[u][t].get(g);
+      for (int i = 0; i < N; ++i) {
+        const F2 d = F2(f[2 * i], f[2 * i + 1]), gy = F2(g[2 * i], g[2 * i + 1]);
+        ag[i] = fma2(gy, mul2(d, r2), ag[i]);
+        ab[i] = add2(ab[i], gy);
+        fma2(d, m2, fma2(mul2(gy, gw[i]), r2, m1)).get(f[2 * i], f[2 * i + 1]);
+      }
+      if (dx && row < rows) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float d = f[e] - mean;
-          o[e] = (g[e] * gw[t * E + e] - m1 - d * m2) * rstd;
-          ag[t * E + e] += g[e] * (d * rstd);  // rows past the end have dy = 0
-          ab[t * E + e] += g[e];
+        for (int t = 0; t < V; ++t) {
+          const int v = sub + t * L;
+          if (FULL || v < nv) Chunk<T, E>::store(dx + row * c + (int64_t)v * E, f + t * E);
         }
-        const int v = sub + t * L;
-        if (dx && row < rows && v < nv) Chunk<T, E>::store(dx + row * c + (int64_t)v * E, o);
       }
     }
   }
   if (!dg_out && !db_out) return;
   // the warp's rows side by side, then the block's warps
+  float a[2 * N], b[2 * N];
 #pragma unroll
-  for (int i = 0; i < V * E; ++i) {
+  for (int i = 0; i < N; ++i) {
+    ag[i].get(a[2 * i], a[2 * i + 1]);
+    ab[i].get(b[2 * i], b[2 * i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * N; ++i) {
 #pragma unroll
     for (int o = L; o < 32; o <<= 1) {
-      ag[i] += __shfl_xor_sync(0xffffffffu, ag[i], o);
-      ab[i] += __shfl_xor_sync(0xffffffffu, ab[i], o);
+      a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
+      b[i] += __shfl_xor_sync(0xffffffffu, b[i], o);
     }
   }
   if (grp == 0) {
 #pragma unroll
-    for (int t = 0; t < V; ++t) {
-      const int v = sub + t * L;
-      if (v < nv)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          sm[(warp * 2) * c + v * E + e] = ag[t * E + e];
-          sm[(warp * 2 + 1) * c + v * E + e] = ab[t * E + e];
-        }
-    }
+    for (int i = 0; i < 2 * N; ++i)
+      if (in(i)) {
+        sm[(warp * 2) * c + channel(i)] = a[i];
+        sm[(warp * 2 + 1) * c + channel(i)] = b[i];
+      }
   }
   __syncthreads();
-  const int64_t part = (int64_t)blockIdx.x * c;
+  const int64_t off = (int64_t)blockIdx.x * part;
   for (int i = threadIdx.x; i < c; i += kWarps * 32) {
-    float a = 0.f, b = 0.f;
+    float sa = 0.f, sb = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      a += sm[(w * 2) * c + i];
-      b += sm[(w * 2 + 1) * c + i];
+      sa += sm[(w * 2) * c + i];
+      sb += sm[(w * 2 + 1) * c + i];
     }
-    if (dg_out) dg_out[part + i] = a;
-    if (db_out) db_out[part + i] = b;
+    if (dg_out) dg_out[off + i] = sa;
+    if (db_out) db_out[off + i] = sb;
   }
 }
 
-// 32 columns by 8 row groups per block: group y adds rows y, y + 8, ..., then the groups are added.
-__global__ void __launch_bounds__(256) k_sum_rows(const float* __restrict__ part, int64_t n, int64_t m,
-                                                  float* __restrict__ out) {
-  __shared__ float sm[8][33];
+// 32 columns by 32 row groups per block: group y adds rows y, y + 32, ..., then the groups are added.
+// Columns below m0 go to out0, the others to out1.
+__global__ void __launch_bounds__(1024) k_sum_rows(const float* __restrict__ part, int64_t n, int64_t m,
+                                                   float* __restrict__ out0, int64_t m0, float* __restrict__ out1) {
+  __shared__ float sm[32][33];
   const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
   if (i < m)
-    for (int64_t r = threadIdx.y; r < n; r += 8) s += part[r * m + i];
+    for (int64_t r = threadIdx.y; r < n; r += 32) s += part[r * m + i];
   sm[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && i < m) {
-#pragma unroll
-    for (int y = 1; y < 8; ++y) s += sm[y][threadIdx.x];
-    out[i] = s;
+  // warp y adds the groups of column y
+  float v = sm[threadIdx.x][threadIdx.y];
+  v = warp_sum(v);
+  const int64_t j = (int64_t)blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && j < m) {
+    if (j < m0)
+      out0[j] = v;
+    else
+      out1[j - m0] = v;
   }
 }
 
@@ -222,46 +233,51 @@ int sm_count() {
   return n;
 }
 
-// Blocks of the row kernel: enough warps to cover the rows, at most four blocks on each SM.
-int64_t grid_blocks(int64_t rows, int rows_per_block) {
+// Blocks of the row kernel: one where the rows are few (a second launch to add the blocks' shares would
+// cost more than the rows: 64 rows of 384 channels 5 us in one block, 9 us in eight and the sum); else
+// enough warps to cover the rows, at most four blocks on each SM.
+int64_t grid_blocks(int64_t rows, int c, int rows_per_block, bool sums) {
+  if (sums && rows * c <= 64 * 512) return 1;
   const int64_t need = (rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sm_count() * 4;
   return need < 1 ? 1 : (need < most ? need : most);
 }
 
-template <class T, int E, int L, int V, int U>
+template <class T, int E, int L, int V, int U, bool FULL>
 int launch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float* db, int64_t rows, int c, float eps,
            float* part, cudaStream_t st) {
-  const int64_t blocks = grid_blocks(rows, kWarps * (32 / L) * U);
+  const int64_t blocks = grid_blocks(rows, c, kWarps * (32 / L) * U, dg || db);
   const size_t smem = (size_t)kWarps * 2 * c * sizeof(float);
-  auto* kern = k_layernorm_bwd<T, E, L, V, U>;
+  auto* kern = k_layernorm_bwd<T, E, L, V, U, FULL>;
   if (smem > 48 * 1024) PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const bool direct = blocks == 1;
-  float* pg = direct ? dg : (dg ? part : nullptr);
-  float* pb = direct ? db : (db ? part + blocks * c : nullptr);
+  const int64_t m0 = dg ? c : 0, m = m0 + (db ? c : 0);  // a partial row: dgamma, then dbeta
+  float* pg = direct || !dg ? dg : part;
+  float* pb = direct || !db ? db : part + m0;
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_layernorm_bwd", 3.0 * (double)rows * c * sizeof(T), 'b');
-    kern<<<(unsigned)blocks, kWarps * 32, smem, st>>>(x, dy, gamma, dx, pg, pb, rows, c, eps);
+    kern<<<(unsigned)blocks, kWarps * 32, smem, st>>>(x, dy, gamma, dx, pg, pb, m, rows, c, eps);
   }
   PF_CHECK_LAUNCH();
-  if (direct) return PF_OK;
-  if (dg) PF_TRY(sum_rows(pg, blocks, c, dg, st));
-  if (db) PF_TRY(sum_rows(pb, blocks, c, db, st));
-  return PF_OK;
+  return direct || m == 0 ? PF_OK : sum_rows(part, blocks, m, dg, m0, db, st);
 }
 
 template <class T, int E>
 int dispatch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float* db, int64_t rows, int c, float eps,
              float* part, cudaStream_t st) {
+  // two chunks per lane and few lanes per row: a row's four sums then take few shuffle steps
   const int nv = c / E;
-#define PF_LN(L, V, U) return launch<T, E, L, V, U>(x, dy, gamma, dx, dg, db, rows, c, eps, part, st)
-  if (nv <= 1) PF_LN(1, 1, 2);
-  if (nv <= 2) PF_LN(2, 1, 2);
-  if (nv <= 4) PF_LN(4, 1, 2);
-  if (nv <= 8) PF_LN(8, 1, 2);
-  if (nv <= 16) PF_LN(16, 1, 2);
-  if (nv <= 32) PF_LN(32, 1, 2);
-  if (nv <= 64) PF_LN(32, 2, 1);
-  if (nv <= 96) PF_LN(32, 3, 1);
+#define PF_LN(L, V, U)                                                                        \
+  return nv == L * V ? launch<T, E, L, V, U, true>(x, dy, gamma, dx, dg, db, rows, c, eps, part, st) \
+                     : launch<T, E, L, V, U, false>(x, dy, gamma, dx, dg, db, rows, c, eps, part, st)
+  if (nv <= 2) PF_LN(1, 2, 1);
+  if (nv <= 4) PF_LN(2, 2, 1);
+  if (nv <= 8) PF_LN(4, 2, 2);
+  if (nv <= 16) PF_LN(8, 2, 2);
+  if (nv <= 32) PF_LN(16, 2, 2);
+  if (nv <= 64) PF_LN(32, 2, 2);
+  if constexpr (E > 1) {
+    if (nv <= 96) PF_LN(32, 3, 1);
+  }
   if (nv <= 128) PF_LN(32, 4, 1);
   if constexpr (E < 8) {
     if (nv <= 256) PF_LN(32, 8, 1);
@@ -276,10 +292,10 @@ int dispatch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, floa
 
 }  // namespace
 
-int sum_rows(const float* part, int64_t n, int64_t m, float* out, cudaStream_t st) {
+int sum_rows(const float* part, int64_t n, int64_t m, float* out0, int64_t m0, float* out1, cudaStream_t st) {
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_sum_rows", 4.0 * (double)(n + 1) * m, 'b');
-    k_sum_rows<<<(unsigned)((m + 31) / 32), dim3(32, 8), 0, st>>>(part, n, m, out);
+    k_sum_rows<<<(unsigned)((m + 31) / 32), dim3(32, 32), 0, st>>>(part, n, m, out0, m0, out1);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;

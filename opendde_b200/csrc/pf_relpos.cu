@@ -25,6 +25,7 @@ namespace train {
 namespace {
 
 constexpr int kRelWarps = 8;
+constexpr int kRelWaves = 4;
 constexpr int kRelRows = 64;  // rows of a block at most (their ids lie in shared memory)
 
 struct RelArgs {
@@ -49,14 +50,17 @@ __device__ __forceinline__ int clip_diff(int a, int b, int lim) {
   return min(max(d, -lim), lim) + lim;
 }
 
-// The columns of one pair: the residue column, and the others packed (token column, symmetry column,
-// same-entity bit; each column is below 2^12).
-__device__ __forceinline__ void pair_cols(const TokId& i, const TokId& j, int R, int S, int& res, int& rest) {
+struct PairCols {
+  int res, tok, sym;  // feature columns; sym carries the same-entity bit above them
+};
+constexpr int kEntBit = 1 << 16;  // above every column (at most 2048)
+__device__ __forceinline__ PairCols pair_cols(const TokId& i, const TokId& j, int R, int S) {
   const bool chain = i.asym == j.asym, ent = i.ent == j.ent;
-  res = chain ? clip_diff(i.res, j.res, R) : 2 * R + 1;
-  const int tok = 2 * R + 2 + ((chain && i.res == j.res) ? clip_diff(i.tok, j.tok, R) : 2 * R + 1);
-  const int sym = 4 * R + 5 + (ent ? clip_diff(i.sym, j.sym, S) : 2 * S + 1);
-  rest = tok | (sym << 12) | ((ent ? 1 : 0) << 24);
+  PairCols p;
+  p.res = chain ? clip_diff(i.res, j.res, R) : 2 * R + 1;
+  p.tok = 2 * R + 2 + ((chain && i.res == j.res) ? clip_diff(i.tok, j.tok, R) : 2 * R + 1);
+  p.sym = 4 * R + 5 + (ent ? clip_diff(i.sym, j.sym, S) + kEntBit : 2 * S + 1);
+  return p;
 }
 
 template <class TW, class T, int G>
@@ -74,27 +78,25 @@ __global__ void __launch_bounds__(kRelWarps * 32) k_relpos_bias(RelArgs a, const
   const int64_t j = ((int64_t)blockIdx.x * kRelWarps + warp) * 32 + lane;
   if (j >= a.n_cols) return;
   const TokId cid = load_id(a.ids, a.col0 + j);
-  int cur_res = -1, cur_rest = -1;
+  PairCols cur{-1, -1, -1};
   float rest_v[G], val[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) rest_v[g] = val[g] = 0.f;
   T* o = out + (int64_t)h0 * a.hs + r0 * a.rs + j;
   for (int i = 0; i < nr; ++i, o += a.rs) {
-    int res, rest;
-    pair_cols(rid[i], cid, a.R, a.S, res, rest);
-    if (res != cur_res || rest != cur_rest) {
-      if (rest != cur_rest) {
-        const int tok = rest & 0xfff, sym = (rest >> 12) & 0xfff;
+    const PairCols p = pair_cols(rid[i], cid, a.R, a.S);
+    const bool new_rest = p.tok != cur.tok || p.sym != cur.sym;
+    if (p.res != cur.res || new_rest) {
+      if (new_rest) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const float* t = tab + g * a.n_feat;
-          rest_v[g] = t[tok] + t[sym] + ((rest >> 24) ? t[4 * a.R + 4] : 0.f);
+          rest_v[g] = t[p.tok] + t[p.sym & (kEntBit - 1)] + (p.sym & kEntBit ? t[4 * a.R + 4] : 0.f);
         }
       }
 #pragma unroll
-      for (int g = 0; g < G; ++g) val[g] = tab[g * a.n_feat + res] + rest_v[g];
-      cur_res = res;
-      cur_rest = rest;
+      for (int g = 0; g < G; ++g) val[g] = tab[g * a.n_feat + p.res] + rest_v[g];
+      cur = p;
     }
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -102,21 +104,63 @@ __global__ void __launch_bounds__(kRelWarps * 32) k_relpos_bias(RelArgs a, const
   }
 }
 
+// tab[g][f] += v[g]: all reads before the writes, which the compiler cannot know to be apart
+template <int G>
+__device__ __forceinline__ void add_column(float* tab, int n_feat, int f, const float* v) {
+  float t[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) t[g] = tab[g * n_feat + f];
+#pragma unroll
+  for (int g = 0; g < G; ++g) tab[g * n_feat + f] = t[g] + v[g];
+}
+
 // Adds each lane's G values to column f of the warp's table; lanes with pred == false add nothing.
-// Every lane of the warp takes part.
+// Every lane of the warp takes part. Lanes that share a column add in lane order, or (all of them in
+// one column: clipped offsets, other chains) through a butterfly.
 template <int G>
 __device__ __forceinline__ void flush(float* tab, int n_feat, bool pred, int f, const float* v) {
   const unsigned live = __ballot_sync(0xffffffffu, pred);
   if (live == 0) return;
-  const unsigned same = __match_any_sync(0xffffffffu, pred ? f : -1);
-  const unsigned lane = threadIdx.x & 31;
-  const int rank = pred ? __popc(same & ((1u << lane) - 1u)) : 0;
-  const int last = __reduce_max_sync(0xffffffffu, rank);
-  for (int r = 0; r <= last; ++r) {
-    if (pred && rank == r) {
+  const unsigned lane = threadIdx.x & 31, before = live & ((1u << lane) - 1u);
+  const bool head = before == 0;  // the first of them, where pred
+  const int prev = __shfl_sync(0xffffffffu, f, head ? lane : 31 - __clz(before));
+  const unsigned starts = __ballot_sync(0xffffffffu, pred && (head || f != prev));
+  if ((starts & (starts - 1)) == 0) {  // one column for all
+    float s[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) tab[g * n_feat + f] += v[g];
+    for (int g = 0; g < G; ++g) s[g] = warp_sum(pred ? v[g] : 0.f);
+    if (pred && head) add_column<G>(tab, n_feat, f, s);
+    __syncwarp();
+    return;
+  }
+  int rank;  // among the lanes of its column
+  if (__all_sync(0xffffffffu, !pred || head || f <= prev) || __all_sync(0xffffffffu, !pred || head || f >= prev)) {
+    // In order, as down a chain: lanes of one column are neighbours. (Matching 32 different columns
+    // against each other takes many times as long.)
+    const int start = 31 - __clz(starts & (0xffffffffu >> (31 - lane)));
+    rank = __popc(before) - __popc(live & ((1u << (start & 31)) - 1u));
+    if (live == 0xffffffffu) {  // sums of neighbours, then one add per column
+      float s[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) s[g] = v[g];
+      for (int d = 1; __any_sync(0xffffffffu, rank >= d); d <<= 1) {
+        const bool same = __shfl_down_sync(0xffffffffu, start, d) == start && lane + d < 32;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float o = __shfl_down_sync(0xffffffffu, s[g], d);
+          if (same) s[g] += o;
+        }
+      }
+      if (rank == 0) add_column<G>(tab, n_feat, f, s);
+      __syncwarp();
+      return;
     }
+  } else {
+    const unsigned same = __match_any_sync(0xffffffffu, pred ? f : -1);
+    rank = __popc(same & ((1u << lane) - 1u));
+  }
+  for (int r = 0; __any_sync(0xffffffffu, pred && rank >= r); ++r) {
+    if (pred && rank == r) add_column<G>(tab, n_feat, f, v);
     __syncwarp();
   }
 }
@@ -138,19 +182,18 @@ __global__ void __launch_bounds__(kRelWarps * 32) k_relpos_bias_bwd(RelArgs a, c
   const int64_t j = ((int64_t)blockIdx.x * kRelWarps + warp) * 32 + lane;
   const bool live = j < a.n_cols;
   const TokId cid = load_id(a.ids, a.col0 + (live ? j : 0));
-  int cur_res = 0, cur_rest = 0;
-  pair_cols(rid[0], cid, a.R, a.S, cur_res, cur_rest);
-  // run: the sum since the residue column last changed; all: since the others last changed, without run
-  float run[G], all[G];
+  PairCols cur = pair_cols(rid[0], cid, a.R, a.S);
+  // Sums since the residue column last changed, before that since the token column did, and before that
+  // since the others did; a change flushes its own sum and the ones inside it.
+  float run[G], tok[G], sym[G];
 #pragma unroll
-  for (int g = 0; g < G; ++g) run[g] = all[g] = 0.f;
-  auto flush_rest = [&](bool pred) {
-    flush<G>(mine, a.n_feat, pred, cur_rest & 0xfff, all);
-    flush<G>(mine, a.n_feat, pred, (cur_rest >> 12) & 0xfff, all);
-    flush<G>(mine, a.n_feat, pred && (cur_rest >> 24), 4 * a.R + 4, all);
+  for (int g = 0; g < G; ++g) run[g] = tok[g] = sym[g] = 0.f;
+  auto flush_sym = [&](bool pred) {
+    flush<G>(mine, a.n_feat, pred, cur.sym & (kEntBit - 1), sym);
+    flush<G>(mine, a.n_feat, pred && (cur.sym & kEntBit), 4 * a.R + 4, sym);
   };
   const T* p = dout + (int64_t)h0 * a.hs + r0 * a.rs + (live ? j : 0);
-  constexpr int U = 4;  // rows in flight
+  constexpr int U = G == 8 ? 4 : 8;  // rows in flight
   for (int i0 = 0; i0 < nr; i0 += U) {
     T x[U][G];
 #pragma unroll
@@ -161,36 +204,46 @@ __global__ void __launch_bounds__(kRelWarps * 32) k_relpos_bias_bwd(RelArgs a, c
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i0 + u < nr) {  // the same for the whole warp
-        int res, rest;
-        pair_cols(rid[i0 + u], cid, a.R, a.S, res, rest);
-        const bool new_res = live && res != cur_res, new_rest = live && rest != cur_rest;
-        if (__any_sync(0xffffffffu, new_res || new_rest)) {
-          const bool out = new_res || new_rest;
-          flush<G>(mine, a.n_feat, out, cur_res, run);
+        const PairCols c = pair_cols(rid[i0 + u], cid, a.R, a.S);
+        const bool new_sym = live && c.sym != cur.sym, new_tok = new_sym || (live && c.tok != cur.tok),
+                   new_res = new_tok || (live && c.res != cur.res);
+        if (__any_sync(0xffffffffu, new_res)) {
+          flush<G>(mine, a.n_feat, new_res, cur.res, run);
 #pragma unroll
           for (int g = 0; g < G; ++g)
-            if (out) {
-              all[g] += run[g];
+            if (new_res) {
+              tok[g] += run[g];
               run[g] = 0.f;
             }
-          if (__any_sync(0xffffffffu, new_rest)) {
-            flush_rest(new_rest);
+          if (__any_sync(0xffffffffu, new_tok)) {
+            flush<G>(mine, a.n_feat, new_tok, cur.tok, tok);
 #pragma unroll
             for (int g = 0; g < G; ++g)
-              if (new_rest) all[g] = 0.f;
+              if (new_tok) {
+                sym[g] += tok[g];
+                tok[g] = 0.f;
+              }
+            if (__any_sync(0xffffffffu, new_sym)) {
+              flush_sym(new_sym);
+#pragma unroll
+              for (int g = 0; g < G; ++g)
+                if (new_sym) sym[g] = 0.f;
+            }
           }
-          cur_res = res;
-          cur_rest = rest;
+          if (live) cur = c;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) run[g] += to_f(x[u][g]);
       }
     }
   }
-  flush<G>(mine, a.n_feat, live, cur_res, run);
+  flush<G>(mine, a.n_feat, live, cur.res, run);
 #pragma unroll
-  for (int g = 0; g < G; ++g) all[g] += run[g];
-  flush_rest(live);
+  for (int g = 0; g < G; ++g) tok[g] += run[g];
+  flush<G>(mine, a.n_feat, live, cur.tok, tok);
+#pragma unroll
+  for (int g = 0; g < G; ++g) sym[g] += tok[g];
+  flush_sym(live);
   __syncthreads();
   // [row chunk x column strip][head][feature]
   float* dst = part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.heads * a.n_feat + (int64_t)h0 * a.n_feat;
@@ -207,15 +260,16 @@ struct RelGrid {
   int64_t strips, chunks, groups;
 };
 
-// Four heads at a time where eight warps' tables for them fit in 64 KB of shared memory (r_max up to
-// about 125), else one. Row chunks: about four blocks per SM, and not so short that the tables'
-// zeroing and adding outweigh the rows.
+// As many heads at a time as eight warps' tables leave room for in 64 KB of shared memory: eight up to
+// 256 features (r_max up to 61), four up to 512, else one. Row chunks: about four blocks per SM, and not
+// so short that the tables' zeroing and adding outweigh the rows.
 RelGrid plan(int64_t n_rows, int64_t n_cols, int heads, int n_feat) {
   RelGrid p;
-  p.G = n_feat <= 512 ? 4 : 1;
+  p.G = n_feat <= 256 && heads > 4 ? 8 : (n_feat <= 512 ? 4 : 1);
   p.strips = (n_cols + kRelWarps * 32 - 1) / (kRelWarps * 32);
   p.groups = (heads + p.G - 1) / p.G;
-  const int64_t want = (148 * 4 + p.strips * p.groups - 1) / (p.strips * p.groups);
+  int64_t want = 148 * kRelWaves * 2 / (p.strips * p.groups);
+  want = want < 1 ? 1 : want;
   int64_t per = (n_rows + want - 1) / want;
   per = per < 16 ? 16 : (per > kRelRows ? kRelRows : per);
   p.rows_per_block = (int)per;
@@ -269,7 +323,10 @@ int relpos_bias(const void* w, int w_dtype, pf_token_ids ids, void* out, int64_t
   const RelGrid p = plan(n_rows, n_cols, heads, relp_n_feat(R, S));
   PF_TRY(check_grid(p));
   const RelArgs a = rel_args(p, ids, row0, n_rows, col0, n_cols, hs, rs, heads, R, S);
-#define PF_REL(TW, T) return p.G == 4 ? launch_fwd<TW, T, 4>(p, a, w, out, st) : launch_fwd<TW, T, 1>(p, a, w, out, st)
+#define PF_REL(TW, T)                                          \
+  return p.G == 8   ? launch_fwd<TW, T, 8>(p, a, w, out, st)   \
+         : p.G == 4 ? launch_fwd<TW, T, 4>(p, a, w, out, st)   \
+                    : launch_fwd<TW, T, 1>(p, a, w, out, st)
   if (w_dtype == PF_F32) {
     if (dtype == PF_F32) PF_REL(float, float);
     PF_REL(float, __nv_bfloat16);
@@ -296,12 +353,17 @@ int relpos_bias_bwd(const void* dbias, int64_t hs, int64_t rs, int dtype, pf_tok
   const RelArgs a = rel_args(p, ids, row0, n_rows, col0, n_cols, hs, rs, heads, R, S);
   const int64_t n = p.strips * p.chunks;
   float* part = n == 1 ? dw : (float*)ws;
+  const int64_t m = (int64_t)heads * n_feat;
+#define PF_REL(T)                                                  \
+  PF_TRY((p.G == 8   ? launch_bwd<T, 8>(p, a, dbias, part, st)     \
+          : p.G == 4 ? launch_bwd<T, 4>(p, a, dbias, part, st)     \
+                     : launch_bwd<T, 1>(p, a, dbias, part, st)))
   if (dtype == PF_F32)
-    PF_TRY((p.G == 4 ? launch_bwd<float, 4>(p, a, dbias, part, st) : launch_bwd<float, 1>(p, a, dbias, part, st)));
+    PF_REL(float);
   else
-    PF_TRY((p.G == 4 ? launch_bwd<__nv_bfloat16, 4>(p, a, dbias, part, st)
-                     : launch_bwd<__nv_bfloat16, 1>(p, a, dbias, part, st)));
-  return n == 1 ? PF_OK : sum_rows(part, n, (int64_t)heads * n_feat, dw, st);
+    PF_REL(__nv_bfloat16);
+#undef PF_REL
+  return n == 1 ? PF_OK : sum_rows(part, n, m, dw, m, nullptr, st);
 }
 
 }  // namespace train

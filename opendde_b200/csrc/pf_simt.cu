@@ -24,7 +24,7 @@ namespace simt {
 // LayerNorm over channels of every position (r, s) of a pair view -> contiguous output
 // out[(r*n_cols + s) * c + ch]. One warp per position; two-pass (mean, then centred
 // variance) like torch's CPU layer_norm.
-template <class T, class TO>
+template <class T, class TO, int MAXV>
 __global__ void k_ln_view(const T* __restrict__ x, int64_t rs, int64_t cs, int64_t n_rows,
                           int64_t n_cols, int c, const float* __restrict__ gamma,
                           const float* __restrict__ beta, float eps, TO* __restrict__ out,
@@ -35,8 +35,7 @@ __global__ void k_ln_view(const T* __restrict__ x, int64_t rs, int64_t cs, int64
   if (pos >= npos) return;
   const int64_t r = pos / n_cols, s = pos - r * n_cols;
   const T* xp = x + r * rs + s * cs;
-  constexpr int MAXV = 32;  // c <= 1024
-  float v[MAXV];
+  float v[MAXV];  // c <= 32 MAXV
   float sum = 0.f;
   const int per = (c + 31) / 32;
 #pragma unroll
@@ -114,69 +113,97 @@ struct VecTraits<__nv_bfloat16> {
   }
 };
 
-template <class T, int L>
+// four values at p (a multiple of four from the start), as one access where the start is aligned
+__device__ __forceinline__ void load_params4(const float* p, bool aligned, float* f) {
+  if (aligned) {
+    const float4 q = __ldg(reinterpret_cast<const float4*>(p));
+    f[0] = q.x, f[1] = q.y, f[2] = q.z, f[3] = q.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __ldg(p + e);
+  }
+}
+
+// V vectors per lane, U groups of rows per warp: the loads of U rows are in flight together and they share
+// one read of gamma and beta (1536^2 rows of 128 bf16: 381 us with U = 1 and scalar parameter reads, see
+// the launch for U).
+template <class T, int L, int V, int U>
 __global__ void __launch_bounds__(256) k_layernorm_rows(const T* __restrict__ x, T* __restrict__ y, int64_t rows,
                                                         int c, const float* __restrict__ gamma,
                                                         const float* __restrict__ beta, float eps) {
-  constexpr int E = VecTraits<T>::E;
-  // vectors per lane: L < 32 is chosen only for rows of fewer than 2L vectors; L = 32 up to c = 1024
-  constexpr int MAXV = L < 32 ? 2 : (1024 / E) / 32;
+  constexpr int E = VecTraits<T>::E, R = 32 / L;
   const int lane = threadIdx.x & 31;
   const int sub = lane & (L - 1);
-  const int64_t row = ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (32 / L) + lane / L;
-  const bool live = row < rows;
+  const int64_t row0 = ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (R * U) + lane / L;
   const int nv = c / E;
-  const uint4* xr = reinterpret_cast<const uint4*>(x + (live ? row : 0) * (int64_t)c);
-  uint4 raw[MAXV];
+  uint4 raw[U][V];
 #pragma unroll
-  for (int t = 0; t < MAXV; ++t) {
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int t = 0; t < V; ++t) {
+      const int64_t row = row0 + u * R;
+      const int v = sub + t * L;
+      raw[u][t] = (row < rows && v < nv) ? __ldg(reinterpret_cast<const uint4*>(x + row * (int64_t)c) + v)
+                                         : make_uint4(0, 0, 0, 0);
+    }
+  float gm[V * E], bt[V * E];
+  const bool ga = ((uintptr_t)gamma & 15) == 0, ba = ((uintptr_t)beta & 15) == 0;
+#pragma unroll
+  for (int t = 0; t < V; ++t) {
     const int v = sub + t * L;
-    raw[t] = (live && v < nv) ? __ldg(xr + v) : make_uint4(0, 0, 0, 0);
-  }
-  float sum = 0.f;
 #pragma unroll
-  for (int t = 0; t < MAXV; ++t) {
-    float f[E];
-    VecTraits<T>::unpack(raw[t], f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += f[e];
-  }
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float mean = sum / (float)c;
-  float sq = 0.f;
-#pragma unroll
-  for (int t = 0; t < MAXV; ++t) {
-    if (sub + t * L < nv) {
-      float f[E];
-      VecTraits<T>::unpack(raw[t], f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float d = f[e] - mean;
-        sq += d * d;
-      }
+    for (int e = 0; e < E; e += 4) {
+      if (gamma && v < nv) load_params4(gamma + v * E + e, ga, gm + t * E + e);
+      if (beta && v < nv) load_params4(beta + v * E + e, ba, bt + t * E + e);
     }
   }
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-  const float rstd = rsqrtf(sq / (float)c + eps);
-  if (!live) return;
-  uint4* yr = reinterpret_cast<uint4*>(y + row * (int64_t)c);
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = row0 + u * R;
+    float sum = 0.f;
 #pragma unroll
-  for (int t = 0; t < MAXV; ++t) {
-    const int v = sub + t * L;
-    if (v < nv) {
+    for (int t = 0; t < V; ++t) {
       float f[E];
-      VecTraits<T>::unpack(raw[t], f);
-      const int ch0 = v * E;
+      VecTraits<T>::unpack(raw[u][t], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float o = (f[e] - mean) * rstd;
-        if (gamma) o *= __ldg(gamma + ch0 + e);
-        if (beta) o += __ldg(beta + ch0 + e);
-        f[e] = o;
+      for (int e = 0; e < E; ++e) sum += f[e];
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float mean = sum / (float)c;
+    float sq = 0.f;
+#pragma unroll
+    for (int t = 0; t < V; ++t) {
+      if (sub + t * L < nv) {
+        float f[E];
+        VecTraits<T>::unpack(raw[u][t], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float d = f[e] - mean;
+          sq += d * d;
+        }
       }
-      yr[v] = VecTraits<T>::pack(f);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    const float rstd = rsqrtf(sq / (float)c + eps);
+    if (row >= rows) continue;
+    uint4* yr = reinterpret_cast<uint4*>(y + row * (int64_t)c);
+#pragma unroll
+    for (int t = 0; t < V; ++t) {
+      const int v = sub + t * L;
+      if (v < nv) {
+        float f[E];
+        VecTraits<T>::unpack(raw[u][t], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float o = (f[e] - mean) * rstd;
+          if (gamma) o *= gm[t * E + e];
+          if (beta) o += bt[t * E + e];
+          f[e] = o;
+        }
+        yr[v] = VecTraits<T>::pack(f);
+      }
     }
   }
 }
@@ -574,7 +601,12 @@ static int ln_view(const T* x, int64_t rs, int64_t cs, int64_t n_rows, int64_t n
   if (P == 0) return PF_OK;
   {
     PF_LAUNCH_SCOPE(st, "k_ln_view");
-    k_ln_view<T, TO><<<nblk(P, 8), 256, 0, st>>>(x, rs, cs, n_rows, n_cols, c, g, b, eps, out, ops);
+    if (c <= 128)
+      k_ln_view<T, TO, 4><<<nblk(P, 8), 256, 0, st>>>(x, rs, cs, n_rows, n_cols, c, g, b, eps, out, ops);
+    else if (c <= 512)
+      k_ln_view<T, TO, 16><<<nblk(P, 8), 256, 0, st>>>(x, rs, cs, n_rows, n_cols, c, g, b, eps, out, ops);
+    else
+      k_ln_view<T, TO, 32><<<nblk(P, 8), 256, 0, st>>>(x, rs, cs, n_rows, n_cols, c, g, b, eps, out, ops);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;
@@ -598,30 +630,51 @@ static int gemm(const TA* A, int64_t sAb, int64_t sAm, const TB* B, int64_t sBb,
   return PF_OK;
 }
 
-template <class T, int L>
+template <class T, int L, int V, int U>
 static int ln_rows_launch(const T* x, T* y, int64_t rows, int c, const float* g, const float* b, float eps,
                           cudaStream_t st) {
-  const int64_t rows_per_block = 8 * (32 / L);
+  const int64_t rows_per_block = 8 * (32 / L) * U;
   const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
   if (blocks > 0x7FFFFFFF) return fail(PF_EUNSUPPORTED, "LayerNorm: %lld rows is too many", (long long)rows);
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_layernorm_rows", 2.0 * (double)rows * c * sizeof(T), 'b');
-    k_layernorm_rows<T, L><<<(unsigned)blocks, 256, 0, st>>>(x, y, rows, c, g, b, eps);
+    k_layernorm_rows<T, L, V, U><<<(unsigned)blocks, 256, 0, st>>>(x, y, rows, c, g, b, eps);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;
+}
+
+// Four groups of rows per warp where that still fills the machine (eight blocks on each of 148 SMs).
+template <class T, int L, int V>
+static int ln_rows_u(const T* x, T* y, int64_t rows, int c, const float* g, const float* b, float eps,
+                     cudaStream_t st) {
+  constexpr int U = V <= 2 ? 4 : (V <= 4 ? 2 : 1);
+  if (rows >= (int64_t)8 * (32 / L) * U * 148 * 8) return ln_rows_launch<T, L, V, U>(x, y, rows, c, g, b, eps, st);
+  return ln_rows_launch<T, L, V, 1>(x, y, rows, c, g, b, eps, st);
 }
 
 template <class T>
 static int ln_rows(const T* x, T* y, int64_t rows, int c, const float* g, const float* b, float eps,
                    cudaStream_t st) {
   const int nv = c * (int)sizeof(T) / 16;
-  if (nv >= 32) return ln_rows_launch<T, 32>(x, y, rows, c, g, b, eps, st);
-  if (nv >= 16) return ln_rows_launch<T, 16>(x, y, rows, c, g, b, eps, st);
-  if (nv >= 8) return ln_rows_launch<T, 8>(x, y, rows, c, g, b, eps, st);
-  if (nv >= 4) return ln_rows_launch<T, 4>(x, y, rows, c, g, b, eps, st);
-  if (nv >= 2) return ln_rows_launch<T, 2>(x, y, rows, c, g, b, eps, st);
-  return ln_rows_launch<T, 1>(x, y, rows, c, g, b, eps, st);
+#define PF_LN_ROWS(L, V) return ln_rows_u<T, L, V>(x, y, rows, c, g, b, eps, st)
+  if constexpr (sizeof(T) == 4) {
+    if (nv > 128) PF_LN_ROWS(32, 8);
+  }
+  if (nv > 96) PF_LN_ROWS(32, 4);
+  if (nv > 64) PF_LN_ROWS(32, 3);
+  if (nv > 32) PF_LN_ROWS(32, 2);
+  if (nv == 32) PF_LN_ROWS(32, 1);
+  if (nv > 16) PF_LN_ROWS(16, 2);
+  if (nv == 16) PF_LN_ROWS(16, 1);
+  if (nv > 8) PF_LN_ROWS(8, 2);
+  if (nv == 8) PF_LN_ROWS(8, 1);
+  if (nv > 4) PF_LN_ROWS(4, 2);
+  if (nv == 4) PF_LN_ROWS(4, 1);
+  if (nv == 3) PF_LN_ROWS(2, 2);
+  if (nv == 2) PF_LN_ROWS(2, 1);
+  PF_LN_ROWS(1, 1);
+#undef PF_LN_ROWS
 }
 
 int layernorm(const void* x, void* y, const float* g, const float* b, int64_t rows, int c,

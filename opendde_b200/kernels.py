@@ -8,6 +8,7 @@ bfloat16 -> PF_BF16 (tcgen05 tensor cores where the shape is covered).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Dict, NamedTuple, Optional
@@ -105,6 +106,12 @@ def make_pack(struct_cls, spec: Dict[str, Optional[torch.Tensor]], f32_names, dt
 
 # ------------------------------------------------------------------------------ ops
 
+def _float_param(p: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if p is None or (p.dtype == torch.float32 and p.is_contiguous()):
+        return p  # read in place
+    return p.detach().float().contiguous()
+
+
 def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
               eps: float = 1e-5) -> torch.Tensor:
     require_cuda(x)
@@ -112,8 +119,7 @@ def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[to
     x = x.contiguous()
     y = torch.empty_like(x)
     c = x.shape[-1]
-    w = None if weight is None else weight.detach().float().contiguous()
-    b = None if bias is None else bias.detach().float().contiguous()
+    w, b = _float_param(weight), _float_param(bias)
     check(_abi.load().pf_layernorm_fwd(x.data_ptr(), y.data_ptr(), _ptr(w), _ptr(b),
                                        x.numel() // c, c, eps, code, stream_ptr()))
     return y
@@ -413,16 +419,25 @@ def diffusion_pair_cond(pack: WeightPack, z_trunk: torch.Tensor, ids, z_out: tor
 # Each call launches on the current stream of its tensors' device, whichever device is current, and
 # can be captured into a CUDA graph (its workspace then lies in the graph's own pool).
 
+_HERE = contextlib.nullcontext()
+
+
 def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
     require_cuda(*ts)
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"tensors lie on different devices: {sorted(map(str, devices))}")
-    return devices.pop()
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors lie on different devices: {dev} and {t.device}")
+    return dev
 
 
-def _float_param(p: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if p is None else p.detach().float().contiguous()
+def _on(dev: torch.device):
+    """A context in which ``dev`` is the current device."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-5,
@@ -437,16 +452,16 @@ def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, weight: Optional[torch.Tens
     c = x.shape[-1]
     if weight is not None and tuple(weight.shape) != (c,):
         raise ValueError(f"weight {tuple(weight.shape)} does not match {c} channels")
-    with torch.cuda.device(dev):
-        x, dy, w = x.detach().contiguous(), dy.detach().contiguous(), _float_param(weight)
-        dx = torch.empty_like(x) if need[0] else None
+    lib = _abi.load()
+    with _on(dev):
+        x, dy, w = x.contiguous(), dy.contiguous(), _float_param(weight)
+        dx = torch.empty_like(x, requires_grad=False) if need[0] else None
         dw = torch.empty(c, device=dev, dtype=torch.float32) if need[1] else None
         db = torch.empty(c, device=dev, dtype=torch.float32) if need[2] else None
         rows = x.numel() // c
-        nbytes = _abi.workspace_bytes("pf_layernorm_bwd_workspace_size", rows, c, code)
-        ws = workspace(nbytes, dev)
-        check(_abi.load().pf_layernorm_bwd(x.data_ptr(), dy.data_ptr(), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db), rows, c,
-                                           eps, code, ws.data_ptr(), ws.numel(), stream_ptr()))
+        ws = workspace(_abi.workspace_bytes("pf_layernorm_bwd_workspace_size", rows, c, code), dev)
+        check(lib.pf_layernorm_bwd(x.data_ptr(), dy.data_ptr(), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db), rows, c, eps,
+                                   code, ws.data_ptr(), ws.numel(), _stream(dev)))
     return dx, dw, db
 
 
@@ -457,30 +472,35 @@ class AttentionSaved(NamedTuple):
     o_lo: Optional[torch.Tensor]
 
 
-def _head_view(t: Optional[torch.Tensor]) -> _abi.HeadView:
-    if t is None:
-        return _abi.HeadView(None, 0, 0, 0)
-    return _abi.HeadView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+_NO_VIEW = (0, 0, 0, 0)
 
 
-def _bias_view(t: Optional[torch.Tensor]) -> _abi.BiasView:
+def _head_view(t: Optional[torch.Tensor]) -> tuple:
+    """pf_head_view of a [B, N, H, d] tensor."""
+    return _NO_VIEW if t is None else (t.data_ptr(), *t.stride()[:3])
+
+
+def _bias_view(t: Optional[torch.Tensor]) -> tuple:
+    """pf_bias_view of a [1 or B, H, n_q, n_k] tensor."""
     if t is None:
-        return _abi.BiasView(None, 0, 0, 0)
-    return _abi.BiasView(t.data_ptr(), 0 if t.shape[0] == 1 else t.stride(0), t.stride(1), t.stride(2))
+        return _NO_VIEW
+    bs, hs, rs, _ = t.stride()
+    return t.data_ptr(), bs if t.shape[0] > 1 else 0, hs, rs
 
 
 def _batched_heads(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dim() not in (3, 4):
+    if t.dim() == 3:
+        t = t[None]
+    elif t.dim() != 4:
         raise ValueError(f"{name} must be [B, N, H, d] or [N, H, d], got shape {tuple(t.shape)}")
-    t = t.detach()
-    t = t[None] if t.dim() == 3 else t
     if t.stride(3) != 1 and t.shape[3] > 1:
         raise ValueError(f"{name} must have contiguous channels")
     return t
 
 
 def _attention_args(q, k, v, bias, mask, scale):
-    """Checked [B, N, H, d] views, the [1 or B, H, n_q, n_k] bias, the float32 mask and the shape."""
+    """Checked [B, N, H, d] views, the [1 or B, H, n_q, n_k] bias, the float32 mask, and the call's fields
+    up to the output."""
     dev = _same_device(q, k, v, bias, mask)
     code = dtype_code(q)
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -489,36 +509,34 @@ def _attention_args(q, k, v, bias, mask, scale):
         raise ValueError("q, k and v must all be batched or all be unbatched")
     q, k, v = _batched_heads(q, "q"), _batched_heads(k, "k"), _batched_heads(v, "v")
     b, n_q, heads, d = q.shape
-    n_k, kv_heads = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+    kb, n_k, kv_heads, kd = k.shape
+    if k.shape != v.shape or kb != b or kd != d:
         raise ValueError(f"attention shapes disagree: q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
     if bias is not None:
-        if bias.dim() not in (3, 4):
+        if bias.dim() == 3:
+            bias = bias[None]
+        elif bias.dim() != 4:
             raise ValueError(f"bias must be [H, n_q, n_k] or [B, H, n_q, n_k], got shape {tuple(bias.shape)}")
-        bias = bias.detach()
-        bias = bias[None] if bias.dim() == 3 else bias
-        if bias.shape[0] not in (1, b) or tuple(bias.shape[1:]) != (heads, n_q, n_k):
+        if bias.shape[0] not in (1, b) or bias.shape[1:] != (heads, n_q, n_k):
             raise ValueError(f"bias {tuple(bias.shape)} is not [1 or {b}, {heads}, {n_q}, {n_k}]")
         if bias.stride(3) != 1 and n_k > 1:
             raise ValueError("bias must have contiguous keys")
         if bias.shape[0] > 1 and bias.stride(0) == 0:
             bias = bias[:1]
-    mv = _abi.MaskView(None, 0, 0)
+    mask_view = (0, 0, 0)
     if mask is not None:
-        if tuple(mask.shape) not in ((n_k,), (b, n_k)):
+        if mask.shape != (b, n_k) and mask.shape != (n_k,):
             raise ValueError(f"mask {tuple(mask.shape)} is not [{n_k}] or [{b}, {n_k}]")
-        mask = mask.detach()
         if mask.dtype != torch.float32:
             if mask.dtype not in (torch.bool, torch.bfloat16, torch.float16, torch.uint8, torch.int32, torch.int64):
                 raise TypeError(f"mask must be boolean or float32 like the pair masks, got {mask.dtype}")
             mask = (mask != 0).to(torch.float32)
-        mask = mask[None].expand(b, n_k) if mask.dim() == 1 else mask
-        mv = mask_view(mask)
+        mask_view = (mask.data_ptr(), mask.stride(0) if mask.dim() == 2 else 0, mask.stride(-1))
     if scale is None:
         scale = 1.0 / math.sqrt(d) if d else 1.0
-    shape = _abi.AttentionShape(b, n_q, n_k, heads, kv_heads, d, float(scale), code,
-                                _abi.PF_F32 if bias is None else dtype_code(bias))
-    return dev, q, k, v, bias, mask, mv, shape
+    shape = (b, n_q, n_k, heads, kv_heads, d, scale, code, _abi.PF_F32 if bias is None else dtype_code(bias))
+    fields = (*shape, *_head_view(q), *_head_view(k), *_head_view(v), *_bias_view(bias), *mask_view)
+    return dev, q, k, v, bias, mask, shape, fields
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -531,18 +549,19 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[
     [n_k]: non-zero where a key is visible; a query that sees none gets 0. ``scale`` defaults to
     1 / sqrt(d). Returns the contiguous output in q's shape; with ``save`` also what
     :func:`attention_bwd` needs."""
-    dev, q4, k4, v4, bias, mask, mv, shape = _attention_args(q, k, v, bias, mask, scale)
-    with torch.cuda.device(dev):
-        o = torch.empty(q4.shape, device=dev, dtype=q.dtype)
+    dev, q4, k4, v4, bias, mask, shape, fields = _attention_args(q, k, v, bias, mask, scale)
+    b, n_q, _, heads = shape[:4]
+    lib = _abi.load()
+    with _on(dev):
+        o = torch.empty(q.shape, device=dev, dtype=q.dtype)
         stats = o_lo = None
         if save:
-            stats = torch.empty((2, shape.batch, shape.heads, shape.n_q), device=dev, dtype=torch.float32)
-            if shape.dtype == _abi.PF_BF16:
+            stats = torch.empty((2, b, heads, n_q), device=dev, dtype=torch.float32)
+            if q.dtype == torch.bfloat16:
                 o_lo = torch.empty(q4.shape, device=dev, dtype=torch.int16)
-        check(_abi.load().pf_attention_fwd(ctypes.byref(shape), _head_view(q4), _head_view(k4), _head_view(v4),
-                                           _bias_view(bias), mv, _head_view(o), _ptr(stats), _ptr(o_lo),
-                                           stream_ptr()))
-    o = o.view(q.shape)
+        call = _abi.ATTENTION_CALL.pack(*fields, *_head_view(o if o.dim() == 4 else o[None]), _ptr(stats) or 0,
+                                        _ptr(o_lo) or 0, *_NO_VIEW * 5)
+        check(lib.pf_attention_fwd(call, _stream(dev)))
     return (o, AttentionSaved(stats, o_lo)) if save else o
 
 
@@ -553,45 +572,45 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     the other arguments are the forward's. dbias has bias's shape and dtype (summed over the batch where
     bias is shared by it) and is None without one. ``need`` drops the ones not wanted (None in their
     place)."""
-    n_batch = None if bias is None else (1 if bias.dim() == 3 else bias.shape[0])
-    dbias_shape = None if bias is None else bias.shape
-    dev, q4, k4, v4, bias, mask, mv, shape = _attention_args(q, k, v, bias, mask, scale)
-    if _same_device(do, o, saved.stats, q) != dev or (saved.o_lo is not None and saved.o_lo.device != dev):
-        raise ValueError("do, o and the saved tensors must lie on q's device")
+    given = bias
+    dev, q4, k4, v4, bias, mask, shape, fields = _attention_args(q, k, v, bias, mask, scale)
+    stats, o_lo = saved
+    _same_device(q, do, o, stats, o_lo)
     for t, name in ((do, "do"), (o, "o")):
         if t.shape != q.shape or t.dtype != q.dtype:
             raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} is not like q {tuple(q.shape)} {q.dtype}")
-    if (tuple(saved.stats.shape) != (2, shape.batch, shape.heads, shape.n_q) or not saved.stats.is_contiguous()
-            or saved.stats.dtype != torch.float32):
+    b, n_q, _, heads = shape[:4]
+    if stats.shape != (2, b, heads, n_q) or not stats.is_contiguous() or stats.dtype != torch.float32:
         raise ValueError("saved does not come from a forward of these shapes")
-    if shape.dtype == _abi.PF_BF16 and (saved.o_lo is None or saved.o_lo.shape != q4.shape
-                                        or saved.o_lo.dtype != torch.int16 or not saved.o_lo.is_contiguous()):
+    if q.dtype == torch.bfloat16 and (o_lo is None or o_lo.shape != q4.shape or o_lo.dtype != torch.int16
+                                      or not o_lo.is_contiguous()):
         raise ValueError("saved does not come from a bfloat16 forward of these shapes")
     do4, o4 = _batched_heads(do, "do"), _batched_heads(o, "o")
-    with torch.cuda.device(dev):
+    lib = _abi.load()
+    with _on(dev):
         dq = torch.empty(q4.shape, device=dev, dtype=q.dtype) if need[0] else None
         dk = dv = dbias = dbias_v = None
         if need[1] or need[2]:
             dk = torch.empty(k4.shape, device=dev, dtype=q.dtype)
             dv = torch.empty(v4.shape, device=dev, dtype=q.dtype)
         if bias is not None and need[3]:
-            if shape.batch == 0:
-                dbias = torch.zeros(dbias_shape, device=dev, dtype=bias.dtype)
-            elif bias.shape[0] == n_batch:
-                dbias = torch.empty(bias.shape, device=dev, dtype=bias.dtype)
-                dbias_v = dbias
-            else:  # one plane expanded over the batch: every entry has a gradient of its own
-                dbias = torch.empty((n_batch,) + tuple(bias.shape[1:]), device=dev, dtype=bias.dtype)
-                dbias_v = dbias
-                bias = bias.expand(dbias.shape).contiguous()
-        nbytes = _abi.workspace_bytes("pf_attention_bwd_workspace_size", ctypes.byref(shape))
-        ws = workspace(nbytes, dev)
-        check(_abi.load().pf_attention_bwd(
-            ctypes.byref(shape), _head_view(q4), _head_view(k4), _head_view(v4), _bias_view(bias), mv, _head_view(o4),
-            saved.stats.data_ptr(), _ptr(saved.o_lo), _head_view(do4), _head_view(dq), _head_view(dk),
-            _head_view(dv), _bias_view(dbias_v), ws.data_ptr(), ws.numel(), stream_ptr()))
-    return (None if dq is None else dq.view(q.shape), dk.view(k.shape) if need[1] else None,
-            dv.view(v.shape) if need[2] else None, None if dbias is None else dbias.view(dbias_shape))
+            if b == 0:
+                dbias = torch.zeros(given.shape, device=dev, dtype=bias.dtype)
+            else:
+                if given.dim() == 4 and given.shape[0] != bias.shape[0]:
+                    # one plane expanded over the batch: every entry has a gradient of its own
+                    bias = given.contiguous()
+                    fields = _attention_args(q, k, v, bias, mask, scale)[-1]
+                dbias = dbias_v = torch.empty(bias.shape, device=dev, dtype=bias.dtype)
+        ws = workspace(_abi.workspace_bytes("pf_attention_bwd_workspace_size", _abi.ATTENTION_SHAPE.pack(*shape)), dev)
+        call = _abi.ATTENTION_CALL.pack(*fields, *_head_view(o4), stats.data_ptr(), _ptr(o_lo) or 0, *_head_view(do4),
+                                        *_head_view(dq), *_head_view(dk), *_head_view(dv), *_bias_view(dbias_v))
+        check(lib.pf_attention_bwd(call, ws.data_ptr(), ws.numel(), _stream(dev)))
+    if q.dim() == 3:
+        dq, dk, dv = (None if t is None else t[0] for t in (dq, dk, dv))
+    if dbias is not None and given.dim() == 3 and dbias.dim() == 4:
+        dbias = dbias[0]
+    return dq, dk if need[1] else None, dv if need[2] else None, dbias
 
 
 def _check_ids(ids, dev) -> int:
@@ -621,12 +640,11 @@ def relpos_bias(weight: torch.Tensor, ids, out: torch.Tensor, row0: int, col0: i
     _plane(out, "out")
     if tuple(weight.shape) != (out.shape[0], 4 * r_max + 2 * s_max + 7):
         raise ValueError(f"weight {tuple(weight.shape)} is not [{out.shape[0]}, {4 * r_max + 2 * s_max + 7}]")
-    w = weight.detach().contiguous()
-    with torch.cuda.device(dev):
-        check(_abi.load().pf_relpos_bias_fwd(w.data_ptr(), dtype_code(w), _abi.TokenIds(*[t.data_ptr() for t in ids]),
-                                             out.data_ptr(), out.stride(0), out.stride(1), code, n_token, row0,
-                                             out.shape[1], col0, out.shape[2], out.shape[0], r_max, s_max,
-                                             stream_ptr()))
+    w, lib = weight.contiguous(), _abi.load()
+    with _on(dev):
+        check(lib.pf_relpos_bias_fwd(w.data_ptr(), dtype_code(w), _abi.TokenIds(*[t.data_ptr() for t in ids]),
+                                     out.data_ptr(), out.stride(0), out.stride(1), code, n_token, row0, out.shape[1],
+                                     col0, out.shape[2], out.shape[0], r_max, s_max, _stream(dev)))
 
 
 def relpos_bias_bwd(dout: torch.Tensor, ids, row0: int, col0: int, r_max: int, s_max: int) -> torch.Tensor:
@@ -636,12 +654,12 @@ def relpos_bias_bwd(dout: torch.Tensor, ids, row0: int, col0: int, r_max: int, s
     code, n_token = dtype_code(dout), _check_ids(ids, dev)
     _plane(dout, "dout")
     heads, rows, cols = dout.shape
-    with torch.cuda.device(dev):
+    lib = _abi.load()
+    with _on(dev):
         nbytes = _abi.workspace_bytes("pf_relpos_bias_bwd_workspace_size", rows, cols, heads, r_max, s_max)
         ws = workspace(nbytes, dev)
         dw = torch.empty((heads, 4 * r_max + 2 * s_max + 7), device=dev, dtype=torch.float32)
-        check(_abi.load().pf_relpos_bias_bwd(dout.data_ptr(), dout.stride(0), dout.stride(1), code,
-                                             _abi.TokenIds(*[t.data_ptr() for t in ids]), dw.data_ptr(), n_token,
-                                             row0, rows, col0, cols, heads, r_max, s_max, ws.data_ptr(), ws.numel(),
-                                             stream_ptr()))
+        check(lib.pf_relpos_bias_bwd(dout.data_ptr(), dout.stride(0), dout.stride(1), code,
+                                     _abi.TokenIds(*[t.data_ptr() for t in ids]), dw.data_ptr(), n_token, row0, rows,
+                                     col0, cols, heads, r_max, s_max, ws.data_ptr(), ws.numel(), _stream(dev)))
     return dw

@@ -19,7 +19,9 @@ NOB, NOM = _abi.BiasView(None, 0, 0, 0), _abi.MaskView(None, 0, 0)
 
 
 def _fwd(shape, q=HV, k=HV, v=HV, bias=NOB, mask=NOM, o=HV):
-    return _abi.load().pf_attention_fwd(ctypes.byref(shape) if shape else None, q, k, v, bias, mask, o, None, None, None)
+    none = _abi.HeadView(None, 0, 0, 0)
+    call = _abi.AttentionCall(shape, q, k, v, bias, mask, o, None, None, none, none, none, none, NOB) if shape else None
+    return _abi.load().pf_attention_fwd(ctypes.byref(call) if shape else None, None)
 
 
 @pytest.mark.parametrize("kw,status", [
@@ -49,8 +51,8 @@ def test_attention_views_refused():
 
 def test_attention_backward_refused():
     def bwd(shape=None, stats=256, o_lo=256, dq=HV, dk=HV, dv=HV, bias=NOB, dbias=NOB, ws=None, nbytes=0):
-        return _abi.load().pf_attention_bwd(ctypes.byref(shape or _shape()), HV, HV, HV, bias, NOM, HV, stats, o_lo, HV,
-                                            dq, dk, dv, dbias, ws, nbytes, None)
+        call = _abi.AttentionCall(shape or _shape(), HV, HV, HV, bias, NOM, HV, stats, o_lo, HV, dq, dk, dv, dbias)
+        return _abi.load().pf_attention_bwd(ctypes.byref(call), ws, nbytes, None)
     null = _abi.HeadView(None, 0, 0, 0)
     plane = _abi.BiasView(256, 80, 20, 5)
     assert bwd(dk=null) == _abi.PF_EINVAL_ARG               # dk and dv come together
