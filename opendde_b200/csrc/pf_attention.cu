@@ -41,15 +41,31 @@ int sum_planes(const Args& a, const float* part, int parts, cudaStream_t st) {
   return PF_OK;
 }
 
-// Parts of the batch for the gradient of a shared bias: about three blocks per SM, and at least four
-// entries each (a part costs a plane written and read).
-int dbias_parts(const pf_attention_shape& s) {
+// How the gradient of a shared bias is computed: with dq in one pass (one block of 16 warps per SM), or by
+// itself (about three blocks per SM), in `parts` parts of the batch of at least four entries each (a part
+// costs a plane written and read).
+struct SharedPlan {
+  bool plane;
+  int parts;
+};
+SharedPlan shared_plan(const pf_attention_shape& s) {
+  SharedPlan p{false, 1};
+  if (s.n_q == 0 || s.n_k == 0) return p;
+  if (s.dtype == PF_BF16 && attn::dq_plane_fits(s.n_q, s.n_k, s.head_dim)) {
+    const int64_t blocks = (s.n_q + 63) / 64 * s.heads;
+    int64_t n = blocks >= 148 ? 1 : 148 / blocks;
+    if (n > s.batch / 4) n = s.batch / 4;
+    if (n < 1) n = 1;
+    // where the last wave of blocks leaves most of the machine idle, the two passes are faster
+    const int64_t waves = (blocks * n + 147) / 148;
+    if (blocks * n * 100 >= waves * 148 * 60) return SharedPlan{true, (int)n};
+  }
   const int64_t rows = s.dtype == PF_BF16 ? 128 : 64, keys = s.dtype == PF_BF16 ? 64 : 32;
   const int64_t blocks = ((s.n_q + rows - 1) / rows) * ((s.n_k + keys - 1) / keys) * s.heads;
-  if (blocks == 0) return 1;
-  int64_t p = (3 * 148 + blocks - 1) / blocks;
-  if (p > s.batch / 4) p = s.batch / 4;
-  return p < 1 ? 1 : (int)p;
+  int64_t n = (3 * 148 + blocks - 1) / blocks;
+  if (n > s.batch / 4) n = s.batch / 4;
+  p.parts = n < 1 ? 1 : (int)n;
+  return p;
 }
 
 Heads heads(const pf_head_view& v) { return Heads{v.ptr, v.batch_stride, v.seq_stride, v.head_stride}; }
@@ -119,7 +135,7 @@ size_t attention_bwd_ws_bytes(const pf_attention_shape& s) {
   Arena ar(nullptr, 0);
   ar.take<float>((size_t)4 * s.batch * s.heads * s.n_q);
   if (s.batch > 1) {
-    const int parts = dbias_parts(s);
+    const int parts = shared_plan(s).parts;
     if (parts > 1) ar.take<float>((size_t)parts * s.heads * s.n_q * s.n_k);
   }
   return ar.used;
@@ -157,23 +173,26 @@ int attention_bwd(const pf_attention_call& c, void* ws, size_t ws_bytes, cudaStr
     a.dv_hs = dv.head_stride;
     PF_TRY(launch(s.dtype, attn::kDkv, a, 4 * pair, st));
   }
-  if (dq.ptr || (dbias.ptr && !shared)) {
-    a.dq = dq.ptr;
-    a.o_bs = dq.batch_stride;
-    a.o_ns = dq.seq_stride;
-    a.o_hs = dq.head_stride;
+  a.dq = dq.ptr;
+  a.o_bs = dq.batch_stride;
+  a.o_ns = dq.seq_stride;
+  a.o_hs = dq.head_stride;
+  const bool sum = shared && s.n_q > 0 && s.n_k > 0;
+  const SharedPlan plan = sum ? shared_plan(s) : SharedPlan{false, 1};
+  if ((dq.ptr || (dbias.ptr && !shared)) && !plan.plane) {
     a.dbias = shared ? nullptr : dbias.ptr;
     PF_TRY(launch(s.dtype, attn::kDq, a, 3 * pair, st));
   }
-  if (shared && s.n_q > 0 && s.n_k > 0) {
-    a.dbias = dbias.ptr;
-    const int parts = dbias_parts(s);
-    float* part = parts > 1 ? ar.take<float>((size_t)parts * s.heads * s.n_q * s.n_k) : nullptr;
-    if (!ar.ok()) return fail(PF_EWORKSPACE, "attention backward: workspace too small");
-    PF_TRY(s.dtype == PF_BF16 ? attn::dbias_bf16(a, part, parts, 2 * pair, st)
-                              : attn::dbias_f32(a, part, parts, 2 * pair, st));
-    if (parts > 1) return sum_planes(a, part, parts, st);
-  }
+  if (!sum) return PF_OK;
+  a.dbias = dbias.ptr;
+  float* part = plan.parts > 1 ? ar.take<float>((size_t)plan.parts * s.heads * s.n_q * s.n_k) : nullptr;
+  if (!ar.ok()) return fail(PF_EWORKSPACE, "attention backward: workspace too small");
+  if (plan.plane)
+    PF_TRY(attn::dq_plane_bf16(a, part, plan.parts, 3 * pair, st));
+  else
+    PF_TRY(s.dtype == PF_BF16 ? attn::dbias_bf16(a, part, plan.parts, 2 * pair, st)
+                              : attn::dbias_f32(a, part, plan.parts, 2 * pair, st));
+  if (plan.parts > 1) return sum_planes(a, part, plan.parts, st);
   return PF_OK;
 }
 

@@ -19,6 +19,7 @@
 
 #include "pf_attention.cuh"
 #include "pf_f32x2.cuh"
+#include "pf_sm100.cuh"
 
 namespace pf {
 namespace train {
@@ -1117,6 +1118,315 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
     }
 }
 
+// ---------------------------------------------------------------- dq and a shared dbias in one pass
+
+// The gradient of a bias that the batch shares is a sum over the batch, dq a sum over the keys: one pass
+// can do both if a block keeps its rows of the [n_q, n_k] plane while it walks over the batch. A block of
+// 16 warps takes 64 rows by all keys of one head and a part of the batch: warp w rows 16 (w % 4).. and
+// the w / 4-th quarter of the keys. Its share of the plane, 16 rows by n_k / 4 keys in fp32, lies in tensor
+// memory as thread-private storage (128 words per thread: up to 1024 keys); a group of 16 keys costs one
+// eight-word load, four packed adds and one store. All keys and values of a batch entry are in shared
+// memory, double-buffered (up to 832 keys of 32 channels), so warps run freely between two entries; the
+// quarters' dq are added through shared memory. Next to dq and dbias apart this saves two of five products
+// and one of two exponentials per score (768 tokens: 4.5 ms apart).
+constexpr int kPlaneThreads = 512;
+constexpr int kPlaneKeys = 832;
+
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
+// the wait takes the loaded registers along, so that no use of them moves above it
+__device__ __forceinline__ void tmem_wait8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+struct PlaneSmem {  // byte offsets
+  int kv, q, cst, vis, end;
+  __host__ __device__ explicit PlaneSmem(int nkp) {
+    const int one = 2 * nkp * 64, red = 4 * 64 * 36 * 4;  // keys and values; the quarters' dq
+    kv = one > red ? one : red;
+    q = 2 * kv;
+    cst = q + 2 * 2 * 64 * 64;
+    vis = cst + 2 * 64 * 16;
+    end = vis + 3 * 32 * 4 + 16;
+  }
+};
+
+template <int BT>
+__global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* part, int parts, int G, int tcols) {
+  constexpr int DP = 32, KS = 2, NB = 4;
+  using S = Tile<DP>;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const int nkp = (int)((a.nk + 15) / 16) * 16;
+  const PlaneSmem L(nkp);
+  const uint32_t s0 = smem_addr(raw);
+  uint32_t* vis = (uint32_t*)(raw + L.vis);  // [3][32] words of visible keys
+  uint32_t* tptr = vis + 96;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rg = warp & 3, sl = warp >> 2;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV);
+  const int pt = id / a.H;
+  const int64_t b0 = a.B * pt / parts, b1 = a.B * (pt + 1) / parts;
+  const int64_t i0 = (int64_t)tile * 64, w0 = i0 + rg * 16;
+  const int words = (nkp + 31) / 32;
+
+  if (warp == 0) {
+    sm100::tmem_alloc(smem_addr(tptr), tcols);
+    sm100::tmem_relinquish();
+  }
+  auto see = [&](int64_t b) {  // the words of entry b
+    for (int w = warp; w < words; w += 16) {
+      const int64_t j = w * 32 + lane;
+      const unsigned m = __ballot_sync(0xffffffffu, j < a.nk && (!a.mask || a.mask[b * a.m_bs + j * a.m_ks] != 0.f));
+      if (lane == 0) vis[(int)(b % 3) * 32 + w] = m;
+    }
+  };
+  auto issue = [&](int64_t b) {
+    const uint32_t* v = vis + (int)(b % 3) * 32;
+    const uint32_t sk = s0 + (int)(b & 1) * L.kv, sv = sk + nkp * S::RB, sq = s0 + L.q + (int)(b & 1) * 8192,
+                   sg = sq + 4096;
+    const bf16 *pk = head_base(a.k, b, kh), *pv = head_base(a.v, b, kh), *pq = head_base(a.q, b, h),
+               *pg = head_base(a.g, b, h);
+    auto rows = [&](uint32_t sm, const bf16* p, int64_t ns, int vec, int64_t r0, int n, int64_t end, bool masked) {
+      if (vec) {
+        for (int i = threadIdx.x; i < n * 4; i += kPlaneThreads) {
+          const int r = i >> 2, c = i & 3;
+          const bool ok = r0 + r < end && c * 8 < a.d && (!masked || ((v[r >> 5] >> (r & 31)) & 1));
+          cp_async16(sm + S::off(r, c), ok ? p + (r0 + r) * ns + c * 8 : p, ok);
+        }
+      } else {
+        for (int i = threadIdx.x; i < n * DP; i += kPlaneThreads) {
+          const int r = i / DP, c = i % DP;
+          const bool ok = r0 + r < end && c < a.d && (!masked || ((v[r >> 5] >> (r & 31)) & 1));
+          const bf16 x = ok ? p[(r0 + r) * ns + c] : from_f<bf16>(0.f);
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(sm + S::off(r, c >> 3) + (c & 7) * 2),
+                       "h"(*reinterpret_cast<const unsigned short*>(&x))
+                       : "memory");
+        }
+      }
+    };
+    rows(sk, pk, a.k.ns, a.vec_k, 0, nkp, a.nk, true);
+    rows(sv, pv, a.v.ns, a.vec_v, 0, nkp, a.nk, true);
+    rows(sq, pq, a.q.ns, a.vec_q, i0, 64, a.nq, false);
+    rows(sg, pg, a.g.ns, a.vec_g, i0, 64, a.nq, false);
+    if (threadIdx.x < 64) {
+      const int64_t i = i0 + threadIdx.x;
+      const float4* pr = (const float4*)a.rows + (b * a.H + h) * a.nq;
+      cp_async16(s0 + L.cst + (int)(b & 1) * 1024 + threadIdx.x * 16, i < a.nq ? pr + i : pr, i < a.nq);
+    }
+    cp_commit();
+  };
+  if (b0 < b1) see(b0);
+  if (b0 + 1 < b1) see(b0 + 1);
+  const char* brow[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int64_t i = w0 + r * 8 + g;
+    brow[r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1);
+  }
+  const int q0 = sl * G;  // the warp's groups: q0 .. q0 + G - 1
+  Bias4<BT> ring[2][2];
+  auto fetch_bias = [&](int slot, int q) {
+    const int64_t j0 = (int64_t)(q0 + q) * 16;
+    if (j0 >= a.nk) return;
+    const bool fast = a.bias_vec && j0 + 16 <= a.nk;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][r], brow[r], j0 + 4 * t, a.nk, fast);
+  };
+  fetch_bias(0, 0);
+  fetch_bias(1, 1);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tbase = *tptr;
+  const uint32_t tm0 = tbase + ((uint32_t)(rg * 32) << 16) + q0 * 8;
+  {
+    const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int q = 0; q < G; ++q) tmem_st8(tm0 + q * 8, zero);
+    sm100::tmem_st_wait();
+  }
+  if (b0 < b1) issue(b0);
+  const F2 scale(a.scale);
+  for (int64_t b = b0; b < b1; ++b) {
+    cp_wait<0>();
+    __syncthreads();
+    if (b + 1 < b1) issue(b + 1);
+    if (b + 2 < b1) see(b + 2);
+    const uint32_t* v = vis + (int)(b % 3) * 32;
+    const uint32_t sk = s0 + (int)(b & 1) * L.kv, sv = sk + nkp * S::RB, sq = s0 + L.q + (int)(b & 1) * 8192,
+                   sg = sq + 4096;
+    const float4* cst = (const float4*)(raw + L.cst + (int)(b & 1) * 1024);
+    uint32_t fq[KS][4], fg[KS][4];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      ldsm4(fq[k], la.at(sq, rg, k));
+      ldsm4(fg[k], la.at(sg, rg, k));
+    }
+    F2 nmx[2], lg[2], nd[2];
+    bool peaked = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float4 c = cst[rg * 16 + r * 8 + g];
+      nmx[r] = F2(-c.x), lg[r] = F2(c.y), nd[r] = F2(c.w);
+      peaked |= c.z != 0.f;
+    }
+    peaked = __any_sync(0xffffffffu, peaked);
+    float acc[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll 1
+    for (int qq = 0; qq < G; qq += 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int q = qq + u, qa = q0 + q;  // group of the warp, of the row
+        const int nextq = q + 2 < G ? q + 2 : q + 2 - G;  // the next entry starts over with the same bias
+        const uint32_t bits = qa * 16 < nkp ? (v[qa >> 1] >> ((qa & 1) * 16)) & 0xffffu : 0;
+        if (bits == 0 || w0 >= a.nq) {
+          fetch_bias(u, nextq);
+          continue;
+        }
+        uint32_t tm[8];
+        tmem_ld8(tm0 + q * 8, tm);
+        float x[2][4], y[2][4];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t r[4], w[4];
+          ldsm4(r, lb.at(sk, qa, k));
+          ldsm4(w, lb.at(sv, qa, k));
+          if (k == 0) {
+            mma0(x[0], fq[k], r[0], r[1]);
+            mma0(x[1], fq[k], r[2], r[3]);
+            mma0(y[0], fg[k], w[0], w[1]);
+            mma0(y[1], fg[k], w[2], w[3]);
+          } else {
+            mma(x[0], fq[k], r[0], r[1]);
+            mma(x[1], fq[k], r[2], r[3]);
+            mma(y[0], fg[k], w[0], w[1]);
+            mma(y[1], fg[k], w[2], w[3]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, ring[u][r], n);
+        fetch_bias(u, nextq);
+        if (bits != 0xffffu) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!((bits >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const F2 p = prob2(&x[n][2 * r], nmx[r], lg[r]);
+            p.get(x[n][2 * r], x[n][2 * r + 1]);
+            mul2(p, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(y[n][2 * r], y[n][2 * r + 1]);
+          }
+        if (peaked) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (x[n][e] == 1.f) y[n][e] = 0.f;
+        }
+        uint32_t da[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) da[i] = pack_bf16(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+        for (int c = 0; c < NB / 2; ++c) {
+          uint32_t f[4];
+          ldsm4_t(f, lt.at(sk, qa, c));
+          mma(acc[2 * c], da, f[0], f[1]);
+          mma(acc[2 * c + 1], da, f[2], f[3]);
+        }
+        tmem_wait8(tm);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float s, s1;
+          add2(F2(__uint_as_float(tm[2 * i]), __uint_as_float(tm[2 * i + 1])),
+               F2(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1]))
+              .get(s, s1);
+          tm[2 * i] = __float_as_uint(s), tm[2 * i + 1] = __float_as_uint(s1);
+        }
+        tmem_st8(tm0 + q * 8, tm);
+      }
+    }
+    sm100::tmem_st_wait();
+    if (a.dq) {
+      __syncthreads();  // entry b's keys and values are done with
+      float* red = (float*)(raw + (int)(b & 1) * L.kv);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          *reinterpret_cast<float2*>(red + (sl * 64 + rg * 16 + r * 8 + g) * 36 + n * 8 + 2 * t) =
+              make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+      __syncthreads();
+      const int row = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 4;
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const float4 x = *reinterpret_cast<const float4*>(red + (s * 64 + row) * 36 + c0);
+        o[0] += x.x, o[1] += x.y, o[2] += x.z, o[3] += x.w;
+      }
+      if (i0 + row < a.nq) {
+        bf16* p = (bf16*)a.dq + b * a.o_bs + (int64_t)h * a.o_hs + (i0 + row) * a.o_ns;
+        const bool vec = pair_ok(a.dq, a.o_bs, a.o_ns, a.o_hs, a.d);
+        store_pair(p, c0, a.d, vec, o[0] * a.scale, o[1] * a.scale);
+        store_pair(p, c0 + 2, a.d, vec, o[2] * a.scale, o[3] * a.scale);
+      }
+    }
+  }
+  cp_commit();
+  cp_wait<0>();
+  // the plane: as k_dbias writes it
+  for (int q = 0; q < G; ++q) {
+    const int64_t j = (int64_t)(q0 + q) * 16 + 4 * t;
+    uint32_t tm[8];
+    __syncwarp();
+    tmem_ld8(tm0 + q * 8, tm);
+    tmem_wait8(tm);
+    if ((int64_t)(q0 + q) * 16 >= a.nk) continue;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + r * 8 + g;
+      if (i >= a.nq) continue;
+      const float v0 = __uint_as_float(tm[2 * r]), v1 = __uint_as_float(tm[2 * r + 1]),
+                  v2 = __uint_as_float(tm[4 + 2 * r]), v3 = __uint_as_float(tm[5 + 2 * r]);
+      const bool whole = (int64_t)(q0 + q) * 16 + 16 <= a.nk;
+      if (parts == 1)
+        store_bias4<BT>(a, (char*)a.dbias + ((int64_t)h * a.db_hs + i * a.db_rs) * (BT == 2 ? 4 : 2), j,
+                        a.db_vec && whole, v0, v1, v2, v3);
+      else
+        store_bias4<2>(a, (char*)(part + (((int64_t)pt * a.H + h) * a.nq + i) * a.nk), j, (a.nk & 3) == 0 && whole,
+                       v0, v1, v2, v3);
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  if (warp == 0) sm100::tmem_dealloc(tbase, tcols);
+}
+
 // ---------------------------------------------------------------- launches
 
 template <class F, class... X>
@@ -1166,6 +1476,26 @@ int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
             parts);
 }
 
+template <int BT>
+int launch_plane(Args a, float* part, int parts, double flops, cudaStream_t st) {
+  const int nkp = (int)((a.nk + 15) / 16) * 16;
+  const int G = ((nkp / 16 + 3) / 4 + 1) / 2 * 2;  // groups of a quarter, an even number
+  int tcols = 32;
+  while (tcols < 4 * G * 8) tcols *= 2;
+  a.tiles = (a.nq + 63) / 64;
+  const int64_t blocks = a.tiles * a.H * parts;
+  if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
+  const int smem = PlaneSmem(nkp).end;
+  auto* kern = k_dq_plane<BT>;
+  PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  {
+    PF_LAUNCH_SCOPE_WORK(st, "k_attn_dq_plane", flops, 'f');
+    kern<<<(unsigned)blocks, kPlaneThreads, smem, st>>>(a, part, parts, G, tcols);
+  }
+  PF_CHECK_LAUNCH();
+  return PF_OK;
+}
+
 }  // namespace
 
 #define PF_ATT_DIM(FN, BT, ...)                    \
@@ -1185,6 +1515,11 @@ int launch_bf16(Kind kind, const Args& a, double flops, cudaStream_t st) {
 int dbias_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
   if (a.bias_f32) PF_ATT_DIM(launch_db, 2, a, part, parts, flops, st);
   PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);
+}
+
+bool dq_plane_fits(int64_t nq, int64_t nk, int d) { return d <= 32 && nk <= kPlaneKeys && nk > 0 && nq > 0; }
+int dq_plane_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
+  return a.bias_f32 ? launch_plane<2>(a, part, parts, flops, st) : launch_plane<1>(a, part, parts, flops, st);
 }
 
 int rows_bf16(const Args& a, const float* stats, Heads o, const int16_t* lo, float* rows, cudaStream_t st) {
