@@ -37,8 +37,7 @@ namespace pf {
 namespace train {
 namespace attn {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kThreads = 128;  // of a block
 
 struct Heads {  // element (b, n, h, e) at p + b*bs + n*ns + h*hs + e
   const void* p;

@@ -1,354 +1,345 @@
-// pf_attention_f32.cu -- the fp32 kernels of pf_attention.cuh: a stationary tile of 64 rows (16 per warp)
-// against streamed tiles of BN rows that cp.async double-buffers in shared memory, with FFMA.
+// pf_attention_f32.cu -- the fp32 kernels of pf_attention.cuh, on the bf16 tensor cores.
+//
+// An fp32 value is the sum of three bf16 values of 8 bits each (its rounding, the rounding of what is
+// left, and the rest), so a product of two fp32 operands is the sum of six bf16 products whose order is
+// 2^0, 2^-8, 2^-8, 2^-16, 2^-16, 2^-16; the three left out are below 2^-24 of the product. The tensor
+// cores add in fp32 but cut off below the last bit of the running sum, which over a long sum would
+// pile up: the small products are added apart from the large ones, and the second product (with p or
+// ds) restarts from zero for every 16 columns and is added to the accumulators by rounded fp32
+// additions. Against the FFMA form of the same kernels, which the multiply-adds bound at 128 per clock
+// and SM (149 rows of 149 tokens, 12 heads of 32, forward plus backward: 1.9 ms), six products at 1024
+// per clock and SM are 1.3 times as many, with a quarter of the instructions.
+//
+// The layout is that of pf_attention_bf16.cu, with every tile in three planes. The streamed tiles are read
+// into registers a tile ahead, split, and stored to the other buffer after the products of the current
+// one. 16 stationary rows per warp, four warps to a block.
 
-#include "pf_attention.cuh"
-#include "pf_f32x2.cuh"
+#include "pf_attention_tc.cuh"
 
 namespace pf {
 namespace train {
 namespace attn {
 namespace {
 
-constexpr int BM = kWarps * 16;  // rows of a stationary tile
-
-// ---------------------------------------------------------------- tiles
-
+// Rows of a streamed tile: four 16-byte loads per thread and operand.
 template <int DP>
-struct Pitch {
-  static constexpr int value = DP + 4;  // rows shifted by 16 bytes: no bank conflicts
+struct Split {
+  static constexpr int KT = 2048 / DP;
+  static constexpr int RB = Tile<DP>::RB;
+  static constexpr int kPlane = KT * RB;   // bytes of a streamed plane
+  static constexpr int kTile3 = 3 * kPlane;
+  static constexpr int kStatPlane = 64 * RB, kStat3 = 3 * kStatPlane;
 };
 
-__device__ __forceinline__ bool key_seen(const Args& a, int64_t b, int64_t j) {
-  return a.mask == nullptr || a.mask[b * a.m_bs + j * a.m_ks] != 0.f;
-}
-
-// Rows [r0, r0 + ROWS) of (b, h) into shared memory, zero past n and d, and where MASKED for masked keys.
-template <int DP, int ROWS, bool MASKED>
-__device__ __forceinline__ void load_tile(float* sm, const Args& a, const Heads& s, int vec, int64_t b, int h, int64_t r0,
-                                          int64_t n) {
-  constexpr int P = Pitch<DP>::value, E = 4, CH = DP / E;
-  const float* base = (const float*)s.p + b * s.bs + (int64_t)h * s.hs;
-  if (vec) {
+__device__ __forceinline__ void split4(const float4& v, uint2 (&w)[3]) {
+  float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = threadIdx.x; i < ROWS * CH; i += kThreads) {
-      const int r = i / CH, c = (i - r * CH) * E;
-      const int64_t row = r0 + r;
-      bool ok = row < n && c < a.d;
-      if (MASKED && ok) ok = key_seen(a, b, row);
-      cp_async16(smem_addr(sm + r * P + c), ok ? base + row * s.ns + c : base, ok);
-    }
-  } else {
-    for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
-      const int r = i / DP, c = i - r * DP;
-      const int64_t row = r0 + r;
-      bool ok = row < n && c < a.d;
-      if (MASKED && ok) ok = key_seen(a, b, row);
-      sm[r * P + c] = ok ? base[row * s.ns + c] : 0.f;
+  for (int p = 0; p < 3; ++p) {
+    w[p].x = pack_bf16(x[0], x[1]);
+    w[p].y = pack_bf16(x[2], x[3]);
+    if (p < 2) {
+      x[0] -= lo_f(w[p].x), x[1] -= hi_f(w[p].x);
+      x[2] -= lo_f(w[p].y), x[3] -= hi_f(w[p].y);
     }
   }
 }
 
-// Which of the BN keys from j0 on are visible, as bits (the same in every lane of a warp).
-template <int BN>
-__device__ __forceinline__ uint64_t seen_bits(const Args& a, int64_t b, int64_t j0) {
-  const int lane = threadIdx.x & 31;
-  uint64_t bits = 0;
+// A tile of KT rows on its way: read, then split and stored.
+template <int DP>
+struct Ahead {
+  float4 v[4];
+  __device__ __forceinline__ void read(const float* base, int64_t ns, int vec, int64_t r0, int64_t n, int d,
+                                       uint64_t live) {
+    constexpr int CH = DP / 4;
 #pragma unroll
-  for (int i = 0; i < BN / 32; ++i) {
-    const int64_t j = j0 + i * 32 + lane;
-    const bool ok = j < a.nk && key_seen(a, b, j);
-    bits |= (uint64_t)__ballot_sync(0xffffffffu, ok) << (32 * i);
-  }
-  return bits;
-}
-template <int BN>
-__device__ __forceinline__ bool all_seen(uint64_t bits) {
-  return bits == (BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1ull);
-}
-
-// ---------------------------------------------------------------- products
-// Register layout of a 16 x 8n accumulator (both types): lane (g, t) = (lane / 4, lane % 4) holds
-// c[n][0..1] = row g, columns 8n + 2t, +1 and c[n][2..3] = row g + 8, the same columns.
-
-template <int DP, int BN>
-struct Prod {
-  static constexpr int P = Pitch<DP>::value;
-  // c = a b^T; pairs hold the sums over even and odd depths
-  static __device__ void nt(float (&c)[BN / 8][4], const float* a, const float* b) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    F2 s[BN / 8][4];
-#pragma unroll
-    for (int n = 0; n < BN / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = F2(0.f);
-#pragma unroll 4
-    for (int k = 0; k < DP; k += 4) {
-      const float4 a0 = *reinterpret_cast<const float4*>(a + g * P + k);
-      const float4 a1 = *reinterpret_cast<const float4*>(a + (g + 8) * P + k);
-      const F2 a0l(a0.x, a0.y), a0h(a0.z, a0.w), a1l(a1.x, a1.y), a1h(a1.z, a1.w);
-#pragma unroll
-      for (int n = 0; n < BN / 8; ++n) {
-        const float4 b0 = *reinterpret_cast<const float4*>(b + (n * 8 + 2 * t) * P + k);
-        const float4 b1 = *reinterpret_cast<const float4*>(b + (n * 8 + 2 * t + 1) * P + k);
-        const F2 b0l(b0.x, b0.y), b0h(b0.z, b0.w), b1l(b1.x, b1.y), b1h(b1.z, b1.w);
-        s[n][0] = fma2(a0h, b0h, fma2(a0l, b0l, s[n][0]));
-        s[n][1] = fma2(a0h, b1h, fma2(a0l, b1l, s[n][1]));
-        s[n][2] = fma2(a1h, b0h, fma2(a1l, b0l, s[n][2]));
-        s[n][3] = fma2(a1h, b1h, fma2(a1l, b1l, s[n][3]));
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < BN / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[n][e] = s[n][e].sum();
-  }
-  // acc += p b; p goes through the warp's scratch rows [16][BN + 4]
-  static __device__ void nn(float (&acc)[DP / 8][4], const float (&p)[BN / 8][4], float* sc, const float* b) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr int Q = BN + 4;
-    __syncwarp();
-#pragma unroll
-    for (int n = 0; n < BN / 8; ++n) {
-      *reinterpret_cast<float2*>(sc + g * Q + n * 8 + 2 * t) = make_float2(p[n][0], p[n][1]);
-      *reinterpret_cast<float2*>(sc + (g + 8) * Q + n * 8 + 2 * t) = make_float2(p[n][2], p[n][3]);
-    }
-    __syncwarp();
-    F2 s[DP / 8][2];
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n) {
-      s[n][0] = F2(acc[n][0], acc[n][1]);
-      s[n][1] = F2(acc[n][2], acc[n][3]);
-    }
-#pragma unroll 2
-    for (int k = 0; k < BN; k += 4) {
-      const float4 a0 = *reinterpret_cast<const float4*>(sc + g * Q + k);
-      const float4 a1 = *reinterpret_cast<const float4*>(sc + (g + 8) * Q + k);
-      const float x0[4] = {a0.x, a0.y, a0.z, a0.w}, x1[4] = {a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const F2 y0(x0[u]), y1(x1[u]);
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n) {
-          const float2 v = *reinterpret_cast<const float2*>(b + (k + u) * P + n * 8 + 2 * t);
-          s[n][0] = fma2(y0, F2(v.x, v.y), s[n][0]);
-          s[n][1] = fma2(y1, F2(v.x, v.y), s[n][1]);
+    for (int j = 0; j < 4; ++j) {
+      const int i = threadIdx.x + j * kThreads, r = i / CH, c = (i - r * CH) * 4;
+      const bool ok = r0 + r < n && c < d && ((live >> (r & 63)) & 1);
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ok) {
+        const float* p = base + (r0 + r) * ns + c;
+        if (vec) {
+          v[j] = *reinterpret_cast<const float4*>(p);
+        } else {
+          v[j].x = p[0];
+          if (c + 1 < d) v[j].y = p[1];
+          if (c + 2 < d) v[j].z = p[2];
+          if (c + 3 < d) v[j].w = p[3];
         }
       }
     }
+  }
+  __device__ __forceinline__ void store(uint32_t sm, int plane, int row0 = 0) const {
+    constexpr int CH = DP / 4;
 #pragma unroll
-    for (int n = 0; n < DP / 8; ++n) {
-      s[n][0].get(acc[n][0], acc[n][1]);
-      s[n][1].get(acc[n][2], acc[n][3]);
+    for (int j = 0; j < 4; ++j) {
+      const int i = threadIdx.x + j * kThreads, r = row0 + i / CH, c = (i - i / CH * CH) * 4;
+      uint2 w[3];
+      split4(v[j], w);
+      const uint32_t at = sm + Tile<DP>::off(r, c >> 3) + (c & 7) * 2;
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + p * plane), "r"(w[p].x), "r"(w[p].y) : "memory");
     }
   }
 };
-
-// ---------------------------------------------------------------- shared-memory plan
-
-template <int DP, int BN>
-struct Smem {
-  static constexpr int P = Pitch<DP>::value;
-  static constexpr int kStat = BM * P, kStream = BN * P;  // elements
-  static constexpr int kScratch = kWarps * 16 * (BN + 4);
-  // nstat stationary tiles, nstream streamed tiles (double-buffered), the products' scratch rows
-  static size_t bytes(int nstat, int nstream) {
-    return ((size_t)nstat * kStat + 2 * (size_t)nstream * kStream + kScratch) * sizeof(float);
+// 64 rows at once
+template <int DP>
+__device__ __forceinline__ void load_stat(uint32_t sm, const float* base, int64_t ns, int vec, int64_t r0, int64_t n,
+                                          int d, uint64_t live) {
+  using S = Split<DP>;
+#pragma unroll 1
+  for (int r = 0; r < 64; r += S::KT) {
+    Ahead<DP> t;
+    t.read(base, ns, vec, r0 + r, n, d, live >> r);
+    t.store(sm, S::kStatPlane, r);
   }
-};
-
-// ---------------------------------------------------------------- scores
-
-__device__ __forceinline__ float ld_bias1(const Args& a, int64_t off) {
-  return a.bias_f32 ? ((const float*)a.bias)[off] : __bfloat162float(((const __nv_bfloat16*)a.bias)[off]);
+}
+__device__ __forceinline__ const float* head_f(const Heads& s, int64_t b, int h) {
+  return (const float*)s.p + b * s.bs + (int64_t)h * s.hs;
 }
 
-// x[n][i] = scale * x[n][i] + bias of rows (i0 + g, i0 + g + 8), keys j0 + 8n + 2t (+1); only visible
-// keys of real rows are read.
-template <int BN>
-__device__ __forceinline__ void add_bias(float (&x)[BN / 8][4], const Args& a, int64_t b, int h, int64_t i0,
-                                         int64_t j0, uint64_t bits) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// x (16 rows by 16 columns) = a b^T over the channels; `fa(plane, k, r)` and `fb(plane, k, r)` give the fragments
+template <int KS, class FA, class FB>
+__device__ __forceinline__ void nt3(float (&x)[2][4], FA fa, FB fb) {
+  float lo[2][4];
 #pragma unroll
-  for (int n = 0; n < BN / 8; ++n)
+  for (int k = 0; k < KS; ++k) {
+    uint32_t a[3][4], b[3][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[n][e] *= a.scale;
-  if (a.bias == nullptr) return;
-  const bool full = all_seen<BN>(bits) && a.bias_vec;
+    for (int p = 0; p < 3; ++p) {
+      fa(p, k, a[p]);
+      fb(p, k, b[p]);
+    }
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int64_t i = i0 + g + 8 * r;
-    if (i >= a.nq) continue;
-    const int64_t off = b * a.b_bs + (int64_t)h * a.b_hs + i * a.b_rs + j0 + 2 * t;
-    if (full && a.bias_f32) {
-      const float* p = (const float*)a.bias + off;
-#pragma unroll
-      for (int n = 0; n < BN / 8; ++n) {
-        const float2 v = *reinterpret_cast<const float2*>(p + n * 8);
-        x[n][2 * r] += v.x;
-        x[n][2 * r + 1] += v.y;
+    for (int n = 0; n < 2; ++n) {
+      if (k == 0) {
+        mma0(lo[n], a[2], b[0][2 * n], b[0][2 * n + 1]);
+        mma0(x[n], a[0], b[0][2 * n], b[0][2 * n + 1]);
+      } else {
+        mma(lo[n], a[2], b[0][2 * n], b[0][2 * n + 1]);
+        mma(x[n], a[0], b[0][2 * n], b[0][2 * n + 1]);
       }
-    } else if (full) {
-      const __nv_bfloat16* p = (const __nv_bfloat16*)a.bias + off;
+      mma(lo[n], a[1], b[1][2 * n], b[1][2 * n + 1]);
+      mma(lo[n], a[0], b[2][2 * n], b[2][2 * n + 1]);
+      mma(lo[n], a[1], b[0][2 * n], b[0][2 * n + 1]);
+      mma(lo[n], a[0], b[1][2 * n], b[1][2 * n + 1]);
+    }
+  }
 #pragma unroll
-      for (int n = 0; n < BN / 8; ++n) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(p + n * 8);
-        x[n][2 * r] += __uint_as_float(v << 16);
-        x[n][2 * r + 1] += __uint_as_float(v & 0xffff0000u);
-      }
-    } else {
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int n = 0; n < BN / 8; ++n)
+    for (int r = 0; r < 2; ++r)
+      add2(F2(x[n][2 * r], x[n][2 * r + 1]), F2(lo[n][2 * r], lo[n][2 * r + 1])).get(x[n][2 * r], x[n][2 * r + 1]);
+}
+// acc += p b for 16 columns of p in three terms; `fb(plane, c, r)` gives the fragments of channels 16 c..
+template <int NB, class FB>
+__device__ __forceinline__ void nn3(float (&acc)[NB][4], const uint32_t (&pa)[3][4], FB fb) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if ((bits >> (n * 8 + 2 * t + e)) & 1) x[n][2 * r + e] += ld_bias1(a, off + n * 8 + e);
+  for (int c = 0; c < NB / 2; ++c) {
+    uint32_t b[3][4];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) fb(p, c, b[p]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      float s[4];
+      mma0(s, pa[2], b[0][2 * n], b[0][2 * n + 1]);
+      mma(s, pa[1], b[1][2 * n], b[1][2 * n + 1]);
+      mma(s, pa[0], b[2][2 * n], b[2][2 * n + 1]);
+      mma(s, pa[1], b[0][2 * n], b[0][2 * n + 1]);
+      mma(s, pa[0], b[1][2 * n], b[1][2 * n + 1]);
+      mma(s, pa[0], b[0][2 * n], b[0][2 * n + 1]);
+      float* d = acc[2 * c + n];
+      add2(F2(d[0], d[1]), F2(s[0], s[1])).get(d[0], d[1]);
+      add2(F2(d[2], d[3]), F2(s[2], s[3])).get(d[2], d[3]);
     }
   }
 }
+// 16 x 16 values in accumulator layout as left operands in three terms (left as their remainder)
+__device__ __forceinline__ void split_a(float (&x)[2][4], uint32_t (&pa)[3][4]) {
+#pragma unroll
+  for (int p = 0; p < 3; ++p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* v = &x[i >> 1][2 * (i & 1)];
+      pa[p][i] = pack_bf16(v[0], v[1]);
+      if (p < 2) add2(F2(v[0], v[1]), F2(-lo_f(pa[p][i]), -hi_f(pa[p][i]))).get(v[0], v[1]);
+    }
+}
 
-template <int BN>
-__device__ __forceinline__ void hide(float (&x)[BN / 8][4], uint64_t bits) {
-  if (all_seen<BN>(bits)) return;
+template <int BT, int R>
+__device__ __forceinline__ void hide16(float (&x)[R][2][4], uint32_t bits) {
+  if (bits == 0xffffu) return;
   const int t = threadIdx.x & 3;
 #pragma unroll
-  for (int n = 0; n < BN / 8; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (!((bits >> (n * 8 + 2 * t + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
+      if (!((bits >> (4 * t + 2 * n + e)) & 1))
+#pragma unroll
+        for (int q = 0; q < R; ++q) x[q][n][e] = x[q][n][2 + e] = -INFINITY;
 }
 
-// p and, in dp's place, ds (see the head of the file)
-template <int BN>
-__device__ __forceinline__ void prob_ds_rows(float (&s)[BN / 8][4], float (&dp)[BN / 8][4], const float* m,
-                                             const float* c, const float* D, const float* peak) {
-#pragma unroll
-  for (int n = 0; n < BN / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p = expf(s[n][e] - m[e >> 1]) * c[e >> 1];
-      s[n][e] = p;
-      dp[n][e] = peak[e >> 1] != 0.f && p == 1.f ? 0.f : p * (dp[n][e] - D[e >> 1]);
-    }
-}
-
-template <int DP>
-__device__ __forceinline__ void store_rows(void* out, int64_t off, int64_t ns, int64_t i0, int64_t n, int d,
-                                           const float (&acc)[DP / 8][4], float f0, float f1) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int64_t i = i0 + g + 8 * r;
-    if (i >= n) continue;
-    float* p = (float*)out + off + i * ns;
-    const float f = r ? f1 : f0;
-#pragma unroll
-    for (int c = 0; c < DP / 8; ++c)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int col = c * 8 + 2 * t + e;
-        if (col < d) p[col] = acc[c][2 * r + e] * f;
-      }
+__device__ __forceinline__ void store2f(float* p, int col, int d, bool vec, float v0, float v1) {
+  if (vec) {
+    if (col < d) *reinterpret_cast<float2*>(p + col) = make_float2(v0, v1);
+  } else {
+    if (col < d) p[col] = v0;
+    if (col + 1 < d) p[col + 1] = v1;
   }
+}
+__device__ __forceinline__ bool pair_ok_f(const void* p, int64_t bs, int64_t ns, int64_t hs, int d) {
+  return ((uintptr_t)p & 7) == 0 && ((bs | ns | hs | d) & 1) == 0;
+}
+template <int KT>
+__device__ __forceinline__ uint64_t tile_bits(float2 raw) {
+  return seen_ballot(raw) & (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
 }
 
 // ---------------------------------------------------------------- forward
 
-template <int DP, int BN>
-__global__ void __launch_bounds__(kThreads) k_attn_fwd(Args a) {
-  using M = Prod<DP, BN>;
-  using S = Smem<DP, BN>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  float* sq = (float*)raw;
-  float* sk = sq + S::kStat;           // [2]
-  float* sv = sk + 2 * S::kStream;     // [2]
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
+  using S = Split<DP>;
+  constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8, HB = KT < 32 ? KT : 32, GQ = HB / 16;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sq = smem_addr(raw), sk = sq + S::kStat3, sv = sk + 2 * S::kTile3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float* sc = sv + 2 * S::kStream + warp * 16 * (BN + 4);
-  int64_t id = blockIdx.x;
-  const int64_t tile = id % a.tiles;
-  id /= a.tiles;
-  const int h = (int)(id % a.H), kh = h / (a.H / a.KV);
-  const int64_t b = id / a.H;
-  const int64_t i0 = tile * BM, w0 = i0 + warp * 16;
-  const int64_t nt = (a.nk + BN - 1) / BN;
-  load_tile<DP, BM, false>(sq, a, a.q, a.vec_q, b, h, i0, a.nq);
-  auto issue = [&](int64_t kt) {
-    const int s = (int)(kt & 1);
-    load_tile<DP, BN, true>(sk + s * S::kStream, a, a.k, a.vec_k, b, kh, kt * BN, a.nk);
-    load_tile<DP, BN, true>(sv + s * S::kStream, a, a.v, a.vec_v, b, kh, kt * BN, a.nk);
-    cp_commit();
-  };
-  float acc[DP / 8][4];
-#pragma unroll
-  for (int n = 0; n < DP / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  if (nt > 0) issue(0);
-  for (int64_t kt = 0; kt < nt; ++kt) {
-    const uint64_t bits = seen_bits<BN>(a, b, kt * BN);
-    cp_wait<0>();
-    __syncthreads();
-    if (kt + 1 < nt) issue(kt + 1);
-    if (bits == 0 || w0 >= a.nq) continue;  // nothing to see, or a warp past the end
-    const int s = (int)(kt & 1);
-    float x[BN / 8][4];
-    M::nt(x, sq + warp * 16 * S::P, sk + s * S::kStream);
-    add_bias<BN>(x, a, b, h, w0, kt * BN, bits);
-    hide<BN>(x, bits);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = m[r];
-#pragma unroll
-      for (int n = 0; n < BN / 8; ++n) mx = fmaxf(mx, fmaxf(x[n][2 * r], x[n][2 * r + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float base = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: every p is 0
-      const float corr = expf(m[r] - base);
-      m[r] = mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < BN / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p = expf(x[n][2 * r + e] - base);
-          x[n][2 * r + e] = p;
-          sum += p;
-        }
-      l[r] = l[r] * corr + sum;
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        acc[n][2 * r] *= corr;
-        acc[n][2 * r + 1] *= corr;
-      }
-    }
-    M::nn(acc, x, sc, sv + s * S::kStream);
-  }
-  cp_commit();
-  cp_wait<0>();
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV);
+  const int64_t b = id / a.H, w0 = (int64_t)tile * 64 + warp * 16;
+  const int nt = (int)((a.nk + KT - 1) / KT);
+  const float *bk = head_f(a.k, b, kh), *bv = head_f(a.v, b, kh);
+  const char* brow[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-    const int64_t i = w0 + g + 8 * r;
+    const int64_t i = w0 + r * 8 + g;
+    brow[r] = bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1);
+  }
+  const F2 scale(a.scale);
+  float acc[NB][4], mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+  uint64_t bits = tile_bits<KT>(seen_raw(a, b, 0));
+  Ahead<DP> pk, pv;
+  load_stat<DP>(sq, head_f(a.q, b, h), a.q.ns, a.vec_q, (int64_t)tile * 64, a.nq, a.d, ~0ull);
+  pk.read(bk, a.k.ns, a.vec_k, 0, a.nk, a.d, bits);
+  pv.read(bv, a.v.ns, a.vec_v, 0, a.nk, a.d, bits);
+  pk.store(sk, S::kPlane);
+  pv.store(sv, S::kPlane);
+  for (int kt = 0; kt < nt; ++kt) {
+    const uint64_t next = tile_bits<KT>(seen_raw(a, b, (int64_t)(kt + 1) * KT));
+    __syncthreads();
+    if (kt + 1 < nt) {
+      pk.read(bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
+      pv.read(bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
+    }
+    if (bits != 0 && w0 < a.nq) {
+      const uint32_t tk = sk + (kt & 1) * S::kTile3, tv = sv + (kt & 1) * S::kTile3;
+#pragma unroll 1
+      for (int hb = 0; hb < KT / HB; ++hb) {
+        const int64_t j0 = (int64_t)kt * KT + hb * HB;
+        const uint32_t hbits = (uint32_t)(bits >> (HB * hb));
+        float x[GQ][2][4];
+#pragma unroll
+        for (int q = 0; q < GQ; ++q) {
+          Bias4<BT> br[2];
+          const bool fast = a.bias_vec && j0 + q * 16 + 16 <= a.nk;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + q * 16 + 4 * t, a.nk, fast);
+          nt3<KS>(x[q], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sq + p * S::kStatPlane, warp, k)); },
+                  [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(tk + p * S::kPlane, hb * GQ + q, k)); });
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) score2<BT>(&x[q][n][2 * r], scale, br[r], n);
+          float(&xq)[1][2][4] = *reinterpret_cast<float(*)[1][2][4]>(&x[q]);
+          hide16<BT, 1>(xq, (hbits >> (16 * q)) & 0xffffu);
+        }
+        float nm[2];
+        bool grew = false;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float v = mx[r];
+#pragma unroll
+          for (int q = 0; q < GQ; ++q)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) v = max3(v, x[q][n][2 * r], x[q][n][2 * r + 1]);
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          nm[r] = v;
+          grew |= v != mx[r];
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float corr = nm[r] == mx[r] ? 1.f : ex2((mx[r] - nm[r]) * kLog2e);
+            mx[r] = nm[r];
+            sum[r] *= corr;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              acc[n][2 * r] *= corr;
+              acc[n][2 * r + 1] *= corr;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const F2 neg(mx[r] == -INFINITY ? 0.f : -mx[r]);  // nothing seen yet: every p is 0
+          F2 s(0.f);
+#pragma unroll
+          for (int q = 0; q < GQ; ++q)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const F2 p = prob2(&x[q][n][2 * r], neg, F2(0.f));
+              p.get(x[q][n][2 * r], x[q][n][2 * r + 1]);
+              s = add2(s, p);
+            }
+          sum[r] += s.sum();
+        }
+#pragma unroll
+        for (int q = 0; q < GQ; ++q) {
+          uint32_t pa[3][4];
+          split_a(x[q], pa);
+          nn3<NB>(acc, pa, [&](int p, int c, uint32_t* f) { ldsm4_t(f, lt.at(tv + p * S::kPlane, hb * GQ + q, c)); });
+        }
+      }
+    }
+    if (kt + 1 < nt) {
+      pk.store(sk + ((kt + 1) & 1) * S::kTile3, S::kPlane);
+      pv.store(sv + ((kt + 1) & 1) * S::kTile3, S::kPlane);
+    }
+    bits = next;
+  }
+  const bool vec = pair_ok_f(a.o, a.o_bs, a.o_ns, a.o_hs, a.d);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float l = sum[r];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t i = w0 + r * 8 + g;
     if (i >= a.nq) continue;
     if (a.stats && t == 0) {
       const int64_t at = (b * a.H + h) * a.nq + i;
-      a.stats[at] = m[r];
-      a.stats[a.rows_plane + at] = l[r];
+      a.stats[at] = mx[r];
+      a.stats[a.rows_plane + at] = l;
     }
     float* o = (float*)a.o + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
 #pragma unroll
-    for (int c = 0; c < DP / 8; ++c)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int col = c * 8 + 2 * t + e;
-        if (col < a.d) o[col] = acc[c][2 * r + e] * inv;
-      }
+    for (int n = 0; n < NB; ++n) store2f(o, n * 8 + 2 * t, a.d, vec, acc[n][2 * r] * inv, acc[n][2 * r + 1] * inv);
   }
 }
 
-// ---------------------------------------------------------------- backward
+// ---------------------------------------------------------------- row constants
 
-// Eight lanes per row (b, i, h): D, and {m, 1 / l, peak, D}; peak = 1 where one key has all of
-// the row's weight in fp32 (l = 1).
+// Eight lanes per row (b, i, h): D, and {m, -log2 l, peak, -D}; peak = 1 where one key has all of the row's
+// weight in fp32 (l = 1).
 __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ stats, Heads o,
                                               float4* __restrict__ rows) {
   const int sub = threadIdx.x & 7;
@@ -357,8 +348,8 @@ __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ 
   const int64_t rr = live ? r : 0;
   const int h = (int)(rr % a.H);
   const int64_t bi = rr / a.H, b = bi / a.nq, i = bi - b * a.nq;
-  const float* po = (const float*)o.p + b * o.bs + i * o.ns + (int64_t)h * o.hs;
-  const float* pg = (const float*)a.g.p + b * a.g.bs + i * a.g.ns + (int64_t)h * a.g.hs;
+  const float* po = head_f(o, b, h) + i * o.ns;
+  const float* pg = head_f(a.g, b, h) + i * a.g.ns;
   float s = 0.f;
   if (live)
     for (int e = sub; e < a.d; e += 8) s += po[e] * pg[e];
@@ -369,267 +360,346 @@ __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ 
   const int64_t at = (b * a.H + h) * a.nq + i;
   const float m = stats[at], l = stats[a.rows_plane + at];
   const bool none = l == 0.f;
-  rows[at] = make_float4(none ? INFINITY : m, none ? 0.f : 1.f / l, l == 1.f ? 1.f : 0.f, none ? 0.f : s);
+  rows[at] = make_float4(none ? INFINITY : m, none ? 0.f : -log2f(l), l == 1.f ? 1.f : 0.f, none ? 0.f : -s);
 }
 
-struct RowConst {
-  float m[2], c[2], peak[2], D[2];
-};
-__device__ __forceinline__ RowConst row_const(const Args& a, int64_t b, int h, int64_t i0) {
-  const int g = (threadIdx.x & 31) >> 2;
-  RowConst r;
+// p from scores and ds in dp's place
+__device__ __forceinline__ void prob_ds(float (&x)[2][4], float (&y)[2][4], const F2 (&nmx)[2], const F2 (&lg)[2],
+                                        const F2 (&nd)[2], bool peaked) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int64_t i = i0 + g + 8 * k;
-    const float4 v = i < a.nq ? ((const float4*)a.rows)[(b * a.H + h) * a.nq + i] : make_float4(INFINITY, 0.f, 0.f, 0.f);
-    r.m[k] = v.x, r.c[k] = v.y, r.peak[k] = v.z, r.D[k] = v.w;
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const F2 p = prob2(&x[n][2 * r], nmx[r], lg[r]);
+      p.get(x[n][2 * r], x[n][2 * r + 1]);
+      mul2(p, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(y[n][2 * r], y[n][2 * r + 1]);
+    }
+  if (peaked) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (x[n][e] == 1.f) y[n][e] = 0.f;
   }
-  return r;
 }
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
+// ---------------------------------------------------------------- dq (and dbias of one batch entry)
 
-// ds of the warp's rows to dbias (real rows, keys below nk)
-template <int BN>
-__device__ __forceinline__ void store_dbias(const Args& a, int64_t b, int h, int64_t i0, int64_t j0,
-                                            const float (&ds)[BN / 8][4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const bool full = j0 + BN <= a.nk && a.db_vec;
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dq(Args a) {
+  using S = Split<DP>;
+  constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sq = smem_addr(raw), sg = sq + S::kStat3, sk = sg + S::kStat3, sv = sk + 2 * S::kTile3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV);
+  const int64_t b = id / a.H, w0 = (int64_t)tile * 64 + warp * 16;
+  const int nt = (int)((a.nk + KT - 1) / KT);
+  const float *bk = head_f(a.k, b, kh), *bv = head_f(a.v, b, kh);
+  const char* brow[2];
+  char* drow[2];
+  F2 nmx[2], lg[2], nd[2];
+  bool peaked = false;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int64_t i = i0 + g + 8 * r;
-    if (i >= a.nq) continue;
-    const int64_t off = b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs + j0 + 2 * t;
+    const int64_t i = w0 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
+    brow[r] = bias_row<BT>(a, b, h, ic);
+    drow[r] = (BT && a.dbias && i < a.nq)
+                  ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs) * (BT == 2 ? 4 : 2)
+                  : nullptr;
+    const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
+    nmx[r] = F2(-c.x), lg[r] = F2(c.y), nd[r] = F2(c.w);
+    peaked |= c.z != 0.f;
+  }
+  peaked = __any_sync(0xffffffffu, peaked);
+  const F2 scale(a.scale);
+  float acc[NB][4];
 #pragma unroll
-    for (int n = 0; n < BN / 8; ++n) {
-      if (full) {
-        if (a.bias_f32)
-          *reinterpret_cast<float2*>((float*)a.dbias + off + n * 8) = make_float2(ds[n][2 * r], ds[n][2 * r + 1]);
-        else
-          *reinterpret_cast<uint32_t*>((__nv_bfloat16*)a.dbias + off + n * 8) =
-              pack2(ds[n][2 * r], ds[n][2 * r + 1]);
-      } else {
+  for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (j0 + n * 8 + 2 * t + e < a.nk) {
-            if (a.bias_f32)
-              ((float*)a.dbias)[off + n * 8 + e] = ds[n][2 * r + e];
-            else
-              ((__nv_bfloat16*)a.dbias)[off + n * 8 + e] = __float2bfloat16_rn(ds[n][2 * r + e]);
-          }
+    for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+  uint64_t bits = tile_bits<KT>(seen_raw(a, b, 0));
+  Ahead<DP> pk, pv;
+  load_stat<DP>(sq, head_f(a.q, b, h), a.q.ns, a.vec_q, (int64_t)tile * 64, a.nq, a.d, ~0ull);
+  load_stat<DP>(sg, head_f(a.g, b, h), a.g.ns, a.vec_g, (int64_t)tile * 64, a.nq, a.d, ~0ull);
+  pk.read(bk, a.k.ns, a.vec_k, 0, a.nk, a.d, bits);
+  pv.read(bv, a.v.ns, a.vec_v, 0, a.nk, a.d, bits);
+  pk.store(sk, S::kPlane);
+  pv.store(sv, S::kPlane);
+  for (int kt = 0; kt < nt; ++kt) {
+    const uint64_t next = tile_bits<KT>(seen_raw(a, b, (int64_t)(kt + 1) * KT));
+    __syncthreads();
+    if (kt + 1 < nt) {
+      pk.read(bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
+      pv.read(bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
+    }
+    if (w0 < a.nq && (bits != 0 || (BT && a.dbias))) {
+      const uint32_t tk = sk + (kt & 1) * S::kTile3, tv = sv + (kt & 1) * S::kTile3;
+#pragma unroll 1
+      for (int q = 0; q < KT / 16; ++q) {
+        const int64_t j0 = (int64_t)kt * KT + q * 16;
+        const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
+        Bias4<BT> br[2];
+        const bool whole = j0 + 16 <= a.nk;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + 4 * t, a.nk, a.bias_vec && whole);
+        float x[1][2][4], y[2][4];
+        nt3<KS>(x[0], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sq + p * S::kStatPlane, warp, k)); },
+                [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(tk + p * S::kPlane, q, k)); });
+        nt3<KS>(y, [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sg + p * S::kStatPlane, warp, k)); },
+                [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(tv + p * S::kPlane, q, k)); });
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
+        hide16<BT, 1>(x, qbits);
+        prob_ds(x[0], y, nmx, lg, nd, peaked);
+        if (BT && a.dbias)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (drow[r])
+              store_bias4<BT>(a, drow[r], j0 + 4 * t, a.db_vec && whole, y[0][2 * r], y[0][2 * r + 1], y[1][2 * r],
+                              y[1][2 * r + 1]);
+        uint32_t da[3][4];
+        split_a(y, da);
+        nn3<NB>(acc, da, [&](int p, int c, uint32_t* f) { ldsm4_t(f, lt.at(tk + p * S::kPlane, q, c)); });
       }
     }
-  }
-}
-
-// dq of one query tile; dbias too where a.dbias is set (one batch entry per bias plane).
-template <int DP, int BN>
-__global__ void __launch_bounds__(kThreads) k_attn_dq(Args a) {
-  using M = Prod<DP, BN>;
-  using S = Smem<DP, BN>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  float* sq = (float*)raw;
-  float* sg = sq + S::kStat;
-  float* sk = sg + S::kStat;        // [2]
-  float* sv = sk + 2 * S::kStream;  // [2]
-  const int warp = threadIdx.x >> 5;
-  float* sc = sv + 2 * S::kStream + warp * 16 * (BN + 4);
-  int64_t id = blockIdx.x;
-  const int64_t tile = id % a.tiles;
-  id /= a.tiles;
-  const int h = (int)(id % a.H), kh = h / (a.H / a.KV);
-  const int64_t b = id / a.H;
-  const int64_t i0 = tile * BM, w0 = i0 + warp * 16;
-  const int64_t nt = (a.nk + BN - 1) / BN;
-  load_tile<DP, BM, false>(sq, a, a.q, a.vec_q, b, h, i0, a.nq);
-  load_tile<DP, BM, false>(sg, a, a.g, a.vec_g, b, h, i0, a.nq);
-  auto issue = [&](int64_t kt) {
-    const int s = (int)(kt & 1);
-    load_tile<DP, BN, true>(sk + s * S::kStream, a, a.k, a.vec_k, b, kh, kt * BN, a.nk);
-    load_tile<DP, BN, true>(sv + s * S::kStream, a, a.v, a.vec_v, b, kh, kt * BN, a.nk);
-    cp_commit();
-  };
-  float acc[DP / 8][4];
-#pragma unroll
-  for (int n = 0; n < DP / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  const RowConst rc = row_const(a, b, h, w0);
-  if (nt > 0) issue(0);
-  for (int64_t kt = 0; kt < nt; ++kt) {
-    const uint64_t bits = seen_bits<BN>(a, b, kt * BN);
-    cp_wait<0>();
-    __syncthreads();
-    if (kt + 1 < nt) issue(kt + 1);
-    const int s = (int)(kt & 1);
-    float x[BN / 8][4], y[BN / 8][4];
-    if (w0 >= a.nq) continue;  // a warp past the end
-    if (bits == 0) {
-#pragma unroll
-      for (int n = 0; n < BN / 8; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
-    } else {
-      M::nt(x, sq + warp * 16 * S::P, sk + s * S::kStream);
-      M::nt(y, sg + warp * 16 * S::P, sv + s * S::kStream);
-      add_bias<BN>(x, a, b, h, w0, kt * BN, bits);
-      hide<BN>(x, bits);
-      prob_ds_rows<BN>(x, y, rc.m, rc.c, rc.D, rc.peak);
-      M::nn(acc, y, sc, sk + s * S::kStream);
+    if (kt + 1 < nt) {
+      pk.store(sk + ((kt + 1) & 1) * S::kTile3, S::kPlane);
+      pv.store(sv + ((kt + 1) & 1) * S::kTile3, S::kPlane);
     }
-    if (a.dbias) store_dbias<BN>(a, b, h, w0, kt * BN, y);
+    bits = next;
   }
-  cp_commit();
-  cp_wait<0>();
-  if (a.dq)
-    store_rows<DP>(a.dq, b * a.o_bs + (int64_t)h * a.o_hs, a.o_ns, w0, a.nq, a.d, acc, a.scale, a.scale);
-}
-
-// dk and dv of one key tile: the transposed scores, keys down the rows.
-template <int DP, int BN>
-__global__ void __launch_bounds__(kThreads) k_attn_dkv(Args a) {
-  using M = Prod<DP, BN>;
-  using S = Smem<DP, BN>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  float* sk = (float*)raw;
-  float* sv = sk + S::kStat;
-  float* sq = sv + S::kStat;        // [2]
-  float* sg = sq + 2 * S::kStream;  // [2]
-  __shared__ float4 cst[2][BN];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float* sc = sg + 2 * S::kStream + warp * 16 * (BN + 4);
-  int64_t id = blockIdx.x;
-  const int64_t tile = id % a.tiles;
-  id /= a.tiles;
-  const int kh = (int)(id % a.KV), group = a.H / a.KV;
-  const int64_t b = id / a.KV;
-  const int64_t j0 = tile * BM, w0 = j0 + warp * 16;
-  const int64_t per = (a.nq + BN - 1) / BN, nt = per * group;
-  load_tile<DP, BM, true>(sk, a, a.k, a.vec_k, b, kh, j0, a.nk);
-  load_tile<DP, BM, true>(sv, a, a.v, a.vec_v, b, kh, j0, a.nk);
-  auto issue = [&](int64_t it) {
-    const int s = (int)(it & 1), h = kh * group + (int)(it / per);
-    const int64_t i0 = (it % per) * BN;
-    load_tile<DP, BN, false>(sq + s * S::kStream, a, a.q, a.vec_q, b, h, i0, a.nq);
-    load_tile<DP, BN, false>(sg + s * S::kStream, a, a.g, a.vec_g, b, h, i0, a.nq);
-    cp_commit();
-    for (int c = threadIdx.x; c < BN; c += kThreads) {
-      const int64_t i = i0 + c;
-      cst[s][c] = i < a.nq ? ((const float4*)a.rows)[(b * a.H + h) * a.nq + i] : make_float4(INFINITY, 0.f, 0.f, 0.f);
-    }
-  };
-  bool seen[2];
+  if (!a.dq) return;
+  const bool vec = pair_ok_f(a.dq, a.o_bs, a.o_ns, a.o_hs, a.d);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int64_t j = w0 + g + 8 * r;
-    seen[r] = j < a.nk && key_seen(a, b, j);
+    const int64_t i = w0 + r * 8 + g;
+    if (i >= a.nq) continue;
+    float* o = (float*)a.dq + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      store2f(o, n * 8 + 2 * t, a.d, vec, acc[n][2 * r] * a.scale, acc[n][2 * r + 1] * a.scale);
   }
-  float dk[DP / 8][4], dv[DP / 8][4];
-#pragma unroll
-  for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
-  const bool any = __syncthreads_or(seen[0] || seen[1]);
-  if (any && nt > 0) {
-    issue(0);
-    for (int64_t it = 0; it < nt; ++it) {
-      const int s = (int)(it & 1), h = kh * group + (int)(it / per);
-      const int64_t i0 = (it % per) * BN;
-      cp_wait<0>();
-      __syncthreads();
-      if (it + 1 < nt) issue(it + 1);
-      if (w0 >= a.nk) continue;  // a warp past the end
-      float x[BN / 8][4], y[BN / 8][4];
-      M::nt(x, sk + warp * 16 * S::P, sq + s * S::kStream);
-      M::nt(y, sv + warp * 16 * S::P, sg + s * S::kStream);
-      const int64_t off = b * a.b_bs + (int64_t)h * a.b_hs + w0 + g;
-#pragma unroll
-      for (int n = 0; n < BN / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = n * 8 + 2 * t + e;
-          const float4 rc = cst[s][c];
-          const bool row = i0 + c < a.nq;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float v = x[n][2 * r + e] * a.scale;
-            if (a.bias && seen[r] && row) v += ld_bias1(a, off + (i0 + c) * a.b_rs + 8 * r);
-            const float p = expf((seen[r] ? v : -INFINITY) - rc.x) * rc.y;
-            x[n][2 * r + e] = p;
-            y[n][2 * r + e] = rc.z != 0.f && p == 1.f ? 0.f : p * (y[n][2 * r + e] - rc.w);
-          }
-        }
-      M::nn(dv, x, sc, sg + s * S::kStream);
-      M::nn(dk, y, sc, sq + s * S::kStream);
-    }
-  }
-  cp_commit();
-  cp_wait<0>();
-  store_rows<DP>(a.dk, b * a.dk_bs + (int64_t)kh * a.dk_hs, a.dk_ns, w0, a.nk, a.d, dk, a.scale, a.scale);
-  store_rows<DP>(a.dv, b * a.dv_bs + (int64_t)kh * a.dv_hs, a.dv_ns, w0, a.nk, a.d, dv, 1.f, 1.f);
 }
 
-// dbias of one 64 x BN tile of the plane of head h, summed over a part of the batch: the result where there
-// is one part, else an fp32 partial plane.
-template <int DP, int BN>
-__global__ void __launch_bounds__(kThreads) k_attn_dbias(Args a, float* part, int parts) {
-  using M = Prod<DP, BN>;
-  using S = Smem<DP, BN>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  float* sm[2] = {(float*)raw, (float*)raw + 2 * S::kStat + 2 * S::kStream};  // q, do, k, v of two batch entries
-  const int warp = threadIdx.x >> 5;
-  int64_t id = blockIdx.x;
-  const int64_t nkt = (a.nk + BN - 1) / BN;
-  const int64_t kt = id % nkt;
-  id /= nkt;
-  const int64_t tile = id % a.tiles;
-  id /= a.tiles;
-  const int h = (int)(id % a.H), kh = h / (a.H / a.KV), pt = (int)(id / a.H);
-  const int64_t b0 = a.B * pt / parts, b1 = a.B * (pt + 1) / parts;
-  const int64_t i0 = tile * BM, w0 = i0 + warp * 16, j0 = kt * BN;
-  auto issue = [&](int64_t b) {
-    float* p = sm[b & 1];
-    load_tile<DP, BM, false>(p, a, a.q, a.vec_q, b, h, i0, a.nq);
-    load_tile<DP, BM, false>(p + S::kStat, a, a.g, a.vec_g, b, h, i0, a.nq);
-    load_tile<DP, BN, true>(p + 2 * S::kStat, a, a.k, a.vec_k, b, kh, j0, a.nk);
-    load_tile<DP, BN, true>(p + 2 * S::kStat + S::kStream, a, a.v, a.vec_v, b, kh, j0, a.nk);
-    cp_commit();
-  };
-  float acc[BN / 8][4];
+// ---------------------------------------------------------------- dk, dv
+
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dkv(Args a) {
+  using S = Split<DP>;
+  constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sk = smem_addr(raw), sv = sk + S::kStat3, sq = sv + S::kStat3, sg = sq + 2 * S::kTile3;
+  float4* cst = (float4*)(raw + 2 * S::kStat3 + 4 * S::kTile3);  // [2][KT]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), ln = lane_bn<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int kh = id % a.KV, group = a.H / a.KV;
+  const int64_t b = id / a.KV, j0 = (int64_t)tile * 64, w0 = j0 + warp * 16;
+  const int per = (int)((a.nq + KT - 1) / KT), nt = per * group;
+  const uint64_t live = seen_ballot(seen_raw(a, b, j0));
+  const uint32_t mine = (uint32_t)(live >> (warp * 16)) & 0xffffu;
+  const bool bfast = a.bias_vec && w0 + 16 <= a.nk;
+  const F2 scale(a.scale);
+  float dk[NB][4], dv[NB][4];
 #pragma unroll
-  for (int n = 0; n < BN / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  if (b0 < b1) issue(b0);
-  for (int64_t b = b0; b < b1; ++b) {
-    const uint64_t bits = seen_bits<BN>(a, b, j0);
-    cp_wait<0>();
-    __syncthreads();
-    if (b + 1 < b1) issue(b + 1);
-    if (bits == 0 || w0 >= a.nq) continue;
-    const float* p = sm[b & 1];
-    const RowConst rc = row_const(a, b, h, w0);
-    float x[BN / 8][4], y[BN / 8][4];
-    M::nt(x, p + warp * 16 * S::P, p + 2 * S::kStat);
-    M::nt(y, p + S::kStat + warp * 16 * S::P, p + 2 * S::kStat + S::kStream);
-    add_bias<BN>(x, a, 0, h, w0, j0, bits);
-    hide<BN>(x, bits);
-    prob_ds_rows<BN>(x, y, rc.m, rc.c, rc.D, rc.peak);
+  for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int n = 0; n < BN / 8; ++n)
+    for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
+  if (live != 0 && nt > 0) {
+    Ahead<DP> pq, pg;
+    float4 pc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto read = [&](int it) {
+      const int h = kh * group + it / per;
+      const int64_t i0 = (int64_t)(it % per) * KT;
+      pq.read(head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+      pg.read(head_f(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+      // a row past the end has p = 0
+      if (threadIdx.x < KT)
+        pc = i0 + threadIdx.x < a.nq ? ((const float4*)a.rows)[(b * a.H + h) * a.nq + i0 + threadIdx.x]
+                                     : make_float4(INFINITY, 0.f, 0.f, 0.f);
+    };
+    auto store = [&](int it) {
+      pq.store(sq + (it & 1) * S::kTile3, S::kPlane);
+      pg.store(sg + (it & 1) * S::kTile3, S::kPlane);
+      if (threadIdx.x < KT) cst[(it & 1) * KT + threadIdx.x] = pc;
+    };
+    load_stat<DP>(sk, head_f(a.k, b, kh), a.k.ns, a.vec_k, j0, a.nk, a.d, live);
+    load_stat<DP>(sv, head_f(a.v, b, kh), a.v.ns, a.vec_v, j0, a.nk, a.d, live);
+    read(0);
+    store(0);
+    for (int it = 0; it < nt; ++it) {
+      __syncthreads();
+      if (it + 1 < nt) read(it + 1);
+      if (mine != 0) {
+        const int h = kh * group + it / per;
+        const int64_t i0 = (int64_t)(it % per) * KT;
+        const uint32_t tq = sq + (it & 1) * S::kTile3, tg = sg + (it & 1) * S::kTile3;
+#pragma unroll 1
+        for (int blk = 0; blk < KT / 16; ++blk) {
+          Bias4<BT> br[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] += y[n][e];
+          for (int r = 0; r < 2; ++r) {
+            const int64_t i = i0 + blk * 16 + r * 8 + g;
+            bias_load<BT>(br[r], bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1), w0 + 4 * t, a.nk, bfast);
+          }
+          float x[1][2][4], y[2][4];
+          nt3<KS>(x[0], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(tq + p * S::kPlane, blk, k)); },
+                  [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sk + p * S::kStatPlane, warp, k)); });
+          nt3<KS>(y, [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(tg + p * S::kPlane, blk, k)); },
+                  [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sv + p * S::kStatPlane, warp, k)); });
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
+          hide16<BT, 1>(x, mine);
+          const float4 c[2] = {cst[(it & 1) * KT + blk * 16 + g], cst[(it & 1) * KT + blk * 16 + 8 + g]};
+          const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)},
+                   nd[2] = {F2(c[0].w), F2(c[1].w)};
+          prob_ds(x[0], y, nmx, lg, nd, __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f));
+          uint32_t u[3][4], w[3][4];
+          split_a(x[0], u);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {  // 8 x 8 blocks transposed, the two off the diagonal changing places
+            w[p][0] = transpose8(u[p][0]), w[p][2] = transpose8(u[p][1]);
+            w[p][1] = transpose8(u[p][2]), w[p][3] = transpose8(u[p][3]);
+          }
+          nn3<NB>(dv, w, [&](int p, int n, uint32_t* f) { ldsm4_t(f, ln.at(tg + p * S::kPlane, blk, n)); });
+          split_a(y, u);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            w[p][0] = transpose8(u[p][0]), w[p][2] = transpose8(u[p][1]);
+            w[p][1] = transpose8(u[p][2]), w[p][3] = transpose8(u[p][3]);
+          }
+          nn3<NB>(dk, w, [&](int p, int n, uint32_t* f) { ldsm4_t(f, ln.at(tq + p * S::kPlane, blk, n)); });
+        }
+      }
+      if (it + 1 < nt) store(it + 1);
+    }
   }
-  cp_commit();
-  cp_wait<0>();
-  if (parts == 1) {
-    store_dbias<BN>(a, 0, h, w0, j0, acc);
-  } else {
-    Args w = a;  // the part's plane in dbias's place
-    w.dbias = part;
-    w.bias_f32 = 1;
-    w.db_vec = (a.nk & 3) == 0;
-    w.db_rs = a.nk;
-    w.db_hs = a.nq * a.nk;
-    w.db_bs = a.H * a.nq * a.nk;
-    store_dbias<BN>(w, pt, h, w0, j0, acc);
+  const bool vk = pair_ok_f(a.dk, a.dk_bs, a.dk_ns, a.dk_hs, a.d), vv = pair_ok_f(a.dv, a.dv_bs, a.dv_ns, a.dv_hs, a.d);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int64_t j = w0 + perm_row(g, r);  // row g + 8 r of the block holds this key
+    if (j >= a.nk) continue;
+    float* ok = (float*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j * a.dk_ns;
+    float* ov = (float*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j * a.dv_ns;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      store2f(ok, n * 8 + 2 * t, a.d, vk, dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
+      store2f(ov, n * 8 + 2 * t, a.d, vv, dv[n][2 * r], dv[n][2 * r + 1]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- dbias shared by the batch
+
+// A 64 x KT tile of one head's plane, summed over the batch entries of a part (see k_dbias of the bf16
+// kernels). One buffer: other blocks of the SM work while this one reads its next entry.
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, float* part, int parts) {
+  using S = Split<DP>;
+  constexpr int KT = S::KT, KS = DP / 16, GQ = KT / 16;
+  extern __shared__ __align__(128) unsigned char raw[];
+  const uint32_t sq = smem_addr(raw), sg = sq + S::kStat3, sk = sg + S::kStat3, sv = sk + S::kTile3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>();
+  unsigned id = blockIdx.x;
+  const unsigned nkt = (unsigned)((a.nk + KT - 1) / KT);
+  const unsigned kt = id % nkt;
+  id /= nkt;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, kh = h / (a.H / a.KV), pt = id / a.H;
+  const int64_t b0 = a.B * pt / parts, b1 = a.B * (pt + 1) / parts;
+  const int64_t i0 = (int64_t)tile * 64, w0 = i0 + warp * 16, j0 = (int64_t)kt * KT;
+  const char* brow[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int64_t i = w0 + r * 8 + g;
+    brow[r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1);
+  }
+  const F2 scale(a.scale);
+  float acc[GQ][2][4];
+#pragma unroll
+  for (int q = 0; q < GQ; ++q)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[q][n][e] = 0.f;
+  for (int64_t b = b0; b < b1; ++b) {
+    const uint64_t bits = tile_bits<KT>(seen_raw(a, b, j0));
+    if (bits == 0) continue;  // the same for the whole block
+    __syncthreads();
+    load_stat<DP>(sq, head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+    load_stat<DP>(sg, head_f(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+    Ahead<DP> pk, pv;
+    pk.read(head_f(a.k, b, kh), a.k.ns, a.vec_k, j0, a.nk, a.d, bits);
+    pv.read(head_f(a.v, b, kh), a.v.ns, a.vec_v, j0, a.nk, a.d, bits);
+    pk.store(sk, S::kPlane);
+    pv.store(sv, S::kPlane);
+    F2 nmx[2], lg[2], nd[2];
+    bool peaked = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + r * 8 + g;
+      const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + (i < a.nq ? i : a.nq - 1)];
+      nmx[r] = F2(-c.x), lg[r] = F2(c.y), nd[r] = F2(c.w);
+      peaked |= c.z != 0.f;
+    }
+    peaked = __any_sync(0xffffffffu, peaked);
+    __syncthreads();
+    if (w0 >= a.nq) continue;
+#pragma unroll
+    for (int q = 0; q < GQ; ++q) {
+      Bias4<BT> br[2];
+      const bool fast = a.bias_vec && j0 + q * 16 + 16 <= a.nk;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + q * 16 + 4 * t, a.nk, fast);
+      float x[1][2][4], y[2][4];
+      nt3<KS>(x[0], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sq + p * S::kStatPlane, warp, k)); },
+              [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sk + p * S::kPlane, q, k)); });
+      nt3<KS>(y, [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sg + p * S::kStatPlane, warp, k)); },
+              [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sv + p * S::kPlane, q, k)); });
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
+      hide16<BT, 1>(x, (uint32_t)(bits >> (16 * q)) & 0xffffu);
+      prob_ds(x[0], y, nmx, lg, nd, peaked);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float* d = &acc[q][n][2 * r];
+          add2(F2(d[0], d[1]), F2(y[n][2 * r], y[n][2 * r + 1])).get(d[0], d[1]);
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int64_t i = w0 + r * 8 + g;
+    if (i >= a.nq) continue;
+#pragma unroll
+    for (int q = 0; q < GQ; ++q) {
+      const int64_t j = j0 + q * 16 + 4 * t;
+      const bool whole = j0 + q * 16 + 16 <= a.nk;
+      const float v0 = acc[q][0][2 * r], v1 = acc[q][0][2 * r + 1], v2 = acc[q][1][2 * r], v3 = acc[q][1][2 * r + 1];
+      if (parts == 1)
+        store_bias4<BT>(a, (char*)a.dbias + ((int64_t)h * a.db_hs + i * a.db_rs) * (BT == 2 ? 4 : 2), j,
+                        a.db_vec && whole, v0, v1, v2, v3);
+      else
+        store_bias4<2>(a, (char*)(part + (((int64_t)pt * a.H + h) * a.nq + i) * a.nk), j, (a.nk & 3) == 0 && whole, v0,
+                       v1, v2, v3);
+    }
   }
 }
 
@@ -649,37 +719,40 @@ int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cud
   return PF_OK;
 }
 
-template <int DP>
+template <int DP, int BT>
 int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
-  constexpr int BN = 32;
-  using S = Smem<DP, BN>;
-  a.tiles = ((kind == kDkv ? a.nk : a.nq) + BM - 1) / BM;
+  using S = Split<DP>;
+  a.tiles = ((kind == kDkv ? a.nk : a.nq) + 63) / 64;
   const int64_t blocks = a.tiles * (kind == kDkv ? a.KV : a.H) * a.B;
-  if (kind == kFwd) return go(k_attn_fwd<DP, BN>, S::bytes(1, 2), blocks, "k_attn_fwd", flops, st, a);
-  if (kind == kDq) return go(k_attn_dq<DP, BN>, S::bytes(2, 2), blocks, "k_attn_dq", flops, st, a);
-  return go(k_attn_dkv<DP, BN>, S::bytes(2, 2), blocks, "k_attn_dkv", flops, st, a);
+  if (kind == kFwd) return go(k_fwd<DP, BT>, S::kStat3 + 4 * S::kTile3, blocks, "k_attn_fwd", flops, st, a);
+  if (kind == kDq) return go(k_dq<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3, blocks, "k_attn_dq", flops, st, a);
+  return go(k_dkv<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16, blocks, "k_attn_dkv", flops, st, a);
 }
-template <int DP>
+template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
-  constexpr int BN = 32;
-  a.tiles = (a.nq + BM - 1) / BM;
-  return go(k_attn_dbias<DP, BN>, Smem<DP, BN>::bytes(4, 2), a.tiles * ((a.nk + BN - 1) / BN) * a.H * parts,
+  using S = Split<DP>;
+  a.tiles = (a.nq + 63) / 64;
+  return go(k_dbias<DP, BT>, 2 * S::kStat3 + 2 * S::kTile3, a.tiles * ((a.nk + S::KT - 1) / S::KT) * a.H * parts,
             "k_attn_dbias", flops, st, a, part, parts);
 }
 
 }  // namespace
 
+#define PF_ATT_DIM(FN, BT, ...)                    \
+  do {                                             \
+    if (a.d <= 32) return FN<32, BT>(__VA_ARGS__); \
+    if (a.d <= 64) return FN<64, BT>(__VA_ARGS__); \
+    return FN<128, BT>(__VA_ARGS__);               \
+  } while (0)
+
 int launch_f32(Kind kind, const Args& a, double flops, cudaStream_t st) {
-  if (a.d <= 32) return launch_t<32>(kind, a, flops, st);
-  if (a.d <= 64) return launch_t<64>(kind, a, flops, st);
-  if (a.d <= 96) return launch_t<96>(kind, a, flops, st);
-  return launch_t<128>(kind, a, flops, st);
+  if (!a.bias) PF_ATT_DIM(launch_t, 0, kind, a, flops, st);
+  if (a.bias_f32) PF_ATT_DIM(launch_t, 2, kind, a, flops, st);
+  PF_ATT_DIM(launch_t, 1, kind, a, flops, st);
 }
 int dbias_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
-  if (a.d <= 32) return launch_db<32>(a, part, parts, flops, st);
-  if (a.d <= 64) return launch_db<64>(a, part, parts, flops, st);
-  if (a.d <= 96) return launch_db<96>(a, part, parts, flops, st);
-  return launch_db<128>(a, part, parts, flops, st);
+  if (a.bias_f32) PF_ATT_DIM(launch_db, 2, a, part, parts, flops, st);
+  PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);
 }
 int rows_f32(const Args& a, const float* stats, Heads o, float* rows, cudaStream_t st) {
   const int64_t blocks = (a.rows_plane + 31) / 32;
