@@ -27,46 +27,56 @@ namespace {
 
 // ---------------------------------------------------------------- forward
 
+// Tiles that are wholly visible and inside, with aligned bias rows, take the body without any checks
+// (FAST): the checks would be half of its instructions.
 template <int DP, int BT, int MT>
 __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
   using S = Tile<DP>;
-  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8;
+  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr int TERMS = BT == 2 ? 3 : 2;  // bf16 values that p is split into (see the head of pf_attention.cuh)
+  constexpr int kV = 2 * kTile * RB;      // from a K tile to its V tile
   extern __shared__ __align__(128) unsigned char raw[];
-  const uint32_t sq = smem_addr(raw), sk = sq + QR * S::RB, sv = sk + 2 * kTile * S::RB;
+  const uint32_t sq = smem_addr(raw), sk = sq + QR * RB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
   unsigned id = blockIdx.x;
   const unsigned tile = id % (unsigned)a.tiles;
   id /= (unsigned)a.tiles;
   const int h = id % a.H, kh = h / (a.H / a.KV);
-  const int64_t b = id / a.H;
+  const int64_t b = id / a.H, nk = a.nk;
   const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT;
-  const int nt = (int)((a.nk + kTile - 1) / kTile);
-  const bf16 *bk = head_base(a.k, b, kh), *bv = head_base(a.v, b, kh);
+  const int nt = (int)((nk + kTile - 1) / kTile);
+  const int bvec = a.bias_vec;
+  const bool work = w0 < a.nq;  // else a warp past the end
   load_rows<DP, QR>(sq, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
+  Stream<DP> ks(head_base(a.k, b, kh), a.k.ns, a.vec_k, 0, nk, a.d), vs(head_base(a.v, b, kh), a.v.ns, a.vec_v, 0, nk, a.d);
   auto issue = [&](int kt, uint64_t live) {
-    const uint32_t s = (kt & 1) * kTile * S::RB;
-    load_rows<DP, kTile>(sk + s, bk, a.k.ns, a.vec_k, (int64_t)kt * kTile, a.nk, a.d, live);
-    load_rows<DP, kTile>(sv + s, bv, a.v.ns, a.vec_v, (int64_t)kt * kTile, a.nk, a.d, live);
+    const uint32_t s = sk + (kt & 1) * kTile * RB;
+    ks.next(s, live, a.vec_k);
+    vs.next(s + kV, live, a.vec_v);
     cp_commit();
   };
-  const char* brow[MT][2];
+  uint32_t ka[KS], va[KS];
+  {
+    const LaneAddr<DP> lb = lane_b<DP>(), lt = lane_bt<DP>();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ka[k] = lb.at(sk, 0, k), va[k] = lt.at(sk + kV, 0, k);
+  }
+  const char* bp[MT][2];  // the lane's first key of the tile, in its rows
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int64_t i = w0 + m * 16 + r * 8 + g;
-      brow[m][r] = bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1);  // rows past the end are not stored
+      bp[m][r] = BT ? bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1) + 4 * t * BS : nullptr;  // such rows are not stored
     }
   Bias4<BT> ring[2][MT][2];
-  auto fetch_bias = [&](int slot, int64_t j0) {  // keys j0 .. j0 + 15
-    if (BT == 0 || j0 >= a.nk) return;
-    const bool fast = a.bias_vec && j0 + 16 <= a.nk;
+  // group q of the tile at key j0 (4 and on: of the next one)
+  auto fetch = [&](int slot, int q, int64_t j0, bool fast) {
+    if (BT == 0) return;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][m][r], brow[m][r], j0 + 4 * t, a.nk, fast);
+      for (int r = 0; r < 2; ++r) bias_get<BT>(ring[slot][m][r], bp[m][r] + q * 16 * BS, j0 + q * 16 + 4 * t, nk, fast);
   };
   const F2 scale(a.scale);
   float acc[MT][NB][4], mx[MT][2], sum[MT][2];
@@ -80,41 +90,23 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
     sum[m][0] = sum[m][1] = 0.f;
   }
   uint32_t fq[MT][KS][4];
-  float2 rawm = seen_raw(a, b, 0);
-  uint64_t bits = seen_ballot(rawm);
+  uint64_t bits = seen_ballot(seen_raw(a, b, 0));
   if (nt > 0) issue(0, bits);
-  rawm = seen_raw(a, b, kTile);
-  fetch_bias(0, 0);
-  fetch_bias(1, 16);
-  for (int kt = 0; kt < nt; ++kt) {
-    const uint64_t next = seen_ballot(rawm);
-    cp_wait<0>();
-    __syncthreads();
-    if (kt == 0) {
+  float2 rawm = seen_raw(a, b, kTile);
+  auto body = [&](auto mode, int64_t j0, uint32_t off, bool nf) {
+    constexpr bool FAST = decltype(mode)::value;
+    uint32_t kc[KS], vc[KS];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int k = 0; k < KS; ++k) ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
-    }
-    if (kt + 1 < nt) issue(kt + 1, next);
-    rawm = seen_raw(a, b, (int64_t)(kt + 2) * kTile);
-    const int64_t j0 = (int64_t)kt * kTile;
-    if (bits == 0 || w0 >= a.nq) {  // no visible key, or a warp past the end
-      fetch_bias(0, j0 + 64);
-      fetch_bias(1, j0 + 80);
-      bits = next;
-      continue;
-    }
-    const uint32_t tk = sk + (kt & 1) * kTile * S::RB, tv = sv + (kt & 1) * kTile * S::RB;
-#pragma unroll
+    for (int k = 0; k < KS; ++k) kc[k] = ka[k] + off, vc[k] = va[k] + off;
+#pragma unroll 1
     for (int hb = 0; hb < 2; ++hb) {  // 32 keys
       float x[MT][4][4];
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
+      unrolled<2>([&](auto Q) {
+        constexpr int q = decltype(Q)::value;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t r[4];
-          ldsm4(r, lb.at(tk, hb * 2 + q, k));
+          ldsm4i<q * 16 * RB>(r, kc[k]);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             if (k == 0) {
@@ -126,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
             }
           }
         }
-      const uint32_t hbits = (uint32_t)(bits >> (32 * hb));
+      });
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -135,19 +127,22 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int r = 0; r < 2; ++r) score2<BT>(&x[m][2 * q + n][2 * r], scale, ring[q][m][r], n);
-        fetch_bias(q, j0 + hb * 32 + q * 16 + 32);
+        fetch(q, 2 * hb + q + 2, j0, hb == 0 ? FAST || (bvec && j0 + (q + 3) * 16 <= nk) : nf);
       }
-      if (hbits != 0xffffffffu) {
+      if (!FAST) {
+        const uint32_t hbits = (uint32_t)(bits >> (32 * hb));
+        if (hbits != 0xffffffffu) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t mine = hbits >> (16 * q + 4 * t);
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t mine = hbits >> (16 * q + 4 * t);
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (!((mine >> (2 * n + e)) & 1))
+              for (int e = 0; e < 2; ++e)
+                if (!((mine >> (2 * n + e)) & 1))
 #pragma unroll
-                for (int m = 0; m < MT; ++m) x[m][2 * q + n][e] = x[m][2 * q + n][2 + e] = -INFINITY;
+                  for (int m = 0; m < MT; ++m) x[m][2 * q + n][e] = x[m][2 * q + n][2 + e] = -INFINITY;
+          }
         }
       }
       bool grew = false;
@@ -183,24 +178,21 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const F2 nm(mx[m][r] == -INFINITY ? 0.f : -mx[m][r]);  // nothing seen yet: every p is 0
+          const F2 neg(mx[m][r] == -INFINITY ? 0.f : -mx[m][r]);  // nothing seen yet: every p is 0
           F2 s2;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const F2 p = prob2(&x[m][n][2 * r], nm, F2(0.f));
+            const F2 p = prob2(&x[m][n][2 * r], neg, F2(0.f));
             p.get(x[m][n][2 * r], x[m][n][2 * r + 1]);
             s2 = n == 0 ? p : add2(s2, p);
           }
-          float s, s1;
-          s2.get(s, s1);
-          s += s1;
-          sum[m][r] += s;
+          sum[m][r] += s2.sum();
         }
+      unrolled<2>([&](auto Q) {
+        constexpr int q = decltype(Q)::value;
+        uint32_t f[KS][4];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t f[NB / 2][4];
-#pragma unroll
-        for (int c = 0; c < NB / 2; ++c) ldsm4_t(f[c], lt.at(tv, hb * 2 + q, c));
+        for (int c = 0; c < KS; ++c) ldsm4_ti<q * 16 * RB>(f[c], vc[c]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -210,16 +202,51 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
             for (int i = 0; i < 4; ++i) {
               float* v = &x[m][2 * q + (i >> 1)][2 * (i & 1)];
               pa[i] = pack_bf16(v[0], v[1]);
-              if (term + 1 < TERMS) add2(F2(v[0], v[1]), F2(-lo_f(pa[i]), -hi_f(pa[i]))).get(v[0], v[1]);
+              if (term + 1 < TERMS) fma2(F2(lo_f(pa[i]), hi_f(pa[i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
             }
 #pragma unroll
-            for (int c = 0; c < NB / 2; ++c) {
+            for (int c = 0; c < KS; ++c) {
               mma(acc[m][2 * c], pa, f[c][0], f[c][1]);
               mma(acc[m][2 * c + 1], pa, f[c][2], f[c][3]);
             }
           }
         }
+      });
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kc[k] += 32 * RB, vc[k] += 32 * RB;
+    }
+  };
+  if (work) {
+    fetch(0, 0, 0, bvec && 16 <= nk);
+    fetch(1, 1, 0, bvec && 32 <= nk);
+  }
+  for (int kt = 0; kt < nt; ++kt) {
+    const uint64_t next = seen_ballot(rawm);
+    const int64_t j0 = (int64_t)kt * kTile;
+    cp_wait<0>();
+    __syncthreads();
+    if (kt == 0) {
+      const LaneAddr<DP> la = lane_a<DP>();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
+    }
+    if (kt + 1 < nt) issue(kt + 1, next);
+    rawm = seen_raw(a, b, j0 + 2 * kTile);
+    if (work) {
+      const bool nf = bvec && j0 + kTile + 32 <= nk;  // the next tile's first two groups
+      const uint32_t off = (kt & 1) * kTile * RB;
+      if (bits == ~0ull && (BT == 0 || bvec)) {
+        body(std::true_type{}, j0, off, nf);
+      } else if (bits != 0) {
+        body(std::false_type{}, j0, off, nf);
+      } else {  // no visible key
+        fetch(0, 4, j0, nf);
+        fetch(1, 5, j0, nf);
       }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) bp[m][0] += kTile * BS, bp[m][1] += kTile * BS;
     }
     bits = next;
   }
@@ -303,56 +330,62 @@ __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ 
 template <int DP, int BT, int MT>
 __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
   using S = Tile<DP>;
-  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8;
+  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
+  constexpr int kV = 2 * kTile * RB;  // from a K tile to its V tile
   extern __shared__ __align__(128) unsigned char raw[];
-  const uint32_t sq = smem_addr(raw), sg = sq + QR * S::RB, sk = sg + QR * S::RB, sv = sk + 2 * kTile * S::RB;
+  const uint32_t sq = smem_addr(raw), sg = sq + QR * RB, sk = sg + QR * RB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
   unsigned id = blockIdx.x;
   const unsigned tile = id % (unsigned)a.tiles;
   id /= (unsigned)a.tiles;
   const int h = id % a.H, kh = h / (a.H / a.KV);
-  const int64_t b = id / a.H;
+  const int64_t b = id / a.H, nk = a.nk;
   const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT;
-  const int nt = (int)((a.nk + kTile - 1) / kTile);
-  const bf16 *bk = head_base(a.k, b, kh), *bv = head_base(a.v, b, kh);
+  const int nt = (int)((nk + kTile - 1) / kTile);
+  const int bvec = a.bias_vec;
+  const bool work = w0 < a.nq, put = BT && a.dbias != nullptr;
   load_rows<DP, QR>(sq, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
   load_rows<DP, QR>(sg, head_base(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+  Stream<DP> ks(head_base(a.k, b, kh), a.k.ns, a.vec_k, 0, nk, a.d), vs(head_base(a.v, b, kh), a.v.ns, a.vec_v, 0, nk, a.d);
   auto issue = [&](int kt, uint64_t live) {
-    const uint32_t s = (kt & 1) * kTile * S::RB;
-    load_rows<DP, kTile>(sk + s, bk, a.k.ns, a.vec_k, (int64_t)kt * kTile, a.nk, a.d, live);
-    load_rows<DP, kTile>(sv + s, bv, a.v.ns, a.vec_v, (int64_t)kt * kTile, a.nk, a.d, live);
+    const uint32_t s = sk + (kt & 1) * kTile * RB;
+    ks.next(s, live, a.vec_k);
+    vs.next(s + kV, live, a.vec_v);
     cp_commit();
   };
-  const char* brow[MT][2];
-  char* drow[MT][2];
+  uint32_t ka[KS], ta[KS];
+  {
+    const LaneAddr<DP> lb = lane_b<DP>(), lt = lane_bt<DP>();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ka[k] = lb.at(sk, 0, k), ta[k] = lt.at(sk, 0, k);
+  }
+  const char* bp[MT][2];  // the lane's first key of the tile, in its rows of the bias and of dbias
+  char* dp[MT][2];
   F2 nmx[MT][2], lg[MT][2], nd[MT][2];
-  const F2 scale(a.scale);
   bool peaked = false;
-  const int bsz = BT == 2 ? 4 : 2;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int64_t i = w0 + m * 16 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
-      brow[m][r] = bias_row<BT>(a, b, h, ic);
-      drow[m][r] = (BT && a.dbias && i < a.nq)
-                       ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs) * bsz
-                       : nullptr;
+      bp[m][r] = BT ? bias_row<BT>(a, b, h, ic) + 4 * t * BS : nullptr;
+      dp[m][r] = (put && i < a.nq) ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs + 4 * t) * BS : nullptr;
       const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
       nmx[m][r] = F2(-c.x), lg[m][r] = F2(c.y), nd[m][r] = F2(c.w);
       peaked |= c.z != 0.f;
     }
   peaked = __any_sync(0xffffffffu, peaked);
+  // what the body without checks needs of the warp's rows
+  const bool plain = !peaked && (BT == 0 || bvec) && (!put || (a.db_vec && w0 + 16 * MT <= a.nq));
   Bias4<BT> ring[2][MT][2];
-  auto fetch_bias = [&](int slot, int64_t j0) {
-    if (BT == 0 || j0 >= a.nk) return;
-    const bool fast = a.bias_vec && j0 + 16 <= a.nk;
+  auto fetch = [&](int slot, int q, int64_t j0, bool fast) {
+    if (BT == 0) return;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][m][r], brow[m][r], j0 + 4 * t, a.nk, fast);
+      for (int r = 0; r < 2; ++r) bias_get<BT>(ring[slot][m][r], bp[m][r] + q * 16 * BS, j0 + q * 16 + 4 * t, nk, fast);
   };
+  const F2 scale(a.scale);
   float acc[MT][NB][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -361,43 +394,24 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
   uint32_t fq[MT][KS][4], fg[MT][KS][4];
-  float2 rawm = seen_raw(a, b, 0);
-  uint64_t bits = seen_ballot(rawm);
+  uint64_t bits = seen_ballot(seen_raw(a, b, 0));
   if (nt > 0) issue(0, bits);
-  rawm = seen_raw(a, b, kTile);
-  fetch_bias(0, 0);
-  fetch_bias(1, 16);
-  for (int kt = 0; kt < nt; ++kt) {
-    const uint64_t next = seen_ballot(rawm);
-    cp_wait<0>();
-    __syncthreads();
-    if (kt == 0) {
+  float2 rawm = seen_raw(a, b, kTile);
+  auto body = [&](auto mode, int64_t j0, uint32_t off, bool nf) {
+    constexpr bool FAST = decltype(mode)::value;
+    uint32_t kc[KS], tc[KS];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
-          ldsm4(fg[m][k], la.at(sg, warp * MT + m, k));
-        }
-    }
-    if (kt + 1 < nt) issue(kt + 1, next);
-    rawm = seen_raw(a, b, (int64_t)(kt + 2) * kTile);
-    const int64_t j0 = (int64_t)kt * kTile;
-    const uint32_t tk = sk + (kt & 1) * kTile * S::RB, tv = sv + (kt & 1) * kTile * S::RB;
-    if (w0 >= a.nq || (bits == 0 && !(BT && a.dbias))) {
-      fetch_bias(0, j0 + 64);
-      fetch_bias(1, j0 + 80);
-      bits = next;
-      continue;
-    }
-#pragma unroll 2
-    for (int q = 0; q < 4; ++q) {  // 16 keys
+    for (int k = 0; k < KS; ++k) kc[k] = ka[k] + off, tc[k] = ta[k] + off;
+#pragma unroll 1
+    for (int hb = 0; hb < 2; ++hb) {
+    unrolled<2>([&](auto Q) {  // 16 keys
+      constexpr int q = decltype(Q)::value;
       float x[MT][2][4], y[MT][2][4];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t r[4], u[4];
-        ldsm4(r, lb.at(tk, q, k));
-        ldsm4(u, lb.at(tv, q, k));
+        ldsm4i<q * 16 * RB>(r, kc[k]);
+        ldsm4i<q * 16 * RB + kV>(u, kc[k]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           if (k == 0) {
@@ -413,16 +427,15 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
           }
         }
       }
-      const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[q & 1][m][r], n);
-      fetch_bias(q & 1, j0 + q * 16 + 32);
-      if (qbits != 0xffffu) {
-        const uint32_t mine = qbits >> (4 * t);
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[q][m][r], n);
+      fetch(q, 2 * hb + q + 2, j0, hb == 0 ? FAST || (bvec && j0 + (q + 3) * 16 <= nk) : nf);
+      if (!FAST) {
+        const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -438,10 +451,10 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const F2 p = prob2(&x[m][n][2 * r], nmx[m][r], lg[m][r]);
-            p.get(x[m][n][2 * r], x[m][n][2 * r + 1]);
+            if (!FAST) p.get(x[m][n][2 * r], x[m][n][2 * r + 1]);
             mul2(p, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[m][r])).get(y[m][n][2 * r], y[m][n][2 * r + 1]);
           }
-      if (peaked) {
+      if (!FAST && peaked) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -450,16 +463,15 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
             for (int e = 0; e < 4; ++e)
               if (x[m][n][e] == 1.f) y[m][n][e] = 0.f;
       }
-      if (BT && a.dbias) {
-        const int64_t j = j0 + q * 16 + 4 * t;
-        const bool fast = a.db_vec && j0 + q * 16 + 16 <= a.nk;
+      if (put) {
+        const int64_t j = j0 + hb * 32 + q * 16 + 4 * t;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
-            if (drow[m][r])
-              store_bias4<BT>(a, drow[m][r], j, fast, y[m][0][2 * r], y[m][0][2 * r + 1], y[m][1][2 * r],
-                              y[m][1][2 * r + 1]);
+            if (FAST || dp[m][r])
+              put_bias4<BT>(dp[m][r] + (hb * 32 + q * 16) * BS, j, nk, FAST || (a.db_vec && j0 + hb * 32 + q * 16 + 16 <= nk),
+                            y[m][0][2 * r], y[m][0][2 * r + 1], y[m][1][2 * r], y[m][1][2 * r + 1]);
       }
       uint32_t da[MT][4];
 #pragma unroll
@@ -467,15 +479,59 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) da[m][i] = pack_bf16(y[m][i >> 1][2 * (i & 1)], y[m][i >> 1][2 * (i & 1) + 1]);
 #pragma unroll
-      for (int c = 0; c < NB / 2; ++c) {
+      for (int c = 0; c < KS; ++c) {
         uint32_t f[4];
-        ldsm4_t(f, lt.at(tk, q, c));
+        ldsm4_ti<q * 16 * RB>(f, tc[c]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           mma(acc[m][2 * c], da[m], f[0], f[1]);
           mma(acc[m][2 * c + 1], da[m], f[2], f[3]);
         }
       }
+    });
+#pragma unroll
+    for (int k = 0; k < KS; ++k) kc[k] += 32 * RB, tc[k] += 32 * RB;
+    }
+  };
+  if (work) {
+    fetch(0, 0, 0, bvec && 16 <= nk);
+    fetch(1, 1, 0, bvec && 32 <= nk);
+  }
+  for (int kt = 0; kt < nt; ++kt) {
+    const uint64_t next = seen_ballot(rawm);
+    const int64_t j0 = (int64_t)kt * kTile;
+    cp_wait<0>();
+    __syncthreads();
+    if (kt == 0) {
+      const LaneAddr<DP> la = lane_a<DP>();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
+          ldsm4(fg[m][k], la.at(sg, warp * MT + m, k));
+        }
+    }
+    if (kt + 1 < nt) issue(kt + 1, next);
+    rawm = seen_raw(a, b, j0 + 2 * kTile);
+    if (work) {
+      const bool nf = bvec && j0 + kTile + 32 <= nk;  // the next tile's first two groups
+      const uint32_t off = (kt & 1) * kTile * RB;
+      if (bits == ~0ull && plain) {
+        body(std::true_type{}, j0, off, nf);
+      } else if (bits != 0 || put) {
+        body(std::false_type{}, j0, off, nf);
+      } else {  // no visible key
+        fetch(0, 4, j0, nf);
+        fetch(1, 5, j0, nf);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          bp[m][r] += kTile * BS;
+          if (dp[m][r]) dp[m][r] += kTile * BS;
+        }
     }
     bits = next;
   }
@@ -502,21 +558,21 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 template <int DP, int BT, int KM>
 __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
   using S = Tile<DP>;
-  constexpr int KR = 64 * KM, KS = DP / 16, NB = DP / 8;
+  constexpr int KR = 64 * KM, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr bool HOLD = DP <= 64;
+  constexpr int kG = 2 * kTile * RB;  // from a Q tile to its dO tile
   extern __shared__ __align__(128) unsigned char raw[];
-  const uint32_t sk = smem_addr(raw), sv = sk + KR * S::RB, sq = sv + KR * S::RB, sg = sq + 2 * kTile * S::RB,
-                 sc = sg + 2 * kTile * S::RB;
+  const uint32_t sk = smem_addr(raw), sv = sk + KR * RB, sq = sv + KR * RB, sc = sq + 2 * kG;
   const float4* cst = (const float4*)(raw + (sc - sk));  // [2][64]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), ln = lane_bn<DP>();
+  const LaneAddr<DP> lb = lane_b<DP>();
   unsigned id = blockIdx.x;
   const unsigned tile = id % (unsigned)a.tiles;
   id /= (unsigned)a.tiles;
   const int kh = id % a.KV, group = a.H / a.KV;
-  const int64_t b = id / a.KV;
+  const int64_t b = id / a.KV, nq = a.nq;
   const int64_t j0 = (int64_t)tile * KR, w0 = j0 + warp * 16 * KM;
-  const int per = (int)((a.nq + kTile - 1) / kTile);
+  const int per = (int)((nq + kTile - 1) / kTile);
   uint64_t live[KM];  // visible keys of the block, 64 at a time
 #pragma unroll
   for (int i = 0; i < KM; ++i) live[i] = seen_ballot(seen_raw(a, b, j0 + 64 * i));
@@ -524,31 +580,20 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
 #pragma unroll
   for (int i = 0; i < KM; ++i) {
     any |= live[i] != 0;
-    load_rows<DP, 64>(sk + i * 64 * S::RB, head_base(a.k, b, kh), a.k.ns, a.vec_k, j0 + 64 * i, a.nk, a.d, live[i]);
-    load_rows<DP, 64>(sv + i * 64 * S::RB, head_base(a.v, b, kh), a.v.ns, a.vec_v, j0 + 64 * i, a.nk, a.d, live[i]);
+    load_rows<DP, 64>(sk + i * 64 * RB, head_base(a.k, b, kh), a.k.ns, a.vec_k, j0 + 64 * i, a.nk, a.d, live[i]);
+    load_rows<DP, 64>(sv + i * 64 * RB, head_base(a.v, b, kh), a.v.ns, a.vec_v, j0 + 64 * i, a.nk, a.d, live[i]);
   }
   // the warp's keys, 16 KM bits
-  const uint32_t mine = (uint32_t)(live[(warp * 16 * KM) / 64] >> ((warp * 16 * KM) & 63)) &
-                        (KM == 2 ? 0xffffffffu : 0xffffu);
-  const bool full = mine == (KM == 2 ? 0xffffffffu : 0xffffu);
+  constexpr uint32_t kAll = KM == 2 ? 0xffffffffu : 0xffffu;
+  const uint32_t mine = (uint32_t)(live[(warp * 16 * KM) / 64] >> ((warp * 16 * KM) & 63)) & kAll;
   const bool bfast = a.bias_vec && w0 + 16 * KM <= a.nk;
-  // head and query tile of the step being loaded
-  int lh = 0, lt = 0, stage = 0;
-  auto issue = [&]() {
-    const int h = kh * group + lh;
-    const int64_t i0 = (int64_t)lt * kTile;
-    const uint32_t s = stage * kTile * S::RB;
-    load_rows<DP, kTile>(sq + s, head_base(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
-    load_rows<DP, kTile>(sg + s, head_base(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
-    if (threadIdx.x < kTile) {
-      const int64_t i = i0 + threadIdx.x;
-      const float4* p = (const float4*)a.rows + (b * a.H + h) * a.nq;
-      cp_async16(sc + (stage * kTile + threadIdx.x) * 16, i < a.nq ? p + i : p, i < a.nq);
-    }
-    cp_commit();
-    stage ^= 1;
-    if (++lt == per) lt = 0, ++lh;
-  };
+  const bool plain = mine == kAll && (BT == 0 || bfast);  // the body without checks
+  uint32_t qa[KS], ta[KS];
+  {
+    const LaneAddr<DP> la = lane_a<DP>(), ln = lane_bn<DP>();
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qa[k] = la.at(sq, 0, k), ta[k] = ln.at(sq, 0, k);
+  }
   const F2 scale(a.scale);
   float dk[KM][NB][4], dv[KM][NB][4];
 #pragma unroll
@@ -559,130 +604,164 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
       for (int e = 0; e < 4; ++e) dk[m][n][e] = dv[m][n][e] = 0.f;
   uint32_t fk[HOLD ? KM : 1][HOLD ? KS : 1][4], fv[HOLD ? KM : 1][HOLD ? KS : 1][4];
   Bias4<BT> ring[2][KM][2];
-  if (any && per > 0) {
-    issue();
-    for (int hh = 0; hh < group; ++hh) {
-      const int h = kh * group + hh;
-      // rows i0 + 16 blk + g (+ 8) of this head into a slot; 0 past the end
-      auto fetch_bias = [&](int slot, int64_t i0) {
-        if (BT == 0) return;
+  const char* bp[2] = {nullptr, nullptr};  // the lane's first key in rows g, g + 8 of the block that is read next
+  const int64_t bstep = a.b_rs * 16 * BS;
+  auto fetch = [&](int slot, int64_t i0, bool fast) {  // rows i0 .. i0 + 15; 0 past the end
+    if (BT == 0) return;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int64_t i = i0 + 8 * r + g;
-          if (i < a.nq) {
-            const char* p = bias_row<BT>(a, b, h, i);
+    for (int r = 0; r < 2; ++r) {
+      const bool row = fast || i0 + 8 * r + g < nq;
 #pragma unroll
-            for (int m = 0; m < KM; ++m) bias_load<BT>(ring[slot][m][r], p, w0 + 16 * m + 4 * t, a.nk, bfast);
+      for (int m = 0; m < KM; ++m) {
+        if (row) {
+          bias_get<BT>(ring[slot][m][r], bp[r] + 16 * m * BS, w0 + 16 * m + 4 * t, a.nk, fast || bfast);
+        } else {
+#pragma unroll
+          for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][m][r].w[w] = 0;
+        }
+      }
+      bp[r] += bstep;
+    }
+  };
+  auto body = [&](auto mode, int64_t i0, int s, bool nf) {
+    constexpr bool FAST = decltype(mode)::value;
+    const uint32_t off = s * kTile * RB;
+    uint32_t qc[KS], tc[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qc[k] = qa[k] + off, tc[k] = ta[k] + off;
+#pragma unroll 1
+    for (int hb = 0; hb < 2; ++hb) {
+    unrolled<2>([&](auto B) {  // 16 queries
+      constexpr int blk = decltype(B)::value;
+      float x[KM][2][4], y[KM][2][4];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t fq[4], fg[4];
+        ldsm4i<blk * 16 * RB>(fq, qc[k]);
+        ldsm4i<blk * 16 * RB + kG>(fg, qc[k]);
+#pragma unroll
+        for (int m = 0; m < KM; ++m) {
+          uint32_t rk[4], rv[4];
+          if (HOLD) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rk[i] = fk[m][k][i], rv[i] = fv[m][k][i];
           } else {
-#pragma unroll
-            for (int m = 0; m < KM; ++m)
-#pragma unroll
-              for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][m][r].w[w] = 0;
+            ldsm4(rk, lb.at(sk, warp * KM + m, k));
+            ldsm4(rv, lb.at(sv, warp * KM + m, k));
+          }
+          if (k == 0) {
+            mma0(x[m][0], fq, rk[0], rk[1]);
+            mma0(x[m][1], fq, rk[2], rk[3]);
+            mma0(y[m][0], fg, rv[0], rv[1]);
+            mma0(y[m][1], fg, rv[2], rv[3]);
+          } else {
+            mma(x[m][0], fq, rk[0], rk[1]);
+            mma(x[m][1], fq, rk[2], rk[3]);
+            mma(y[m][0], fg, rv[0], rv[1]);
+            mma(y[m][1], fg, rv[2], rv[3]);
           }
         }
+      }
+      const float4 c[2] = {cst[s * kTile + hb * 32 + blk * 16 + g], cst[s * kTile + hb * 32 + blk * 16 + 8 + g]};
+      const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)}, nd[2] = {F2(c[0].w), F2(c[1].w)};
+#pragma unroll
+      for (int m = 0; m < KM; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[blk][m][r], n);
+      fetch(blk, i0 + hb * 32 + blk * 16 + 32, hb == 0 ? FAST : nf);
+      if (!FAST) {
+#pragma unroll
+        for (int m = 0; m < KM; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!((mine >> (16 * m + 4 * t + 2 * n + e)) & 1)) x[m][n][e] = x[m][n][2 + e] = -INFINITY;
+      }
+      const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
+      uint32_t pa[KM][4], da[KM][4];
+#pragma unroll
+      for (int m = 0; m < KM; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float p[2], ds[2];
+            const F2 p2 = prob2(&x[m][n][2 * r], nmx[r], lg[r]);
+            p2.get(p[0], p[1]);
+            mul2(p2, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
+            if (peaked) {
+              if (p[0] == 1.f) ds[0] = 0.f;
+              if (p[1] == 1.f) ds[1] = 0.f;
+            }
+            pa[m][2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
+            da[m][2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
+          }
+#pragma unroll
+      for (int n = 0; n < KS; ++n) {
+        uint32_t fg[4], fq[4];
+        ldsm4_ti<blk * 16 * RB + kG>(fg, tc[n]);
+        ldsm4_ti<blk * 16 * RB>(fq, tc[n]);
+#pragma unroll
+        for (int m = 0; m < KM; ++m) {
+          mma(dv[m][2 * n], pa[m], fg[0], fg[1]);
+          mma(dv[m][2 * n + 1], pa[m], fg[2], fg[3]);
+          mma(dk[m][2 * n], da[m], fq[0], fq[1]);
+          mma(dk[m][2 * n + 1], da[m], fq[2], fq[3]);
+        }
+      }
+    });
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qc[k] += 32 * RB, tc[k] += 32 * RB;
+    }
+  };
+  if (any && per > 0) {
+    int it = 0;
+    for (int hh = 0; hh < group; ++hh) {
+      const int h = kh * group + hh;
+      Stream<DP> qs(head_base(a.q, b, h), a.q.ns, a.vec_q, 0, nq, a.d), gs(head_base(a.g, b, h), a.g.ns, a.vec_g, 0, nq, a.d);
+      const float4* pr = (const float4*)a.rows + (b * a.H + h) * nq;
+      auto issue = [&](int qt, int s) {
+        const uint64_t rows = first_bits(nq - (int64_t)qt * kTile);
+        qs.next(sq + s * kTile * RB, rows, a.vec_q);
+        gs.next(sq + kG + s * kTile * RB, rows, a.vec_g);
+        if (threadIdx.x < kTile) {
+          const int64_t i = (int64_t)qt * kTile + threadIdx.x;
+          cp_async16(sc + (s * kTile + threadIdx.x) * 16, i < nq ? pr + i : pr, i < nq);
+        }
+        cp_commit();
       };
-      fetch_bias(0, 0);
-      fetch_bias(1, 16);
-      for (int qt = 0; qt < per; ++qt) {
-        const int s = (hh * per + qt) & 1;
+      if (hh > 0) __syncthreads();  // the last head's tiles are done with
+      issue(0, it & 1);
+      if (BT) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) bp[r] = bias_row<BT>(a, b, h, 8 * r + g) + (w0 + 4 * t) * BS;
+      }
+      fetch(0, 0, false);
+      fetch(1, 16, false);
+      for (int qt = 0; qt < per; ++qt, ++it) {
+        const int s = it & 1;
         cp_wait<0>();
         __syncthreads();
-        if (HOLD && hh == 0 && qt == 0) {
+        if (HOLD && it == 0) {
 #pragma unroll
           for (int m = 0; m < (HOLD ? KM : 1); ++m)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
+            for (int k = 0; k < (HOLD ? KS : 1); ++k) {
               ldsm4(fk[m][k], lb.at(sk, warp * KM + m, k));
               ldsm4(fv[m][k], lb.at(sv, warp * KM + m, k));
             }
         }
-        if (lh < group) issue();
+        if (qt + 1 < per) issue(qt + 1, s ^ 1);
         if (mine == 0) continue;  // none of the warp's keys is visible
-        const uint32_t tq = sq + s * kTile * S::RB, tg = sg + s * kTile * S::RB;
         const int64_t i0 = (int64_t)qt * kTile;
-#pragma unroll 2
-        for (int blk = 0; blk < 4; ++blk) {  // 16 queries
-          float x[KM][2][4], y[KM][2][4];
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            uint32_t fq[4], fg[4];
-            ldsm4(fq, la.at(tq, blk, k));
-            ldsm4(fg, la.at(tg, blk, k));
-#pragma unroll
-            for (int m = 0; m < KM; ++m) {
-              uint32_t rk[4], rv[4];
-              if (HOLD) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rk[i] = fk[m][k][i], rv[i] = fv[m][k][i];
-              } else {
-                ldsm4(rk, lb.at(sk, warp * KM + m, k));
-                ldsm4(rv, lb.at(sv, warp * KM + m, k));
-              }
-              if (k == 0) {
-                mma0(x[m][0], fq, rk[0], rk[1]);
-                mma0(x[m][1], fq, rk[2], rk[3]);
-                mma0(y[m][0], fg, rv[0], rv[1]);
-                mma0(y[m][1], fg, rv[2], rv[3]);
-              } else {
-                mma(x[m][0], fq, rk[0], rk[1]);
-                mma(x[m][1], fq, rk[2], rk[3]);
-                mma(y[m][0], fg, rv[0], rv[1]);
-                mma(y[m][1], fg, rv[2], rv[3]);
-              }
-            }
-          }
-          const float4 c[2] = {cst[s * kTile + blk * 16 + g], cst[s * kTile + blk * 16 + 8 + g]};
-          const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)},
-                   nd[2] = {F2(c[0].w), F2(c[1].w)};
-#pragma unroll
-          for (int m = 0; m < KM; ++m)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[blk & 1][m][r], n);
-          fetch_bias(blk & 1, i0 + blk * 16 + 32);
-          if (!full) {
-#pragma unroll
-            for (int m = 0; m < KM; ++m)
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if (!((mine >> (16 * m + 4 * t + 2 * n + e)) & 1)) x[m][n][e] = x[m][n][2 + e] = -INFINITY;
-          }
-          const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
-          uint32_t pa[KM][4], da[KM][4];
-#pragma unroll
-          for (int m = 0; m < KM; ++m)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                float p[2], ds[2];
-                const F2 p2 = prob2(&x[m][n][2 * r], nmx[r], lg[r]);
-                p2.get(p[0], p[1]);
-                mul2(p2, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
-                if (peaked) {
-                  if (p[0] == 1.f) ds[0] = 0.f;
-                  if (p[1] == 1.f) ds[1] = 0.f;
-                }
-                pa[m][2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
-                da[m][2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
-              }
-#pragma unroll
-          for (int n = 0; n < NB / 2; ++n) {
-            uint32_t fg[4], fq[4];
-            ldsm4_t(fg, ln.at(tg, blk, n));
-            ldsm4_t(fq, ln.at(tq, blk, n));
-#pragma unroll
-            for (int m = 0; m < KM; ++m) {
-              mma(dv[m][2 * n], pa[m], fg[0], fg[1]);
-              mma(dv[m][2 * n + 1], pa[m], fg[2], fg[3]);
-              mma(dk[m][2 * n], da[m], fq[0], fq[1]);
-              mma(dk[m][2 * n + 1], da[m], fq[2], fq[3]);
-            }
-          }
-        }
+        const bool nf = plain && i0 + kTile + 32 <= nq;  // the next tile's first two blocks
+        if (plain && i0 + kTile <= nq)
+          body(std::true_type{}, i0, s, nf);
+        else
+          body(std::false_type{}, i0, s, nf);
       }
     }
   }

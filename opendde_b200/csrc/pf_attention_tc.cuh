@@ -2,6 +2,8 @@
 // pf_attention_f32_tc.cu): swizzled shared tiles and their ldmatrix addresses, products, visible keys, bias
 // fragments, scores. See pf_attention_bf16.cu for the layout.
 #pragma once
+#include <type_traits>
+
 #include "pf_attention.cuh"
 #include "pf_f32x2.cuh"
 
@@ -72,6 +74,27 @@ __device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
+// the same at a constant offset from the address
+template <int OFF>
+__device__ __forceinline__ void ldsm4i(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr), "n"(OFF));
+}
+template <int OFF>
+__device__ __forceinline__ void ldsm4_ti(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr), "n"(OFF));
+}
+// f(0) .. f(N - 1) with constant arguments
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<N, I + 1>(f);
+  }
+}
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -122,6 +145,49 @@ __device__ __forceinline__ const bf16* head_base(const Heads& s, int64_t b, int 
   return (const bf16*)s.p + b * s.bs + (int64_t)h * s.hs;
 }
 
+// One operand's tiles of 64 rows, one after the other: a thread keeps its place in the tile, so a tile costs
+// an add and a copy for each of its chunks.
+template <int DP>
+struct Stream {
+  static constexpr int CH = Tile<DP>::CH;
+  static constexpr bool kPlain = kThreads % CH == 0;  // else rows and chunks of a thread change from pass to pass
+  static constexpr int RP = kThreads / CH, PASSES = kPlain ? kTile / RP : 1;
+  const bf16* base;
+  const char* p;
+  int64_t ns, step, r0, n;
+  uint32_t dst;
+  int row, d, vec;
+  bool col;
+  // rows r0, r0 + 64, ... of `base`, which has n
+  __device__ __forceinline__ Stream(const bf16* base, int64_t ns, int vec, int64_t r0, int64_t n, int d)
+      : base(base), ns(ns), r0(r0), n(n), d(d), vec(vec && kPlain) {
+    row = threadIdx.x / CH;
+    const int c = threadIdx.x - row * CH;
+    p = (const char*)(base + (r0 + row) * ns + c * 8);
+    step = RP * ns * 2;
+    dst = Tile<DP>::off(row, c);
+    col = c * 8 < d;
+  }
+  // rows without a bit in `live`, which has none past the end, are zero
+  __device__ __forceinline__ void next(uint32_t sm, uint64_t live, int vec16) {
+    if (vec) {
+      const uint32_t half[2] = {(uint32_t)live, (uint32_t)(live >> 32)};
+#pragma unroll
+      for (int j = 0; j < PASSES; ++j) {
+        const bool ok = col && ((half[j * RP / 32] >> (row + j * RP % 32)) & 1);
+        // 128 channels: rows 8 apart differ in one bit of the swizzle
+        const uint32_t at = DP == 128 ? (dst ^ ((j & 1) << 5)) : dst;
+        cp_async16(sm + at + j * RP * Tile<DP>::RB, p + j * step, ok);
+      }
+      p += PASSES * step;
+    } else {
+      load_rows<DP, kTile>(sm, base, ns, vec16, r0, n, d, live);
+    }
+    r0 += kTile;
+  }
+};
+__device__ __forceinline__ uint64_t first_bits(int64_t n) { return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1); }
+
 // ---------------------------------------------------------------- visible keys
 
 // Mask values of keys j0 + lane and j0 + 32 + lane (0 past the end), read a tile ahead of their use.
@@ -155,15 +221,15 @@ __device__ __forceinline__ const char* bias_row(const Args& a, int64_t b, int h,
   if (BT == 0) return nullptr;
   return (const char*)a.bias + (b * a.b_bs + (int64_t)h * a.b_hs + i * a.b_rs) * (BT == 2 ? 4 : 2);
 }
-// keys j .. j + 3 of the row at p; `fast`: all exist and are aligned together
+// keys j .. j + 3, the first of them at p; `fast`: all exist and are aligned together
 template <int BT>
-__device__ __forceinline__ void bias_load(Bias4<BT>& r, const char* p, int64_t j, int64_t nk, bool fast) {
+__device__ __forceinline__ void bias_get(Bias4<BT>& r, const char* p, int64_t j, int64_t nk, bool fast) {
   if (BT == 1) {
     if (fast) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p + j * 2);
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
       r.w[0] = v.x, r.w[1] = v.y;
     } else {
-      const unsigned short* q = (const unsigned short*)p + j;
+      const unsigned short* q = (const unsigned short*)p;
       uint32_t e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) e[i] = j + i < nk ? q[i] : 0;
@@ -171,14 +237,19 @@ __device__ __forceinline__ void bias_load(Bias4<BT>& r, const char* p, int64_t j
     }
   } else if (BT == 2) {
     if (fast) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + j * 4);
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
       r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
     } else {
-      const uint32_t* q = (const uint32_t*)p + j;
+      const uint32_t* q = (const uint32_t*)p;
 #pragma unroll
       for (int i = 0; i < 4; ++i) r.w[i] = j + i < nk ? q[i] : 0;
     }
   }
+}
+// the same of the row at p
+template <int BT>
+__device__ __forceinline__ void bias_load(Bias4<BT>& r, const char* p, int64_t j, int64_t nk, bool fast) {
+  bias_get<BT>(r, p + j * (BT == 2 ? 4 : 2), j, nk, fast);
 }
 template <int BT>
 __device__ __forceinline__ float bias_val(const Bias4<BT>& r, int i) {
@@ -207,31 +278,38 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// one row's four columns of a group as stored by the products: x[0][2r..] then x[1][2r..]
+// one row's four columns of a group as the products leave them, x[0][2r..] then x[1][2r..]: keys j .. j + 3,
+// the first of them at p
 template <int BT>
-__device__ __forceinline__ void store_bias4(const Args& a, char* p, int64_t j, bool fast, float v0, float v1, float v2,
-                                            float v3) {
+__device__ __forceinline__ void put_bias4(char* p, int64_t j, int64_t nk, bool fast, float v0, float v1, float v2,
+                                          float v3) {
   if (BT == 2) {
-    float* q = (float*)p + j;
+    float* q = (float*)p;
     if (fast) {
       *reinterpret_cast<float4*>(q) = make_float4(v0, v1, v2, v3);
     } else {
-      if (j < a.nk) q[0] = v0;
-      if (j + 1 < a.nk) q[1] = v1;
-      if (j + 2 < a.nk) q[2] = v2;
-      if (j + 3 < a.nk) q[3] = v3;
+      if (j < nk) q[0] = v0;
+      if (j + 1 < nk) q[1] = v1;
+      if (j + 2 < nk) q[2] = v2;
+      if (j + 3 < nk) q[3] = v3;
     }
   } else {
-    bf16* q = (bf16*)p + j;
+    bf16* q = (bf16*)p;
     if (fast) {
       *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf16(v0, v1), pack_bf16(v2, v3));
     } else {
-      if (j < a.nk) q[0] = __float2bfloat16_rn(v0);
-      if (j + 1 < a.nk) q[1] = __float2bfloat16_rn(v1);
-      if (j + 2 < a.nk) q[2] = __float2bfloat16_rn(v2);
-      if (j + 3 < a.nk) q[3] = __float2bfloat16_rn(v3);
+      if (j < nk) q[0] = __float2bfloat16_rn(v0);
+      if (j + 1 < nk) q[1] = __float2bfloat16_rn(v1);
+      if (j + 2 < nk) q[2] = __float2bfloat16_rn(v2);
+      if (j + 3 < nk) q[3] = __float2bfloat16_rn(v3);
     }
   }
+}
+// the same of the row at p
+template <int BT>
+__device__ __forceinline__ void store_bias4(const Args& a, char* p, int64_t j, bool fast, float v0, float v1, float v2,
+                                            float v3) {
+  put_bias4<BT>(p + j * (BT == 2 ? 4 : 2), j, a.nk, fast, v0, v1, v2, v3);
 }
 
 // 8 consecutive accumulator columns of a row, two per lane
