@@ -1006,10 +1006,10 @@ struct PlaneSmem {  // byte offsets
 
 template <int BT>
 __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* part, int parts, int G, int tcols) {
-  constexpr int DP = 32, KS = 2, NB = 4;
+  constexpr int DP = 32, KS = 2, NB = 4, BS = BT == 2 ? 4 : 2;
   using S = Tile<DP>;
   extern __shared__ __align__(128) unsigned char raw[];
-  const int nkp = (int)((a.nk + 15) / 16) * 16;
+  const int nkp = (int)((a.nk + 31) / 32) * 32;
   const PlaneSmem L(nkp);
   const uint32_t s0 = smem_addr(raw);
   uint32_t* vis = (uint32_t*)(raw + L.vis);  // [3][32] words of visible keys
@@ -1024,7 +1024,7 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
   const int pt = id / a.H;
   const int64_t b0 = a.B * pt / parts, b1 = a.B * (pt + 1) / parts;
   const int64_t i0 = (int64_t)tile * 64, w0 = i0 + rg * 16;
-  const int words = (nkp + 31) / 32;
+  const int words = nkp / 32;
 
   if (warp == 0) {
     sm100::tmem_alloc(smem_addr(tptr), tcols);
@@ -1043,28 +1043,43 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
                    sg = sq + 4096;
     const bf16 *pk = head_base(a.k, b, kh), *pv = head_base(a.v, b, kh), *pq = head_base(a.q, b, h),
                *pg = head_base(a.g, b, h);
-    auto rows = [&](uint32_t sm, const bf16* p, int64_t ns, int vec, int64_t r0, int n, int64_t end, bool masked) {
+    const int row = threadIdx.x >> 2, c = threadIdx.x & 3;
+    const uint32_t dst = S::off(row, c);  // rows 128 apart have the same swizzle
+    const bool col = c * 8 < a.d;
+    auto keys = [&](uint32_t sm, const bf16* p, int64_t ns, int vec) {
       if (vec) {
-        for (int i = threadIdx.x; i < n * 4; i += kPlaneThreads) {
-          const int r = i >> 2, c = i & 3;
-          const bool ok = r0 + r < end && c * 8 < a.d && (!masked || ((v[r >> 5] >> (r & 31)) & 1));
-          cp_async16(sm + S::off(r, c), ok ? p + (r0 + r) * ns + c * 8 : p, ok);
-        }
+        const char* q = (const char*)(p + row * ns + c * 8);
+        const int64_t step = ns * 256;
+        for (int r = row; r < nkp; r += 128, q += step, sm += 128 * S::RB)
+          cp_async16(sm + dst, q, col && ((v[r >> 5] >> (r & 31)) & 1));  // no bits past the end
       } else {
-        for (int i = threadIdx.x; i < n * DP; i += kPlaneThreads) {
-          const int r = i / DP, c = i % DP;
-          const bool ok = r0 + r < end && c < a.d && (!masked || ((v[r >> 5] >> (r & 31)) & 1));
-          const bf16 x = ok ? p[(r0 + r) * ns + c] : from_f<bf16>(0.f);
-          asm volatile("st.shared.b16 [%0], %1;" ::"r"(sm + S::off(r, c >> 3) + (c & 7) * 2),
+        for (int i = threadIdx.x; i < nkp * DP; i += kPlaneThreads) {
+          const int r = i / DP, e = i % DP;
+          const bool ok = e < a.d && ((v[r >> 5] >> (r & 31)) & 1);
+          const bf16 x = ok ? p[r * ns + e] : from_f<bf16>(0.f);
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(sm + S::off(r, e >> 3) + (e & 7) * 2),
                        "h"(*reinterpret_cast<const unsigned short*>(&x))
                        : "memory");
         }
       }
     };
-    rows(sk, pk, a.k.ns, a.vec_k, 0, nkp, a.nk, true);
-    rows(sv, pv, a.v.ns, a.vec_v, 0, nkp, a.nk, true);
-    rows(sq, pq, a.q.ns, a.vec_q, i0, 64, a.nq, false);
-    rows(sg, pg, a.g.ns, a.vec_g, i0, 64, a.nq, false);
+    auto queries = [&](uint32_t sm, const bf16* p, int64_t ns, int vec) {
+      if (vec) {
+        if (row < 64) cp_async16(sm + dst, p + (i0 + row) * ns + c * 8, col && i0 + row < a.nq);
+      } else {
+        for (int i = threadIdx.x; i < 64 * DP; i += kPlaneThreads) {
+          const int r = i / DP, e = i % DP;
+          const bf16 x = e < a.d && i0 + r < a.nq ? p[(i0 + r) * ns + e] : from_f<bf16>(0.f);
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(sm + S::off(r, e >> 3) + (e & 7) * 2),
+                       "h"(*reinterpret_cast<const unsigned short*>(&x))
+                       : "memory");
+        }
+      }
+    };
+    keys(sk, pk, a.k.ns, a.vec_k);
+    keys(sv, pv, a.v.ns, a.vec_v);
+    queries(sq, pq, a.q.ns, a.vec_q);
+    queries(sg, pg, a.g.ns, a.vec_g);
     if (threadIdx.x < 64) {
       const int64_t i = i0 + threadIdx.x;
       const float4* pr = (const float4*)a.rows + (b * a.H + h) * a.nq;
@@ -1074,23 +1089,21 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
   };
   if (b0 < b1) see(b0);
   if (b0 + 1 < b1) see(b0 + 1);
-  const char* brow[2];
+  const int q0 = sl * G;  // the warp's groups: q0 .. q0 + G - 1, in pairs
+  const char* brow[2];    // the lane's first key of the first pair
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int64_t i = w0 + r * 8 + g;
-    brow[r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1);
+    brow[r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1) + (q0 * 16 + 4 * t) * BS;
   }
-  const int q0 = sl * G;  // the warp's groups: q0 .. q0 + G - 1
   Bias4<BT> ring[2][2];
-  auto fetch_bias = [&](int slot, int q) {
-    const int64_t j0 = (int64_t)(q0 + q) * 16;
-    if (j0 >= a.nk) return;
-    const bool fast = a.bias_vec && j0 + 16 <= a.nk;
+  auto fetch = [&](int u, const char* const (&p)[2], int64_t j, bool fast) {  // group u of the pair at key j
 #pragma unroll
-    for (int r = 0; r < 2; ++r) bias_load<BT>(ring[slot][r], brow[r], j0 + 4 * t, a.nk, fast);
+    for (int r = 0; r < 2; ++r) bias_get<BT>(ring[u][r], p[r] + u * 16 * BS, j + u * 16 + 4 * t, a.nk, fast);
   };
-  fetch_bias(0, 0);
-  fetch_bias(1, 1);
+  auto inside = [&](int64_t j) { return a.bias_vec && j + 32 <= a.nk; };
+  fetch(0, brow, q0 * 16, inside(q0 * 16));
+  fetch(1, brow, q0 * 16, inside(q0 * 16));
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
@@ -1132,25 +1145,24 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll 1
-    for (int qq = 0; qq < G; qq += 2) {
+    uint32_t ka[KS], ta[KS];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int q = qq + u, qa = q0 + q;  // group of the warp, of the row
-        const int nextq = q + 2 < G ? q + 2 : q + 2 - G;  // the next entry starts over with the same bias
-        const uint32_t bits = qa * 16 < nkp ? (v[qa >> 1] >> ((qa & 1) * 16)) & 0xffffu : 0;
-        if (bits == 0 || w0 >= a.nq) {
-          fetch_bias(u, nextq);
-          continue;
-        }
+    for (int k = 0; k < KS; ++k) ka[k] = lb.at(sk, q0, k), ta[k] = lt.at(sk, q0, k);
+    const uint32_t dv = sv - sk;
+    uint32_t tm_at = tm0;
+    const char* bp[2] = {brow[0], brow[1]};
+    auto pair = [&](auto mode, uint32_t bits, int64_t nj, bool nf) {
+      constexpr bool FAST = decltype(mode)::value;
+      unrolled<2>([&](auto U) {
+        constexpr int u = decltype(U)::value;
         uint32_t tm[8];
-        tmem_ld8(tm0 + q * 8, tm);
+        tmem_ld8(tm_at + u * 8, tm);
         float x[2][4], y[2][4];
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t r[4], w[4];
-          ldsm4(r, lb.at(sk, qa, k));
-          ldsm4(w, lb.at(sv, qa, k));
+          ldsm4i<u * 16 * S::RB>(r, ka[k]);
+          ldsm4i<u * 16 * S::RB>(w, ka[k] + dv);
           if (k == 0) {
             mma0(x[0], fq[k], r[0], r[1]);
             mma0(x[1], fq[k], r[2], r[3]);
@@ -1167,23 +1179,23 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, ring[u][r], n);
-        fetch_bias(u, nextq);
-        if (bits != 0xffffu) {
+        fetch(u, bp, nj, nf);
+        if (!FAST) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (!((bits >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
+              if (!((bits >> (u * 16 + 4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const F2 p = prob2(&x[n][2 * r], nmx[r], lg[r]);
-            p.get(x[n][2 * r], x[n][2 * r + 1]);
+            if (!FAST) p.get(x[n][2 * r], x[n][2 * r + 1]);
             mul2(p, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(y[n][2 * r], y[n][2 * r + 1]);
           }
-        if (peaked) {
+        if (!FAST && peaked) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -1194,9 +1206,9 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
 #pragma unroll
         for (int i = 0; i < 4; ++i) da[i] = pack_bf16(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1]);
 #pragma unroll
-        for (int c = 0; c < NB / 2; ++c) {
+        for (int c = 0; c < KS; ++c) {
           uint32_t f[4];
-          ldsm4_t(f, lt.at(sk, qa, c));
+          ldsm4_ti<u * 16 * S::RB>(f, ta[c]);
           mma(acc[2 * c], da, f[0], f[1]);
           mma(acc[2 * c + 1], da, f[2], f[3]);
         }
@@ -1209,8 +1221,31 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
               .get(s, s1);
           tm[2 * i] = __float_as_uint(s), tm[2 * i + 1] = __float_as_uint(s1);
         }
-        tmem_st8(tm0 + q * 8, tm);
+        tmem_st8(tm_at + u * 8, tm);
+      });
+    };
+#pragma unroll 1
+    for (int qq = 0; qq < G; qq += 2) {
+      const int word = (q0 + qq) >> 1;
+      const uint32_t bits = word < words ? v[word] : 0;
+      const bool last = qq + 2 >= G;  // the next entry starts over with the same bias
+#pragma unroll
+      for (int r = 0; r < 2; ++r) bp[r] = last ? brow[r] : bp[r] + 32 * BS;
+      const int64_t nj = (int64_t)(q0 + (last ? 0 : qq + 2)) * 16;
+      const bool nf = inside(nj);
+      if (w0 < a.nq) {
+        if (bits == 0xffffffffu && !peaked) {
+          pair(std::true_type{}, bits, nj, nf);
+        } else if (bits != 0) {
+          pair(std::false_type{}, bits, nj, nf);
+        } else {  // no visible key
+          fetch(0, bp, nj, nf);
+          fetch(1, bp, nj, nf);
+        }
       }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) ka[k] += 32 * S::RB, ta[k] += 32 * S::RB;
+      tm_at += 16;
     }
     sm100::tmem_st_wait();
     if (a.dq) {
@@ -1320,7 +1355,7 @@ int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
 
 template <int BT>
 int launch_plane(Args a, float* part, int parts, double flops, cudaStream_t st) {
-  const int nkp = (int)((a.nk + 15) / 16) * 16;
+  const int nkp = (int)((a.nk + 31) / 32) * 32;  // whole pairs of groups
   const int G = ((nkp / 16 + 3) / 4 + 1) / 2 * 2;  // groups of a quarter, an even number
   int tcols = 32;
   while (tcols < 4 * G * 8) tcols *= 2;
