@@ -171,7 +171,6 @@ int attention_bwd(const pf_attention_call& c, void* ws, size_t ws_bytes, cudaStr
     a.dv_bs = dv.batch_stride;
     a.dv_ns = dv.seq_stride;
     a.dv_hs = dv.head_stride;
-    PF_TRY(launch(s.dtype, attn::kDkv, a, 4 * pair, st));
   }
   a.dq = dq.ptr;
   a.o_bs = dq.batch_stride;
@@ -179,10 +178,11 @@ int attention_bwd(const pf_attention_call& c, void* ws, size_t ws_bytes, cudaStr
   a.o_hs = dq.head_stride;
   const bool sum = shared && s.n_q > 0 && s.n_k > 0;
   const SharedPlan plan = sum ? shared_plan(s) : SharedPlan{false, 1};
-  if ((dq.ptr || (dbias.ptr && !shared)) && !plan.plane) {
-    a.dbias = shared ? nullptr : dbias.ptr;
-    PF_TRY(launch(s.dtype, attn::kDq, a, 3 * pair, st));
-  }
+  a.dbias = shared ? nullptr : dbias.ptr;
+  const bool by_rows = (dq.ptr || a.dbias) && !plan.plane;
+  if (by_rows || dk.ptr)
+    PF_TRY(launch(s.dtype, !by_rows ? attn::kDkv : (dk.ptr ? attn::kDqDkv : attn::kDq), a,
+                  (by_rows ? 3 * pair : 0.0) + (dk.ptr ? 4 * pair : 0.0), st));
   if (!sum) return PF_OK;
   a.dbias = dbias.ptr;
   float* part = plan.parts > 1 ? ar.take<float>((size_t)plan.parts * s.heads * s.n_q * s.n_k) : nullptr;

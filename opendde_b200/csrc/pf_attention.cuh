@@ -83,10 +83,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-enum Kind { kFwd, kDq, kDkv };
+enum Kind { kFwd, kDq, kDkv, kDqDkv };
 
 // One translation unit per storage type. launch_*: the forward, dq (with dbias of one batch entry per
-// plane where a.dbias is set) or dk and dv; dbias_*: the gradient of a shared bias, from `parts` partial
+// plane where a.dbias is set), dk and dv, or all three; dbias_*: the gradient of a shared bias, from `parts` partial
 // planes [parts][H][n_q][n_k] in `part` where parts > 1; rows_*: the row constants, 16 bytes per row.
 int launch_bf16(Kind kind, const Args& a, double flops, cudaStream_t st);
 int launch_f32(Kind kind, const Args& a, double flops, cudaStream_t st);

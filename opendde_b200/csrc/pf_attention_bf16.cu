@@ -296,48 +296,63 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
 
 // ---------------------------------------------------------------- row constants
 
-// Eight lanes per row (b, i, h): D, and {m, -log2 l, peak, -D}; peak = 1 where one key has all of the
-// row's weight in fp32 (l = 1).
+// D, and {m, -log2 l, peak, -D} of the rows (b, h, i), i fastest; peak = 1 where one key has all of the
+// row's weight in fp32 (l = 1). L lanes per row, eight channels each (VEC: as one access of o, its low
+// halves and do).
+template <int L, bool VEC>
 __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ stats, Heads o,
                                               const int16_t* __restrict__ lo, float4* __restrict__ rows) {
-  const int sub = threadIdx.x & 7;
-  const int64_t r = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  const bool live = r < a.rows_plane;
-  const int64_t rr = live ? r : 0;
-  const int h = (int)(rr % a.H);
-  const int64_t bi = rr / a.H, b = bi / a.nq, i = bi - b * a.nq;
-  const bf16* po = head_base(o, b, h) + i * o.ns;
-  const bf16* pg = head_base(a.g, b, h) + i * a.g.ns;
+  const int sub = threadIdx.x & (L - 1);
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const bool live = at < a.rows_plane;
+  const int64_t r = live ? at : 0, bh = r / a.nq, i = r - bh * a.nq, b = bh / a.H;
+  const int h = (int)(bh - b * a.H), c = sub * 8;
+  const bf16* po = head_base(o, b, h) + i * o.ns + c;
+  const bf16* pg = head_base(a.g, b, h) + i * a.g.ns + c;
+  const int16_t* pl = lo + ((b * a.nq + i) * a.H + h) * a.d + c;
   float s = 0.f;
-  if (live)
-    for (int e = sub; e < a.d; e += 8) {
-      float v = to_f(po[e]);
-      if (v == v) v = __uint_as_float(__float_as_uint(v) + (int)lo[rr * a.d + e]);
-      s += v * to_f(pg[e]);
+  if (VEC) {
+    if (live && c < a.d) {
+      const uint4 vo = *reinterpret_cast<const uint4*>(po), vg = *reinterpret_cast<const uint4*>(pg),
+                  vl = *reinterpret_cast<const uint4*>(pl);
+      const uint32_t wo[4] = {vo.x, vo.y, vo.z, vo.w}, wg[4] = {vg.x, vg.y, vg.z, vg.w}, wl[4] = {vl.x, vl.y, vl.z, vl.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float a0 = lo_f(wo[k]), a1 = hi_f(wo[k]);
+        const int l0 = (int)(wl[k] << 16) >> 16, l1 = (int)wl[k] >> 16;
+        s += (a0 == a0 ? __uint_as_float(__float_as_uint(a0) + l0) : a0) * lo_f(wg[k]);
+        s += (a1 == a1 ? __uint_as_float(__float_as_uint(a1) + l1) : a1) * hi_f(wg[k]);
+      }
     }
-  s += __shfl_xor_sync(0xffffffffu, s, 1);
-  s += __shfl_xor_sync(0xffffffffu, s, 2);
-  s += __shfl_xor_sync(0xffffffffu, s, 4);
+  } else if (live) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < a.d) {
+        float v = to_f(po[e]);
+        if (v == v) v = __uint_as_float(__float_as_uint(v) + (int)pl[e]);
+        s += v * to_f(pg[e]);
+      }
+  }
+#pragma unroll
+  for (int k = 1; k < L; k <<= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (!live || sub) return;
-  const int64_t at = (b * a.H + h) * a.nq + i;
   const float m = stats[at], l = stats[a.rows_plane + at];
-  const bool none = l == 0.f;
+  const bool none = l == 0.f;  // sees nothing: p = exp(t - inf) = 0
   rows[at] = make_float4(none ? INFINITY : m, none ? 0.f : -log2f(l), l == 1.f ? 1.f : 0.f, none ? 0.f : -s);
 }
 
 // ---------------------------------------------------------------- dq (and dbias of one batch entry)
 
 template <int DP, int BT, int MT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
+__device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
   constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr int kV = 2 * kTile * RB;  // from a K tile to its V tile
   extern __shared__ __align__(128) unsigned char raw[];
   const uint32_t sq = smem_addr(raw), sg = sq + QR * RB, sk = sg + QR * RB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  unsigned id = blockIdx.x;
-  const unsigned tile = id % (unsigned)a.tiles;
-  id /= (unsigned)a.tiles;
+  const unsigned tile = id % (unsigned)tiles;
+  id /= (unsigned)tiles;
   const int h = id % a.H, kh = h / (a.H / a.KV);
   const int64_t b = id / a.H, nk = a.nk;
   const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT;
@@ -556,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
 
 // 16 KM keys per warp; HOLD: their fragments stay in registers.
 template <int DP, int BT, int KM>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
+__device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
   constexpr int KR = 64 * KM, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr bool HOLD = DP <= 64;
@@ -566,9 +581,8 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
   const float4* cst = (const float4*)(raw + (sc - sk));  // [2][64]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const LaneAddr<DP> lb = lane_b<DP>();
-  unsigned id = blockIdx.x;
-  const unsigned tile = id % (unsigned)a.tiles;
-  id /= (unsigned)a.tiles;
+  const unsigned tile = id % (unsigned)tiles;
+  id /= (unsigned)tiles;
   const int kh = id % a.KV, group = a.H / a.KV;
   const int64_t b = id / a.KV, nq = a.nq;
   const int64_t j0 = (int64_t)tile * KR, w0 = j0 + warp * 16 * KM;
@@ -782,6 +796,23 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
         store_pair(ov, n * 8 + 2 * t, a.d, vv, dv[m][n][2 * r], dv[m][n][2 * r + 1]);
       }
     }
+}
+
+template <int DP, int BT, int MT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
+  dq_block<DP, BT, MT>(a, blockIdx.x, a.tiles);
+}
+template <int DP, int BT, int KM>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
+  dkv_block<DP, BT, KM>(a, blockIdx.x, a.tiles);
+}
+// Both in one launch, dk and dv in the first blocks: where neither fills the machine they run side by side.
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dqkv(Args a, unsigned dkv_blocks) {
+  if (blockIdx.x < dkv_blocks)
+    dkv_block<DP, BT, 1>(a, blockIdx.x, (a.nk + 63) / 64);
+  else
+    dq_block<DP, BT, 1>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
 
 // ---------------------------------------------------------------- dbias shared by the batch
@@ -1323,26 +1354,45 @@ template <int DP, int BT>
 int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   constexpr size_t RB = Tile<DP>::RB;
   // two row blocks per warp where the accumulators leave room for them and there are blocks enough
-  const int64_t rows = kind == kDkv ? a.nk : a.nq, heads = (kind == kDkv ? a.KV : a.H) * a.B;
-  const int64_t t1 = (rows + 63) / 64, t2 = (rows + 127) / 128;
-  const bool two = DP == 32 && t2 * heads >= 3 * 148;
-  a.tiles = two ? t2 : t1;
-  const int64_t blocks = a.tiles * heads;
-  if (blocks == 0) return PF_OK;
-  switch (kind) {
-    case kFwd:
-      if constexpr (DP == 32)
-        if (two) return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
-      return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
-    case kDq:
-      if constexpr (DP == 32)
-        if (two) return go(k_dq<DP, BT, 2>, (256 + 4 * kTile) * RB, blocks, "k_attn_dq", flops, st, a);
-      return go(k_dq<DP, BT, 1>, (128 + 4 * kTile) * RB, blocks, "k_attn_dq", flops, st, a);
-    default:
-      if constexpr (DP == 32)
-        if (two) return go(k_dkv<DP, BT, 2>, (256 + 4 * kTile) * RB + 2048, blocks, "k_attn_dkv", flops, st, a);
-      return go(k_dkv<DP, BT, 1>, (128 + 4 * kTile) * RB + 2048, blocks, "k_attn_dkv", flops, st, a);
+  auto grid = [&](int64_t rows, int64_t heads, bool& two) {
+    const int64_t t1 = (rows + 63) / 64, t2 = (rows + 127) / 128;
+    two = DP == 32 && t2 * heads >= 3 * 148;
+    a.tiles = two ? t2 : t1;
+    return a.tiles * heads;
+  };
+  bool two = false;
+  if (kind == kFwd) {
+    const int64_t blocks = grid(a.nq, a.H * a.B, two);
+    if (blocks == 0) return PF_OK;
+    if constexpr (DP == 32)
+      if (two) return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
+    return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
   }
+  const size_t smem1 = (128 + 4 * kTile) * RB + 2048, smem2 = (256 + 4 * kTile) * RB + 2048;
+  const bool want_q = kind != kDkv, want_kv = kind != kDq;
+  if (want_q && want_kv) {
+    bool two_q, two_kv;
+    const int64_t bq = grid(a.nq, a.H * a.B, two_q), bkv = grid(a.nk, a.KV * a.B, two_kv);
+    if (!two_q && !two_kv && bq > 0 && bkv > 0)
+      return go(k_dqkv<DP, BT>, smem1, bq + bkv, "k_attn_dqkv", flops, st, a, (unsigned)bkv);
+  }
+  if (want_kv) {
+    const int64_t blocks = grid(a.nk, a.KV * a.B, two);
+    if (blocks > 0) {
+      if constexpr (DP == 32)
+        if (two) PF_TRY(go(k_dkv<DP, BT, 2>, smem2, blocks, "k_attn_dkv", flops * (want_q ? 4. / 7 : 1), st, a));
+      if (!two) PF_TRY(go(k_dkv<DP, BT, 1>, smem1, blocks, "k_attn_dkv", flops * (want_q ? 4. / 7 : 1), st, a));
+    }
+  }
+  if (want_q) {
+    const int64_t blocks = grid(a.nq, a.H * a.B, two);
+    if (blocks > 0) {
+      if constexpr (DP == 32)
+        if (two) return go(k_dq<DP, BT, 2>, smem2, blocks, "k_attn_dq", flops * (want_kv ? 3. / 7 : 1), st, a);
+      return go(k_dq<DP, BT, 1>, smem1, blocks, "k_attn_dq", flops * (want_kv ? 3. / 7 : 1), st, a);
+    }
+  }
+  return PF_OK;
 }
 
 template <int DP, int BT>
@@ -1400,11 +1450,16 @@ int dq_plane_bf16(const Args& a, float* part, int parts, double flops, cudaStrea
 }
 
 int rows_bf16(const Args& a, const float* stats, Heads o, const int16_t* lo, float* rows, cudaStream_t st) {
-  const int64_t blocks = (a.rows_plane + 31) / 32;
+  const int lanes = a.d <= 32 ? 4 : (a.d <= 64 ? 8 : 16);
+  const int64_t blocks = (a.rows_plane * lanes + 255) / 256;
   if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: too many rows");
+  const bool vec = a.vec_g && ((uintptr_t)o.p | (uintptr_t)lo) % 16 == 0 && ((o.bs | o.ns | o.hs) & 7) == 0;
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_attn_rows", (6.0 * a.d + 24.0) * (double)a.rows_plane, 'b');
-    k_rows<<<(unsigned)blocks, 256, 0, st>>>(a, stats, o, lo, (float4*)rows);
+    auto* kern = lanes == 4   ? (vec ? k_rows<4, true> : k_rows<4, false>)
+                 : lanes == 8 ? (vec ? k_rows<8, true> : k_rows<8, false>)
+                              : (vec ? k_rows<16, true> : k_rows<16, false>);
+    kern<<<(unsigned)blocks, 256, 0, st>>>(a, stats, o, lo, (float4*)rows);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;

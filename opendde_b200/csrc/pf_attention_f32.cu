@@ -338,26 +338,32 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
 
 // ---------------------------------------------------------------- row constants
 
-// Eight lanes per row (b, i, h): D, and {m, -log2 l, peak, -D}; peak = 1 where one key has all of the row's
-// weight in fp32 (l = 1).
+// D, and {m, -log2 l, peak, -D} of the rows (b, h, i), i fastest; peak = 1 where one key has all of the
+// row's weight in fp32 (l = 1). L lanes per row, four channels each (VEC: as one access).
+template <int L, bool VEC>
 __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ stats, Heads o,
                                               float4* __restrict__ rows) {
-  const int sub = threadIdx.x & 7;
-  const int64_t r = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  const bool live = r < a.rows_plane;
-  const int64_t rr = live ? r : 0;
-  const int h = (int)(rr % a.H);
-  const int64_t bi = rr / a.H, b = bi / a.nq, i = bi - b * a.nq;
-  const float* po = head_f(o, b, h) + i * o.ns;
-  const float* pg = head_f(a.g, b, h) + i * a.g.ns;
+  const int sub = threadIdx.x & (L - 1);
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const bool live = at < a.rows_plane;
+  const int64_t r = live ? at : 0, bh = r / a.nq, i = r - bh * a.nq, b = bh / a.H;
+  const int h = (int)(bh - b * a.H), c = sub * 4;
+  const float* po = head_f(o, b, h) + i * o.ns + c;
+  const float* pg = head_f(a.g, b, h) + i * a.g.ns + c;
   float s = 0.f;
-  if (live)
-    for (int e = sub; e < a.d; e += 8) s += po[e] * pg[e];
-  s += __shfl_xor_sync(0xffffffffu, s, 1);
-  s += __shfl_xor_sync(0xffffffffu, s, 2);
-  s += __shfl_xor_sync(0xffffffffu, s, 4);
+  if (VEC) {
+    if (live && c < a.d) {
+      const float4 x = *reinterpret_cast<const float4*>(po), y = *reinterpret_cast<const float4*>(pg);
+      s = x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+    }
+  } else if (live) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < a.d) s += po[e] * pg[e];
+  }
+#pragma unroll
+  for (int k = 1; k < L; k <<= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (!live || sub) return;
-  const int64_t at = (b * a.H + h) * a.nq + i;
   const float m = stats[at], l = stats[a.rows_plane + at];
   const bool none = l == 0.f;
   rows[at] = make_float4(none ? INFINITY : m, none ? 0.f : -log2f(l), l == 1.f ? 1.f : 0.f, none ? 0.f : -s);
@@ -386,16 +392,15 @@ __device__ __forceinline__ void prob_ds(float (&x)[2][4], float (&y)[2][4], cons
 // ---------------------------------------------------------------- dq (and dbias of one batch entry)
 
 template <int DP, int BT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dq(Args a) {
+__device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Split<DP>;
   constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8;
   extern __shared__ __align__(128) unsigned char raw[];
   const uint32_t sq = smem_addr(raw), sg = sq + S::kStat3, sk = sg + S::kStat3, sv = sk + 2 * S::kTile3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
-  unsigned id = blockIdx.x;
-  const unsigned tile = id % (unsigned)a.tiles;
-  id /= (unsigned)a.tiles;
+  const unsigned tile = id % (unsigned)tiles;
+  id /= (unsigned)tiles;
   const int h = id % a.H, kh = h / (a.H / a.KV);
   const int64_t b = id / a.H, w0 = (int64_t)tile * 64 + warp * 16;
   const int nt = (int)((a.nk + KT - 1) / KT);
@@ -491,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dq(Args a) {
 // ---------------------------------------------------------------- dk, dv
 
 template <int DP, int BT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dkv(Args a) {
+__device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Split<DP>;
   constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -499,9 +504,8 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dkv(Args a) {
   float4* cst = (float4*)(raw + 2 * S::kStat3 + 4 * S::kTile3);  // [2][KT]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), ln = lane_bn<DP>();
-  unsigned id = blockIdx.x;
-  const unsigned tile = id % (unsigned)a.tiles;
-  id /= (unsigned)a.tiles;
+  const unsigned tile = id % (unsigned)tiles;
+  id /= (unsigned)tiles;
   const int kh = id % a.KV, group = a.H / a.KV;
   const int64_t b = id / a.KV, j0 = (int64_t)tile * 64, w0 = j0 + warp * 16;
   const int per = (int)((a.nq + KT - 1) / KT), nt = per * group;
@@ -598,6 +602,16 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dkv(Args a) {
       store2f(ov, n * 8 + 2 * t, a.d, vv, dv[n][2 * r], dv[n][2 * r + 1]);
     }
   }
+}
+
+// dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
+// run side by side.
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dqkv(Args a, unsigned dkv_blocks) {
+  if (blockIdx.x < dkv_blocks)
+    dkv_block<DP, BT>(a, blockIdx.x, (a.nk + 63) / 64);
+  else
+    dq_block<DP, BT>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
 
 // ---------------------------------------------------------------- dbias shared by the batch
@@ -722,11 +736,14 @@ int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cud
 template <int DP, int BT>
 int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   using S = Split<DP>;
-  a.tiles = ((kind == kDkv ? a.nk : a.nq) + 63) / 64;
-  const int64_t blocks = a.tiles * (kind == kDkv ? a.KV : a.H) * a.B;
-  if (kind == kFwd) return go(k_fwd<DP, BT>, S::kStat3 + 4 * S::kTile3, blocks, "k_attn_fwd", flops, st, a);
-  if (kind == kDq) return go(k_dq<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3, blocks, "k_attn_dq", flops, st, a);
-  return go(k_dkv<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16, blocks, "k_attn_dkv", flops, st, a);
+  const int64_t tq = (a.nq + 63) / 64, tk = (a.nk + 63) / 64;
+  if (kind == kFwd) {
+    a.tiles = tq;
+    return go(k_fwd<DP, BT>, S::kStat3 + 4 * S::kTile3, tq * a.H * a.B, "k_attn_fwd", flops, st, a);
+  }
+  const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
+  return go(k_dqkv<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16, bq + bkv,
+            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a, (unsigned)bkv);
 }
 template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
@@ -755,11 +772,16 @@ int dbias_f32(const Args& a, float* part, int parts, double flops, cudaStream_t 
   PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);
 }
 int rows_f32(const Args& a, const float* stats, Heads o, float* rows, cudaStream_t st) {
-  const int64_t blocks = (a.rows_plane + 31) / 32;
+  const int lanes = a.d <= 32 ? 8 : (a.d <= 64 ? 16 : 32);
+  const int64_t blocks = (a.rows_plane * lanes + 255) / 256;
   if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: too many rows");
+  const bool vec = a.vec_g && (uintptr_t)o.p % 16 == 0 && ((o.bs | o.ns | o.hs) & 3) == 0;
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_attn_rows", (8.0 * a.d + 24.0) * (double)a.rows_plane, 'b');
-    k_rows<<<(unsigned)blocks, 256, 0, st>>>(a, stats, o, (float4*)rows);
+    auto* kern = lanes == 8    ? (vec ? k_rows<8, true> : k_rows<8, false>)
+                 : lanes == 16 ? (vec ? k_rows<16, true> : k_rows<16, false>)
+                               : (vec ? k_rows<32, true> : k_rows<32, false>);
+    kern<<<(unsigned)blocks, 256, 0, st>>>(a, stats, o, (float4*)rows);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;

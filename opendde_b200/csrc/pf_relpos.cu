@@ -261,8 +261,9 @@ struct RelGrid {
 };
 
 // As many heads at a time as eight warps' tables leave room for in 64 KB of shared memory: eight up to
-// 256 features (r_max up to 61), four up to 512, else one. Row chunks: about four blocks per SM, and not
-// so short that the tables' zeroing and adding outweigh the rows.
+// 256 features (r_max up to 61), four up to 512, else one. Row chunks: about eight blocks per SM (two run
+// at a time; the warps on the diagonal of a chain take several times as long as the others, and shorter
+// chunks even that out: 16 rows 84 us, 32 rows 97 us at 1536 tokens and 16 heads), of at least four rows.
 RelGrid plan(int64_t n_rows, int64_t n_cols, int heads, int n_feat) {
   RelGrid p;
   p.G = n_feat <= 256 && heads > 4 ? 8 : (n_feat <= 512 ? 4 : 1);
@@ -271,7 +272,7 @@ RelGrid plan(int64_t n_rows, int64_t n_cols, int heads, int n_feat) {
   int64_t want = 148 * kRelWaves * 2 / (p.strips * p.groups);
   want = want < 1 ? 1 : want;
   int64_t per = (n_rows + want - 1) / want;
-  per = per < 16 ? 16 : (per > kRelRows ? kRelRows : per);
+  per = per < 4 ? 4 : (per > kRelRows ? kRelRows : per);
   p.rows_per_block = (int)per;
   p.chunks = (n_rows + per - 1) / per;
   return p;
