@@ -78,7 +78,7 @@ constexpr int kWarps = 8;
 
 // L lanes per row, V chunks of E channels per lane, U rows of a lane in flight; FULL: c = L V E.
 template <class T, int E, int L, int V, int U, bool FULL>
-__global__ void __launch_bounds__(kWarps * 32) k_layernorm_bwd(const T* x, const T* dy,
+__global__ void __launch_bounds__(kWarps * 32, 2) k_layernorm_bwd(const T* x, const T* dy,
                                                                const float* __restrict__ gamma, T* dx, float* dg_out,
                                                                float* db_out, int64_t part, int64_t rows, int c,
                                                                float eps) {

@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "pf_common.cuh"
+#include "pf_f32x2.cuh"
 #include "pf_prof.h"
 #include "pf_simt.h"
 
@@ -64,9 +65,10 @@ __global__ void k_ln_view(const T* __restrict__ x, int64_t rs, int64_t cs, int64
     if (t < per) {
       int ch = t * 32 + lane;
       if (ch < c) {
-        float y = (v[t] - mean) * rstd;
-        if (gamma) y = y * gamma[ch];
-        if (beta) y = y + beta[ch];
+        // each rounded by itself, whatever the compiler would contract
+        float y = __fmul_rn(v[t] - mean, rstd);
+        if (gamma) y = __fmul_rn(y, gamma[ch]);
+        if (beta) y = __fadd_rn(y, beta[ch]);
         op[ch] = from_f<TO>(y);
       }
     }
@@ -146,63 +148,65 @@ __global__ void __launch_bounds__(256) k_layernorm_rows(const T* __restrict__ x,
       raw[u][t] = (row < rows && v < nv) ? __ldg(reinterpret_cast<const uint4*>(x + row * (int64_t)c) + v)
                                          : make_uint4(0, 0, 0, 0);
     }
-  float gm[V * E], bt[V * E];
+  F2 gm[V * E / 2];
+  float bt[V * E];
   const bool ga = ((uintptr_t)gamma & 15) == 0, ba = ((uintptr_t)beta & 15) == 0;
 #pragma unroll
   for (int t = 0; t < V; ++t) {
     const int v = sub + t * L;
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
-      if (gamma && v < nv) load_params4(gamma + v * E + e, ga, gm + t * E + e);
+      float f[4];
+      if (gamma && v < nv) {
+        load_params4(gamma + v * E + e, ga, f);
+        gm[(t * E + e) / 2] = F2(f[0], f[1]), gm[(t * E + e) / 2 + 1] = F2(f[2], f[3]);
+      }
       if (beta && v < nv) load_params4(beta + v * E + e, ba, bt + t * E + e);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t row = row0 + u * R;
+    float f[V * E];
+#pragma unroll
+    for (int t = 0; t < V; ++t) VecTraits<T>::unpack(raw[u][t], *reinterpret_cast<float(*)[E]>(f + t * E));
     float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < V; ++t) {
-      float f[E];
-      VecTraits<T>::unpack(raw[u][t], f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += f[e];
-    }
+    for (int i = 0; i < V * E; ++i) sum += f[i];
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float mean = sum / (float)c;
+    const F2 neg(-mean);
     float sq = 0.f;
 #pragma unroll
     for (int t = 0; t < V; ++t) {
-      if (sub + t * L < nv) {
-        float f[E];
-        VecTraits<T>::unpack(raw[u][t], f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float d = f[e] - mean;
-          sq += d * d;
-        }
+      for (int i = t * E; i < (t + 1) * E; i += 2) add2(F2(f[i], f[i + 1]), neg).get(f[i], f[i + 1]);
+      if (sub + t * L < nv) {
+#pragma unroll
+        for (int i = t * E; i < (t + 1) * E; ++i) sq = fmaf(f[i], f[i], sq);
       }
     }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-    const float rstd = rsqrtf(sq / (float)c + eps);
+    const F2 rstd(rsqrtf(sq / (float)c + eps));
     if (row >= rows) continue;
     uint4* yr = reinterpret_cast<uint4*>(y + row * (int64_t)c);
 #pragma unroll
     for (int t = 0; t < V; ++t) {
       const int v = sub + t * L;
       if (v < nv) {
-        float f[E];
-        VecTraits<T>::unpack(raw[u][t], f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float o = (f[e] - mean) * rstd;
-          if (gamma) o *= gm[t * E + e];
-          if (beta) o += bt[t * E + e];
-          f[e] = o;
+        for (int i = t * E / 2; i < (t + 1) * E / 2; ++i) {
+          F2 o = mul2(F2(f[2 * i], f[2 * i + 1]), rstd);
+          if (gamma) o = mul2(o, gm[i]);
+          o.get(f[2 * i], f[2 * i + 1]);
+          if (beta) {  // a rounded sum of the rounded product
+            f[2 * i] = __fadd_rn(f[2 * i], bt[2 * i]);
+            f[2 * i + 1] = __fadd_rn(f[2 * i + 1], bt[2 * i + 1]);
+          }
         }
-        yr[v] = VecTraits<T>::pack(f);
+        __stcs(yr + v, VecTraits<T>::pack(*reinterpret_cast<float(*)[E]>(f + t * E)));
       }
     }
   }
