@@ -42,7 +42,7 @@ int sum_planes(const Args& a, const float* part, int parts, cudaStream_t st) {
 }
 
 // How the gradient of a shared bias is computed: with dq in one pass (one block of 16 warps per SM), or by
-// itself (about three blocks per SM), in `parts` parts of the batch of at least four entries each (a part
+// itself (as many blocks as run at a time), in `parts` parts of the batch of at least four entries each (a part
 // costs a plane written and read).
 struct SharedPlan {
   bool plane;
@@ -60,9 +60,12 @@ SharedPlan shared_plan(const pf_attention_shape& s) {
     const int64_t waves = (blocks * n + 147) / 148;
     if (blocks * n * 100 >= waves * 148 * 60) return SharedPlan{true, (int)n};
   }
-  const int64_t rows = s.dtype == PF_BF16 ? 128 : 64, keys = s.dtype == PF_BF16 ? 64 : 32;
+  // tiles of the kernels and how many blocks an SM holds
+  const bool bf16 = s.dtype == PF_BF16;
+  const int64_t rows = bf16 ? 128 : 64, keys = bf16 || s.head_dim <= 32 ? 64 : (s.head_dim <= 64 ? 32 : 16);
   const int64_t blocks = ((s.n_q + rows - 1) / rows) * ((s.n_k + keys - 1) / keys) * s.heads;
-  int64_t n = (3 * 148 + blocks - 1) / blocks;
+  const int64_t fit = (s.head_dim <= 32 ? (bf16 ? 3 : 4) : 1) * 148;
+  int64_t n = blocks >= fit ? 1 : fit / blocks;
   if (n > s.batch / 4) n = s.batch / 4;
   p.parts = n < 1 ? 1 : (int)n;
   return p;

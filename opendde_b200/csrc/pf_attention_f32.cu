@@ -38,8 +38,8 @@ __device__ __forceinline__ void split4(const float4& v, uint2 (&w)[3]) {
     w[p].x = pack_bf16(x[0], x[1]);
     w[p].y = pack_bf16(x[2], x[3]);
     if (p < 2) {
-      x[0] -= lo_f(w[p].x), x[1] -= hi_f(w[p].x);
-      x[2] -= lo_f(w[p].y), x[3] -= hi_f(w[p].y);
+      fma2(F2(lo_f(w[p].x), hi_f(w[p].x)), F2(-1.f), F2(x[0], x[1])).get(x[0], x[1]);
+      fma2(F2(lo_f(w[p].y), hi_f(w[p].y)), F2(-1.f), F2(x[2], x[3])).get(x[2], x[3]);
     }
   }
 }
@@ -163,7 +163,7 @@ __device__ __forceinline__ void split_a(float (&x)[2][4], uint32_t (&pa)[3][4]) 
     for (int i = 0; i < 4; ++i) {
       float* v = &x[i >> 1][2 * (i & 1)];
       pa[p][i] = pack_bf16(v[0], v[1]);
-      if (p < 2) add2(F2(v[0], v[1]), F2(-lo_f(pa[p][i]), -hi_f(pa[p][i]))).get(v[0], v[1]);
+      if (p < 2) fma2(F2(lo_f(pa[p][i]), hi_f(pa[p][i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
     }
 }
 
