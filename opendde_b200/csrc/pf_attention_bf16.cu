@@ -1,11 +1,10 @@
 // pf_attention_bf16.cu -- the bf16 kernels of pf_attention.cuh on warp-level tensor-core products.
 //
-// Work of one warp: 16 MT query rows against groups of 16 keys (forward, dq, dbias), or 16 KM keys
+// Work of one warp: 16 or 32 query rows against groups of 16 keys (forward, dq, dbias), or 16 keys
 // against groups of 16 queries (dk, dv); four warps to a block, streamed tiles of 64 rows
 // double-buffered by cp.async. For the heads of 24 and 32 channels of this package a 16 x 16 block of
 // scores costs two to four products of depth 32 next to 256 exponentials, so the kernels are bound by
-// the issue of products, exponentials and the arithmetic around them, not by memory: two row blocks
-// per warp (MT = 2, KM = 2) use every streamed fragment twice.
+// the issue of products, exponentials and the arithmetic around them, not by memory.
 //
 // Columns of a group of 16 keys are permuted so that a lane's four columns are four neighbouring keys
 // (lane t of a quad: keys 4t..4t+3 in place of 2t, 2t+1, 2t+8, 2t+9): a bias row is then read, and a
@@ -30,7 +29,7 @@ namespace {
 // Tiles that are wholly visible and inside, with aligned bias rows, take the body without any checks
 // (FAST): the checks would be half of its instructions.
 template <int DP, int BT, int MT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_fwd(Args a) {
+__global__ void __launch_bounds__(kThreads, DP == 32 ? (MT == 1 ? 4 : 3) : 2) k_fwd(Args a) {
   using S = Tile<DP>;
   constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr int TERMS = BT == 2 ? 3 : 2;  // bf16 values that p is split into (see the head of pf_attention.cuh)
@@ -343,10 +342,10 @@ __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ 
 
 // ---------------------------------------------------------------- dq (and dbias of one batch entry)
 
-template <int DP, int BT, int MT>
+template <int DP, int BT>
 __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
-  constexpr int QR = 64 * MT, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
+  constexpr int QR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr int kV = 2 * kTile * RB;  // from a K tile to its V tile
   extern __shared__ __align__(128) unsigned char raw[];
   const uint32_t sq = smem_addr(raw), sg = sq + QR * RB, sk = sg + QR * RB;
@@ -355,7 +354,7 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   id /= (unsigned)tiles;
   const int h = id % a.H, kh = h / (a.H / a.KV);
   const int64_t b = id / a.H, nk = a.nk;
-  const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16 * MT;
+  const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16;
   const int nt = (int)((nk + kTile - 1) / kTile);
   const int bvec = a.bias_vec;
   const bool work = w0 < a.nq, put = BT && a.dbias != nullptr;
@@ -374,41 +373,35 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
 #pragma unroll
     for (int k = 0; k < KS; ++k) ka[k] = lb.at(sk, 0, k), ta[k] = lt.at(sk, 0, k);
   }
-  const char* bp[MT][2];  // the lane's first key of the tile, in its rows of the bias and of dbias
-  char* dp[MT][2];
-  F2 nmx[MT][2], lg[MT][2], nd[MT][2];
+  const char* bp[2];  // the lane's first key of the tile, in its rows of the bias and of dbias
+  char* dp[2];
+  F2 nmx[2], lg[2], nd[2];
   bool peaked = false;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int64_t i = w0 + m * 16 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
-      bp[m][r] = BT ? bias_row<BT>(a, b, h, ic) + 4 * t * BS : nullptr;
-      dp[m][r] = (put && i < a.nq) ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs + 4 * t) * BS : nullptr;
+      const int64_t i = w0 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
+      bp[r] = BT ? bias_row<BT>(a, b, h, ic) + 4 * t * BS : nullptr;
+      dp[r] = (put && i < a.nq) ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs + 4 * t) * BS : nullptr;
       const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
-      nmx[m][r] = F2(-c.x), lg[m][r] = F2(c.y), nd[m][r] = F2(c.w);
+      nmx[r] = F2(-c.x), lg[r] = F2(c.y), nd[r] = F2(c.w);
       peaked |= c.z != 0.f;
     }
   peaked = __any_sync(0xffffffffu, peaked);
   // what the body without checks needs of the warp's rows
-  const bool plain = !peaked && (BT == 0 || bvec) && (!put || (a.db_vec && w0 + 16 * MT <= a.nq));
-  Bias4<BT> ring[2][MT][2];
+  const bool plain = !peaked && (BT == 0 || bvec) && (!put || (a.db_vec && w0 + 16 <= a.nq));
+  Bias4<BT> ring[2][2];
   auto fetch = [&](int slot, int q, int64_t j0, bool fast) {
     if (BT == 0) return;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) bias_get<BT>(ring[slot][m][r], bp[m][r] + q * 16 * BS, j0 + q * 16 + 4 * t, nk, fast);
+      for (int r = 0; r < 2; ++r) bias_get<BT>(ring[slot][r], bp[r] + q * 16 * BS, j0 + q * 16 + 4 * t, nk, fast);
   };
   const F2 scale(a.scale);
-  float acc[MT][NB][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
+  float acc[NB][4];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  uint32_t fq[MT][KS][4], fg[MT][KS][4];
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+  uint32_t fq[KS][4], fg[KS][4];
   uint64_t bits = seen_ballot(seen_raw(a, b, 0));
   if (nt > 0) issue(0, bits);
   float2 rawm = seen_raw(a, b, kTile);
@@ -421,33 +414,30 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
     for (int hb = 0; hb < 2; ++hb) {
     unrolled<2>([&](auto Q) {  // 16 keys
       constexpr int q = decltype(Q)::value;
-      float x[MT][2][4], y[MT][2][4];
+      float x[2][4], y[2][4];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t r[4], u[4];
         ldsm4i<q * 16 * RB>(r, kc[k]);
         ldsm4i<q * 16 * RB + kV>(u, kc[k]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        {
           if (k == 0) {
-            mma0(x[m][0], fq[m][k], r[0], r[1]);
-            mma0(x[m][1], fq[m][k], r[2], r[3]);
-            mma0(y[m][0], fg[m][k], u[0], u[1]);
-            mma0(y[m][1], fg[m][k], u[2], u[3]);
+            mma0(x[0], fq[k], r[0], r[1]);
+            mma0(x[1], fq[k], r[2], r[3]);
+            mma0(y[0], fg[k], u[0], u[1]);
+            mma0(y[1], fg[k], u[2], u[3]);
           } else {
-            mma(x[m][0], fq[m][k], r[0], r[1]);
-            mma(x[m][1], fq[m][k], r[2], r[3]);
-            mma(y[m][0], fg[m][k], u[0], u[1]);
-            mma(y[m][1], fg[m][k], u[2], u[3]);
+            mma(x[0], fq[k], r[0], r[1]);
+            mma(x[1], fq[k], r[2], r[3]);
+            mma(y[0], fg[k], u[0], u[1]);
+            mma(y[1], fg[k], u[2], u[3]);
           }
         }
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[q][m][r], n);
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, ring[q][r], n);
       fetch(q, 2 * hb + q + 2, j0, hb == 0 ? FAST || (bvec && j0 + (q + 3) * 16 <= nk) : nf);
       if (!FAST) {
         const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
@@ -456,51 +446,41 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (!((mine >> (2 * n + e)) & 1))
-#pragma unroll
-              for (int m = 0; m < MT; ++m) x[m][n][e] = x[m][n][2 + e] = -INFINITY;
+      x[n][e] = x[n][2 + e] = -INFINITY;
       }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const F2 p = prob2(&x[m][n][2 * r], nmx[m][r], lg[m][r]);
-            if (!FAST) p.get(x[m][n][2 * r], x[m][n][2 * r + 1]);
-            mul2(p, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[m][r])).get(y[m][n][2 * r], y[m][n][2 * r + 1]);
+            const F2 p = prob2(&x[n][2 * r], nmx[r], lg[r]);
+            if (!FAST) p.get(x[n][2 * r], x[n][2 * r + 1]);
+            mul2(p, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(y[n][2 * r], y[n][2 * r + 1]);
           }
       if (!FAST && peaked) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (x[m][n][e] == 1.f) y[m][n][e] = 0.f;
+              if (x[n][e] == 1.f) y[n][e] = 0.f;
       }
       if (put) {
         const int64_t j = j0 + hb * 32 + q * 16 + 4 * t;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
           for (int r = 0; r < 2; ++r)
-            if (FAST || dp[m][r])
-              put_bias4<BT>(dp[m][r] + (hb * 32 + q * 16) * BS, j, nk, FAST || (a.db_vec && j0 + hb * 32 + q * 16 + 16 <= nk),
-                            y[m][0][2 * r], y[m][0][2 * r + 1], y[m][1][2 * r], y[m][1][2 * r + 1]);
+            if (FAST || dp[r])
+              put_bias4<BT>(dp[r] + (hb * 32 + q * 16) * BS, j, nk, FAST || (a.db_vec && j0 + hb * 32 + q * 16 + 16 <= nk),
+                            y[0][2 * r], y[0][2 * r + 1], y[1][2 * r], y[1][2 * r + 1]);
       }
-      uint32_t da[MT][4];
+      uint32_t da[4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) da[m][i] = pack_bf16(y[m][i >> 1][2 * (i & 1)], y[m][i >> 1][2 * (i & 1) + 1]);
+        for (int i = 0; i < 4; ++i) da[i] = pack_bf16(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1]);
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         uint32_t f[4];
         ldsm4_ti<q * 16 * RB>(f, tc[c]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          mma(acc[m][2 * c], da[m], f[0], f[1]);
-          mma(acc[m][2 * c + 1], da[m], f[2], f[3]);
+        {
+          mma(acc[2 * c], da, f[0], f[1]);
+          mma(acc[2 * c + 1], da, f[2], f[3]);
         }
       }
     });
@@ -520,11 +500,9 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
     if (kt == 0) {
       const LaneAddr<DP> la = lane_a<DP>();
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
         for (int k = 0; k < KS; ++k) {
-          ldsm4(fq[m][k], la.at(sq, warp * MT + m, k));
-          ldsm4(fg[m][k], la.at(sg, warp * MT + m, k));
+          ldsm4(fq[k], la.at(sq, warp, k));
+          ldsm4(fg[k], la.at(sg, warp, k));
         }
     }
     if (kt + 1 < nt) issue(kt + 1, next);
@@ -541,11 +519,9 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
         fetch(1, 5, j0, nf);
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
         for (int r = 0; r < 2; ++r) {
-          bp[m][r] += kTile * BS;
-          if (dp[m][r]) dp[m][r] += kTile * BS;
+          bp[r] += kTile * BS;
+          if (dp[r]) dp[r] += kTile * BS;
         }
     }
     bits = next;
@@ -555,25 +531,24 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   if (!a.dq) return;
   const bool vec = pair_ok(a.dq, a.o_bs, a.o_ns, a.o_hs, a.d);
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int64_t i = w0 + m * 16 + r * 8 + g;
+      const int64_t i = w0 + r * 8 + g;
       if (i >= a.nq) continue;
       bf16* o = (bf16*)a.dq + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
-        store_pair(o, n * 8 + 2 * t, a.d, vec, acc[m][n][2 * r] * a.scale, acc[m][n][2 * r + 1] * a.scale);
+        store_pair(o, n * 8 + 2 * t, a.d, vec, acc[n][2 * r] * a.scale, acc[n][2 * r + 1] * a.scale);
     }
 }
 
 // ---------------------------------------------------------------- dk, dv
 
-// 16 KM keys per warp; HOLD: their fragments stay in registers.
-template <int DP, int BT, int KM>
+// 16 keys per warp (32 need 168 registers where 16 need 128, and three blocks on an SM are slower than four:
+// 768 tokens 2.1 against 1.9 ms); HOLD: their fragments stay in registers.
+template <int DP, int BT>
 __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
-  constexpr int KR = 64 * KM, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
+  constexpr int KR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr bool HOLD = DP <= 64;
   constexpr int kG = 2 * kTile * RB;  // from a Q tile to its dO tile
   extern __shared__ __align__(128) unsigned char raw[];
@@ -585,22 +560,14 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
   id /= (unsigned)tiles;
   const int kh = id % a.KV, group = a.H / a.KV;
   const int64_t b = id / a.KV, nq = a.nq;
-  const int64_t j0 = (int64_t)tile * KR, w0 = j0 + warp * 16 * KM;
+  const int64_t j0 = (int64_t)tile * KR, w0 = j0 + warp * 16;
   const int per = (int)((nq + kTile - 1) / kTile);
-  uint64_t live[KM];  // visible keys of the block, 64 at a time
-#pragma unroll
-  for (int i = 0; i < KM; ++i) live[i] = seen_ballot(seen_raw(a, b, j0 + 64 * i));
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < KM; ++i) {
-    any |= live[i] != 0;
-    load_rows<DP, 64>(sk + i * 64 * RB, head_base(a.k, b, kh), a.k.ns, a.vec_k, j0 + 64 * i, a.nk, a.d, live[i]);
-    load_rows<DP, 64>(sv + i * 64 * RB, head_base(a.v, b, kh), a.v.ns, a.vec_v, j0 + 64 * i, a.nk, a.d, live[i]);
-  }
-  // the warp's keys, 16 KM bits
-  constexpr uint32_t kAll = KM == 2 ? 0xffffffffu : 0xffffu;
-  const uint32_t mine = (uint32_t)(live[(warp * 16 * KM) / 64] >> ((warp * 16 * KM) & 63)) & kAll;
-  const bool bfast = a.bias_vec && w0 + 16 * KM <= a.nk;
+  const uint64_t live = seen_ballot(seen_raw(a, b, j0));  // visible keys of the block
+  load_rows<DP, 64>(sk, head_base(a.k, b, kh), a.k.ns, a.vec_k, j0, a.nk, a.d, live);
+  load_rows<DP, 64>(sv, head_base(a.v, b, kh), a.v.ns, a.vec_v, j0, a.nk, a.d, live);
+  constexpr uint32_t kAll = 0xffffu;
+  const uint32_t mine = (uint32_t)(live >> (warp * 16)) & kAll;  // and of the warp
+  const bool bfast = a.bias_vec && w0 + 16 <= a.nk;
   const bool plain = mine == kAll && (BT == 0 || bfast);  // the body without checks
   uint32_t qa[KS], ta[KS];
   {
@@ -609,15 +576,13 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     for (int k = 0; k < KS; ++k) qa[k] = la.at(sq, 0, k), ta[k] = ln.at(sq, 0, k);
   }
   const F2 scale(a.scale);
-  float dk[KM][NB][4], dv[KM][NB][4];
-#pragma unroll
-  for (int m = 0; m < KM; ++m)
+  float dk[NB][4], dv[NB][4];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dk[m][n][e] = dv[m][n][e] = 0.f;
-  uint32_t fk[HOLD ? KM : 1][HOLD ? KS : 1][4], fv[HOLD ? KM : 1][HOLD ? KS : 1][4];
-  Bias4<BT> ring[2][KM][2];
+      for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
+  uint32_t fk[HOLD ? KS : 1][4], fv[HOLD ? KS : 1][4];
+  Bias4<BT> ring[2][2];
   const char* bp[2] = {nullptr, nullptr};  // the lane's first key in rows g, g + 8 of the block that is read next
   const int64_t bstep = a.b_rs * 16 * BS;
   auto fetch = [&](int slot, int64_t i0, bool fast) {  // rows i0 .. i0 + 15; 0 past the end
@@ -625,13 +590,12 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const bool row = fast || i0 + 8 * r + g < nq;
-#pragma unroll
-      for (int m = 0; m < KM; ++m) {
+      {
         if (row) {
-          bias_get<BT>(ring[slot][m][r], bp[r] + 16 * m * BS, w0 + 16 * m + 4 * t, a.nk, fast || bfast);
+          bias_get<BT>(ring[slot][r], bp[r], w0 + 4 * t, a.nk, fast || bfast);
         } else {
 #pragma unroll
-          for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][m][r].w[w] = 0;
+          for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][r].w[w] = 0;
         }
       }
       bp[r] += bstep;
@@ -647,83 +611,75 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     for (int hb = 0; hb < 2; ++hb) {
     unrolled<2>([&](auto B) {  // 16 queries
       constexpr int blk = decltype(B)::value;
-      float x[KM][2][4], y[KM][2][4];
+      float x[2][4], y[2][4];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t fq[4], fg[4];
         ldsm4i<blk * 16 * RB>(fq, qc[k]);
         ldsm4i<blk * 16 * RB + kG>(fg, qc[k]);
-#pragma unroll
-        for (int m = 0; m < KM; ++m) {
+        {
           uint32_t rk[4], rv[4];
           if (HOLD) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rk[i] = fk[m][k][i], rv[i] = fv[m][k][i];
+            for (int i = 0; i < 4; ++i) rk[i] = fk[k][i], rv[i] = fv[k][i];
           } else {
-            ldsm4(rk, lb.at(sk, warp * KM + m, k));
-            ldsm4(rv, lb.at(sv, warp * KM + m, k));
+            ldsm4(rk, lb.at(sk, warp, k));
+            ldsm4(rv, lb.at(sv, warp, k));
           }
           if (k == 0) {
-            mma0(x[m][0], fq, rk[0], rk[1]);
-            mma0(x[m][1], fq, rk[2], rk[3]);
-            mma0(y[m][0], fg, rv[0], rv[1]);
-            mma0(y[m][1], fg, rv[2], rv[3]);
+            mma0(x[0], fq, rk[0], rk[1]);
+            mma0(x[1], fq, rk[2], rk[3]);
+            mma0(y[0], fg, rv[0], rv[1]);
+            mma0(y[1], fg, rv[2], rv[3]);
           } else {
-            mma(x[m][0], fq, rk[0], rk[1]);
-            mma(x[m][1], fq, rk[2], rk[3]);
-            mma(y[m][0], fg, rv[0], rv[1]);
-            mma(y[m][1], fg, rv[2], rv[3]);
+            mma(x[0], fq, rk[0], rk[1]);
+            mma(x[1], fq, rk[2], rk[3]);
+            mma(y[0], fg, rv[0], rv[1]);
+            mma(y[1], fg, rv[2], rv[3]);
           }
         }
       }
       const float4 c[2] = {cst[s * kTile + hb * 32 + blk * 16 + g], cst[s * kTile + hb * 32 + blk * 16 + 8 + g]};
       const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)}, nd[2] = {F2(c[0].w), F2(c[1].w)};
 #pragma unroll
-      for (int m = 0; m < KM; ++m)
-#pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) score2<BT>(&x[m][n][2 * r], scale, ring[blk][m][r], n);
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, ring[blk][r], n);
       fetch(blk, i0 + hb * 32 + blk * 16 + 32, hb == 0 ? FAST : nf);
       if (!FAST) {
-#pragma unroll
-        for (int m = 0; m < KM; ++m)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (!((mine >> (16 * m + 4 * t + 2 * n + e)) & 1)) x[m][n][e] = x[m][n][2 + e] = -INFINITY;
+              if (!((mine >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
       }
       const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
-      uint32_t pa[KM][4], da[KM][4];
-#pragma unroll
-      for (int m = 0; m < KM; ++m)
+      uint32_t pa[4], da[4];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             float p[2], ds[2];
-            const F2 p2 = prob2(&x[m][n][2 * r], nmx[r], lg[r]);
+            const F2 p2 = prob2(&x[n][2 * r], nmx[r], lg[r]);
             p2.get(p[0], p[1]);
-            mul2(p2, add2(F2(y[m][n][2 * r], y[m][n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
+            mul2(p2, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
             if (peaked) {
               if (p[0] == 1.f) ds[0] = 0.f;
               if (p[1] == 1.f) ds[1] = 0.f;
             }
-            pa[m][2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
-            da[m][2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
+            pa[2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
+            da[2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
           }
 #pragma unroll
       for (int n = 0; n < KS; ++n) {
         uint32_t fg[4], fq[4];
         ldsm4_ti<blk * 16 * RB + kG>(fg, tc[n]);
         ldsm4_ti<blk * 16 * RB>(fq, tc[n]);
-#pragma unroll
-        for (int m = 0; m < KM; ++m) {
-          mma(dv[m][2 * n], pa[m], fg[0], fg[1]);
-          mma(dv[m][2 * n + 1], pa[m], fg[2], fg[3]);
-          mma(dk[m][2 * n], da[m], fq[0], fq[1]);
-          mma(dk[m][2 * n + 1], da[m], fq[2], fq[3]);
+        {
+          mma(dv[2 * n], pa, fg[0], fg[1]);
+          mma(dv[2 * n + 1], pa, fg[2], fg[3]);
+          mma(dk[2 * n], da, fq[0], fq[1]);
+          mma(dk[2 * n + 1], da, fq[2], fq[3]);
         }
       }
     });
@@ -731,7 +687,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     for (int k = 0; k < KS; ++k) qc[k] += 32 * RB, tc[k] += 32 * RB;
     }
   };
-  if (any && per > 0) {
+  if (live != 0 && per > 0) {
     int it = 0;
     for (int hh = 0; hh < group; ++hh) {
       const int h = kh * group + hh;
@@ -761,11 +717,9 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
         __syncthreads();
         if (HOLD && it == 0) {
 #pragma unroll
-          for (int m = 0; m < (HOLD ? KM : 1); ++m)
-#pragma unroll
             for (int k = 0; k < (HOLD ? KS : 1); ++k) {
-              ldsm4(fk[m][k], lb.at(sk, warp * KM + m, k));
-              ldsm4(fv[m][k], lb.at(sv, warp * KM + m, k));
+              ldsm4(fk[k], lb.at(sk, warp, k));
+              ldsm4(fv[k], lb.at(sv, warp, k));
             }
         }
         if (qt + 1 < per) issue(qt + 1, s ^ 1);
@@ -783,36 +737,27 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
   cp_wait<0>();
   const bool vk = pair_ok(a.dk, a.dk_bs, a.dk_ns, a.dk_hs, a.d), vv = pair_ok(a.dv, a.dv_bs, a.dv_ns, a.dv_hs, a.d);
 #pragma unroll
-  for (int m = 0; m < KM; ++m)
-#pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int64_t j = w0 + 16 * m + perm_row(g, r);  // row g + 8 r of the block holds this key
+      const int64_t j = w0 + perm_row(g, r);  // row g + 8 r of the block holds this key
       if (j >= a.nk) continue;
       bf16* ok = (bf16*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j * a.dk_ns;
       bf16* ov = (bf16*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j * a.dv_ns;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        store_pair(ok, n * 8 + 2 * t, a.d, vk, dk[m][n][2 * r] * a.scale, dk[m][n][2 * r + 1] * a.scale);
-        store_pair(ov, n * 8 + 2 * t, a.d, vv, dv[m][n][2 * r], dv[m][n][2 * r + 1]);
+        store_pair(ok, n * 8 + 2 * t, a.d, vk, dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
+        store_pair(ov, n * 8 + 2 * t, a.d, vv, dv[n][2 * r], dv[n][2 * r + 1]);
       }
     }
 }
 
-template <int DP, int BT, int MT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dq(Args a) {
-  dq_block<DP, BT, MT>(a, blockIdx.x, a.tiles);
-}
-template <int DP, int BT, int KM>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dkv(Args a) {
-  dkv_block<DP, BT, KM>(a, blockIdx.x, a.tiles);
-}
-// Both in one launch, dk and dv in the first blocks: where neither fills the machine they run side by side.
+// dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
+// run side by side.
 template <int DP, int BT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 2) k_dqkv(Args a, unsigned dkv_blocks) {
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 2) k_dqkv(Args a, unsigned dkv_blocks) {
   if (blockIdx.x < dkv_blocks)
-    dkv_block<DP, BT, 1>(a, blockIdx.x, (a.nk + 63) / 64);
+    dkv_block<DP, BT>(a, blockIdx.x, (a.nk + 63) / 64);
   else
-    dq_block<DP, BT, 1>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
+    dq_block<DP, BT>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
 
 // ---------------------------------------------------------------- dbias shared by the batch
@@ -1339,6 +1284,7 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
 
 template <class F, class... X>
 int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cudaStream_t st, X... x) {
+  if (blocks == 0) return PF_OK;
   if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
   if (smem > 40 * 1024)
     PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -1353,46 +1299,23 @@ int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cud
 template <int DP, int BT>
 int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   constexpr size_t RB = Tile<DP>::RB;
-  // two row blocks per warp where the accumulators leave room for them and there are blocks enough
-  auto grid = [&](int64_t rows, int64_t heads, bool& two) {
-    const int64_t t1 = (rows + 63) / 64, t2 = (rows + 127) / 128;
-    two = DP == 32 && t2 * heads >= 3 * 148;
-    a.tiles = two ? t2 : t1;
-    return a.tiles * heads;
-  };
-  bool two = false;
+  const int64_t tq = (a.nq + 63) / 64, tk = (a.nk + 63) / 64;
   if (kind == kFwd) {
-    const int64_t blocks = grid(a.nq, a.H * a.B, two);
-    if (blocks == 0) return PF_OK;
-    if constexpr (DP == 32)
-      if (two) return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
-    return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, blocks, "k_attn_fwd", flops, st, a);
-  }
-  const size_t smem1 = (128 + 4 * kTile) * RB + 2048, smem2 = (256 + 4 * kTile) * RB + 2048;
-  const bool want_q = kind != kDkv, want_kv = kind != kDq;
-  if (want_q && want_kv) {
-    bool two_q, two_kv;
-    const int64_t bq = grid(a.nq, a.H * a.B, two_q), bkv = grid(a.nk, a.KV * a.B, two_kv);
-    if (!two_q && !two_kv && bq > 0 && bkv > 0)
-      return go(k_dqkv<DP, BT>, smem1, bq + bkv, "k_attn_dqkv", flops, st, a, (unsigned)bkv);
-  }
-  if (want_kv) {
-    const int64_t blocks = grid(a.nk, a.KV * a.B, two);
-    if (blocks > 0) {
-      if constexpr (DP == 32)
-        if (two) PF_TRY(go(k_dkv<DP, BT, 2>, smem2, blocks, "k_attn_dkv", flops * (want_q ? 4. / 7 : 1), st, a));
-      if (!two) PF_TRY(go(k_dkv<DP, BT, 1>, smem1, blocks, "k_attn_dkv", flops * (want_q ? 4. / 7 : 1), st, a));
+    // two row blocks per warp where the accumulators leave room for them and there are blocks enough (768 rows
+    // of 768 tokens: 1.5 against 1.7 ms)
+    if constexpr (DP == 32) {
+      const int64_t t2 = (a.nq + 127) / 128;
+      if (t2 * a.H * a.B >= 3 * 148) {
+        a.tiles = t2;
+        return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, t2 * a.H * a.B, "k_attn_fwd", flops, st, a);
+      }
     }
+    a.tiles = tq;
+    return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, tq * a.H * a.B, "k_attn_fwd", flops, st, a);
   }
-  if (want_q) {
-    const int64_t blocks = grid(a.nq, a.H * a.B, two);
-    if (blocks > 0) {
-      if constexpr (DP == 32)
-        if (two) return go(k_dq<DP, BT, 2>, smem2, blocks, "k_attn_dq", flops * (want_kv ? 3. / 7 : 1), st, a);
-      return go(k_dq<DP, BT, 1>, smem1, blocks, "k_attn_dq", flops * (want_kv ? 3. / 7 : 1), st, a);
-    }
-  }
-  return PF_OK;
+  const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
+  return go(k_dqkv<DP, BT>, (128 + 4 * kTile) * RB + 2048, bq + bkv,
+            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a, (unsigned)bkv);
 }
 
 template <int DP, int BT>
