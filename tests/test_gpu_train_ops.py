@@ -140,6 +140,24 @@ def test_attention_shared_bias(n, H, mask, dtype, bias_dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,nq,nk,H,KV,d,mask,bias_dtype", [
+    (40, 100, 130, 4, 4, 24, "holes", BF16), (37, 64, 255, 8, 2, 20, None, F32), (150, 40, 33, 4, 4, 32, "pad", BF16),
+    (9, 130, 832, 4, 4, 32, "pad", F32), (9, 130, 833, 4, 4, 32, None, BF16), (21, 97, 65, 16, 16, 3, "holes", F32),
+    (6, 200, 190, 4, 2, 64, "pad", BF16), (5, 1, 400, 4, 4, 32, None, F32)])
+def test_attention_shared_bias_over_a_long_batch(B, nq, nk, H, KV, d, mask, bias_dtype, dtype, cuda_device):
+    """The plane's gradient as a sum over the batch, in one pass with dq or by itself, whole and in parts; the keys up
+    to and past what one pass holds; a batch larger than its parts."""
+    args = _att(B, nq, nk, H, KV, d, dtype, cuda_device, "shared", bias_dtype, mask)
+    got = _verify(args)
+    q, k, v, do, bias, mt = args
+    o, saved = kernels.attention(q, k, v, bias, mt, save=True)
+    alone = kernels.attention_bwd(do, q, k, v, o, saved, bias, mt, need=(False, False, False, True))
+    assert alone[:3] == (None, None, None) and torch.equal(alone[3], got["dbias"])
+    again = _run(*args)
+    assert all(torch.equal(again[name], got[name]) for name in got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("d", [1, 3, 8, 33, 40, 64, 65, 96, 100, 128])
 def test_attention_head_dims(d, dtype, cuda_device):
     _verify(_att(2, 70, 45, 2, 1, d, dtype, cuda_device, "batch", dtype, "holes"))
@@ -247,6 +265,14 @@ def test_attention_large_logits(cuda_device):
     q, k, v, do, bias, _ = _att(1, 50, 60, 2, 2, 32, F32, cuda_device, "batch", F32)
     _verify((q * 20, k * 10, v, do, bias, None))
     _verify((q, k, v, do, bias * 300, None))
+
+
+def test_attention_peaked_rows_keep_small_gradients(cuda_device):
+    """Rows whose probability is 1 in fp32 at one key: its ds is 0, the other keys keep theirs, however small."""
+    for dtype in (F32, BF16):
+        q, k, v, do, bias, _ = _att(3, 66, 70, 2, 2, 32, dtype, cuda_device, "shared", F32)
+        bias[:, :, ::2, 5] += 30.0  # every other row
+        _verify((q, k, v, do, bias, None))
 
 
 def test_attention_parts_scale_and_repeat(cuda_device):
