@@ -194,21 +194,34 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? (MT == 1 ? 4 : 3) : 2) k_
         for (int c = 0; c < KS; ++c) ldsm4_ti<q * 16 * RB>(f[c], vc[c]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
+          uint32_t pa[TERMS][4];
 #pragma unroll
-          for (int term = 0; term < TERMS; ++term) {
-            uint32_t pa[4];
+          for (int term = 0; term < TERMS; ++term)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float* v = &x[m][2 * q + (i >> 1)][2 * (i & 1)];
-              pa[i] = pack_bf16(v[0], v[1]);
-              if (term + 1 < TERMS) fma2(F2(lo_f(pa[i]), hi_f(pa[i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
+              pa[term][i] = pack_bf16(v[0], v[1]);
+              if (term + 1 < TERMS) fma2(F2(lo_f(pa[term][i]), hi_f(pa[term][i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
             }
 #pragma unroll
-            for (int c = 0; c < KS; ++c) {
-              mma(acc[m][2 * c], pa, f[c][0], f[c][1]);
-              mma(acc[m][2 * c + 1], pa, f[c][2], f[c][3]);
+          for (int c = 0; c < KS; ++c)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              float* d = acc[m][2 * c + n];
+              if (BT == 2) {
+                // the products cut off below the last bit of their sum: start from zero, small terms first,
+                // and add the group by rounded additions
+                float part[4];
+                mma0(part, pa[TERMS - 1], f[c][2 * n], f[c][2 * n + 1]);
+#pragma unroll
+                for (int term = TERMS - 2; term >= 0; --term) mma(part, pa[term], f[c][2 * n], f[c][2 * n + 1]);
+                add2(F2(d[0], d[1]), F2(part[0], part[1])).get(d[0], d[1]);
+                add2(F2(d[2], d[3]), F2(part[2], part[3])).get(d[2], d[3]);
+              } else {
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) mma(d, pa[term], f[c][2 * n], f[c][2 * n + 1]);
+              }
             }
-          }
         }
       });
 #pragma unroll
@@ -342,7 +355,7 @@ __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ 
 
 // ---------------------------------------------------------------- dq (and dbias of one batch entry)
 
-template <int DP, int BT>
+template <int DP, int BT, int TERMS>
 __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
   constexpr int QR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
@@ -471,16 +484,23 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
               put_bias4<BT>(dp[r] + (hb * 32 + q * 16) * BS, j, nk, FAST || (a.db_vec && j0 + hb * 32 + q * 16 + 16 <= nk),
                             y[0][2 * r], y[0][2 * r + 1], y[1][2 * r], y[1][2 * r + 1]);
       }
-      uint32_t da[4];
+      uint32_t da[TERMS][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) da[i] = pack_bf16(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1]);
+      for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* v = &y[i >> 1][2 * (i & 1)];
+          da[term][i] = pack_bf16(v[0], v[1]);
+          if (term + 1 < TERMS) fma2(F2(lo_f(da[term][i]), hi_f(da[term][i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
+        }
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         uint32_t f[4];
         ldsm4_ti<q * 16 * RB>(f, tc[c]);
-        {
-          mma(acc[2 * c], da, f[0], f[1]);
-          mma(acc[2 * c + 1], da, f[2], f[3]);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) {
+          mma(acc[2 * c], da[term], f[0], f[1]);
+          mma(acc[2 * c + 1], da[term], f[2], f[3]);
         }
       }
     });
@@ -545,7 +565,7 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
 
 // 16 keys per warp (32 need 168 registers where 16 need 128, and three blocks on an SM are slower than four:
 // 768 tokens 2.1 against 1.9 ms); HOLD: their fragments stay in registers.
-template <int DP, int BT>
+template <int DP, int BT, int TERMS>
 __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
   constexpr int KR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
@@ -654,32 +674,41 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
               if (!((mine >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
       }
       const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
-      uint32_t pa[4], da[4];
+      uint32_t pa[TERMS][4], da[TERMS][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float p[2], ds[2];
-            const F2 p2 = prob2(&x[n][2 * r], nmx[r], lg[r]);
-            p2.get(p[0], p[1]);
-            mul2(p2, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
-            if (peaked) {
-              if (p[0] == 1.f) ds[0] = 0.f;
-              if (p[1] == 1.f) ds[1] = 0.f;
-            }
-            pa[2 * r + n] = transpose8(pack_bf16(p[0], p[1]));
-            da[2 * r + n] = transpose8(pack_bf16(ds[0], ds[1]));
+        for (int r = 0; r < 2; ++r) {
+          float p[2], ds[2];
+          const F2 p2 = prob2(&x[n][2 * r], nmx[r], lg[r]);
+          p2.get(p[0], p[1]);
+          mul2(p2, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
+          if (peaked) {
+            if (p[0] == 1.f) ds[0] = 0.f;
+            if (p[1] == 1.f) ds[1] = 0.f;
           }
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
+            const uint32_t a = pack_bf16(p[0], p[1]), c = pack_bf16(ds[0], ds[1]);
+            pa[term][2 * r + n] = transpose8(a);
+            da[term][2 * r + n] = transpose8(c);
+            if (term + 1 < TERMS) {
+              p[0] -= lo_f(a), p[1] -= hi_f(a);
+              ds[0] -= lo_f(c), ds[1] -= hi_f(c);
+            }
+          }
+        }
 #pragma unroll
       for (int n = 0; n < KS; ++n) {
         uint32_t fg[4], fq[4];
         ldsm4_ti<blk * 16 * RB + kG>(fg, tc[n]);
         ldsm4_ti<blk * 16 * RB>(fq, tc[n]);
-        {
-          mma(dv[2 * n], pa, fg[0], fg[1]);
-          mma(dv[2 * n + 1], pa, fg[2], fg[3]);
-          mma(dk[2 * n], da, fq[0], fq[1]);
-          mma(dk[2 * n + 1], da, fq[2], fq[3]);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) {
+          mma(dv[2 * n], pa[term], fg[0], fg[1]);
+          mma(dv[2 * n + 1], pa[term], fg[2], fg[3]);
+          mma(dk[2 * n], da[term], fq[0], fq[1]);
+          mma(dk[2 * n + 1], da[term], fq[2], fq[3]);
         }
       }
     });
@@ -752,12 +781,12 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
 
 // dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
 // run side by side.
-template <int DP, int BT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 2) k_dqkv(Args a, unsigned dkv_blocks) {
+template <int DP, int BT, int TERMS>
+__global__ void __launch_bounds__(kThreads, DP == 32 && TERMS == 1 ? 4 : 2) k_dqkv(Args a, unsigned dkv_blocks) {
   if (blockIdx.x < dkv_blocks)
-    dkv_block<DP, BT>(a, blockIdx.x, (a.nk + 63) / 64);
+    dkv_block<DP, BT, TERMS>(a, blockIdx.x, (a.nk + 63) / 64);
   else
-    dq_block<DP, BT>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
+    dq_block<DP, BT, TERMS>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
 
 // ---------------------------------------------------------------- dbias shared by the batch
@@ -1314,8 +1343,11 @@ int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
     return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, tq * a.H * a.B, "k_attn_fwd", flops, st, a);
   }
   const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
-  return go(k_dqkv<DP, BT>, (128 + 4 * kTile) * RB + 2048, bq + bkv,
-            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a, (unsigned)bkv);
+  // p and ds as two bf16 values where the blocks do not fill the machine and the second costs nothing
+  const size_t smem = (128 + 4 * kTile) * RB + 2048;
+  const char* name = kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv");
+  if (bq + bkv <= 148) return go(k_dqkv<DP, BT, 2>, smem, bq + bkv, name, flops, st, a, (unsigned)bkv);
+  return go(k_dqkv<DP, BT, 1>, smem, bq + bkv, name, flops, st, a, (unsigned)bkv);
 }
 
 template <int DP, int BT>
