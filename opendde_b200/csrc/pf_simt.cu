@@ -127,8 +127,8 @@ __device__ __forceinline__ void load_params4(const float* p, bool aligned, float
 }
 
 // V vectors per lane, U groups of rows per warp: the loads of U rows are in flight together and they share
-// one read of gamma and beta (1536^2 rows of 128 bf16: 381 us with U = 1 and scalar parameter reads, see
-// the launch for U).
+// one read of gamma and beta. 1536^2 rows of 128 bf16: 232 us, 5.2 TB/s (381 us with U = 1 and scalar
+// parameter reads).
 template <class T, int L, int V, int U>
 __global__ void __launch_bounds__(256) k_layernorm_rows(const T* __restrict__ x, T* __restrict__ y, int64_t rows,
                                                         int c, const float* __restrict__ gamma,
