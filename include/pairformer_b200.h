@@ -495,7 +495,9 @@ PF_API int pf_copy_regions_dma(const pf_copy_region* regions, int32_t n_regions,
  *   dq = scale ds k,  dk = scale ds^T q,  dv = p^T do,  dbias = ds
  * dk and dv add the query heads that share a key head; dbias adds the batch where it is shared. The
  * backward recomputes p from the row statistics that the forward kept. A query that sees no key has
- * o = 0 and gradients 0; keys the mask drops are not read. */
+ * o = 0 and gradients 0; keys the mask drops are not read. p, ds and (fp32) all operands are multiplied
+ * as sums of bf16 values: an infinity, or a value above 3.389e38, of q, k, v or do at a visible place
+ * gives NaN. The bias may hold infinities. */
 typedef struct {
   int64_t batch, n_q, n_k;
   int32_t heads, kv_heads, head_dim; /* kv_heads divides heads; head_dim in [1, 128]   */

@@ -1,5 +1,5 @@
 // pf_attention_tc.cuh -- building blocks of the tensor-core attention kernels (pf_attention_bf16.cu,
-// pf_attention_f32_tc.cu): swizzled shared tiles and their ldmatrix addresses, products, visible keys, bias
+// pf_attention_f32.cu): swizzled shared tiles and their ldmatrix addresses, products, visible keys, bias
 // fragments, scores. See pf_attention_bf16.cu for the layout.
 #pragma once
 #include <type_traits>
@@ -15,7 +15,6 @@ namespace {
 using bf16 = __nv_bfloat16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;  // rows of a streamed tile
-
 
 // ---------------------------------------------------------------- shared tiles
 
