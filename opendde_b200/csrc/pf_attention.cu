@@ -41,9 +41,9 @@ int sum_planes(const Args& a, const float* part, int parts, cudaStream_t st) {
   return PF_OK;
 }
 
-// How the gradient of a shared bias is computed: with dq in one pass (one block of 16 warps per SM), or by
-// itself (as many blocks as run at a time), in `parts` parts of the batch of at least four entries each (a part
-// costs a plane written and read).
+// How the gradient of a shared bias is computed: with dq in one pass (bf16: one block of 16 warps per SM; fp32:
+// three blocks of four, or two above 256 keys), or by itself (as many blocks as run at a time), in `parts` parts
+// of the batch of at least four entries each (a part costs a plane written and read).
 struct SharedPlan {
   bool plane;
   int parts;
@@ -51,17 +51,17 @@ struct SharedPlan {
 SharedPlan shared_plan(const pf_attention_shape& s) {
   SharedPlan p{false, 1};
   if (s.n_q == 0 || s.n_k == 0) return p;
-  if (s.dtype == PF_BF16 && attn::dq_plane_fits(s.n_q, s.n_k, s.head_dim)) {
-    const int64_t blocks = (s.n_q + 63) / 64 * s.heads;
-    int64_t n = blocks >= 148 ? 1 : 148 / blocks;
+  const bool bf16 = s.dtype == PF_BF16;
+  if (bf16 ? attn::dq_plane_bf16_fits(s.n_k, s.head_dim) : attn::dq_plane_f32_fits(s.n_k, s.head_dim)) {
+    const int64_t blocks = (s.n_q + 63) / 64 * s.heads, fit = 148 * (bf16 ? 1 : (s.n_k <= 256 ? 3 : 2));
+    int64_t n = blocks >= fit ? 1 : fit / blocks;
     if (n > s.batch / 4) n = s.batch / 4;
     if (n < 1) n = 1;
     // where the last wave of blocks leaves most of the machine idle, the two passes are faster
-    const int64_t waves = (blocks * n + 147) / 148;
-    if (blocks * n * 100 >= waves * 148 * 60) return SharedPlan{true, (int)n};
+    const int64_t waves = (blocks * n + fit - 1) / fit;
+    if (blocks * n * 100 >= waves * fit * 60) return SharedPlan{true, (int)n};
   }
   // tiles of the kernels and how many blocks an SM holds
-  const bool bf16 = s.dtype == PF_BF16;
   const int64_t rows = bf16 ? 128 : 64, keys = bf16 || s.head_dim <= 32 ? 64 : (s.head_dim <= 64 ? 32 : 16);
   const int64_t blocks = ((s.n_q + rows - 1) / rows) * ((s.n_k + keys - 1) / keys) * s.heads;
   const int64_t fit = (s.head_dim <= 32 ? (bf16 ? 3 : 4) : 1) * 148;
@@ -191,7 +191,8 @@ int attention_bwd(const pf_attention_call& c, void* ws, size_t ws_bytes, cudaStr
   float* part = plan.parts > 1 ? ar.take<float>((size_t)plan.parts * s.heads * s.n_q * s.n_k) : nullptr;
   if (!ar.ok()) return fail(PF_EWORKSPACE, "attention backward: workspace too small");
   if (plan.plane)
-    PF_TRY(attn::dq_plane_bf16(a, part, plan.parts, 3 * pair, st));
+    PF_TRY(s.dtype == PF_BF16 ? attn::dq_plane_bf16(a, part, plan.parts, 3 * pair, st)
+                              : attn::dq_plane_f32(a, part, plan.parts, 3 * pair, st));
   else
     PF_TRY(s.dtype == PF_BF16 ? attn::dbias_bf16(a, part, plan.parts, 2 * pair, st)
                               : attn::dbias_f32(a, part, plan.parts, 2 * pair, st));

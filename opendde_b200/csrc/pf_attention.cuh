@@ -94,7 +94,9 @@ int launch_f32(Kind kind, const Args& a, double flops, cudaStream_t st);
 int dbias_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st);
 int dbias_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st);
 // dq and the gradient of a shared bias in one pass, where it fits; parts as for dbias_*
-bool dq_plane_fits(int64_t nq, int64_t nk, int d);
+bool dq_plane_bf16_fits(int64_t nk, int d);
+bool dq_plane_f32_fits(int64_t nk, int d);
+int dq_plane_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st);
 int dq_plane_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st);
 int rows_bf16(const Args& a, const float* stats, Heads o, const int16_t* lo, float* rows, cudaStream_t st);
 int rows_f32(const Args& a, const float* stats, Heads o, float* rows, cudaStream_t st);

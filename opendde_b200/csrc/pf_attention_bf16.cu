@@ -981,24 +981,6 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
 constexpr int kPlaneThreads = 512;
 constexpr int kPlaneKeys = 832;
 
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr));
-}
-// the wait takes the loaded registers along, so that no use of them moves above it
-__device__ __forceinline__ void tmem_wait8(uint32_t (&r)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-
 struct PlaneSmem {  // byte offsets
   int kv, q, cst, vis, end;
   __host__ __device__ explicit PlaneSmem(int nkp) {
@@ -1401,7 +1383,7 @@ int dbias_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t
   PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);
 }
 
-bool dq_plane_fits(int64_t nq, int64_t nk, int d) { return d <= 32 && nk <= kPlaneKeys && nk > 0 && nq > 0; }
+bool dq_plane_bf16_fits(int64_t nk, int d) { return d <= 32 && nk <= kPlaneKeys; }
 int dq_plane_bf16(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
   return a.bias_f32 ? launch_plane<2>(a, part, parts, flops, st) : launch_plane<1>(a, part, parts, flops, st);
 }

@@ -8,7 +8,7 @@
 // ds) restarts from zero for every 16 columns and is added to the accumulators by rounded fp32
 // additions. Against the FFMA form of the same kernels, which the multiply-adds bound at 128 per clock
 // and SM (149 rows of 149 tokens, 12 heads of 32, forward plus backward: 1.9 ms), six products at 1024
-// per clock and SM are 1.3 times as many, with a quarter of the instructions (1.1 ms; 0.7 ms of products).
+// per clock and SM are 1.3 times as many, with a quarter of the instructions (0.79 ms; 0.55 ms of products).
 // An infinity splits into an infinity and a NaN: at a visible place it gives NaN.
 //
 // The layout is that of pf_attention_bf16.cu, with every tile in three planes. The streamed tiles are read
@@ -16,6 +16,7 @@
 // one. 16 stationary rows per warp, four warps to a block.
 
 #include "pf_attention_tc.cuh"
+#include "pf_sm100.cuh"
 
 namespace pf {
 namespace train {
@@ -246,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
       for (int hb = 0; hb < KT / HB; ++hb) {
         const int64_t j0 = (int64_t)kt * KT + hb * HB;
         const uint32_t hbits = (uint32_t)(bits >> (HB * hb));
+        if ((hbits & (HB == 32 ? ~0u : 0xffffu)) == 0) continue;  // no visible key
         float x[GQ][2][4];
 #pragma unroll
         for (int q = 0; q < GQ; ++q) {
@@ -390,20 +392,21 @@ __device__ __forceinline__ void prob_ds(float (&x)[2][4], float (&y)[2][4], cons
   }
 }
 
-// ---------------------------------------------------------------- dq (and dbias of one batch entry)
+// ---------------------------------------------------------------- dq (and dbias)
 
-template <int DP, int BT>
-__device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
+// dq of rows [64 tile, 64 tile + 64) of (b, h). dbias of the entry is written where a.dbias is set; PLANE: added to
+// the sums of the entries before, eight words of tensor memory per lane for each 16 keys, from tm0.
+template <int DP, int BT, bool PLANE>
+__device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigned tile, uint32_t tm0) {
   using S = Split<DP>;
   constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8;
   extern __shared__ __align__(128) unsigned char raw[];
   const uint32_t sq = smem_addr(raw), sg = sq + S::kStat3, sk = sg + S::kStat3, sv = sk + 2 * S::kTile3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), lt = lane_bt<DP>();
-  const unsigned tile = id % (unsigned)tiles;
-  id /= (unsigned)tiles;
-  const int h = id % a.H, kh = h / (a.H / a.KV);
-  const int64_t b = id / a.H, w0 = (int64_t)tile * 64 + warp * 16;
+  const int kh = h / (a.H / a.KV);
+  const int64_t w0 = (int64_t)tile * 64 + warp * 16;
+  const bool put = BT && !PLANE && a.dbias;
   const int nt = (int)((a.nk + KT - 1) / KT);
   const float *bk = head_f(a.k, b, kh), *bv = head_f(a.v, b, kh);
   const char* brow[2];
@@ -414,7 +417,7 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   for (int r = 0; r < 2; ++r) {
     const int64_t i = w0 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
     brow[r] = bias_row<BT>(a, b, h, ic);
-    drow[r] = (BT && a.dbias && i < a.nq)
+    drow[r] = (put && i < a.nq)
                   ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs) * (BT == 2 ? 4 : 2)
                   : nullptr;
     const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
@@ -443,12 +446,13 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
       pk.read(bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
       pv.read(bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
     }
-    if (w0 < a.nq && (bits != 0 || (BT && a.dbias))) {
+    if (w0 < a.nq && (bits != 0 || put)) {
       const uint32_t tk = sk + (kt & 1) * S::kTile3, tv = sv + (kt & 1) * S::kTile3;
 #pragma unroll 1
       for (int q = 0; q < KT / 16; ++q) {
         const int64_t j0 = (int64_t)kt * KT + q * 16;
         const uint32_t qbits = (uint32_t)(bits >> (16 * q)) & 0xffffu;
+        if (qbits == 0 && (!put || j0 >= a.nk)) continue;  // no visible key, and nothing to write
         Bias4<BT> br[2];
         const bool whole = j0 + 16 <= a.nk;
 #pragma unroll
@@ -464,7 +468,22 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
           for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
         hide16<BT, 1>(x, qbits);
         prob_ds(x[0], y, nmx, lg, nd, peaked);
-        if (BT && a.dbias)
+        if (PLANE) {
+          uint32_t tm[8];
+          const uint32_t at = tm0 + (uint32_t)(kt * (KT / 16) + q) * 8;
+          tmem_ld8(at, tm);
+          tmem_wait8(tm);
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            float s0, s1;
+            add2(F2(__uint_as_float(tm[i]), __uint_as_float(tm[i + 1])), F2(y[i >> 2][i & 3], y[i >> 2][(i & 3) + 1]))
+                .get(s0, s1);
+            tm[i] = __float_as_uint(s0), tm[i + 1] = __float_as_uint(s1);
+          }
+          tmem_st8(at, tm);
+          if (!a.dq) continue;
+        }
+        if (put)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
             if (drow[r])
@@ -492,6 +511,74 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
     for (int n = 0; n < NB; ++n)
       store2f(o, n * 8 + 2 * t, a.d, vec, acc[n][2 * r] * a.scale, acc[n][2 * r + 1] * a.scale);
   }
+}
+
+template <int DP, int BT>
+__device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
+  const unsigned tile = id % (unsigned)tiles;
+  id /= (unsigned)tiles;
+  dq_rows<DP, BT, false>(a, id / a.H, id % a.H, tile, 0);
+}
+
+// dq and the gradient of a bias that the batch shares in one pass (see k_dq_plane of the bf16 kernels): a block
+// takes 64 rows of one head through a part of the batch, and its rows of the plane lie in tensor memory, 128
+// columns for up to 256 keys (three blocks per SM) or 256 for up to 512 (two). Next to dq and dbias apart this
+// saves two of five products: 149 rows of 149 tokens, 12 heads, 0.28 ms against 0.48 ms.
+constexpr int kPlaneKeys = 512;
+
+template <int BT>
+__global__ void __launch_bounds__(kThreads, 3) k_dq_plane(Args a, float* part, int parts, int tcols, int tptr_at) {
+  extern __shared__ __align__(128) unsigned char raw[];
+  uint32_t* tptr = (uint32_t*)(raw + tptr_at);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned id = blockIdx.x;
+  const unsigned tile = id % (unsigned)a.tiles;
+  id /= (unsigned)a.tiles;
+  const int h = id % a.H, pt = id / a.H;
+  const int64_t b0 = a.B * pt / parts, b1 = a.B * (pt + 1) / parts;
+  const int64_t w0 = (int64_t)tile * 64 + warp * 16;
+  const int groups = (int)((a.nk + 15) / 16);
+  if (warp == 0) {
+    sm100::tmem_alloc(smem_addr(tptr), tcols);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tbase = *tptr, tm0 = tbase + ((uint32_t)(warp * 32) << 16);
+  const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int q = 0; q < groups; ++q) tmem_st8(tm0 + q * 8, zero);
+  sm100::tmem_st_wait();
+  for (int64_t b = b0; b < b1; ++b) {
+    if (b > b0) __syncthreads();  // the last entry's tiles are done with
+    dq_rows<32, BT, true>(a, b, h, tile, tm0);
+    sm100::tmem_st_wait();
+  }
+  for (int q = 0; q < groups; ++q) {
+    uint32_t tm[8];
+    __syncwarp();
+    tmem_ld8(tm0 + q * 8, tm);
+    tmem_wait8(tm);
+    const int64_t j = (int64_t)q * 16 + 4 * t;
+    const bool whole = (int64_t)q * 16 + 16 <= a.nk;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t i = w0 + r * 8 + g;
+      if (i >= a.nq) continue;
+      const float v0 = __uint_as_float(tm[2 * r]), v1 = __uint_as_float(tm[2 * r + 1]),
+                  v2 = __uint_as_float(tm[4 + 2 * r]), v3 = __uint_as_float(tm[5 + 2 * r]);
+      if (parts == 1)
+        store_bias4<BT>(a, (char*)a.dbias + ((int64_t)h * a.db_hs + i * a.db_rs) * (BT == 2 ? 4 : 2), j,
+                        a.db_vec && whole, v0, v1, v2, v3);
+      else
+        store_bias4<2>(a, (char*)(part + (((int64_t)pt * a.H + h) * a.nq + i) * a.nk), j, (a.nk & 3) == 0 && whole, v0,
+                       v1, v2, v3);
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  if (warp == 0) sm100::tmem_dealloc(tbase, tcols);
 }
 
 // ---------------------------------------------------------------- dk, dv
@@ -550,6 +637,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
         const uint32_t tq = sq + (it & 1) * S::kTile3, tg = sg + (it & 1) * S::kTile3;
 #pragma unroll 1
         for (int blk = 0; blk < KT / 16; ++blk) {
+          if (i0 + blk * 16 >= a.nq) break;
           Bias4<BT> br[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -675,6 +763,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, fl
     if (w0 >= a.nq) continue;
 #pragma unroll
     for (int q = 0; q < GQ; ++q) {
+      if (((uint32_t)(bits >> (16 * q)) & 0xffffu) == 0) continue;  // no visible key
       Bias4<BT> br[2];
       const bool fast = a.bias_vec && j0 + q * 16 + 16 <= a.nk;
 #pragma unroll
@@ -754,6 +843,17 @@ int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
             "k_attn_dbias", flops, st, a, part, parts);
 }
 
+template <int BT>
+int launch_plane(Args a, float* part, int parts, double flops, cudaStream_t st) {
+  using S = Split<32>;
+  const int tcols = a.nk <= 256 ? 128 : 256;
+  const int tiles = 2 * S::kStat3 + 4 * S::kTile3;
+  // room for as many blocks as tensor memory holds
+  const size_t smem = tcols == 128 ? tiles + 16 : 100 * 1024;
+  a.tiles = (a.nq + 63) / 64;
+  return go(k_dq_plane<BT>, smem, a.tiles * a.H * parts, "k_attn_dq_plane", flops, st, a, part, parts, tcols, tiles);
+}
+
 }  // namespace
 
 #define PF_ATT_DIM(FN, BT, ...)                    \
@@ -771,6 +871,10 @@ int launch_f32(Kind kind, const Args& a, double flops, cudaStream_t st) {
 int dbias_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
   if (a.bias_f32) PF_ATT_DIM(launch_db, 2, a, part, parts, flops, st);
   PF_ATT_DIM(launch_db, 1, a, part, parts, flops, st);
+}
+bool dq_plane_f32_fits(int64_t nk, int d) { return d <= 32 && nk <= kPlaneKeys; }
+int dq_plane_f32(const Args& a, float* part, int parts, double flops, cudaStream_t st) {
+  return a.bias_f32 ? launch_plane<2>(a, part, parts, flops, st) : launch_plane<1>(a, part, parts, flops, st);
 }
 int rows_f32(const Args& a, const float* stats, Heads o, float* rows, cudaStream_t st) {
   const int lanes = a.d <= 32 ? 8 : (a.d <= 64 ? 16 : 32);

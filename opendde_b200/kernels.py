@@ -36,7 +36,7 @@ def require_cuda(*ts: Optional[torch.Tensor]) -> None:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def pair_view(t: torch.Tensor) -> PairView:

@@ -158,6 +158,16 @@ def test_attention_shared_bias_over_a_long_batch(B, nq, nk, H, KV, d, mask, bias
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,nq,nk,H,KV,d,mask,bias_dtype", [
+    (96, 130, 149, 4, 4, 24, "holes", F32), (100, 65, 256, 6, 3, 32, "pad", BF16), (99, 70, 257, 4, 4, 32, None, F32),
+    (100, 67, 512, 4, 1, 30, "holes", F32), (100, 65, 513, 4, 4, 32, "pad", F32)])
+def test_attention_shared_bias_with_blocks_for_every_sm(B, nq, nk, H, KV, d, mask, bias_dtype, dtype, cuda_device):
+    """As above where the batch's parts fill the machine, which fp32 takes for its one pass: up to 256, up to 512 and
+    above 512 keys."""
+    test_attention_shared_bias_over_a_long_batch(B, nq, nk, H, KV, d, mask, bias_dtype, dtype, cuda_device)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("d", [1, 3, 8, 33, 40, 64, 65, 96, 100, 128])
 def test_attention_head_dims(d, dtype, cuda_device):
     _verify(_att(2, 70, 45, 2, 1, d, dtype, cuda_device, "batch", dtype, "holes"))
