@@ -46,73 +46,95 @@ __device__ __forceinline__ void split4(const float4& v, uint2 (&w)[3]) {
   }
 }
 
-// A tile of KT rows on its way: read, then split and stored.
+// A thread's place in the tiles of KT rows of one operand: four 16-byte loads, rows `row` + RP i.
+template <int DP>
+struct Place {
+  static constexpr int CH = DP / 4, RP = kThreads / CH;
+  int row, col;
+  uint32_t dst;
+  __device__ __forceinline__ Place() {
+    row = threadIdx.x / CH;
+    col = (threadIdx.x - row * CH) * 4;
+    dst = Tile<DP>::off(row, col >> 3) + (col & 7) * 2;
+  }
+  // the offset of load i: rows RP apart have the same swizzle (32 channels) or differ in one bit of it
+  __device__ __forceinline__ uint32_t at(int i) const {
+    const uint32_t x = DP == 32 ? 0 : (DP == 64 ? (i & 1) * 2 : (i & 1) * 4 + (i >> 1) * 2);
+    return (dst ^ (x << 4)) + i * RP * Tile<DP>::RB;
+  }
+};
+
+// A tile on its way: read, then split and stored.
 template <int DP>
 struct Ahead {
+  using P = Place<DP>;
   float4 v[4];
-  __device__ __forceinline__ void read(const float* base, int64_t ns, int vec, int64_t r0, int64_t n, int d,
+  // rows r0.. of `base`; those without a bit in `live`, which has none past the end, are zero
+  __device__ __forceinline__ void read(const P& at, const float* base, int64_t ns, int vec, int64_t r0, int d,
                                        uint64_t live) {
-    constexpr int CH = DP / 4;
+    const float* p = base + (r0 + at.row) * ns + at.col;
+    const uint64_t mine = at.col < d ? live >> at.row : 0;
+    const uint32_t half[2] = {(uint32_t)mine, (uint32_t)(mine >> 32)};
+    const int64_t step = ns * P::RP;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = threadIdx.x + j * kThreads, r = i / CH, c = (i - r * CH) * 4;
-      const bool ok = r0 + r < n && c < d && ((live >> (r & 63)) & 1);
-      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (ok) {
-        const float* p = base + (r0 + r) * ns + c;
+    for (int i = 0; i < 4; ++i, p += step) {
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if ((half[i * P::RP / 32] >> (i * P::RP % 32)) & 1) {
         if (vec) {
-          v[j] = *reinterpret_cast<const float4*>(p);
+          v[i] = *reinterpret_cast<const float4*>(p);
         } else {
-          v[j].x = p[0];
-          if (c + 1 < d) v[j].y = p[1];
-          if (c + 2 < d) v[j].z = p[2];
-          if (c + 3 < d) v[j].w = p[3];
+          v[i].x = p[0];
+          if (at.col + 1 < d) v[i].y = p[1];
+          if (at.col + 2 < d) v[i].z = p[2];
+          if (at.col + 3 < d) v[i].w = p[3];
         }
       }
     }
   }
-  __device__ __forceinline__ void store(uint32_t sm, int plane, int row0 = 0) const {
-    constexpr int CH = DP / 4;
+  template <int PLANE>
+  __device__ __forceinline__ void store(const P& at, uint32_t sm) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = threadIdx.x + j * kThreads, r = row0 + i / CH, c = (i - i / CH * CH) * 4;
+    for (int i = 0; i < 4; ++i) {
       uint2 w[3];
-      split4(v[j], w);
-      const uint32_t at = sm + Tile<DP>::off(r, c >> 3) + (c & 7) * 2;
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + p * plane), "r"(w[p].x), "r"(w[p].y) : "memory");
+      split4(v[i], w);
+      const uint32_t to = sm + at.at(i);
+      unrolled<3>([&](auto Q) {
+        constexpr int p = decltype(Q)::value;
+        asm volatile("st.shared.v2.b32 [%0+%3], {%1, %2};" ::"r"(to), "r"(w[p].x), "r"(w[p].y), "n"(p * PLANE)
+                     : "memory");
+      });
     }
   }
 };
 // 64 rows at once
 template <int DP>
-__device__ __forceinline__ void load_stat(uint32_t sm, const float* base, int64_t ns, int vec, int64_t r0, int64_t n,
-                                          int d, uint64_t live) {
+__device__ __forceinline__ void load_stat(const Place<DP>& at, uint32_t sm, const float* base, int64_t ns, int vec,
+                                          int64_t r0, int d, uint64_t live) {
   using S = Split<DP>;
 #pragma unroll 1
   for (int r = 0; r < 64; r += S::KT) {
     Ahead<DP> t;
-    t.read(base, ns, vec, r0 + r, n, d, live >> r);
-    t.store(sm, S::kStatPlane, r);
+    t.read(at, base, ns, vec, r0 + r, d, live >> r);
+    t.template store<S::kStatPlane>(at, sm + r * S::RB);
   }
 }
 __device__ __forceinline__ const float* head_f(const Heads& s, int64_t b, int h) {
   return (const float*)s.p + b * s.bs + (int64_t)h * s.hs;
 }
 
-// x (16 rows by 16 columns) = a b^T over the channels; `fa(plane, k, r)` and `fb(plane, k, r)` give the fragments
-template <int KS, class FA, class FB>
-__device__ __forceinline__ void nt3(float (&x)[2][4], FA fa, FB fb) {
+// x (16 rows by 16 columns) = a b^T over the channels: the lane's addresses of the operands' first planes for each
+// 16 channels, PA and PB bytes between the planes
+template <int KS, int PA, int PB>
+__device__ __forceinline__ void nt3(float (&x)[2][4], const uint32_t (&aa)[KS], const uint32_t (&ba)[KS]) {
   float lo[2][4];
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
     uint32_t a[3][4], b[3][4];
-#pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      fa(p, k, a[p]);
-      fb(p, k, b[p]);
-    }
+    unrolled<3>([&](auto P) {
+      constexpr int p = decltype(P)::value;
+      ldsm4i<p * PA>(a[p], aa[k]);
+      ldsm4i<p * PB>(b[p], ba[k]);
+    });
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       if (k == 0) {
@@ -134,14 +156,16 @@ __device__ __forceinline__ void nt3(float (&x)[2][4], FA fa, FB fb) {
     for (int r = 0; r < 2; ++r)
       add2(F2(x[n][2 * r], x[n][2 * r + 1]), F2(lo[n][2 * r], lo[n][2 * r + 1])).get(x[n][2 * r], x[n][2 * r + 1]);
 }
-// acc += p b for 16 columns of p in three terms; `fb(plane, c, r)` gives the fragments of channels 16 c..
-template <int NB, class FB>
-__device__ __forceinline__ void nn3(float (&acc)[NB][4], const uint32_t (&pa)[3][4], FB fb) {
+// acc += p b for 16 columns of p in three terms: the lane's addresses of b's first plane for each 16 channels
+template <int NB, int PB>
+__device__ __forceinline__ void nn3(float (&acc)[NB][4], const uint32_t (&pa)[3][4], const uint32_t (&ba)[NB / 2]) {
 #pragma unroll
   for (int c = 0; c < NB / 2; ++c) {
     uint32_t b[3][4];
-#pragma unroll
-    for (int p = 0; p < 3; ++p) fb(p, c, b[p]);
+    unrolled<3>([&](auto P) {
+      constexpr int p = decltype(P)::value;
+      ldsm4_ti<p * PB>(b[p], ba[c]);
+    });
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       float s[4];
@@ -156,6 +180,11 @@ __device__ __forceinline__ void nn3(float (&acc)[NB][4], const uint32_t (&pa)[3]
       add2(F2(d[2], d[3]), F2(s[2], s[3])).get(d[2], d[3]);
     }
   }
+}
+template <int DP>
+__device__ __forceinline__ void addresses(uint32_t (&to)[DP / 16], const LaneAddr<DP>& l, uint32_t base, int blk) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) to[k] = l.at(base, blk, k);
 }
 // 16 x 16 values in accumulator layout as left operands in three terms (left as their remainder)
 __device__ __forceinline__ void split_a(float (&x)[2][4], uint32_t (&pa)[3][4]) {
@@ -229,17 +258,21 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
     for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
   uint64_t bits = tile_bits<KT>(seen_raw(a, b, 0));
   Ahead<DP> pk, pv;
-  load_stat<DP>(sq, head_f(a.q, b, h), a.q.ns, a.vec_q, (int64_t)tile * 64, a.nq, a.d, ~0ull);
-  pk.read(bk, a.k.ns, a.vec_k, 0, a.nk, a.d, bits);
-  pv.read(bv, a.v.ns, a.vec_v, 0, a.nk, a.d, bits);
-  pk.store(sk, S::kPlane);
-  pv.store(sv, S::kPlane);
+  const Place<DP> place;
+  load_stat<DP>(place, sq, head_f(a.q, b, h), a.q.ns, a.vec_q, (int64_t)tile * 64, a.d,
+                first_bits(a.nq - (int64_t)tile * 64));
+  pk.read(place, bk, a.k.ns, a.vec_k, 0, a.d, bits);
+  pv.read(place, bv, a.v.ns, a.vec_v, 0, a.d, bits);
+  pk.template store<S::kPlane>(place, sk);
+  pv.template store<S::kPlane>(place, sv);
+  uint32_t qa[KS];
+  addresses<DP>(qa, la, sq, warp);
   for (int kt = 0; kt < nt; ++kt) {
     const uint64_t next = tile_bits<KT>(seen_raw(a, b, (int64_t)(kt + 1) * KT));
     __syncthreads();
     if (kt + 1 < nt) {
-      pk.read(bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
-      pv.read(bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
+      pk.read(place, bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.d, next);
+      pv.read(place, bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.d, next);
     }
     if (bits != 0 && w0 < a.nq) {
       const uint32_t tk = sk + (kt & 1) * S::kTile3, tv = sv + (kt & 1) * S::kTile3;
@@ -255,8 +288,9 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
           const bool fast = a.bias_vec && j0 + q * 16 + 16 <= a.nk;
 #pragma unroll
           for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + q * 16 + 4 * t, a.nk, fast);
-          nt3<KS>(x[q], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sq + p * S::kStatPlane, warp, k)); },
-                  [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(tk + p * S::kPlane, hb * GQ + q, k)); });
+          uint32_t ba[KS];
+          addresses<DP>(ba, lb, tk, hb * GQ + q);
+          nt3<KS, S::kStatPlane, S::kPlane>(x[q], qa, ba);
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -309,13 +343,15 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
         for (int q = 0; q < GQ; ++q) {
           uint32_t pa[3][4];
           split_a(x[q], pa);
-          nn3<NB>(acc, pa, [&](int p, int c, uint32_t* f) { ldsm4_t(f, lt.at(tv + p * S::kPlane, hb * GQ + q, c)); });
+          uint32_t ba[KS];
+          addresses<DP>(ba, lt, tv, hb * GQ + q);
+          nn3<NB, S::kPlane>(acc, pa, ba);
         }
       }
     }
     if (kt + 1 < nt) {
-      pk.store(sk + ((kt + 1) & 1) * S::kTile3, S::kPlane);
-      pv.store(sv + ((kt + 1) & 1) * S::kTile3, S::kPlane);
+      pk.template store<S::kPlane>(place, sk + ((kt + 1) & 1) * S::kTile3);
+      pv.template store<S::kPlane>(place, sv + ((kt + 1) & 1) * S::kTile3);
     }
     bits = next;
   }
@@ -433,18 +469,23 @@ __device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigne
     for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
   uint64_t bits = tile_bits<KT>(seen_raw(a, b, 0));
   Ahead<DP> pk, pv;
-  load_stat<DP>(sq, head_f(a.q, b, h), a.q.ns, a.vec_q, (int64_t)tile * 64, a.nq, a.d, ~0ull);
-  load_stat<DP>(sg, head_f(a.g, b, h), a.g.ns, a.vec_g, (int64_t)tile * 64, a.nq, a.d, ~0ull);
-  pk.read(bk, a.k.ns, a.vec_k, 0, a.nk, a.d, bits);
-  pv.read(bv, a.v.ns, a.vec_v, 0, a.nk, a.d, bits);
-  pk.store(sk, S::kPlane);
-  pv.store(sv, S::kPlane);
+  const Place<DP> place;
+  const uint64_t rows = first_bits(a.nq - (int64_t)tile * 64);
+  load_stat<DP>(place, sq, head_f(a.q, b, h), a.q.ns, a.vec_q, (int64_t)tile * 64, a.d, rows);
+  load_stat<DP>(place, sg, head_f(a.g, b, h), a.g.ns, a.vec_g, (int64_t)tile * 64, a.d, rows);
+  pk.read(place, bk, a.k.ns, a.vec_k, 0, a.d, bits);
+  pv.read(place, bv, a.v.ns, a.vec_v, 0, a.d, bits);
+  pk.template store<S::kPlane>(place, sk);
+  pv.template store<S::kPlane>(place, sv);
+  uint32_t qa[KS], ga[KS];
+  addresses<DP>(qa, la, sq, warp);
+  addresses<DP>(ga, la, sg, warp);
   for (int kt = 0; kt < nt; ++kt) {
     const uint64_t next = tile_bits<KT>(seen_raw(a, b, (int64_t)(kt + 1) * KT));
     __syncthreads();
     if (kt + 1 < nt) {
-      pk.read(bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
-      pv.read(bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.nk, a.d, next);
+      pk.read(place, bk, a.k.ns, a.vec_k, (int64_t)(kt + 1) * KT, a.d, next);
+      pv.read(place, bv, a.v.ns, a.vec_v, (int64_t)(kt + 1) * KT, a.d, next);
     }
     if (w0 < a.nq && (bits != 0 || put)) {
       const uint32_t tk = sk + (kt & 1) * S::kTile3, tv = sv + (kt & 1) * S::kTile3;
@@ -458,10 +499,11 @@ __device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigne
 #pragma unroll
         for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + 4 * t, a.nk, a.bias_vec && whole);
         float x[1][2][4], y[2][4];
-        nt3<KS>(x[0], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sq + p * S::kStatPlane, warp, k)); },
-                [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(tk + p * S::kPlane, q, k)); });
-        nt3<KS>(y, [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sg + p * S::kStatPlane, warp, k)); },
-                [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(tv + p * S::kPlane, q, k)); });
+        uint32_t ba[KS];
+        addresses<DP>(ba, lb, tk, q);
+        nt3<KS, S::kStatPlane, S::kPlane>(x[0], qa, ba);
+        addresses<DP>(ba, lb, tv, q);
+        nt3<KS, S::kStatPlane, S::kPlane>(y, ga, ba);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -491,12 +533,13 @@ __device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigne
                               y[1][2 * r + 1]);
         uint32_t da[3][4];
         split_a(y, da);
-        nn3<NB>(acc, da, [&](int p, int c, uint32_t* f) { ldsm4_t(f, lt.at(tk + p * S::kPlane, q, c)); });
+        addresses<DP>(ba, lt, tk, q);
+        nn3<NB, S::kPlane>(acc, da, ba);
       }
     }
     if (kt + 1 < nt) {
-      pk.store(sk + ((kt + 1) & 1) * S::kTile3, S::kPlane);
-      pv.store(sv + ((kt + 1) & 1) * S::kTile3, S::kPlane);
+      pk.template store<S::kPlane>(place, sk + ((kt + 1) & 1) * S::kTile3);
+      pv.template store<S::kPlane>(place, sv + ((kt + 1) & 1) * S::kTile3);
     }
     bits = next;
   }
@@ -608,24 +651,29 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
   if (live != 0 && nt > 0) {
     Ahead<DP> pq, pg;
+    const Place<DP> place;
     float4 pc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto read = [&](int it) {
       const int h = kh * group + it / per;
       const int64_t i0 = (int64_t)(it % per) * KT;
-      pq.read(head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
-      pg.read(head_f(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+      const uint64_t rows = first_bits(a.nq - i0) & (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
+      pq.read(place, head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.d, rows);
+      pg.read(place, head_f(a.g, b, h), a.g.ns, a.vec_g, i0, a.d, rows);
       // a row past the end has p = 0
       if (threadIdx.x < KT)
         pc = i0 + threadIdx.x < a.nq ? ((const float4*)a.rows)[(b * a.H + h) * a.nq + i0 + threadIdx.x]
                                      : make_float4(INFINITY, 0.f, 0.f, 0.f);
     };
     auto store = [&](int it) {
-      pq.store(sq + (it & 1) * S::kTile3, S::kPlane);
-      pg.store(sg + (it & 1) * S::kTile3, S::kPlane);
+      pq.template store<S::kPlane>(place, sq + (it & 1) * S::kTile3);
+      pg.template store<S::kPlane>(place, sg + (it & 1) * S::kTile3);
       if (threadIdx.x < KT) cst[(it & 1) * KT + threadIdx.x] = pc;
     };
-    load_stat<DP>(sk, head_f(a.k, b, kh), a.k.ns, a.vec_k, j0, a.nk, a.d, live);
-    load_stat<DP>(sv, head_f(a.v, b, kh), a.v.ns, a.vec_v, j0, a.nk, a.d, live);
+    load_stat<DP>(place, sk, head_f(a.k, b, kh), a.k.ns, a.vec_k, j0, a.d, live);
+    load_stat<DP>(place, sv, head_f(a.v, b, kh), a.v.ns, a.vec_v, j0, a.d, live);
+    uint32_t ka[KS], va[KS];
+    addresses<DP>(ka, lb, sk, warp);
+    addresses<DP>(va, lb, sv, warp);
     read(0);
     store(0);
     for (int it = 0; it < nt; ++it) {
@@ -645,10 +693,11 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
             bias_load<BT>(br[r], bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1), w0 + 4 * t, a.nk, bfast);
           }
           float x[1][2][4], y[2][4];
-          nt3<KS>(x[0], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(tq + p * S::kPlane, blk, k)); },
-                  [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sk + p * S::kStatPlane, warp, k)); });
-          nt3<KS>(y, [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(tg + p * S::kPlane, blk, k)); },
-                  [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sv + p * S::kStatPlane, warp, k)); });
+          uint32_t aa[KS];
+          addresses<DP>(aa, la, tq, blk);
+          nt3<KS, S::kPlane, S::kStatPlane>(x[0], aa, ka);
+          addresses<DP>(aa, la, tg, blk);
+          nt3<KS, S::kPlane, S::kStatPlane>(y, aa, va);
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -665,14 +714,16 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
             w[p][0] = transpose8(u[p][0]), w[p][2] = transpose8(u[p][1]);
             w[p][1] = transpose8(u[p][2]), w[p][3] = transpose8(u[p][3]);
           }
-          nn3<NB>(dv, w, [&](int p, int n, uint32_t* f) { ldsm4_t(f, ln.at(tg + p * S::kPlane, blk, n)); });
+          addresses<DP>(aa, ln, tg, blk);
+          nn3<NB, S::kPlane>(dv, w, aa);
           split_a(y, u);
 #pragma unroll
           for (int p = 0; p < 3; ++p) {
             w[p][0] = transpose8(u[p][0]), w[p][2] = transpose8(u[p][1]);
             w[p][1] = transpose8(u[p][2]), w[p][3] = transpose8(u[p][3]);
           }
-          nn3<NB>(dk, w, [&](int p, int n, uint32_t* f) { ldsm4_t(f, ln.at(tq + p * S::kPlane, blk, n)); });
+          addresses<DP>(aa, ln, tq, blk);
+          nn3<NB, S::kPlane>(dk, w, aa);
         }
       }
       if (it + 1 < nt) store(it + 1);
@@ -731,6 +782,10 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, fl
     brow[r] = bias_row<BT>(a, 0, h, i < a.nq ? i : a.nq - 1);
   }
   const F2 scale(a.scale);
+  const Place<DP> place;
+  uint32_t qa[KS], ga[KS];
+  addresses<DP>(qa, la, sq, warp);
+  addresses<DP>(ga, la, sg, warp);
   float acc[GQ][2][4];
 #pragma unroll
   for (int q = 0; q < GQ; ++q)
@@ -742,13 +797,13 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, fl
     const uint64_t bits = tile_bits<KT>(seen_raw(a, b, j0));
     if (bits == 0) continue;  // the same for the whole block
     __syncthreads();
-    load_stat<DP>(sq, head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.nq, a.d, ~0ull);
-    load_stat<DP>(sg, head_f(a.g, b, h), a.g.ns, a.vec_g, i0, a.nq, a.d, ~0ull);
+    load_stat<DP>(place, sq, head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.d, first_bits(a.nq - i0));
+    load_stat<DP>(place, sg, head_f(a.g, b, h), a.g.ns, a.vec_g, i0, a.d, first_bits(a.nq - i0));
     Ahead<DP> pk, pv;
-    pk.read(head_f(a.k, b, kh), a.k.ns, a.vec_k, j0, a.nk, a.d, bits);
-    pv.read(head_f(a.v, b, kh), a.v.ns, a.vec_v, j0, a.nk, a.d, bits);
-    pk.store(sk, S::kPlane);
-    pv.store(sv, S::kPlane);
+    pk.read(place, head_f(a.k, b, kh), a.k.ns, a.vec_k, j0, a.d, bits);
+    pv.read(place, head_f(a.v, b, kh), a.v.ns, a.vec_v, j0, a.d, bits);
+    pk.template store<S::kPlane>(place, sk);
+    pv.template store<S::kPlane>(place, sv);
     F2 nmx[2], lg[2], nd[2];
     bool peaked = false;
 #pragma unroll
@@ -769,10 +824,11 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, fl
 #pragma unroll
       for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + q * 16 + 4 * t, a.nk, fast);
       float x[1][2][4], y[2][4];
-      nt3<KS>(x[0], [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sq + p * S::kStatPlane, warp, k)); },
-              [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sk + p * S::kPlane, q, k)); });
-      nt3<KS>(y, [&](int p, int k, uint32_t* f) { ldsm4(f, la.at(sg + p * S::kStatPlane, warp, k)); },
-              [&](int p, int k, uint32_t* f) { ldsm4(f, lb.at(sv + p * S::kPlane, q, k)); });
+      uint32_t ba[KS];
+      addresses<DP>(ba, lb, sk, q);
+      nt3<KS, S::kStatPlane, S::kPlane>(x[0], qa, ba);
+      addresses<DP>(ba, lb, sv, q);
+      nt3<KS, S::kStatPlane, S::kPlane>(y, ga, ba);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll

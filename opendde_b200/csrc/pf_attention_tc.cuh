@@ -229,9 +229,15 @@ __device__ __forceinline__ void bias_get(Bias4<BT>& r, const char* p, int64_t j,
       r.w[0] = v.x, r.w[1] = v.y;
     } else {
       const unsigned short* q = (const unsigned short*)p;
+      const int left = (int)(nk - j < 4 ? nk - j : 4);
       uint32_t e[4];
+      if (left == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = j + i < nk ? q[i] : 0;
+        for (int i = 0; i < 4; ++i) e[i] = q[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = i < left ? q[i] : 0;
+      }
       r.w[0] = e[0] | (e[1] << 16), r.w[1] = e[2] | (e[3] << 16);
     }
   } else if (BT == 2) {
@@ -240,8 +246,14 @@ __device__ __forceinline__ void bias_get(Bias4<BT>& r, const char* p, int64_t j,
       r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
     } else {
       const uint32_t* q = (const uint32_t*)p;
+      const int left = (int)(nk - j < 4 ? nk - j : 4);
+      if (left == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r.w[i] = j + i < nk ? q[i] : 0;
+        for (int i = 0; i < 4; ++i) r.w[i] = q[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = i < left ? q[i] : 0;
+      }
     }
   }
 }
