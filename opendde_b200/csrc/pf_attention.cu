@@ -43,32 +43,40 @@ int sum_planes(const Args& a, const float* part, int parts, cudaStream_t st) {
 
 // How the gradient of a shared bias is computed: with dq in one pass (bf16: one block of 16 warps per SM; fp32:
 // three blocks of four, or two above 256 keys), or by itself (as many blocks as run at a time), in `parts` parts
-// of the batch of at least four entries each (a part costs a plane written and read).
+// of the batch.
 struct SharedPlan {
   bool plane;
   int parts;
 };
+// Parts of at least four entries each for `blocks` blocks per part of which `fit` run at a time: the fewest waves
+// of blocks per part (512 tokens, four heads, bf16: 9 parts of 32 blocks fill two waves to 97 %, 4 parts one to
+// 86 %; 900 tokens: 480 blocks in one part would be two waves for the work of one), against what a part costs,
+// a plane written and read and a block's first entry, about two and a half entries' work. `time`: in units
+// of the work on a full machine.
+int best_parts(int64_t blocks, int64_t fit, int64_t batch, double* time) {
+  const int64_t most = batch / 4 < 1 ? 1 : batch / 4, cap = fit / blocks > 16 ? fit / blocks : 16;
+  int best = 1;
+  for (int64_t n = 1; n <= most && n <= cap; ++n) {
+    const double waves = (double)((blocks * n + fit - 1) / fit);
+    const double t = waves * fit / (double)(blocks * n) + (n > 1 ? 2.5 * n / (double)batch : 0.0);
+    if (n == 1 || t < *time) *time = t, best = (int)n;
+  }
+  return best;
+}
 SharedPlan shared_plan(const pf_attention_shape& s) {
-  SharedPlan p{false, 1};
-  if (s.n_q == 0 || s.n_k == 0) return p;
+  if (s.n_q == 0 || s.n_k == 0 || s.batch == 0) return SharedPlan{false, 1};
   const bool bf16 = s.dtype == PF_BF16;
+  double time = 0.0;
   if (bf16 ? attn::dq_plane_bf16_fits(s.n_k, s.head_dim) : attn::dq_plane_f32_fits(s.n_k, s.head_dim)) {
-    const int64_t blocks = (s.n_q + 63) / 64 * s.heads, fit = 148 * (bf16 ? 1 : (s.n_k <= 256 ? 3 : 2));
-    int64_t n = blocks >= fit ? 1 : fit / blocks;
-    if (n > s.batch / 4) n = s.batch / 4;
-    if (n < 1) n = 1;
-    // where the last wave of blocks leaves most of the machine idle, the two passes are faster
-    const int64_t waves = (blocks * n + fit - 1) / fit;
-    if (blocks * n * 100 >= waves * fit * 60) return SharedPlan{true, (int)n};
+    const int fit = 148 * (bf16 ? 1 : (s.n_k <= 256 ? 3 : 2));
+    const int n = best_parts((s.n_q + 63) / 64 * s.heads, fit, s.batch, &time);
+    // where most of the machine would stay idle, the two passes are faster
+    if (time < 1.7) return SharedPlan{true, n};
   }
   // tiles of the kernels and how many blocks an SM holds
   const int64_t rows = bf16 ? 128 : 64, keys = bf16 || s.head_dim <= 32 ? 64 : (s.head_dim <= 64 ? 32 : 16);
   const int64_t blocks = ((s.n_q + rows - 1) / rows) * ((s.n_k + keys - 1) / keys) * s.heads;
-  const int64_t fit = (s.head_dim <= 32 ? (bf16 ? 3 : 4) : 1) * 148;
-  int64_t n = blocks >= fit ? 1 : fit / blocks;
-  if (n > s.batch / 4) n = s.batch / 4;
-  p.parts = n < 1 ? 1 : (int)n;
-  return p;
+  return SharedPlan{false, best_parts(blocks, (s.head_dim <= 32 ? (bf16 ? 3 : 4) : 1) * 148, s.batch, &time)};
 }
 
 Heads heads(const pf_head_view& v) { return Heads{v.ptr, v.batch_stride, v.seq_stride, v.head_stride}; }

@@ -498,6 +498,19 @@ def _batched_heads(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
+def _quads(bias: torch.Tensor, b: int) -> torch.Tensor:
+    """The bias with rows that start on four elements. Others are read one element at a time, and a plane that
+    many batch entries share, once for each: from 2^24 scores the copy costs less (768 against 767 tokens, four
+    heads, bfloat16, forward and backward: 6.3 against 10.3 ms without the copy)."""
+    _, h, n_q, n_k = bias.shape
+    if b < 8 or b * h * n_q * n_k < 1 << 24:
+        return bias
+    if not (bias.stride(1) % 4 or bias.stride(2) % 4 or bias.data_ptr() % (4 * bias.element_size())):
+        return bias
+    rows = torch.empty((1, h, n_q, -(-n_k // 4) * 4), device=bias.device, dtype=bias.dtype)[..., :n_k]
+    return rows.copy_(bias.detach())
+
+
 def _attention_args(q, k, v, bias, mask, scale):
     """Checked [B, N, H, d] views, the [1 or B, H, n_q, n_k] bias, the float32 mask, and the call's fields
     up to the output."""
@@ -523,6 +536,8 @@ def _attention_args(q, k, v, bias, mask, scale):
             raise ValueError("bias must have contiguous keys")
         if bias.shape[0] > 1 and bias.stride(0) == 0:
             bias = bias[:1]
+        if bias.shape[0] == 1:
+            bias = _quads(bias, b)
     mask_view = (0, 0, 0)
     if mask is not None:
         if mask.shape != (b, n_k) and mask.shape != (n_k,):

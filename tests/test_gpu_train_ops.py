@@ -167,6 +167,24 @@ def test_attention_shared_bias_with_blocks_for_every_sm(B, nq, nk, H, KV, d, mas
     test_attention_shared_bias_over_a_long_batch(B, nq, nk, H, KV, d, mask, bias_dtype, dtype, cuda_device)
 
 
+@pytest.mark.parametrize("dtype,bias_dtype", [(F32, F32), (BF16, BF16), (BF16, F32)])
+def test_attention_large_shared_bias_of_any_alignment(dtype, bias_dtype, cuda_device):
+    """Enough scores (2^24) that a plane with rows off four elements is copied: odd strides, a base off 16 bytes, and
+    one plane expanded over the batch; the plane itself stays as it was."""
+    B, n, H = 47, 301, 4
+    q, k, v, do, bias, mask = _att(B, n, n, H, H, 16, dtype, cuda_device, "shared", bias_dtype, "pad")
+    buf = torch.full((H * n * 303 + 1,), float("nan"), device=cuda_device, dtype=bias_dtype)
+    odd = torch.as_strided(buf, (1, H, n, n), (1, n * 303, 303, 1), 1)
+    odd.copy_(bias)
+    kept = buf.clone()
+    got = _verify((q, k, v, do, odd, mask))
+    assert torch.equal(buf.view(torch.uint8), kept.view(torch.uint8))
+    o, saved = kernels.attention(q, k, v, odd.expand(B, H, n, n), mask, save=True)
+    assert torch.equal(o, got["o"])
+    each = kernels.attention_bwd(do, q, k, v, o, saved, odd[0], mask)[3]
+    assert each.shape == (H, n, n) and torch.equal(each, got["dbias"][0])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("d", [1, 3, 8, 33, 40, 64, 65, 96, 100, 128])
 def test_attention_head_dims(d, dtype, cuda_device):
