@@ -440,6 +440,11 @@ def _stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
+def _empty(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous room like ``t`` (empty_like takes half the time of empty, but follows t's strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-5,
                   need=(True, True, True)):
     """(dx, dweight, dbias) of :func:`layernorm` for the output's gradient ``dy`` (see
@@ -455,9 +460,10 @@ def layernorm_bwd(x: torch.Tensor, dy: torch.Tensor, weight: Optional[torch.Tens
     lib = _abi.load()
     with _on(dev):
         x, dy, w = x.contiguous(), dy.contiguous(), _float_param(weight)
-        dx = torch.empty_like(x, requires_grad=False) if need[0] else None
-        dw = torch.empty(c, device=dev, dtype=torch.float32) if need[1] else None
-        db = torch.empty(c, device=dev, dtype=torch.float32) if need[2] else None
+        dx = torch.empty_like(x) if need[0] else None
+        sums = (lambda: torch.empty(c, device=dev, dtype=torch.float32)) if w is None else lambda: torch.empty_like(w)
+        dw = sums() if need[1] else None
+        db = sums() if need[2] else None
         rows = x.numel() // c
         ws = workspace(_abi.workspace_bytes("pf_layernorm_bwd_workspace_size", rows, c, code), dev)
         check(lib.pf_layernorm_bwd(x.data_ptr(), dy.data_ptr(), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db), rows, c, eps,
@@ -489,10 +495,10 @@ def _bias_view(t: Optional[torch.Tensor]) -> tuple:
 
 
 def _batched_heads(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dim() == 3:
+    if t.dim() != 4:
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [B, N, H, d] or [N, H, d], got shape {tuple(t.shape)}")
         t = t[None]
-    elif t.dim() != 4:
-        raise ValueError(f"{name} must be [B, N, H, d] or [N, H, d], got shape {tuple(t.shape)}")
     if t.stride(3) != 1 and t.shape[3] > 1:
         raise ValueError(f"{name} must have contiguous channels")
     return t
@@ -515,8 +521,8 @@ def _attention_args(q, k, v, bias, mask, scale):
     """Checked [B, N, H, d] views, the [1 or B, H, n_q, n_k] bias, the float32 mask, and the call's fields
     up to the output."""
     dev = _same_device(q, k, v, bias, mask)
-    code = dtype_code(q)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    code, dtype = dtype_code(q), q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"q, k and v must share the dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     if not q.dim() == k.dim() == v.dim():
         raise ValueError("q, k and v must all be batched or all be unbatched")
@@ -568,12 +574,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[
     b, n_q, _, heads = shape[:4]
     lib = _abi.load()
     with _on(dev):
-        o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        o = _empty(q)
         stats = o_lo = None
         if save:
-            stats = torch.empty((2, b, heads, n_q), device=dev, dtype=torch.float32)
+            stats = q.new_empty((2, b, heads, n_q), dtype=torch.float32)
             if q.dtype == torch.bfloat16:
-                o_lo = torch.empty(q4.shape, device=dev, dtype=torch.int16)
+                o_lo = torch.empty_like(o if o.dim() == 4 else o[None], dtype=torch.int16)
         call = _abi.ATTENTION_CALL.pack(*fields, *_head_view(o if o.dim() == 4 else o[None]), _ptr(stats) or 0,
                                         _ptr(o_lo) or 0, *_NO_VIEW * 5)
         check(lib.pf_attention_fwd(call, _stream(dev)))
@@ -603,11 +609,10 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     do4, o4 = _batched_heads(do, "do"), _batched_heads(o, "o")
     lib = _abi.load()
     with _on(dev):
-        dq = torch.empty(q4.shape, device=dev, dtype=q.dtype) if need[0] else None
+        dq = _empty(q4) if need[0] else None
         dk = dv = dbias = dbias_v = None
         if need[1] or need[2]:
-            dk = torch.empty(k4.shape, device=dev, dtype=q.dtype)
-            dv = torch.empty(v4.shape, device=dev, dtype=q.dtype)
+            dk, dv = _empty(k4), _empty(v4)
         if bias is not None and need[3]:
             if b == 0:
                 dbias = torch.zeros(given.shape, device=dev, dtype=bias.dtype)
@@ -616,7 +621,7 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
                     # one plane expanded over the batch: every entry has a gradient of its own
                     bias = given.contiguous()
                     fields = _attention_args(q, k, v, bias, mask, scale)[-1]
-                dbias = dbias_v = torch.empty(bias.shape, device=dev, dtype=bias.dtype)
+                dbias = dbias_v = _empty(bias)
         ws = workspace(_abi.workspace_bytes("pf_attention_bwd_workspace_size", _abi.ATTENTION_SHAPE.pack(*shape)), dev)
         call = _abi.ATTENTION_CALL.pack(*fields, *_head_view(o4), stats.data_ptr(), _ptr(o_lo) or 0, *_head_view(do4),
                                         *_head_view(dq), *_head_view(dk), *_head_view(dv), *_bias_view(dbias_v))
@@ -673,7 +678,7 @@ def relpos_bias_bwd(dout: torch.Tensor, ids, row0: int, col0: int, r_max: int, s
     with _on(dev):
         nbytes = _abi.workspace_bytes("pf_relpos_bias_bwd_workspace_size", rows, cols, heads, r_max, s_max)
         ws = workspace(nbytes, dev)
-        dw = torch.empty((heads, 4 * r_max + 2 * s_max + 7), device=dev, dtype=torch.float32)
+        dw = dout.new_empty((heads, 4 * r_max + 2 * s_max + 7), dtype=torch.float32)
         check(lib.pf_relpos_bias_bwd(dout.data_ptr(), dout.stride(0), dout.stride(1), code,
                                      _abi.TokenIds(*[t.data_ptr() for t in ids]), dw.data_ptr(), n_token, row0, rows,
                                      col0, cols, heads, r_max, s_max, ws.data_ptr(), ws.numel(), _stream(dev)))
