@@ -10,7 +10,10 @@
 //
 // A warp walks over rows and keeps its lanes' share of dgamma and dbeta in registers; a block adds
 // its warps' shares through shared memory and writes one partial row, and k_sum_rows adds the partial
-// rows in a fixed order (no atomics: equal inputs give equal bits). One block writes the result itself.
+// rows in a fixed order (no atomics: equal inputs give equal bits). Few rows are one cluster of blocks, which add
+// their rows through distributed shared memory in the same launch.
+
+#include <cooperative_groups.h>
 
 #include "pf_common.cuh"
 #include "pf_f32x2.cuh"
@@ -74,14 +77,17 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+namespace cg = cooperative_groups;
 constexpr int kWarps = 8;
+constexpr int kRanks = 8;             // blocks of the cluster that takes few rows
+constexpr int64_t kFew = 4 * 64 * 512;  // elements of those
 
 // L lanes per row, V chunks of E channels per lane, U rows of a lane in flight; FULL: c = L V E.
 template <class T, int E, int L, int V, int U, bool FULL>
 __global__ void __launch_bounds__(kWarps * 32, 2) k_layernorm_bwd(const T* x, const T* dy,
                                                                const float* __restrict__ gamma, T* dx, float* dg_out,
                                                                float* db_out, int64_t part, int64_t rows, int c,
-                                                               float eps) {
+                                                               float eps, int ranks) {
   constexpr int R = 32 / L;  // rows of a warp side by side
   constexpr int N = V * E / 2;  // channel pairs of a lane
   extern __shared__ float sm[];
@@ -199,8 +205,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_layernorm_bwd(const T* x, co
       sa += sm[(w * 2) * c + i];
       sb += sm[(w * 2 + 1) * c + i];
     }
-    if (dg_out) dg_out[off + i] = sa;
-    if (db_out) db_out[off + i] = sb;
+    if (ranks > 1) {
+      sm[i] = sa;  // this thread alone has read column i
+      sm[c + i] = sb;
+    } else {
+      if (dg_out) dg_out[off + i] = sa;
+      if (db_out) db_out[off + i] = sb;
+    }
+  }
+  if (ranks > 1) {  // the grid is one cluster: each block adds a share of the columns over all of them
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int share = (2 * c + ranks - 1) / ranks, i1 = min(2 * c, ((int)blockIdx.x + 1) * share);
+    for (int i = blockIdx.x * share + threadIdx.x; i < i1; i += kWarps * 32) {
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < kRanks; ++r) s += *cluster.map_shared_rank(sm + i, r);
+      if (i < c) {
+        if (dg_out) dg_out[i] = s;
+      } else {
+        if (db_out) db_out[i - c] = s;
+      }
+    }
+    cluster.sync();  // no block leaves while others read its sums
   }
 }
 
@@ -233,11 +260,13 @@ int sm_count() {
   return n;
 }
 
-// Blocks of the row kernel: one where the rows are few (64 rows of 384 channels, by events around each
-// launch: 14 us in one block, 9 us in eight and 9 more to add their shares); else enough warps to cover the
-// rows, at most four blocks on each SM (two run at a time).
+// Blocks of the row kernel: a cluster of eight where the rows are few (64 rows of 384 channels, called and replayed:
+// 17.8 and 3.5 us against 21 to 25 and 4.1 us in two launches, and 14 us in one block; 1024 rows of 128: 17.8 and
+// 5.8 against 21 and 5.7 us; 2048: 17.9 and 8.2 against 21 and 5.7 us); else enough warps to cover the rows, at
+// most four blocks on each SM (two run at a time).
+bool few_rows(int64_t rows, int c) { return rows * c <= kFew; }
 int64_t grid_blocks(int64_t rows, int c, int rows_per_block, bool sums) {
-  if (sums && rows * c <= 64 * 512) return 1;
+  if (sums && few_rows(rows, c)) return kRanks;
   const int64_t need = (rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sm_count() * 4;
   return need < 1 ? 1 : (need < most ? need : most);
 }
@@ -249,13 +278,20 @@ int launch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float*
   const size_t smem = (size_t)kWarps * 2 * c * sizeof(float);
   auto* kern = k_layernorm_bwd<T, E, L, V, U, FULL>;
   if (smem > 48 * 1024) PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const bool direct = blocks == 1;
+  const bool cluster = (dg || db) && few_rows(rows, c), direct = blocks == 1 || cluster;
   const int64_t m0 = dg ? c : 0, m = m0 + (db ? c : 0);  // a partial row: dgamma, then dbeta
   float* pg = direct || !dg ? dg : part;
   float* pb = direct || !db ? db : part + m0;
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_layernorm_bwd", 3.0 * (double)rows * c * sizeof(T), 'b');
-    kern<<<(unsigned)blocks, kWarps * 32, smem, st>>>(x, dy, gamma, dx, pg, pb, m, rows, c, eps);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kRanks, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.attrs = &attr, cfg.numAttrs = cluster ? 1 : 0;
+    PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x, dy, gamma, dx, pg, pb, m, rows, c, eps, cluster ? kRanks : 1));
   }
   PF_CHECK_LAUNCH();
   return direct || m == 0 ? PF_OK : sum_rows(part, blocks, m, dg, m0, db, st);
