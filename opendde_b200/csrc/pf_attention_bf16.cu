@@ -368,6 +368,7 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   id /= (unsigned)tiles;
   const int h = id % a.H, kh = h / (a.H / a.KV);
   const int64_t b = id / a.H, nk = a.nk;
+  if (b >= a.B) return;  // makes up a whole cluster
   const int64_t i0 = (int64_t)tile * QR, w0 = i0 + warp * 16;
   const int nt = (int)((nk + kTile - 1) / kTile);
   const int bvec = a.bias_vec;
@@ -567,7 +568,7 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
 // 16 keys per warp (32 need 168 registers where 16 need 128, and three blocks on an SM are slower than four:
 // 768 tokens 2.1 against 1.9 ms); HOLD: their fragments stay in registers.
 template <int DP, int BT, int TERMS>
-__device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles) {
+__device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles, int rank, int ranks) {
   using S = Tile<DP>;
   constexpr int KR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
   constexpr bool HOLD = DP <= 64;
@@ -719,7 +720,8 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
   };
   if (live != 0 && per > 0) {
     int it = 0;
-    for (int hh = 0; hh < group; ++hh) {
+    const int heads = group / ranks, first = rank * heads;
+    for (int hh = first; hh < first + heads; ++hh) {
       const int h = kh * group + hh;
       Stream<DP> qs(head_base(a.q, b, h), a.q.ns, a.vec_q, 0, nq, a.d), gs(head_base(a.g, b, h), a.g.ns, a.vec_g, 0, nq, a.d);
       const float4* pr = (const float4*)a.rows + (b * a.H + h) * nq;
@@ -733,7 +735,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
         }
         cp_commit();
       };
-      if (hh > 0) __syncthreads();  // the last head's tiles are done with
+      if (hh > first) __syncthreads();  // the last head's tiles are done with
       issue(0, it & 1);
       if (BT) {
 #pragma unroll
@@ -766,6 +768,18 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
   cp_commit();
   cp_wait<0>();
   const bool vk = pair_ok(a.dk, a.dk_bs, a.dk_ns, a.dk_hs, a.d), vv = pair_ok(a.dv, a.dv_bs, a.dv_ns, a.dv_hs, a.d);
+  if (ranks > 1) {
+    bf16* pk = (bf16*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j0 * a.dk_ns;
+    bf16* pv = (bf16*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j0 * a.dv_ns;
+    sum_ranks<DP>(raw, dk, dv, ranks, rank, [&](int which, int row, int c, float v0, float v1) {
+      if (j0 + row >= a.nk) return;
+      if (which == 0)
+        store_pair(pk + row * a.dk_ns, c, a.d, vk, v0 * a.scale, v1 * a.scale);
+      else
+        store_pair(pv + row * a.dv_ns, c, a.d, vv, v0, v1);
+    });
+    return;
+  }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int64_t j = w0 + perm_row(g, r);  // row g + 8 r of the block holds this key
@@ -783,9 +797,10 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
 // dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
 // run side by side.
 template <int DP, int BT, int TERMS>
-__global__ void __launch_bounds__(kThreads, DP == 32 && TERMS == 1 ? 4 : 2) k_dqkv(Args a, unsigned dkv_blocks) {
+__global__ void __launch_bounds__(kThreads, DP == 32 && TERMS == 1 ? 4 : 2)
+    k_dqkv(Args a, unsigned dkv_blocks, int ranks) {
   if (blockIdx.x < dkv_blocks)
-    dkv_block<DP, BT, TERMS>(a, blockIdx.x, (a.nk + 63) / 64);
+    dkv_block<DP, BT, TERMS>(a, blockIdx.x / ranks, (a.nk + 63) / 64, blockIdx.x % ranks, ranks);
   else
     dq_block<DP, BT, TERMS>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
@@ -1295,20 +1310,6 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
 
 // ---------------------------------------------------------------- launches
 
-template <class F, class... X>
-int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cudaStream_t st, X... x) {
-  if (blocks == 0) return PF_OK;
-  if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
-  if (smem > 40 * 1024)
-    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  {
-    PF_LAUNCH_SCOPE_WORK(st, name, flops, 'f');
-    kern<<<(unsigned)blocks, kThreads, smem, st>>>(x...);
-  }
-  PF_CHECK_LAUNCH();
-  return PF_OK;
-}
-
 template <int DP, int BT>
 int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   constexpr size_t RB = Tile<DP>::RB;
@@ -1320,25 +1321,29 @@ int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
       const int64_t t2 = (a.nq + 127) / 128;
       if (t2 * a.H * a.B >= 3 * 148) {
         a.tiles = t2;
-        return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, t2 * a.H * a.B, "k_attn_fwd", flops, st, a);
+        return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, t2 * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
       }
     }
     a.tiles = tq;
-    return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, tq * a.H * a.B, "k_attn_fwd", flops, st, a);
+    return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
   }
   const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
-  // p and ds as two bf16 values where the blocks do not fill the machine and the second costs nothing
+  // p and ds as two bf16 values where all blocks, wanted here or not, do not fill the machine and the second
+  // costs nothing
   const size_t smem = (128 + 4 * kTile) * RB + 2048;
   const char* name = kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv");
-  if (bq + bkv <= 148) return go(k_dqkv<DP, BT, 2>, smem, bq + bkv, name, flops, st, a, (unsigned)bkv);
-  return go(k_dqkv<DP, BT, 1>, smem, bq + bkv, name, flops, st, a, (unsigned)bkv);
+  const int ranks = bkv == 0 ? 1 : dkv_ranks(a, bkv, tq * a.H * a.B);
+  const int64_t bk = bkv * ranks, blocks = (bk + bq + ranks - 1) / ranks * ranks;
+  if (tq * a.H * a.B + tk * a.KV * a.B <= 148)
+    return go(k_dqkv<DP, BT, 2>, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
+  return go(k_dqkv<DP, BT, 1>, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
 }
 
 template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
   constexpr size_t smem = 2 * ((size_t)(256 + 128) * Tile<DP>::RB + 2048);
   a.tiles = (a.nq + 127) / 128;
-  return go(k_dbias<DP, BT>, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, "k_attn_dbias", flops, st, a, part,
+  return go(k_dbias<DP, BT>, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, 1, "k_attn_dbias", flops, st, a, part,
             parts);
 }
 

@@ -560,7 +560,8 @@ template <int DP, int BT>
 __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
   const unsigned tile = id % (unsigned)tiles;
   id /= (unsigned)tiles;
-  dq_rows<DP, BT, false>(a, id / a.H, id % a.H, tile, 0);
+  if (id / a.H < a.B)  // else it makes up a whole cluster
+    dq_rows<DP, BT, false>(a, id / a.H, id % a.H, tile, 0);
 }
 
 // dq and the gradient of a bias that the batch shares in one pass (see k_dq_plane of the bf16 kernels): a block
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_dq_plane(Args a, float* part, i
 // ---------------------------------------------------------------- dk, dv
 
 template <int DP, int BT>
-__device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles) {
+__device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles, int rank, int ranks) {
   using S = Split<DP>;
   constexpr int KT = S::KT, KS = DP / 16, NB = DP / 8;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -637,9 +638,9 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
   const LaneAddr<DP> la = lane_a<DP>(), lb = lane_b<DP>(), ln = lane_bn<DP>();
   const unsigned tile = id % (unsigned)tiles;
   id /= (unsigned)tiles;
-  const int kh = id % a.KV, group = a.H / a.KV;
+  const int kh = id % a.KV, group = a.H / a.KV, heads = group / ranks, h0 = kh * group + rank * heads;
   const int64_t b = id / a.KV, j0 = (int64_t)tile * 64, w0 = j0 + warp * 16;
-  const int per = (int)((a.nq + KT - 1) / KT), nt = per * group;
+  const int per = (int)((a.nq + KT - 1) / KT), nt = per * heads;
   const uint64_t live = seen_ballot(seen_raw(a, b, j0));
   const uint32_t mine = (uint32_t)(live >> (warp * 16)) & 0xffffu;
   const bool bfast = a.bias_vec && w0 + 16 <= a.nk;
@@ -654,7 +655,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     const Place<DP> place;
     float4 pc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto read = [&](int it) {
-      const int h = kh * group + it / per;
+      const int h = h0 + it / per;
       const int64_t i0 = (int64_t)(it % per) * KT;
       const uint64_t rows = first_bits(a.nq - i0) & (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
       pq.read(place, head_f(a.q, b, h), a.q.ns, a.vec_q, i0, a.d, rows);
@@ -680,7 +681,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
       __syncthreads();
       if (it + 1 < nt) read(it + 1);
       if (mine != 0) {
-        const int h = kh * group + it / per;
+        const int h = h0 + it / per;
         const int64_t i0 = (int64_t)(it % per) * KT;
         const uint32_t tq = sq + (it & 1) * S::kTile3, tg = sg + (it & 1) * S::kTile3;
 #pragma unroll 1
@@ -730,6 +731,18 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     }
   }
   const bool vk = pair_ok_f(a.dk, a.dk_bs, a.dk_ns, a.dk_hs, a.d), vv = pair_ok_f(a.dv, a.dv_bs, a.dv_ns, a.dv_hs, a.d);
+  if (ranks > 1) {
+    float* pk = (float*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j0 * a.dk_ns;
+    float* pv = (float*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j0 * a.dv_ns;
+    sum_ranks<DP>(raw, dk, dv, ranks, rank, [&](int which, int row, int c, float v0, float v1) {
+      if (j0 + row >= a.nk) return;
+      if (which == 0)
+        store2f(pk + row * a.dk_ns, c, a.d, vk, v0 * a.scale, v1 * a.scale);
+      else
+        store2f(pv + row * a.dv_ns, c, a.d, vv, v0, v1);
+    });
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int64_t j = w0 + perm_row(g, r);  // row g + 8 r of the block holds this key
@@ -747,9 +760,9 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
 // dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
 // run side by side.
 template <int DP, int BT>
-__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dqkv(Args a, unsigned dkv_blocks) {
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dqkv(Args a, unsigned dkv_blocks, int ranks) {
   if (blockIdx.x < dkv_blocks)
-    dkv_block<DP, BT>(a, blockIdx.x, (a.nk + 63) / 64);
+    dkv_block<DP, BT>(a, blockIdx.x / ranks, (a.nk + 63) / 64, blockIdx.x % ranks, ranks);
   else
     dq_block<DP, BT>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
@@ -865,37 +878,26 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, fl
 
 // ---------------------------------------------------------------- launches
 
-template <class F, class... X>
-int go(F* kern, size_t smem, int64_t blocks, const char* name, double flops, cudaStream_t st, X... x) {
-  if (blocks == 0) return PF_OK;
-  if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
-  if (smem > 40 * 1024)
-    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  {
-    PF_LAUNCH_SCOPE_WORK(st, name, flops, 'f');
-    kern<<<(unsigned)blocks, kThreads, smem, st>>>(x...);
-  }
-  PF_CHECK_LAUNCH();
-  return PF_OK;
-}
-
 template <int DP, int BT>
 int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   using S = Split<DP>;
   const int64_t tq = (a.nq + 63) / 64, tk = (a.nk + 63) / 64;
   if (kind == kFwd) {
     a.tiles = tq;
-    return go(k_fwd<DP, BT>, S::kStat3 + 4 * S::kTile3, tq * a.H * a.B, "k_attn_fwd", flops, st, a);
+    return go(k_fwd<DP, BT>, S::kStat3 + 4 * S::kTile3, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
   }
   const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
-  return go(k_dqkv<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16, bq + bkv,
-            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a, (unsigned)bkv);
+  const int ranks = bkv == 0 ? 1 : dkv_ranks(a, bkv, tq * a.H * a.B);
+  const int64_t bk = bkv * ranks, blocks = (bk + bq + ranks - 1) / ranks * ranks;
+  return go(k_dqkv<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16, blocks, ranks,
+            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a, (unsigned)bk,
+            ranks);
 }
 template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
   using S = Split<DP>;
   a.tiles = (a.nq + 63) / 64;
-  return go(k_dbias<DP, BT>, 2 * S::kStat3 + 2 * S::kTile3, a.tiles * ((a.nk + S::KT - 1) / S::KT) * a.H * parts,
+  return go(k_dbias<DP, BT>, 2 * S::kStat3 + 2 * S::kTile3, a.tiles * ((a.nk + S::KT - 1) / S::KT) * a.H * parts, 1,
             "k_attn_dbias", flops, st, a, part, parts);
 }
 
@@ -907,7 +909,7 @@ int launch_plane(Args a, float* part, int parts, double flops, cudaStream_t st) 
   // room for as many blocks as tensor memory holds
   const size_t smem = tcols == 128 ? tiles + 16 : 100 * 1024;
   a.tiles = (a.nq + 63) / 64;
-  return go(k_dq_plane<BT>, smem, a.tiles * a.H * parts, "k_attn_dq_plane", flops, st, a, part, parts, tcols, tiles);
+  return go(k_dq_plane<BT>, smem, a.tiles * a.H * parts, 1, "k_attn_dq_plane", flops, st, a, part, parts, tcols, tiles);
 }
 
 }  // namespace

@@ -2,6 +2,8 @@
 // pf_attention_f32.cu): swizzled shared tiles and their ldmatrix addresses, products, visible keys, bias
 // fragments, scores. See pf_attention_bf16.cu for the layout.
 #pragma once
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "pf_attention.cuh"
@@ -334,6 +336,73 @@ __device__ __forceinline__ void store_pair(bf16* p, int col, int d, bool vec, fl
 }
 __device__ __forceinline__ bool pair_ok(const void* p, int64_t bs, int64_t ns, int64_t hs, int d) {
   return ((uintptr_t)p & 3) == 0 && ((bs | ns | hs | d) & 1) == 0;
+}
+
+// ---------------------------------------------------------------- dk, dv of a cluster
+
+// Blocks of a launch with `cluster` blocks to a cluster (1: none).
+template <class F, class... X>
+int go(F* kern, size_t smem, int64_t blocks, int cluster, const char* name, double flops, cudaStream_t st, X... x) {
+  if (blocks == 0) return PF_OK;
+  if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
+  if (smem > 40 * 1024)
+    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  {
+    PF_LAUNCH_SCOPE_WORK(st, name, flops, 'f');
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.attrs = &attr, cfg.numAttrs = cluster > 1 ? 1 : 0;
+    PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x...));
+  }
+  PF_CHECK_LAUNCH();
+  return PF_OK;
+}
+
+// The blocks of a cluster that the query heads of a key head are shared out to: a power of two up to eight, where
+// there is room for them next to dq's blocks (computed or not: the same bits either way), two blocks on each SM.
+// 3 x 301 queries by 517 keys, 2 key heads of 4 query heads each, bf16, with dq: 44 us in one block, 37 us in two,
+// 38 us in four.
+inline int dkv_ranks(const Args& a, int64_t blocks, int64_t dq_blocks) {
+  int ranks = 1;
+  while (ranks < 8 && a.H / a.KV % (2 * ranks) == 0 && 2 * ranks * blocks + dq_blocks <= 2 * 148) ranks *= 2;
+  return ranks;
+}
+
+// The sum over the cluster's blocks, in their order, of x and y (a warp's 16 keys each, as the products leave
+// them): each block adds a share of the 64 keys from all blocks' shared memory and passes them to store(which,
+// key, channel, v0, v1).
+template <int DP, class Store>
+__device__ __forceinline__ void sum_ranks(unsigned char* raw, const float (&x)[DP / 8][4], const float (&y)[DP / 8][4],
+                                          int ranks, int rank, Store store) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  float* red = (float*)raw;  // [2][64][DP]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  __syncthreads();  // the tiles are done with
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      float* p = red + (warp * 16 + perm_row(g, r)) * DP + n * 8 + 2 * t;
+      *reinterpret_cast<float2*>(p) = make_float2(x[n][2 * r], x[n][2 * r + 1]);
+      *reinterpret_cast<float2*>(p + 64 * DP) = make_float2(y[n][2 * r], y[n][2 * r + 1]);
+    }
+  cluster.sync();
+  const int keys = 64 / ranks;
+  for (int i = threadIdx.x; i < keys * DP; i += kThreads) {  // pairs of channels
+    const int c = i % (DP / 2) * 2, k = i / (DP / 2), which = k / keys, row = rank * keys + k % keys;
+    float2 s = make_float2(0.f, 0.f);
+    for (int q = 0; q < ranks; ++q) {
+      const float2 v = *cluster.map_shared_rank(reinterpret_cast<float2*>(red + (which * 64 + row) * DP + c), q);
+      s.x += v.x, s.y += v.y;
+    }
+    store(which, row, c, s.x, s.y);
+  }
+  cluster.sync();  // no block leaves while others read its sums
 }
 
 // ---------------------------------------------------------------- tensor memory as thread-private storage

@@ -202,6 +202,28 @@ def test_attention_lengths_and_shared_heads(B, nq, nk, H, KV, bias, mask, dtype,
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,nq,nk,H,KV,d,bias,mask", [
+    (1, 70, 130, 8, 1, 128, "batch", "pad"), (2, 65, 67, 16, 2, 96, None, "holes"), (1, 100, 64, 6, 2, 40, "batch", None),
+    (1, 33, 200, 12, 2, 24, "shared", "pad"), (1, 1, 1, 16, 1, 8, "batch", None), (2, 129, 90, 4, 1, 64, "shared", None),
+    (1, 64, 65, 32, 2, 32, "batch", "pad"), (3, 301, 517, 8, 2, 64, None, "holes"), (2, 0, 70, 8, 2, 32, None, None)])
+def test_attention_key_heads_of_many_query_heads(B, nq, nk, H, KV, d, bias, mask, dtype, cuda_device):
+    """dk and dv add up to sixteen query heads, shared out to blocks in twos, fours and eights or not at all (three)."""
+    args = _att(B, nq, nk, H, KV, d, dtype, cuda_device, bias, F32, mask)
+    got = _verify(args) if nq else _run(*args)
+    again = _run(*args)
+    assert all(torch.equal(again[name], got[name]) for name in got)
+    if nq == 0:
+        assert not got["dk"].any() and not got["dv"].any()
+    q, k, v, do, bt, mt = args
+    views = torch.zeros(B, nk, KV, 3 * d, device=cuda_device, dtype=dtype)
+    views[..., d:2 * d], views[..., 2 * d:] = k, v
+    o, saved = kernels.attention(q, views[..., d:2 * d], views[..., 2 * d:], bt, mt, save=True)
+    far = kernels.attention_bwd(do, q, views[..., d:2 * d], views[..., 2 * d:], o, saved, bt, mt,
+                                need=(False, True, True, False))
+    assert torch.equal(far[1], got["dk"]) and torch.equal(far[2], got["dv"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_one_visible_key_has_no_score_gradient(dtype, cuda_device):
     q, k, v, do, bias, _ = _att(2, 40, 33, 2, 2, 24, dtype, cuda_device, "batch", F32)
     mask = torch.zeros(2, 33, device=cuda_device)
