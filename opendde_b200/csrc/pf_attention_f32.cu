@@ -8,7 +8,7 @@
 // ds) restarts from zero for every 16 columns and is added to the accumulators by rounded fp32
 // additions. Against the FFMA form of the same kernels, which the multiply-adds bound at 128 per clock
 // and SM (149 rows of 149 tokens, 12 heads of 32, forward plus backward: 1.9 ms), six products at 1024
-// per clock and SM are 1.3 times as many, with a quarter of the instructions (0.79 ms; 0.55 ms of products).
+// per clock and SM are 1.3 times as many, with a quarter of the instructions (0.76 ms; 0.55 ms of products).
 // An infinity splits into an infinity and a NaN: at a visible place it gives NaN.
 //
 // The layout is that of pf_attention_bf16.cu, with every tile in three planes. The streamed tiles are read
