@@ -16,9 +16,8 @@
 //          and adds ds in registers, so the sum has a fixed order and needs no atomics
 //
 // Precision: scores, softmax statistics, D, accumulators and the sum over a shared bias's batch are fp32
-// in both storage types. bf16: in the backward p and ds are rounded to bf16 as operands of the second
-// product (one rounding of the operand's own type; as two bf16 values where the problem is small and the
-// second costs nothing). ds is a difference of dp and D, so an error of o
+// in both storage types. bf16: in the backward p and ds are multiplied as sums of two
+// bf16 values, so that a gradient is rounded once, to its own type. ds is a difference of dp and D, so an error of o
 // would be its largest: the forward multiplies p as a sum of two bf16 values (three where the bias is
 // fp32, whose gradient then keeps fp32's accuracy), D is formed from o before its rounding, and for
 // that the forward keeps the 16 bits of o that the rounding dropped.

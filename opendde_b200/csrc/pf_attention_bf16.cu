@@ -5,7 +5,7 @@
 // double-buffered by cp.async. For the heads of 24 and 32 channels of this package a 16 x 16 block of
 // scores costs two to four products of depth 32 next to 256 exponentials, so the kernels are bound by
 // the issue of products, exponentials and the arithmetic around them, not by memory: 768 rows of 768
-// tokens, four heads, forward 1.5 ms, dk and dv 1.9 ms, dq with dbias 2.2 ms (0.6, 0.8 and 0.6 ms of products).
+// tokens, four heads, forward 1.5 ms, dk and dv 2.4 ms, dq with dbias 2.5 ms (0.6, 1.2 and 0.8 ms of products).
 //
 // Columns of a group of 16 keys are permuted so that a lane's four columns are four neighbouring keys
 // (lane t of a quad: keys 4t..4t+3 in place of 2t, 2t+1, 2t+8, 2t+9): a bias row is then read, and a
@@ -354,9 +354,26 @@ __global__ void __launch_bounds__(256) k_rows(Args a, const float* __restrict__ 
   rows[at] = make_float4(none ? INFINITY : m, none ? 0.f : -log2f(l), l == 1.f ? 1.f : 0.f, none ? 0.f : -s);
 }
 
+// bf16 values that p and ds are split into as operands of the second product, whatever the size of the problem: 16
+// bits of them, so that a gradient is the fp32 one rounded once (1e-4 from the rounded fp64 value, 2-norm). One
+// value would leave 2.7e-3 there, and take 2.0 instead of 2.4 ms for dk and dv and 2.3 instead of 2.5 ms for dq and
+// dbias of 768 rows of 768 tokens, four heads.
+constexpr int kTerms = 2;
+// 16 x 16 values in accumulator layout as left operands (left as what the last term drops)
+__device__ __forceinline__ void split_terms(uint32_t (&da)[kTerms][4], float (&y)[2][4]) {
+#pragma unroll
+  for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* v = &y[i >> 1][2 * (i & 1)];
+      da[term][i] = pack_bf16(v[0], v[1]);
+      if (term + 1 < kTerms) fma2(F2(lo_f(da[term][i]), hi_f(da[term][i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
+    }
+}
+
 // ---------------------------------------------------------------- dq (and dbias of one batch entry)
 
-template <int DP, int BT, int TERMS>
+template <int DP, int BT>
 __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t tiles) {
   using S = Tile<DP>;
   constexpr int QR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
@@ -486,21 +503,14 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
               put_bias4<BT>(dp[r] + (hb * 32 + q * 16) * BS, j, nk, FAST || (a.db_vec && j0 + hb * 32 + q * 16 + 16 <= nk),
                             y[0][2 * r], y[0][2 * r + 1], y[1][2 * r], y[1][2 * r + 1]);
       }
-      uint32_t da[TERMS][4];
-#pragma unroll
-      for (int term = 0; term < TERMS; ++term)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* v = &y[i >> 1][2 * (i & 1)];
-          da[term][i] = pack_bf16(v[0], v[1]);
-          if (term + 1 < TERMS) fma2(F2(lo_f(da[term][i]), hi_f(da[term][i])), F2(-1.f), F2(v[0], v[1])).get(v[0], v[1]);
-        }
+      uint32_t da[kTerms][4];
+      split_terms(da, y);
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         uint32_t f[4];
         ldsm4_ti<q * 16 * RB>(f, tc[c]);
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
+        for (int term = 0; term < kTerms; ++term) {
           mma(acc[2 * c], da[term], f[0], f[1]);
           mma(acc[2 * c + 1], da[term], f[2], f[3]);
         }
@@ -566,8 +576,8 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
 // ---------------------------------------------------------------- dk, dv
 
 // 16 keys per warp (32 need 168 registers where 16 need 128, and three blocks on an SM are slower than four:
-// 768 tokens 2.1 against 1.9 ms); HOLD: their fragments stay in registers.
-template <int DP, int BT, int TERMS>
+// 768 tokens 2.5 against 2.4 ms); HOLD: their fragments stay in registers.
+template <int DP, int BT>
 __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t tiles, int rank, int ranks) {
   using S = Tile<DP>;
   constexpr int KR = 64, KS = DP / 16, NB = DP / 8, RB = S::RB, BS = BT == 2 ? 4 : 2;
@@ -676,7 +686,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
               if (!((mine >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
       }
       const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
-      uint32_t pa[TERMS][4], da[TERMS][4];
+      uint32_t pa[kTerms][4], da[kTerms][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -690,13 +700,13 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
             if (p[1] == 1.f) ds[1] = 0.f;
           }
 #pragma unroll
-          for (int term = 0; term < TERMS; ++term) {
+          for (int term = 0; term < kTerms; ++term) {
             const uint32_t a = pack_bf16(p[0], p[1]), c = pack_bf16(ds[0], ds[1]);
             pa[term][2 * r + n] = transpose8(a);
             da[term][2 * r + n] = transpose8(c);
-            if (term + 1 < TERMS) {
-              p[0] -= lo_f(a), p[1] -= hi_f(a);
-              ds[0] -= lo_f(c), ds[1] -= hi_f(c);
+            if (term + 1 < kTerms) {
+              fma2(F2(lo_f(a), hi_f(a)), F2(-1.f), F2(p[0], p[1])).get(p[0], p[1]);
+              fma2(F2(lo_f(c), hi_f(c)), F2(-1.f), F2(ds[0], ds[1])).get(ds[0], ds[1]);
             }
           }
         }
@@ -706,7 +716,7 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
         ldsm4_ti<blk * 16 * RB + kG>(fg, tc[n]);
         ldsm4_ti<blk * 16 * RB>(fq, tc[n]);
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
+        for (int term = 0; term < kTerms; ++term) {
           mma(dv[2 * n], pa[term], fg[0], fg[1]);
           mma(dv[2 * n + 1], pa[term], fg[2], fg[3]);
           mma(dk[2 * n], da[term], fq[0], fq[1]);
@@ -796,13 +806,12 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
 
 // dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
 // run side by side.
-template <int DP, int BT, int TERMS>
-__global__ void __launch_bounds__(kThreads, DP == 32 && TERMS == 1 ? 4 : 2)
-    k_dqkv(Args a, unsigned dkv_blocks, int ranks) {
+template <int DP, int BT>
+__global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 2) k_dqkv(Args a, unsigned dkv_blocks, int ranks) {
   if (blockIdx.x < dkv_blocks)
-    dkv_block<DP, BT, TERMS>(a, blockIdx.x / ranks, (a.nk + 63) / 64, blockIdx.x % ranks, ranks);
+    dkv_block<DP, BT>(a, blockIdx.x / ranks, (a.nk + 63) / 64, blockIdx.x % ranks, ranks);
   else
-    dq_block<DP, BT, TERMS>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
+    dq_block<DP, BT>(a, blockIdx.x - dkv_blocks, (a.nq + 63) / 64);
 }
 
 // ---------------------------------------------------------------- dbias shared by the batch
@@ -991,8 +1000,8 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_dbias(Args a, fl
 // eight-word load, four packed adds and one store. All keys and values of a batch entry are in shared
 // memory, double-buffered (up to 832 keys of 32 channels), so warps run freely between two entries; the
 // quarters' dq are added through shared memory. Next to dq and dbias apart this saves two of five products
-// and one of two exponentials per score (768 rows of 768 tokens, four heads: 2.2 ms, 4.5 ms apart). It is bound
-// by instruction issue (2.1 per clock and SM, 22 per score).
+// and one of two exponentials per score (768 rows of 768 tokens, four heads: 2.5 ms; apart, 900 rows of 900, 1.6
+// times the scores: 6.8 ms). It is bound by instruction issue.
 constexpr int kPlaneThreads = 512;
 constexpr int kPlaneKeys = 832;
 
@@ -1206,16 +1215,6 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
             for (int e = 0; e < 4; ++e)
               if (x[n][e] == 1.f) y[n][e] = 0.f;
         }
-        uint32_t da[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) da[i] = pack_bf16(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1]);
-#pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          uint32_t f[4];
-          ldsm4_ti<u * 16 * S::RB>(f, ta[c]);
-          mma(acc[2 * c], da, f[0], f[1]);
-          mma(acc[2 * c + 1], da, f[2], f[3]);
-        }
         tmem_wait8(tm);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1226,6 +1225,18 @@ __global__ void __launch_bounds__(kPlaneThreads, 1) k_dq_plane(Args a, float* pa
           tm[2 * i] = __float_as_uint(s), tm[2 * i + 1] = __float_as_uint(s1);
         }
         tmem_st8(tm_at + u * 8, tm);
+        uint32_t da[kTerms][4];
+        split_terms(da, y);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+          uint32_t f[4];
+          ldsm4_ti<u * 16 * S::RB>(f, ta[c]);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) {
+            mma(acc[2 * c], da[term], f[0], f[1]);
+            mma(acc[2 * c + 1], da[term], f[2], f[3]);
+          }
+        }
       });
     };
 #pragma unroll 1
@@ -1328,15 +1339,11 @@ int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
     return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
   }
   const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
-  // p and ds as two bf16 values where all blocks, wanted here or not, do not fill the machine and the second
-  // costs nothing
   const size_t smem = (128 + 4 * kTile) * RB + 2048;
   const char* name = kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv");
   const int ranks = bkv == 0 ? 1 : dkv_ranks(a, bkv, tq * a.H * a.B);
   const int64_t bk = bkv * ranks, blocks = (bk + bq + ranks - 1) / ranks * ranks;
-  if (tq * a.H * a.B + tk * a.KV * a.B <= 148)
-    return go(k_dqkv<DP, BT, 2>, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
-  return go(k_dqkv<DP, BT, 1>, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
+  return go(k_dqkv<DP, BT>, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
 }
 
 template <int DP, int BT>

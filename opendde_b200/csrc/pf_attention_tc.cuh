@@ -364,8 +364,8 @@ int go(F* kern, size_t smem, int64_t blocks, int cluster, const char* name, doub
 
 // The blocks of a cluster that the query heads of a key head are shared out to: a power of two up to eight, where
 // there is room for them next to dq's blocks (computed or not: the same bits either way), two blocks on each SM.
-// 3 x 301 queries by 517 keys, 2 key heads of 4 query heads each, bf16, with dq: 44 us in one block, 37 us in two,
-// 38 us in four.
+// 3 x 301 queries by 517 keys, 2 key heads of 4 query heads each, bf16, one term of p and ds, with dq: 44 us in one
+// block, 37 us in two, 38 us in four.
 inline int dkv_ranks(const Args& a, int64_t blocks, int64_t dq_blocks) {
   int ranks = 1;
   while (ranks < 8 && a.H / a.KV % (2 * ranks) == 0 && 2 * ranks * blocks + dq_blocks <= 2 * 148) ranks *= 2;

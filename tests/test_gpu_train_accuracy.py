@@ -1,0 +1,26 @@
+"""Attention and its gradients against fp64 in the 2-norm (bounds: train_accuracy_support.py)."""
+import pytest
+import torch
+
+from test_gpu_train_ops import _att, _run
+from train_accuracy_support import BF16_TOL, FP32_TOL, distance
+from train_ops_support import attention_ref
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("B,nq,nk,H,KV,d,bias,bias_dtype,mask", [
+    (160, 160, 160, 4, 4, 32, "shared", BF16, "pad"),     # dq and the plane's gradient in one pass
+    (40, 100, 900, 4, 4, 32, "shared", F32, None),        # apart, the plane past what one pass holds
+    (1, 700, 700, 16, 16, 24, "batch", F32, None), (64, 200, 190, 4, 2, 32, None, None, "holes"),
+    (6, 300, 257, 8, 8, 64, "batch", BF16, "pad"), (5, 200, 320, 8, 2, 96, None, None, None),
+    (4, 300, 300, 8, 8, 128, "shared", F32, "pad"), (1, 40, 45, 2, 2, 32, "batch", BF16, None)])
+def test_bf16_outputs_are_rounded_once(B, nq, nk, H, KV, d, bias, bias_dtype, mask, cuda_device):
+    """Whatever the size of the problem and the kernels that it takes: nothing but the rounding to bf16 shows."""
+    args = _att(B, nq, nk, H, KV, d, BF16, cuda_device, bias, bias_dtype, mask)
+    val, _ = attention_ref(*args)
+    got = _run(*args)
+    far = {name: distance(got[name], val[name]) for name in val}
+    tol = {name: FP32_TOL if got[name].dtype == F32 else BF16_TOL for name in far}
+    assert all(far[name] <= tol[name] for name in far), far
