@@ -1332,26 +1332,28 @@ int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
       const int64_t t2 = (a.nq + 127) / 128;
       if (t2 * a.H * a.B >= 3 * 148) {
         a.tiles = t2;
-        return go(k_fwd<DP, BT, 2>, (128 + 4 * kTile) * RB, t2 * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
+        constexpr size_t smem = (128 + 4 * kTile) * RB;
+        return go<k_fwd<DP, BT, 2>>(smem, smem, t2 * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
       }
     }
     a.tiles = tq;
-    return go(k_fwd<DP, BT, 1>, (64 + 4 * kTile) * RB, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
+    constexpr size_t smem = (64 + 4 * kTile) * RB;
+    return go<k_fwd<DP, BT, 1>>(smem, smem, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
   }
   const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
-  const size_t smem = (128 + 4 * kTile) * RB + 2048;
+  constexpr size_t smem = (128 + 4 * kTile) * RB + 2048;
   const char* name = kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv");
   const int ranks = bkv == 0 ? 1 : dkv_ranks(a, bkv, tq * a.H * a.B);
   const int64_t bk = bkv * ranks, blocks = (bk + bq + ranks - 1) / ranks * ranks;
-  return go(k_dqkv<DP, BT>, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
+  return go<k_dqkv<DP, BT>>(smem, smem, blocks, ranks, name, flops, st, a, (unsigned)bk, ranks);
 }
 
 template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
   constexpr size_t smem = 2 * ((size_t)(256 + 128) * Tile<DP>::RB + 2048);
   a.tiles = (a.nq + 127) / 128;
-  return go(k_dbias<DP, BT>, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, 1, "k_attn_dbias", flops, st, a, part,
-            parts);
+  return go<k_dbias<DP, BT>>(smem, smem, a.tiles * ((a.nk + 63) / 64) * a.H * parts, 1, "k_attn_dbias", flops, st, a,
+                             part, parts);
 }
 
 template <int BT>
@@ -1364,11 +1366,10 @@ int launch_plane(Args a, float* part, int parts, double flops, cudaStream_t st) 
   const int64_t blocks = a.tiles * a.H * parts;
   if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
   const int smem = PlaneSmem(nkp).end;
-  auto* kern = k_dq_plane<BT>;
-  PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  PF_TRY(room_for_shared<k_dq_plane<BT>>(PlaneSmem(kPlaneKeys).end));
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_attn_dq_plane", flops, 'f');
-    kern<<<(unsigned)blocks, kPlaneThreads, smem, st>>>(a, part, parts, G, tcols);
+    k_dq_plane<BT><<<(unsigned)blocks, kPlaneThreads, smem, st>>>(a, part, parts, G, tcols);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;

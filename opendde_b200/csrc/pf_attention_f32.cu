@@ -884,32 +884,37 @@ int launch_t(Kind kind, Args a, double flops, cudaStream_t st) {
   const int64_t tq = (a.nq + 63) / 64, tk = (a.nk + 63) / 64;
   if (kind == kFwd) {
     a.tiles = tq;
-    return go(k_fwd<DP, BT>, S::kStat3 + 4 * S::kTile3, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
+    constexpr size_t smem = S::kStat3 + 4 * S::kTile3;
+    return go<k_fwd<DP, BT>>(smem, smem, tq * a.H * a.B, 1, "k_attn_fwd", flops, st, a);
   }
   const int64_t bq = kind == kDkv ? 0 : tq * a.H * a.B, bkv = kind == kDq ? 0 : tk * a.KV * a.B;
   const int ranks = bkv == 0 ? 1 : dkv_ranks(a, bkv, tq * a.H * a.B);
   const int64_t bk = bkv * ranks, blocks = (bk + bq + ranks - 1) / ranks * ranks;
-  return go(k_dqkv<DP, BT>, 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16, blocks, ranks,
-            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a, (unsigned)bk,
-            ranks);
+  constexpr size_t smem = 2 * S::kStat3 + 4 * S::kTile3 + 2 * S::KT * 16;
+  return go<k_dqkv<DP, BT>>(smem, smem, blocks, ranks,
+                            kind == kDq ? "k_attn_dq" : (kind == kDkv ? "k_attn_dkv" : "k_attn_dqkv"), flops, st, a,
+                            (unsigned)bk, ranks);
 }
 template <int DP, int BT>
 int launch_db(Args a, float* part, int parts, double flops, cudaStream_t st) {
   using S = Split<DP>;
   a.tiles = (a.nq + 63) / 64;
-  return go(k_dbias<DP, BT>, 2 * S::kStat3 + 2 * S::kTile3, a.tiles * ((a.nk + S::KT - 1) / S::KT) * a.H * parts, 1,
-            "k_attn_dbias", flops, st, a, part, parts);
+  constexpr size_t smem = 2 * S::kStat3 + 2 * S::kTile3;
+  return go<k_dbias<DP, BT>>(smem, smem, a.tiles * ((a.nk + S::KT - 1) / S::KT) * a.H * parts, 1, "k_attn_dbias", flops,
+                             st, a, part, parts);
 }
 
 template <int BT>
 int launch_plane(Args a, float* part, int parts, double flops, cudaStream_t st) {
   using S = Split<32>;
   const int tcols = a.nk <= 256 ? 128 : 256;
-  const int tiles = 2 * S::kStat3 + 4 * S::kTile3;
+  constexpr int tiles = 2 * S::kStat3 + 4 * S::kTile3;
   // room for as many blocks as tensor memory holds
-  const size_t smem = tcols == 128 ? tiles + 16 : 100 * 1024;
+  constexpr size_t most = 100 * 1024;
+  const size_t smem = tcols == 128 ? tiles + 16 : most;
   a.tiles = (a.nq + 63) / 64;
-  return go(k_dq_plane<BT>, smem, a.tiles * a.H * parts, 1, "k_attn_dq_plane", flops, st, a, part, parts, tcols, tiles);
+  return go<k_dq_plane<BT>>(smem, most, a.tiles * a.H * parts, 1, "k_attn_dq_plane", flops, st, a, part, parts, tcols,
+                            tiles);
 }
 
 }  // namespace

@@ -340,13 +340,13 @@ __device__ __forceinline__ bool pair_ok(const void* p, int64_t bs, int64_t ns, i
 
 // ---------------------------------------------------------------- dk, dv of a cluster
 
-// Blocks of a launch with `cluster` blocks to a cluster (1: none).
-template <class F, class... X>
-int go(F* kern, size_t smem, int64_t blocks, int cluster, const char* name, double flops, cudaStream_t st, X... x) {
+// `blocks` blocks of kernel K with `cluster` of them to a cluster (1: none) and `smem` bytes of shared memory, of
+// which other calls take `most` at most.
+template <auto K, class... X>
+int go(size_t smem, size_t most, int64_t blocks, int cluster, const char* name, double flops, cudaStream_t st, X... x) {
   if (blocks == 0) return PF_OK;
   if (blocks > 0x7fffffffll) return fail(PF_EUNSUPPORTED, "attention: %lld tiles are too many", (long long)blocks);
-  if (smem > 40 * 1024)
-    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  PF_TRY(room_for_shared<K>(most));
   {
     PF_LAUNCH_SCOPE_WORK(st, name, flops, 'f');
     cudaLaunchAttribute attr{};
@@ -356,7 +356,7 @@ int go(F* kern, size_t smem, int64_t blocks, int cluster, const char* name, doub
     cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cfg.attrs = &attr, cfg.numAttrs = cluster > 1 ? 1 : 0;
-    PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x...));
+    PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, K, x...));
   }
   PF_CHECK_LAUNCH();
   return PF_OK;

@@ -276,8 +276,8 @@ int launch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float*
            float* part, cudaStream_t st) {
   const int64_t blocks = grid_blocks(rows, c, kWarps * (32 / L) * U, dg || db);
   const size_t smem = (size_t)kWarps * 2 * c * sizeof(float);
-  auto* kern = k_layernorm_bwd<T, E, L, V, U, FULL>;
-  if (smem > 48 * 1024) PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  constexpr auto* kern = k_layernorm_bwd<T, E, L, V, U, FULL>;
+  PF_TRY(room_for_shared<kern>((size_t)kWarps * 2 * L * V * E * sizeof(float)));  // the instance's widest rows
   const bool cluster = (dg || db) && few_rows(rows, c), direct = blocks == 1 || cluster;
   const int64_t m0 = dg ? c : 0, m = m0 + (db ? c : 0);  // a partial row: dgamma, then dbeta
   float* pg = direct || !dg ? dg : part;

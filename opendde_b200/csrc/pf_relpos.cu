@@ -305,13 +305,11 @@ int launch_fwd(const RelGrid& p, const RelArgs& a, const void* w, void* out, cud
 template <class T, int G>
 int launch_bwd(const RelGrid& p, const RelArgs& a, const void* dout, float* part, cudaStream_t st) {
   const size_t smem = (size_t)kRelWarps * G * a.n_feat * sizeof(float);
-  auto* kern = k_relpos_bias_bwd<T, G>;
-  if (smem > 40 * 1024)
-    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  PF_TRY((room_for_shared<k_relpos_bias_bwd<T, G>>(64 * 1024)));  // see plan()
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_relpos_bias_bwd", (double)a.heads * a.n_rows * a.n_cols * sizeof(T), 'b');
-    kern<<<dim3((unsigned)p.strips, (unsigned)p.chunks, (unsigned)p.groups), kRelWarps * 32, smem, st>>>(
-        a, (const T*)dout, part);
+    k_relpos_bias_bwd<T, G><<<dim3((unsigned)p.strips, (unsigned)p.chunks, (unsigned)p.groups), kRelWarps * 32, smem,
+                              st>>>(a, (const T*)dout, part);
   }
   PF_CHECK_LAUNCH();
   return PF_OK;

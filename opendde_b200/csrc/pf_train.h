@@ -3,10 +3,27 @@
 // the gradient of its table (pf_relpos.cu).
 #pragma once
 #include <cuda_runtime.h>
+
+#include <atomic>
+
 #include "../../include/pairformer_b200.h"
+#include "pf_common.cuh"
+#include "pf_tmap.h"
 
 namespace pf {
 namespace train {
+
+// Lets kernel K take up to `most` bytes of dynamic shared memory, once per device. The limit is one per kernel and
+// device for all host threads, so it is the largest that any call needs and never lowered: a limit set to each call's
+// own size would fail another thread's larger launch.
+template <auto K>
+int room_for_shared(size_t most) {
+  static std::atomic<unsigned long long> done{0};
+  return once_per_device(done, [&]() -> int {
+    PF_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    return PF_OK;
+  });
+}
 
 size_t layernorm_bwd_ws_bytes(int64_t rows, int c, int dtype);
 int layernorm_bwd(const void* x, const void* dy, const float* gamma, void* dx, float* dgamma, float* dbeta,
