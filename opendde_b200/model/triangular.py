@@ -269,23 +269,40 @@ class TriangleAttention(nn.Module):
 
         return _batched(one, x, mask)
 
-    def differentiable(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def differentiable(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                       uniform_rows: bool = False) -> torch.Tensor:
         """The update of one [N, N, c_in] pair tensor with gradients of x and of the parameters: the layer norm and
         the attention over rows (which share the triangle bias) are this package's kernels, the projections are
-        library products. A non-zero ``mask`` entry is a visible key; a row without any attends to all of its keys
-        (a constant added to every logit changes nothing)."""
+        library products.
+
+        A row's keys are those of its largest ``mask`` value (values from 1 on count as 1), which is what
+        softmax(scores + inf (mask - 1)) comes to. Where that value is below 1, in padded rows above all, the scores
+        vanish next to inf in fp32: ``forward`` averages v over the row's keys. ``uniform_rows`` does the same here
+        (such rows then have no gradient of q, k and the bias); without it their softmax is over the scores, as in
+        exact arithmetic."""
         kernels.require_cuda(x, mask)
         if x.dim() != 3 or x.shape[0] != x.shape[1]:
             raise ValueError("differentiable takes one [N, N, c_in] pair tensor")
-        seen = None if mask is None else mask != 0
+        if mask is not None and mask.shape != x.shape[:2]:
+            raise ValueError(f"mask {tuple(mask.shape)} is not {tuple(x.shape[:2])}")
+        seen = mean = None
+        if mask is not None and mask.numel():
+            seen = mask.detach().to(device=x.device, dtype=torch.float32).clamp(max=1)
         if not self.starting:
             x, seen = x.transpose(0, 1), None if seen is None else seen.t()
         if seen is not None:
-            seen = (seen | ~seen.any(-1, keepdim=True)).to(device=x.device, dtype=torch.float32)
+            top = seen.amax(-1, keepdim=True)
+            seen = (seen == top).to(torch.float32)
+            if uniform_rows:
+                mean = seen.masked_fill(top >= 1, 0)
+                seen = seen - mean
+                mean = mean / mean.sum(-1, keepdim=True).clamp(min=1)
         y = self.layer_norm.differentiable(x)
         heads = (*y.shape[:2], self.no_heads, self.c_hidden)
         q, k, v, g, bias = (F.linear(y, m.weight.to(y.dtype)) for m in (
             self.mha.linear_q, self.mha.linear_k, self.mha.linear_v, self.mha.linear_g, self.linear))
-        o = autograd.attention(q.view(heads), k.view(heads), v.view(heads), bias.permute(2, 0, 1), seen)
-        out = F.linear(o.flatten(2) * torch.sigmoid(g), self.mha.linear_o.weight.to(y.dtype))
+        o = autograd.attention(q.view(heads), k.view(heads), v.view(heads), bias.permute(2, 0, 1), seen).flatten(2)
+        if mean is not None:  # o is 0 in these rows
+            o = o + torch.bmm(mean.to(v.dtype)[:, None], v)
+        out = F.linear(o * torch.sigmoid(g), self.mha.linear_o.weight.to(y.dtype))
         return out if self.starting else out.transpose(0, 1)

@@ -1,0 +1,85 @@
+"""The modules' differentiable forms next to their forward, and on masks that are not 0 and 1."""
+import pytest
+import torch
+
+from oracle import pairformer_oracle as O
+from opendde_b200.model import TriangleAttention
+from opendde_b200.utils import make_inputs, ragged_pair_mask, seeded_init_
+from test_gpu_autograd import TOL, _compare
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _pair_mask(n, device):
+    """Holes; a row that is masked, one of equal fractions, one of several; a fraction beside full keys; a value
+    above 1."""
+    mask = ragged_pair_mask(n, seed=8, drop=0.2, full_rows=[4])
+    mask[0, ::3] = 0.5
+    mask[0, 1] = 1.0
+    mask[7] = 0.25
+    mask[9] = torch.arange(n) % 4 * 0.125
+    mask[11, 2] = 1.5
+    mask[11, 3] = 1.0
+    return mask.to(device)
+
+
+def _triangle_attention(z, mask, p, heads, starting, uniform):
+    """The update in z's type: each row's keys are those of its largest mask value; a row whose largest is below 1
+    is a softmax over its scores, or the plain mean of v over its keys."""
+    if not starting:
+        z, mask = z.transpose(0, 1), mask.t()
+    n = z.shape[0]
+    x = O.layer_norm(z, p["layer_norm.weight"], p["layer_norm.bias"], 1e-5)
+    q, k, v, g = (O.linear(x, p[f"mha.linear_{m}.weight"]).view(n, n, heads, -1).transpose(1, 2) for m in "qkvg")
+    t = q @ k.transpose(2, 3) / q.shape[-1] ** 0.5 + O.linear(x, p["linear.weight"]).permute(2, 0, 1)
+    m = mask.clamp(max=1)
+    top = m.amax(-1, keepdim=True)
+    if uniform:
+        t = t.masked_fill((top < 1)[:, None, None], 0.0)
+    o = torch.softmax(t.masked_fill((m != top)[:, None, None], float("-inf")), -1) @ v
+    out = O.linear((o * torch.sigmoid(g)).transpose(1, 2).flatten(2), p["mha.linear_o.weight"])
+    return out if starting else out.transpose(0, 1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("starting", [True, False])
+@pytest.mark.parametrize("uniform", [True, False])
+def test_triangle_attention_masks(uniform, starting, dtype, cuda_device):
+    _, z, _ = make_inputs(29, c_z=64, seed=6, with_s=False)
+    mask = _pair_mask(29, cuda_device)
+    if not starting:
+        mask = mask.t()
+    mod = TriangleAttention(c_in=64, c_hidden=32, no_heads=2, starting=starting)
+    # the form above is the oracle's: with its 1e9 the scores of a row without a full key survive in fp64, with 1e30
+    # they vanish as they do in fp32 with 1e9
+    p64 = {name: t.double() for name, t in seeded_init_(mod, seed=3, perturb_1d=True).items()}
+    m64 = mask.cpu().double()
+    want = O.triangle_attention(z.double(), m64.clamp(max=1), p64, 2, starting=starting, inf=1e30 if uniform else 1e9)
+    same = _triangle_attention(z.double(), m64, p64, 2, starting, uniform)
+    assert (want - same).norm() <= 1e-5 * want.norm()
+    _compare(mod, cuda_device, dtype, [z], lambda p, z: _triangle_attention(z, mask.double(), p, 2, starting, uniform),
+             lambda m, z: m.differentiable(z, mask, uniform_rows=uniform), TOL[dtype])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("starting", [True, False])
+def test_triangle_attention_follows_forward(starting, dtype, cuda_device):
+    """The same update as the inference forward, masked rows and fractions beside full keys included, within what both
+    may be off (bf16: forward's scores are fp16 values, 2e-2 as for its parity with the reference)."""
+    _, z, _ = make_inputs(40, c_z=64, seed=6, with_s=False)
+    mask = ragged_pair_mask(40, seed=8, drop=0.2, full_rows=[4, 39])
+    mask[0, ::3] = 0.5
+    mask[0, 1] = 1.0
+    mask = mask.to(cuda_device) if starting else mask.t().to(cuda_device)
+    mod = TriangleAttention(c_in=64, c_hidden=32, no_heads=2, starting=starting)
+    seeded_init_(mod, seed=3, perturb_1d=True)
+    mod, z = mod.to(cuda_device), z.to(cuda_device, dtype)
+    with torch.no_grad():
+        want, got = mod(z, mask), mod.differentiable(z, mask, uniform_rows=True)
+        every = mod.differentiable(z), mod(z)
+    tol = TOL[F32] if dtype == F32 else 2e-2
+    for a, b in ((got, want), every):
+        assert ((a.double() - b.double()).norm() / b.double().norm()).item() <= tol
+    with pytest.raises(ValueError, match="mask"):
+        mod.differentiable(z, mask[:, :-1])
