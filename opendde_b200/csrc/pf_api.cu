@@ -83,9 +83,9 @@ int pf_set_option(int option, int64_t value) {
 int pf_layernorm_fwd(const void* x, void* y, const float* gamma, const float* beta, int64_t rows,
                      int32_t c, float eps, int32_t dtype, void* stream) {
   PF_TRY(check_dtype(dtype));
-  if (!x || !y) return fail(PF_EINVAL_ARG, "layernorm: null input/output");
   if (rows < 0 || c <= 0 || c > 1024) return fail(PF_EINVAL_SHAPE, "layernorm: rows=%lld c=%d", (long long)rows, c);
   if (rows == 0) return PF_OK;
+  if (!x || !y) return fail(PF_EINVAL_ARG, "layernorm: null input/output");
   // LayerNorm is fused into every producing tensor-core kernel; the standalone entry point runs
   // a row kernel with 128-bit loads and stores in both dtypes (HBM-bound, no MMA to feed), or
   // the scalar warp-per-row kernel when rows are not whole 16-byte vectors.

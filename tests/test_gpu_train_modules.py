@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from oracle import pairformer_oracle as O
-from opendde_b200.model import TriangleAttention
+from opendde_b200.model import LayerNorm, TriangleAttention
 from opendde_b200.utils import make_inputs, ragged_pair_mask, seeded_init_
 from test_gpu_autograd import TOL, _compare
 
@@ -83,3 +83,16 @@ def test_triangle_attention_follows_forward(starting, dtype, cuda_device):
         assert ((a.double() - b.double()).norm() / b.double().norm()).item() <= tol
     with pytest.raises(ValueError, match="mask"):
         mod.differentiable(z, mask[:, :-1])
+
+
+def test_no_tokens(cuda_device):
+    """The forms of nothing: shapes and zero gradients, no error."""
+    x = torch.zeros(0, 0, 64, device=cuda_device, requires_grad=True)
+    ln = LayerNorm(64).to(cuda_device)
+    ln.differentiable(x).sum().backward()
+    assert x.grad.shape == x.shape and not ln.weight.grad.any()
+    mod = TriangleAttention(c_in=64, c_hidden=32, no_heads=2).to(cuda_device)
+    for mask in (None, torch.ones(0, 0, device=cuda_device)):
+        out = mod.differentiable(x, mask, uniform_rows=True)
+        out.sum().backward()
+        assert out.shape == x.shape and not mod.mha.linear_q.weight.grad.any()
