@@ -118,7 +118,8 @@ class AttentionPairBias(nn.Module):
                        extra_attn_bias: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``forward(a, None, z)`` of one [N, c_a] single and [N, N, c_z] pair representation with gradients of a, z,
         ``extra_attn_bias`` and the parameters: layer norms and attention are this package's kernels, the
-        projections are library products. The bias is float32 whatever a is, as in ``forward``."""
+        projections are library products. The bias is a float32 product whatever a and z are, as in ``forward``, and
+        its gradient stays float32 up to the weight and the normalised z."""
         kernels.require_cuda(a, z, extra_attn_bias)
         if a.dim() != 2 or z.dim() != 3:
             raise ValueError("differentiable takes one [N, c_a] and one [N, N, c_z] tensor")
@@ -127,8 +128,8 @@ class AttentionPairBias(nn.Module):
         b_q = att.linear_q.bias
         q = F.linear(y, att.linear_q.weight.to(y.dtype), None if b_q is None else b_q.to(y.dtype))
         k, v, g = (F.linear(y, m.weight.to(y.dtype)) for m in (att.linear_k, att.linear_v, att.linear_g))
-        w_z = self.linear_nobias_z.weight.to(z.dtype)
-        bias = F.linear(self.layernorm_z.differentiable(z), w_z).permute(2, 0, 1).to(torch.float32)
+        bias = F.linear(self.layernorm_z.differentiable(z).float(), self.linear_nobias_z.weight.float())
+        bias = bias.permute(2, 0, 1)
         if extra_attn_bias is not None:
             e = extra_attn_bias.to(device=a.device, dtype=torch.float32)
             bias = bias + (e if e.dim() == 3 else e[None])

@@ -3,9 +3,11 @@ import pytest
 import torch
 
 from oracle import pairformer_oracle as O
-from opendde_b200.model import LayerNorm, TriangleAttention
+from opendde_b200 import autograd
+from opendde_b200.model import AttentionPairBias, LayerNorm, TriangleAttention
 from opendde_b200.utils import make_inputs, ragged_pair_mask, seeded_init_
 from test_gpu_autograd import TOL, _compare
+from train_ops_support import U
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -96,3 +98,35 @@ def test_no_tokens(cuda_device):
         out = mod.differentiable(x, mask, uniform_rows=True)
         out.sum().backward()
         assert out.shape == x.shape and not mod.mha.linear_q.weight.grad.any()
+
+
+def test_attention_pair_bias_is_fp32(cuda_device, monkeypatch):
+    """bf16 inputs: the bias that attention gets is the fp32 product of the normalised pair tensor and the weight, as
+    in forward, and its gradient reaches the weight unrounded. Sums of 64 and n^2 products."""
+    n = 50
+    s, z, _ = make_inputs(n, c_z=64, c_s=96, seed=5)
+    mod = AttentionPairBias(has_s=False, create_offset_ln_z=True, n_heads=4, c_a=96, c_z=64)
+    seeded_init_(mod, seed=3, perturb_1d=True)
+    mod, s, z = mod.to(cuda_device), s.to(cuda_device, BF16), z.to(cuda_device, BF16)
+    w = mod.linear_nobias_z.weight
+    with torch.no_grad():
+        w.copy_(w.to(BF16))  # forward multiplies bf16 weights
+    seen, attention = {}, autograd.attention
+
+    def record(q, k, v, bias, *rest):
+        seen["bias"] = bias.detach()
+        bias.register_hook(lambda g: seen.update(grad=g))
+        return attention(q, k, v, bias, *rest)
+    monkeypatch.setattr(autograd, "attention", record)
+    out = mod.differentiable(s, z)
+    out.backward(torch.randn(out.shape, generator=torch.Generator().manual_seed(1)).to(cuda_device, BF16))
+    y, w64 = mod.layernorm_z(z).double(), w.detach().double()
+    assert seen["bias"].dtype == seen["grad"].dtype == F32
+    far = (seen["bias"].double() - (y @ w64.t()).permute(2, 0, 1)).abs()
+    assert (far <= 72 * U * (y.abs() @ w64.abs().t()).permute(2, 0, 1)).all()
+    g = seen["grad"].double()
+    far = (w.grad.double() - torch.einsum("hij,ijc->hc", g, y)).abs()
+    assert (far <= 16 * n * U * torch.einsum("hij,ijc->hc", g.abs(), y.abs())).all()
+    # forward's own bias rounds its normalised input to bf16 as well
+    rel = (seen["bias"].double() - mod.pair_bias(z).double()).norm() / seen["bias"].double().norm()
+    assert rel.item() <= 2.0 ** -8
