@@ -4,10 +4,10 @@ import torch
 
 from oracle import pairformer_oracle as O
 from opendde_b200 import autograd
-from opendde_b200.model import AttentionPairBias, LayerNorm, TriangleAttention
+from opendde_b200.model import AttentionPairBias, LayerNorm, RelativePositionEncoding, TriangleAttention
 from opendde_b200.utils import make_inputs, ragged_pair_mask, seeded_init_
 from test_gpu_autograd import TOL, _compare
-from train_ops_support import U
+from train_ops_support import U, relpos_columns, token_ids
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -130,3 +130,41 @@ def test_attention_pair_bias_is_fp32(cuda_device, monkeypatch):
     # forward's own bias rounds its normalised input to bf16 as well
     rel = (seen["bias"].double() - mod.pair_bias(z).double()).norm() / seen["bias"].double().norm()
     assert rel.item() <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_single_update_with_a_relative_position_bias(dtype, cuda_device):
+    """s + AttentionPairBias(s, z) with RelativePositionEncoding.head_bias as extra_attn_bias: outputs and gradients of
+    s, z, every parameter and the table against fp64 autograd of the same formula."""
+    n, heads = 37, 4
+    s, z, _ = make_inputs(n, c_z=64, c_s=96, seed=5)
+    ids = token_ids(n, 2, cuda_device)
+    relpe = RelativePositionEncoding(r_max=8, s_max=2, c_z=heads).to(cuda_device)
+    feats = relpe.generate_relp(dict(zip(("asym_id", "residue_index", "entity_id", "token_index", "sym_id"), ids)))["relp"]
+    mod = AttentionPairBias(has_s=False, create_offset_ln_z=False, n_heads=heads, c_a=96, c_z=64)
+    p = {k: t.double().to(cuda_device).requires_grad_() for k, t in seeded_init_(mod, seed=3, perturb_1d=True).items()}
+    mod = mod.to(cuda_device)
+    s, z = s.to(cuda_device, dtype).requires_grad_(), z.to(cuda_device, dtype).requires_grad_()
+    table = relpe.linear_no_bias.weight
+    got = s + mod.differentiable(s, z, relpe.head_bias(feats))
+
+    s64, z64, t64 = (t.detach().double().requires_grad_() for t in (s, z, table))
+    y = O.layer_norm(s64, p["layernorm_a.weight"], p["layernorm_a.bias"], 1e-5)
+    q = O.linear(y, p["attention.linear_q.weight"], p["attention.linear_q.bias"])
+    k, v, g = (O.linear(y, p[f"attention.linear_{m}.weight"]) for m in "kvg")
+    q, k, v = (t.view(n, heads, -1).transpose(0, 1) for t in (q, k, v))
+    bias = O.linear(O.layer_norm(z64, p["layernorm_z.weight"], None, 1e-5), p["linear_nobias_z.weight"]).permute(2, 0, 1)
+    bias = bias + torch.einsum("ijf,hf->hij", relpos_columns(ids, slice(0, n), slice(0, n), 8, 2), t64)
+    o = (torch.softmax(q @ k.transpose(1, 2) / q.shape[-1] ** 0.5 + bias, -1) @ v).transpose(0, 1).flatten(1)
+    want = s64 + O.linear(o * torch.sigmoid(g), p["attention.linear_o.weight"])
+
+    dy = torch.randn(n, 96, generator=torch.Generator().manual_seed(2)).to(cuda_device, dtype)
+    names = [k for k, _ in mod.named_parameters()]
+    assert set(names) == set(p)
+    gg = torch.autograd.grad(got, [s, z, table] + [t for _, t in mod.named_parameters()], dy)
+    gw = torch.autograd.grad(want, [s64, z64, t64] + [p[k] for k in names], dy.double())
+    for name, a, b in zip(["out", "s", "z", "table"] + names, (got,) + gg, (want,) + gw):
+        assert ((a.double() - b).norm() / b.norm()).item() <= TOL[dtype], name
+    with torch.no_grad():  # the inference form of the same call
+        want = s + mod(s, None, z, extra_attn_bias=relpe.head_bias(feats))
+    assert ((got.double() - want.double()).norm() / want.double().norm()).item() <= TOL[dtype]
