@@ -495,6 +495,14 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
             for (int e = 0; e < 4; ++e)
               if (x[n][e] == 1.f) y[n][e] = 0.f;
       }
+      if (!FAST) {  // a hidden key's ds is 0, whatever do holds
+        const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!((mine >> (2 * n + e)) & 1)) y[n][e] = y[n][2 + e] = 0.f;
+      }
       if (put) {
         const int64_t j = j0 + hb * 32 + q * 16 + 4 * t;
 #pragma unroll

@@ -199,7 +199,7 @@ __device__ __forceinline__ void split_a(float (&x)[2][4], uint32_t (&pa)[3][4]) 
 }
 
 template <int BT, int R>
-__device__ __forceinline__ void hide16(float (&x)[R][2][4], uint32_t bits) {
+__device__ __forceinline__ void hide16(float (&x)[R][2][4], uint32_t bits, float hidden = -INFINITY) {
   if (bits == 0xffffu) return;
   const int t = threadIdx.x & 3;
 #pragma unroll
@@ -208,7 +208,7 @@ __device__ __forceinline__ void hide16(float (&x)[R][2][4], uint32_t bits) {
     for (int e = 0; e < 2; ++e)
       if (!((bits >> (4 * t + 2 * n + e)) & 1))
 #pragma unroll
-        for (int q = 0; q < R; ++q) x[q][n][e] = x[q][n][2 + e] = -INFINITY;
+        for (int q = 0; q < R; ++q) x[q][n][e] = x[q][n][2 + e] = hidden;
 }
 
 __device__ __forceinline__ void store2f(float* p, int col, int d, bool vec, float v0, float v1) {
@@ -498,7 +498,8 @@ __device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigne
         const bool whole = j0 + 16 <= a.nk;
 #pragma unroll
         for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + 4 * t, a.nk, a.bias_vec && whole);
-        float x[1][2][4], y[2][4];
+        float x[1][2][4], ys[1][2][4];
+        float(&y)[2][4] = ys[0];
         uint32_t ba[KS];
         addresses<DP>(ba, lb, tk, q);
         nt3<KS, S::kStatPlane, S::kPlane>(x[0], qa, ba);
@@ -510,6 +511,7 @@ __device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigne
           for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
         hide16<BT, 1>(x, qbits);
         prob_ds(x[0], y, nmx, lg, nd, peaked);
+        hide16<BT, 1>(ys, qbits, 0.f);  // a hidden key's ds is 0, whatever do holds
         if (PLANE) {
           uint32_t tm[8];
           const uint32_t at = tm0 + (uint32_t)(kt * (KT / 16) + q) * 8;

@@ -1,0 +1,28 @@
+"""Edges of the training operators on the GPU."""
+import pytest
+import torch
+
+from test_gpu_train_ops import _att, _run
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("bias", [None, "shared", "batch"])
+@pytest.mark.parametrize("n_q,n_k,d", [(70, 80, 32), (33, 200, 64)])
+def test_attention_padded_entries_may_hold_anything(n_q, n_k, d, bias, bad, dtype, cuda_device):
+    """A batch entry whose keys are all masked has output and gradients 0 whatever its queries and the gradient of its
+    output hold; the other entries and a shared bias's gradient keep their bits."""
+    q, k, v, do, bt, mask = _att(9, n_q, n_k, 2, 2, d, dtype, cuda_device, bias, F32, "holes")
+    want = _run(q, k, v, do, bt, mask)
+    gone = (mask == 0).all(1)
+    assert gone.sum() == 1
+    q2, do2 = q.clone(), do.clone()
+    q2[gone], do2[gone] = bad, bad
+    got = _run(q2, k, v, do2, bt, mask)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+        if not (name == "dbias" and bias == "shared"):
+            assert not got[name][gone].any(), name
