@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from test_gpu_train_ops import _att, _run
+from opendde_b200 import kernels
+from test_gpu_train_ops import _att, _rand, _run
+from train_ops_support import check, layernorm_ref
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -26,3 +28,18 @@ def test_attention_padded_entries_may_hold_anything(n_q, n_k, d, bias, bad, dtyp
         assert torch.equal(got[name], want[name]), name
         if not (name == "dbias" and bias == "shared"):
             assert not got[name][gone].any(), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,c", [(2600, 513), (2100, 640), (3001, 768), (2000, 769), (1800, 896), (2500, 1000),
+                                    (1500, 1001), (3000, 1024), (600, 1023)])
+def test_layernorm_bwd_of_many_wide_rows(rows, c, dtype, cuda_device):
+    """More than 512 channels, several rows to each warp, partial sums of many blocks."""
+    x, dy = _rand((rows, c), dtype, cuda_device, 1, 2.0), _rand((rows, c), dtype, cuda_device, 2)
+    w = _rand((c,), F32, cuda_device, 3, 0.3) + 1
+    val, bound = layernorm_ref(x, dy, w, 1e-5)
+    got = dict(zip(("dx", "dw", "db"), kernels.layernorm_bwd(x, dy, w)))
+    for name in got:
+        check(got[name], val[name], bound[name], name)
+    again = dict(zip(got, kernels.layernorm_bwd(x, dy, w)))
+    assert all(torch.equal(got[name], again[name]) for name in got)
