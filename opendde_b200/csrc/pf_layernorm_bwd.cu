@@ -79,8 +79,7 @@ __device__ __forceinline__ float group_sum(float v) {
 
 namespace cg = cooperative_groups;
 constexpr int kWarps = 8;
-constexpr int kRanks = 8;             // blocks of the cluster that takes few rows
-constexpr int64_t kFew = 4 * 64 * 512;  // elements of those
+constexpr int kRanks = 8;  // blocks of the cluster that takes few rows
 
 // Blocks on an SM: two (128 registers) where a lane has up to 16 channels, and at 768 bf16 channels exactly; more
 // channels need the registers of one block (two: 0.3 to 1.4 KB of spills; 30000 rows of 1024, bf16 109 against 59 us,
@@ -265,13 +264,16 @@ int sm_count() {
   return n;
 }
 
-// Blocks of the row kernel: a cluster of eight where the rows are few (64 rows of 384 channels, called and replayed:
-// 17.8 and 3.5 us against 21 to 25 and 4.1 us in two launches, and 14 us in one block; 1024 rows of 128: 17.8 and
-// 5.8 against 21 and 5.7 us; 2048: 17.9 and 8.2 against 21 and 5.7 us); else enough warps to cover the rows, at
-// most four blocks on each SM (two run at a time).
-bool few_rows(int64_t rows, int c) { return rows * c <= kFew; }
-int64_t grid_blocks(int64_t rows, int c, int rows_per_block, bool sums) {
-  if (sums && few_rows(rows, c)) return kRanks;
+// Blocks of the row kernel for rows of `chunk` rows per block and step, `values` values of a lane in flight: a cluster
+// of eight where the rows are few steps of it, up to four of 16 values, two of 32 (called and replayed, us, fp32: 64
+// rows of 384 channels, one step, 18 and 4.7 against 21 to 25 and 6.2 in two launches; 128 rows of 1024, two steps, 20
+// and 8 against 24 and 8; 1024 rows of 128, four steps, 18 and 8 against 21 and 6; 3500 rows of 37, 28 steps, 25 and
+// 25 against 22 and 8); else enough warps to cover the rows, at most four blocks on each SM.
+bool few_rows(int64_t rows, int chunk, int values) {
+  const int steps = values > 16 ? 64 / values : 4;
+  return rows <= (int64_t)steps * kRanks * chunk;
+}
+int64_t grid_blocks(int64_t rows, int rows_per_block) {
   const int64_t need = (rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sm_count() * 4;
   return need < 1 ? 1 : (need < most ? need : most);
 }
@@ -279,11 +281,13 @@ int64_t grid_blocks(int64_t rows, int c, int rows_per_block, bool sums) {
 template <class T, int E, int L, int V, int U, bool FULL>
 int launch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float* db, int64_t rows, int c, float eps,
            float* part, cudaStream_t st) {
-  const int64_t blocks = grid_blocks(rows, c, kWarps * (32 / L) * U, dg || db);
+  constexpr int rows_per_block = kWarps * (32 / L) * U;
+  const bool cluster = (dg || db) && few_rows(rows, rows_per_block, U * V * E);
+  const int64_t blocks = cluster ? kRanks : grid_blocks(rows, rows_per_block);
   const size_t smem = (size_t)kWarps * 2 * c * sizeof(float);
   constexpr auto* kern = k_layernorm_bwd<T, E, L, V, U, FULL>;
   PF_TRY(room_for_shared<kern>((size_t)kWarps * 2 * L * V * E * sizeof(float)));  // the instance's widest rows
-  const bool cluster = (dg || db) && few_rows(rows, c), direct = blocks == 1 || cluster;
+  const bool direct = blocks == 1 || cluster;
   const int64_t m0 = dg ? c : 0, m = m0 + (db ? c : 0);  // a partial row: dgamma, then dbeta
   float* pg = direct || !dg ? dg : part;
   float* pb = direct || !db ? db : part + m0;

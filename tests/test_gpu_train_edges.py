@@ -43,3 +43,18 @@ def test_layernorm_bwd_of_many_wide_rows(rows, c, dtype, cuda_device):
         check(got[name], val[name], bound[name], name)
     again = dict(zip(got, kernels.layernorm_bwd(x, dy, w)))
     assert all(torch.equal(got[name], again[name]) for name in got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c,limits", [(37, (512,)), (65, (256,)), (128, (1024,)), (384, (128, 256)), (512, (256,)),
+                                      (768, (128,)), (1001, (128,)), (1024, (128,)), (7, (1024, 2048)), (16, (4096,))])
+def test_layernorm_bwd_where_the_launches_change(c, limits, dtype, cuda_device):
+    """One cluster up to some number of rows, two launches from there on; a call that wants dx alone has neither sums."""
+    w = _rand((c,), F32, cuda_device, 3, 0.3) + 1
+    for rows in (r + more for r in limits for more in (0, 1)):
+        x, dy = _rand((rows, c), dtype, cuda_device, 1, 2.0), _rand((rows, c), dtype, cuda_device, 2)
+        val, bound = layernorm_ref(x, dy, w, 1e-5)
+        got = kernels.layernorm_bwd(x, dy, w)
+        for name, t in zip(("dx", "dw", "db"), got):
+            check(t, val[name], bound[name], f"{name} of {rows}")
+        assert torch.equal(kernels.layernorm_bwd(x, dy, w, need=(True, False, False))[0], got[0])
