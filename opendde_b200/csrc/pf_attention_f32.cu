@@ -198,17 +198,15 @@ __device__ __forceinline__ void split_a(float (&x)[2][4], uint32_t (&pa)[3][4]) 
     }
 }
 
-template <int BT, int R>
-__device__ __forceinline__ void hide16(float (&x)[R][2][4], uint32_t bits, float hidden = -INFINITY) {
+// `hidden` in place of the columns without a bit
+__device__ __forceinline__ void hide16(float (&x)[2][4], uint32_t bits, float hidden = -INFINITY) {
   if (bits == 0xffffu) return;
   const int t = threadIdx.x & 3;
 #pragma unroll
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (!((bits >> (4 * t + 2 * n + e)) & 1))
-#pragma unroll
-        for (int q = 0; q < R; ++q) x[q][n][e] = x[q][n][2 + e] = hidden;
+      if (!((bits >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = hidden;
 }
 
 __device__ __forceinline__ void store2f(float* p, int col, int d, bool vec, float v0, float v1) {
@@ -295,8 +293,7 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 3 : 1) k_fwd(Args a) {
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int r = 0; r < 2; ++r) score2<BT>(&x[q][n][2 * r], scale, br[r], n);
-          float(&xq)[1][2][4] = *reinterpret_cast<float(*)[1][2][4]>(&x[q]);
-          hide16<BT, 1>(xq, (hbits >> (16 * q)) & 0xffffu);
+          hide16(x[q], (hbits >> (16 * q)) & 0xffffu);
         }
         float nm[2];
         bool grew = false;
@@ -498,20 +495,19 @@ __device__ __forceinline__ void dq_rows(const Args& a, int64_t b, int h, unsigne
         const bool whole = j0 + 16 <= a.nk;
 #pragma unroll
         for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + 4 * t, a.nk, a.bias_vec && whole);
-        float x[1][2][4], ys[1][2][4];
-        float(&y)[2][4] = ys[0];
+        float x[2][4], y[2][4];
         uint32_t ba[KS];
         addresses<DP>(ba, lb, tk, q);
-        nt3<KS, S::kStatPlane, S::kPlane>(x[0], qa, ba);
+        nt3<KS, S::kStatPlane, S::kPlane>(x, qa, ba);
         addresses<DP>(ba, lb, tv, q);
         nt3<KS, S::kStatPlane, S::kPlane>(y, ga, ba);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
-        hide16<BT, 1>(x, qbits);
-        prob_ds(x[0], y, nmx, lg, nd, peaked);
-        hide16<BT, 1>(ys, qbits, 0.f);  // a hidden key's ds is 0, whatever do holds
+          for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, br[r], n);
+        hide16(x, qbits);
+        prob_ds(x, y, nmx, lg, nd, peaked);
+        hide16(y, qbits, 0.f);  // a hidden key's ds is 0, whatever do holds
         if (PLANE) {
           uint32_t tm[8];
           const uint32_t at = tm0 + (uint32_t)(kt * (KT / 16) + q) * 8;
@@ -695,23 +691,23 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
             const int64_t i = i0 + blk * 16 + r * 8 + g;
             bias_load<BT>(br[r], bias_row<BT>(a, b, h, i < a.nq ? i : a.nq - 1), w0 + 4 * t, a.nk, bfast);
           }
-          float x[1][2][4], y[2][4];
+          float x[2][4], y[2][4];
           uint32_t aa[KS];
           addresses<DP>(aa, la, tq, blk);
-          nt3<KS, S::kPlane, S::kStatPlane>(x[0], aa, ka);
+          nt3<KS, S::kPlane, S::kStatPlane>(x, aa, ka);
           addresses<DP>(aa, la, tg, blk);
           nt3<KS, S::kPlane, S::kStatPlane>(y, aa, va);
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
-          hide16<BT, 1>(x, mine);
+            for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, br[r], n);
+          hide16(x, mine);
           const float4 c[2] = {cst[(it & 1) * KT + blk * 16 + g], cst[(it & 1) * KT + blk * 16 + 8 + g]};
           const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)},
                    nd[2] = {F2(c[0].w), F2(c[1].w)};
-          prob_ds(x[0], y, nmx, lg, nd, __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f));
+          prob_ds(x, y, nmx, lg, nd, __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f));
           uint32_t u[3][4], w[3][4];
-          split_a(x[0], u);
+          split_a(x, u);
 #pragma unroll
           for (int p = 0; p < 3; ++p) {  // 8 x 8 blocks transposed, the two off the diagonal changing places
             w[p][0] = transpose8(u[p][0]), w[p][2] = transpose8(u[p][1]);
@@ -838,18 +834,18 @@ __global__ void __launch_bounds__(kThreads, DP == 32 ? 4 : 1) k_dbias(Args a, fl
       const bool fast = a.bias_vec && j0 + q * 16 + 16 <= a.nk;
 #pragma unroll
       for (int r = 0; r < 2; ++r) bias_load<BT>(br[r], brow[r], j0 + q * 16 + 4 * t, a.nk, fast);
-      float x[1][2][4], y[2][4];
+      float x[2][4], y[2][4];
       uint32_t ba[KS];
       addresses<DP>(ba, lb, sk, q);
-      nt3<KS, S::kStatPlane, S::kPlane>(x[0], qa, ba);
+      nt3<KS, S::kStatPlane, S::kPlane>(x, qa, ba);
       addresses<DP>(ba, lb, sv, q);
       nt3<KS, S::kStatPlane, S::kPlane>(y, ga, ba);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) score2<BT>(&x[0][n][2 * r], scale, br[r], n);
-      hide16<BT, 1>(x, (uint32_t)(bits >> (16 * q)) & 0xffffu);
-      prob_ds(x[0], y, nmx, lg, nd, peaked);
+        for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, br[r], n);
+      hide16(x, (uint32_t)(bits >> (16 * q)) & 0xffffu);
+      prob_ds(x, y, nmx, lg, nd, peaked);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll

@@ -283,14 +283,13 @@ int launch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float*
            float* part, cudaStream_t st) {
   constexpr int rows_per_block = kWarps * (32 / L) * U;
   const bool cluster = (dg || db) && few_rows(rows, rows_per_block, U * V * E);
-  const int64_t blocks = cluster ? kRanks : grid_blocks(rows, rows_per_block);
+  const int64_t blocks = cluster ? kRanks : grid_blocks(rows, rows_per_block);  // more than one where sums are wanted
   const size_t smem = (size_t)kWarps * 2 * c * sizeof(float);
   constexpr auto* kern = k_layernorm_bwd<T, E, L, V, U, FULL>;
   PF_TRY(room_for_shared<kern>((size_t)kWarps * 2 * L * V * E * sizeof(float)));  // the instance's widest rows
-  const bool direct = blocks == 1 || cluster;
   const int64_t m0 = dg ? c : 0, m = m0 + (db ? c : 0);  // a partial row: dgamma, then dbeta
-  float* pg = direct || !dg ? dg : part;
-  float* pb = direct || !db ? db : part + m0;
+  float* pg = cluster || !dg ? dg : part;
+  float* pb = cluster || !db ? db : part + m0;
   {
     PF_LAUNCH_SCOPE_WORK(st, "k_layernorm_bwd", 3.0 * (double)rows * c * sizeof(T), 'b');
     cudaLaunchAttribute attr{};
@@ -303,7 +302,7 @@ int launch(const T* x, const T* dy, const float* gamma, T* dx, float* dg, float*
     PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, x, dy, gamma, dx, pg, pb, m, rows, c, eps, cluster ? kRanks : 1));
   }
   PF_CHECK_LAUNCH();
-  return direct || m == 0 ? PF_OK : sum_rows(part, blocks, m, dg, m0, db, st);
+  return cluster || m == 0 ? PF_OK : sum_rows(part, blocks, m, dg, m0, db, st);
 }
 
 template <class T, int E>
@@ -346,9 +345,11 @@ int sum_rows(const float* part, int64_t n, int64_t m, float* out0, int64_t m0, f
   return PF_OK;
 }
 
-// Two partial rows (dgamma, dbeta) per block of the largest grid; the size depends on the channel
-// count alone, and a problem of one block needs none of it.
-size_t layernorm_bwd_ws_bytes(int64_t, int c, int) { return (size_t)sm_count() * 4 * 2 * c * sizeof(float); }
+// Two partial rows (dgamma, dbeta) per block of the largest grid that these rows can have: every instance takes at
+// least one row per warp and step.
+size_t layernorm_bwd_ws_bytes(int64_t rows, int c, int) {
+  return (size_t)grid_blocks(rows, kWarps) * 2 * c * sizeof(float);
+}
 
 int layernorm_bwd(const void* x, const void* dy, const float* gamma, void* dx, float* dgamma, float* dbeta,
                   int64_t rows, int c, float eps, int dtype, void* ws, size_t, cudaStream_t st) {
