@@ -1,7 +1,8 @@
 // pf_relp.cuh -- the relative-position feature of a token pair as the indices of its one-hot
 // entries (RelativePositionEncoding, opendde/model/modules/embedders.py:124-179, 226-290), shared
-// by the trunk's pair input (pf_trunk.cu) and the diffusion pair conditioning (pf_heads.cu), with
-// the 4-channel vector accesses of their one-warp-per-position kernels.
+// by the trunk's pair input (pf_trunk.cu), the diffusion pair conditioning (pf_heads.cu) and the
+// relative-position bias of attention heads (pf_relpos.cu), with the 4-channel vector accesses of the
+// first two's one-warp-per-position kernels.
 //
 // The feature vector is [residue offset (2R + 2) | token offset (2R + 2) | same entity (1) |
 // symmetry-copy offset (2S + 2)], R = r_max, S = s_max: three one-hots and one bit. Its product
@@ -22,23 +23,36 @@ struct RelpIndex {
 
 __host__ __device__ __forceinline__ int relp_n_feat(int r_max, int s_max) { return 4 * r_max + 2 * s_max + 7; }
 
-__device__ __forceinline__ int relp_clip(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+// The ids of one token.
+struct RelpIds {
+  int asym, res, ent, tok, sym;
+};
+__device__ __forceinline__ RelpIds relp_ids(const pf_token_ids& p, int64_t i) {
+  return RelpIds{p.asym_id[i], p.residue_index[i], p.entity_id[i], p.token_index[i], p.sym_id[i]};
+}
+
+// a - b clipped to [-lim, lim], plus lim; the difference saturates, so no pair of ids wraps around
+__device__ __forceinline__ int relp_offset(int a, int b, int lim) {
+  int d;
+  asm("sub.sat.s32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return min(max(d, -lim), lim) + lim;
+}
 
 // Residue offset clipped to [0, 2R] within a chain (2R + 1 across chains); token offset clipped
 // the same way within one residue of one chain (2R + 1 otherwise); symmetry-copy offset clipped to
 // [0, 2S] within an entity (2S + 1 across entities).
-__device__ __forceinline__ RelpIndex relp_index(const pf_token_ids& ids, int64_t i, int64_t j, int R, int S) {
-  const bool same_chain = ids.asym_id[i] == ids.asym_id[j];
-  const int res_i = ids.residue_index[i], res_j = ids.residue_index[j];
-  const bool same_res = res_i == res_j;
+__device__ __forceinline__ RelpIndex relp_index(const RelpIds& i, const RelpIds& j, int R, int S) {
+  const bool chain = i.asym == j.asym;
   RelpIndex x;
-  x.same_ent = ids.entity_id[i] == ids.entity_id[j];
-  x.res = same_chain ? relp_clip(res_i - res_j + R, 0, 2 * R) : 2 * R + 1;
-  x.tok = 2 * R + 2 +
-          ((same_chain && same_res) ? relp_clip(ids.token_index[i] - ids.token_index[j] + R, 0, 2 * R) : 2 * R + 1);
+  x.same_ent = i.ent == j.ent;
+  x.res = chain ? relp_offset(i.res, j.res, R) : 2 * R + 1;
+  x.tok = 2 * R + 2 + ((chain && i.res == j.res) ? relp_offset(i.tok, j.tok, R) : 2 * R + 1);
   x.ent = 4 * R + 4;
-  x.chn = 4 * R + 5 + (x.same_ent ? relp_clip(ids.sym_id[i] - ids.sym_id[j] + S, 0, 2 * S) : 2 * S + 1);
+  x.chn = 4 * R + 5 + (x.same_ent ? relp_offset(i.sym, j.sym, S) : 2 * S + 1);
   return x;
+}
+__device__ __forceinline__ RelpIndex relp_index(const pf_token_ids& ids, int64_t i, int64_t j, int R, int S) {
+  return relp_index(relp_ids(ids, i), relp_ids(ids, j), R, S);
 }
 
 // Four consecutive channels as fp32, from / to the storage type (8-byte bf16 or 16-byte fp32

@@ -36,49 +36,30 @@ struct RelArgs {
   int heads, R, S, n_feat, rows_per_block;
 };
 
-struct TokId {
-  int asym, res, ent, tok, sym;
-};
-
-__device__ __forceinline__ TokId load_id(const pf_token_ids& p, int64_t i) {
-  return TokId{p.asym_id[i], p.residue_index[i], p.entity_id[i], p.token_index[i], p.sym_id[i]};
-}
-
-// a - b clipped to [-lim, lim], plus lim; the difference saturates, so no pair of ids wraps around
-__device__ __forceinline__ int clip_diff(int a, int b, int lim) {
-  int d;
-  asm("sub.sat.s32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return min(max(d, -lim), lim) + lim;
-}
-
 struct PairCols {
   int res, tok, sym;  // feature columns; sym carries the same-entity bit above them
 };
 constexpr int kEntBit = 1 << 16;  // above every column (at most 2048)
-__device__ __forceinline__ PairCols pair_cols(const TokId& i, const TokId& j, int R, int S) {
-  const bool chain = i.asym == j.asym, ent = i.ent == j.ent;
-  PairCols p;
-  p.res = chain ? clip_diff(i.res, j.res, R) : 2 * R + 1;
-  p.tok = 2 * R + 2 + ((chain && i.res == j.res) ? clip_diff(i.tok, j.tok, R) : 2 * R + 1);
-  p.sym = 4 * R + 5 + (ent ? clip_diff(i.sym, j.sym, S) + kEntBit : 2 * S + 1);
-  return p;
+__device__ __forceinline__ PairCols pair_cols(const RelpIds& i, const RelpIds& j, int R, int S) {
+  const RelpIndex x = relp_index(i, j, R, S);
+  return PairCols{x.res, x.tok, x.chn + (x.same_ent ? kEntBit : 0)};
 }
 
 template <class TW, class T, int G>
 __global__ void __launch_bounds__(kRelWarps * 32) k_relpos_bias(RelArgs a, const TW* __restrict__ w, T* out) {
   extern __shared__ float tab[];  // [G][n_feat]
-  __shared__ TokId rid[kRelRows];
+  __shared__ RelpIds rid[kRelRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h0 = blockIdx.z * G, nh = min(G, a.heads - h0);
   const int64_t r0 = (int64_t)blockIdx.y * a.rows_per_block;
   const int nr = (int)min((int64_t)a.rows_per_block, a.n_rows - r0);
   for (int i = threadIdx.x; i < G * a.n_feat; i += blockDim.x)
     tab[i] = i < nh * a.n_feat ? to_f(w[(int64_t)h0 * a.n_feat + i]) : 0.f;
-  for (int i = threadIdx.x; i < nr; i += blockDim.x) rid[i] = load_id(a.ids, a.row0 + r0 + i);
+  for (int i = threadIdx.x; i < nr; i += blockDim.x) rid[i] = relp_ids(a.ids, a.row0 + r0 + i);
   __syncthreads();
   const int64_t j = ((int64_t)blockIdx.x * kRelWarps + warp) * 32 + lane;
   if (j >= a.n_cols) return;
-  const TokId cid = load_id(a.ids, a.col0 + j);
+  const RelpIds cid = relp_ids(a.ids, a.col0 + j);
   PairCols cur{-1, -1, -1};
   float rest_v[G], val[G];
 #pragma unroll
@@ -170,19 +151,19 @@ template <class T, int G>
 __global__ void __launch_bounds__(kRelWarps * 32) k_relpos_bias_bwd(RelArgs a, const T* __restrict__ dout,
                                                                     float* part) {
   extern __shared__ float tab[];  // [kRelWarps][G][n_feat]
-  __shared__ TokId rid[kRelRows];
+  __shared__ RelpIds rid[kRelRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h0 = blockIdx.z * G, nh = min(G, a.heads - h0);
   const int64_t r0 = (int64_t)blockIdx.y * a.rows_per_block;
   const int nr = (int)min((int64_t)a.rows_per_block, a.n_rows - r0);
   const int per_warp = G * a.n_feat;
   for (int i = threadIdx.x; i < kRelWarps * per_warp; i += blockDim.x) tab[i] = 0.f;
-  for (int i = threadIdx.x; i < nr; i += blockDim.x) rid[i] = load_id(a.ids, a.row0 + r0 + i);
+  for (int i = threadIdx.x; i < nr; i += blockDim.x) rid[i] = relp_ids(a.ids, a.row0 + r0 + i);
   __syncthreads();
   float* mine = tab + warp * per_warp;
   const int64_t j = ((int64_t)blockIdx.x * kRelWarps + warp) * 32 + lane;
   const bool live = j < a.n_cols;
-  const TokId cid = load_id(a.ids, a.col0 + (live ? j : 0));
+  const RelpIds cid = relp_ids(a.ids, a.col0 + (live ? j : 0));
   PairCols cur = pair_cols(rid[0], cid, a.R, a.S);
   // Sums since the residue column last changed, before that since the token column did, and before that
   // since the others did; a change flushes its own sum and the ones inside it.

@@ -5,6 +5,7 @@ import torch
 from oracle import pairformer_oracle as O
 from opendde_b200 import autograd
 from opendde_b200.model import AttentionPairBias, LayerNorm, RelativePositionEncoding, TriangleAttention
+from opendde_b200.model.trunk_init import trunk_pair_init
 from opendde_b200.utils import make_inputs, ragged_pair_mask, seeded_init_
 from test_gpu_autograd import TOL, _compare
 from train_ops_support import U, relpos_columns, token_ids
@@ -168,3 +169,24 @@ def test_single_update_with_a_relative_position_bias(dtype, cuda_device):
     with torch.no_grad():  # the inference form of the same call
         want = s + mod(s, None, z, extra_attn_bias=relpe.head_bias(feats))
     assert ((got.double() - want.double()).norm() / want.double().norm()).item() <= TOL[dtype]
+
+
+def test_pair_input_and_head_bias_have_the_same_features(cuda_device):
+    """The trunk's pair input (of a zero single input: the relative-position term alone) and the head bias of one table
+    are the same sums of columns, also for ids at the ends of int32, whose differences do not fit."""
+    n, c = 50, 64
+    ids = list(token_ids(n, 3, cuda_device))
+    lim = torch.iinfo(torch.int32)
+    at = torch.arange(n, device=cuda_device)
+    ids[1] = torch.where(at % 2 == 0, lim.min, lim.max).int()
+    ids[3] = torch.where(at % 5 == 0, lim.max, lim.min).int()
+    ids[4] = torch.where(at % 3 == 0, lim.min, lim.max).int()
+    relpe = RelativePositionEncoding(r_max=32, s_max=2, c_z=c).to(cuda_device)
+    feats = relpe.generate_relp(dict(zip(("asym_id", "residue_index", "entity_id", "token_index", "sym_id"), ids)))["relp"]
+    one, two, bond = (torch.nn.Linear(k, c, bias=False).to(cuda_device) for k in (96, 96, 1))
+    z = trunk_pair_init(torch.zeros(n, 96, device=cuda_device), one, two, relpe, bond, feats, None)
+    w = relpe.linear_no_bias.weight.detach().double()
+    hot = relpos_columns(ids, slice(0, n), slice(0, n), 32, 2)
+    bound = 8 * U * (hot @ w.abs().t())
+    assert ((z.double() - hot @ w.t()).abs() <= bound).all()
+    assert ((relpe.head_bias(feats).permute(1, 2, 0).double() - hot @ w.t()).abs() <= bound).all()
