@@ -525,8 +525,9 @@ typedef struct {
  * stats (fp32 [2][batch][heads][n_q]: the rows' maximum and sum) and, in bf16, o_lo (16 bits per
  * element, [batch][n_q][heads][head_dim] contiguous: what the rounding of o dropped) are written by the
  * forward for the backward; both may be NULL where none follows. The fields from d_o on are the
- * backward's: dq.ptr, dbias.ptr, and dk.ptr together with dv.ptr, may be NULL (not computed). Outputs
- * are overwritten and may not overlap an input. */
+ * backward's: dq.ptr, dbias.ptr, and dk.ptr together with dv.ptr, may be NULL (not computed). dbias may have
+ * batch stride 0 (the sum over the batch) where the bias has; a shared bias may also have a gradient per entry.
+ * Outputs are overwritten and may not overlap an input. */
 typedef struct {
   pf_attention_shape shape;
   pf_head_view q, k, v;
@@ -540,7 +541,10 @@ typedef struct {
 } pf_attention_call;
 
 PF_API int pf_attention_fwd(const pf_attention_call* call, void* stream);
+/* What pf_attention_bwd needs for any call of a shape, and for one call (less where no dbias is summed over the
+ * batch; its pointers are only compared with NULL). */
 PF_API int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* bytes);
+PF_API int pf_attention_bwd_call_workspace_size(const pf_attention_call* call, size_t* bytes);
 PF_API int pf_attention_bwd(const pf_attention_call* call, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Relative-position bias -----------------------------------------------------------------

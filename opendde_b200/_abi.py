@@ -60,7 +60,7 @@ EXPORTED = (
     "pf_confidence_pair_init_workspace_size", "pf_confidence_pair_init_fwd",
     "pf_diffusion_pair_cond_workspace_size", "pf_diffusion_pair_cond_fwd",
     "pf_layernorm_bwd_workspace_size", "pf_layernorm_bwd",
-    "pf_attention_fwd", "pf_attention_bwd_workspace_size", "pf_attention_bwd",
+    "pf_attention_fwd", "pf_attention_bwd_workspace_size", "pf_attention_bwd_call_workspace_size", "pf_attention_bwd",
     "pf_relpos_bias_fwd", "pf_relpos_bias_bwd_workspace_size", "pf_relpos_bias_bwd",
 )
 
@@ -161,9 +161,8 @@ class AttentionCall(Structure):
 
 # The same bytes from plain numbers (shape; q, k, v; bias; mask; o; stats, o_lo; d_o, dq, dk, dv; dbias): filling the
 # nested structures one by one would cost more than a small launch.
-ATTENTION_SHAPE = struct.Struct("@3q3if2i")
 ATTENTION_CALL = struct.Struct("@3q3if2i" + "P3q" * 3 + "P3q" + "P2q" + "P3q" + "2P" + "P3q" * 4 + "P3q")
-assert ATTENTION_SHAPE.size == ctypes.sizeof(AttentionShape) and ATTENTION_CALL.size == ctypes.sizeof(AttentionCall)
+assert ATTENTION_CALL.size == ctypes.sizeof(AttentionCall)
 
 
 _lib = None
@@ -259,9 +258,10 @@ def load(path: str = LIB_PATH):
         "pf_layernorm_bwd_workspace_size": ([c_int64, c_int32, c_int32, sz], c_int),
         "pf_layernorm_bwd": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float,
                               c_int32, c_void_p, c_size_t, c_void_p], c_int),
-        # the call and the shape as packed bytes (ATTENTION_CALL, ATTENTION_SHAPE) or structures
+        # the call as packed bytes (ATTENTION_CALL) or a structure
         "pf_attention_fwd": ([c_void_p, c_void_p], c_int),
         "pf_attention_bwd_workspace_size": ([c_void_p, sz], c_int),
+        "pf_attention_bwd_call_workspace_size": ([c_void_p, sz], c_int),
         "pf_attention_bwd": ([c_void_p, c_void_p, c_size_t, c_void_p], c_int),
         "pf_relpos_bias_fwd": ([c_void_p, c_int32, TokenIds, c_void_p, c_int64, c_int64, c_int32, c_int64, c_int64,
                                 c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p], c_int),

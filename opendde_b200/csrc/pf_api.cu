@@ -860,7 +860,15 @@ int pf_attention_fwd(const pf_attention_call* call, void* stream) {
 int pf_attention_bwd_workspace_size(const pf_attention_shape* shape, size_t* bytes) {
   PF_TRY(check_attention(shape));
   if (!bytes) return fail(PF_EINVAL_ARG, "bytes is NULL");
-  *bytes = train::attention_bwd_ws_bytes(*shape);
+  *bytes = train::attention_bwd_ws_bytes(*shape, true);
+  return PF_OK;
+}
+
+int pf_attention_bwd_call_workspace_size(const pf_attention_call* call, size_t* bytes) {
+  if (!call) return fail(PF_EINVAL_ARG, "attention backward: null call");
+  PF_TRY(check_attention(&call->shape));
+  if (!bytes) return fail(PF_EINVAL_ARG, "bytes is NULL");
+  *bytes = train::attention_bwd_ws_bytes(call->shape, call->dbias.ptr && call->dbias.batch_stride == 0);
   return PF_OK;
 }
 
@@ -869,7 +877,7 @@ int pf_attention_bwd(const pf_attention_call* call, void* workspace, size_t work
   const pf_attention_call& c = *call;
   const pf_attention_shape& s = c.shape;
   size_t need;
-  PF_TRY(pf_attention_bwd_workspace_size(&s, &need));
+  PF_TRY(pf_attention_bwd_call_workspace_size(call, &need));
   set_path("attention");
   if ((c.dk.ptr == nullptr) != (c.dv.ptr == nullptr))
     return fail(PF_EINVAL_ARG, "attention backward: dk and dv are computed together");
@@ -886,10 +894,11 @@ int pf_attention_bwd(const pf_attention_call* call, void* workspace, size_t work
     return fail(PF_EINVAL_ARG, "attention backward: bad view of a gradient");
   if (c.dbias.ptr) {
     if (!bias_ok(c.dbias, s.bias_dtype) || (s.n_q > 1 && c.dbias.row_stride < s.n_k) ||
-        (s.heads > 1 && c.dbias.head_stride < s.n_k))
+        (s.heads > 1 && c.dbias.head_stride < s.n_k) ||
+        (s.batch > 1 && c.dbias.batch_stride != 0 && c.dbias.batch_stride < s.n_k))
       return fail(PF_EINVAL_ARG, "attention backward: bad dbias view");
-    if (s.batch > 1 && (c.bias.batch_stride == 0) != (c.dbias.batch_stride == 0))
-      return fail(PF_EINVAL_ARG, "attention backward: dbias is shared by the batch exactly where the bias is");
+    if (s.batch > 1 && c.bias.batch_stride != 0 && c.dbias.batch_stride == 0)
+      return fail(PF_EINVAL_ARG, "attention backward: dbias is shared by the batch and the bias is not");
     if (s.batch == 0) return fail(PF_EINVAL_SHAPE, "attention backward: dbias of an empty batch");
   }
   if (!rows && !keys) return PF_OK;

@@ -140,12 +140,11 @@ int attention_fwd(const pf_attention_call& c, cudaStream_t st) {
   return launch(s.dtype, attn::kFwd, a, 4.0 * s.batch * s.heads * s.n_q * s.n_k * s.head_dim, st);
 }
 
-// The row constants (16 bytes per row), then the partial planes of a shared bias's gradient. Sized as if
-// the bias were shared: a caller need not say.
-size_t attention_bwd_ws_bytes(const pf_attention_shape& s) {
+// The row constants (16 bytes per row), then the partial planes of a gradient that is summed over the batch.
+size_t attention_bwd_ws_bytes(const pf_attention_shape& s, bool shared_dbias) {
   Arena ar(nullptr, 0);
   ar.take<float>((size_t)4 * s.batch * s.heads * s.n_q);
-  if (s.batch > 1) {
+  if (shared_dbias && s.batch > 1) {
     const int parts = shared_plan(s).parts;
     if (parts > 1) ar.take<float>((size_t)parts * s.heads * s.n_q * s.n_k);
   }

@@ -32,7 +32,7 @@ int layernorm_bwd(const void* x, const void* dy, const float* gamma, void* dx, f
 // Column sums of n rows of m values, in a fixed order: columns below m0 to out0, the others to out1.
 int sum_rows(const float* part, int64_t n, int64_t m, float* out0, int64_t m0, float* out1, cudaStream_t st);
 
-size_t attention_bwd_ws_bytes(const pf_attention_shape& s);
+size_t attention_bwd_ws_bytes(const pf_attention_shape& s, bool shared_dbias);
 int attention_fwd(const pf_attention_call& c, cudaStream_t st);
 int attention_bwd(const pf_attention_call& c, void* ws, size_t ws_bytes, cudaStream_t st);
 

@@ -616,15 +616,14 @@ def attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
         if bias is not None and need[3]:
             if b == 0:
                 dbias = torch.zeros(given.shape, device=dev, dtype=bias.dtype)
+            elif given.dim() == 4 and given.shape[0] != bias.shape[0]:
+                # one plane expanded over the batch: every entry has a gradient of its own
+                dbias = dbias_v = torch.empty(given.shape, device=dev, dtype=bias.dtype)
             else:
-                if given.dim() == 4 and given.shape[0] != bias.shape[0]:
-                    # one plane expanded over the batch: every entry has a gradient of its own
-                    bias = given.contiguous()
-                    fields = _attention_args(q, k, v, bias, mask, scale)[-1]
                 dbias = dbias_v = _empty(bias)
-        ws = workspace(_abi.workspace_bytes("pf_attention_bwd_workspace_size", _abi.ATTENTION_SHAPE.pack(*shape)), dev)
         call = _abi.ATTENTION_CALL.pack(*fields, *_head_view(o4), stats.data_ptr(), _ptr(o_lo) or 0, *_head_view(do4),
                                         *_head_view(dq), *_head_view(dk), *_head_view(dv), *_bias_view(dbias_v))
+        ws = workspace(_abi.workspace_bytes("pf_attention_bwd_call_workspace_size", call), dev)
         check(lib.pf_attention_bwd(call, ws.data_ptr(), ws.numel(), _stream(dev)))
     if q.dim() == 3:
         dq, dk, dv = (None if t is None else t[0] for t in (dq, dk, dv))

@@ -58,3 +58,20 @@ def test_layernorm_bwd_where_the_launches_change(c, limits, dtype, cuda_device):
         for name, t in zip(("dx", "dw", "db"), got):
             check(t, val[name], bound[name], f"{name} of {rows}")
         assert torch.equal(kernels.layernorm_bwd(x, dy, w, need=(True, False, False))[0], got[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_gradient_of_an_expanded_plane_needs_no_copies(dtype, cuda_device):
+    """One plane expanded over the batch: a gradient for each entry, and no room for a plane of each beside it."""
+    B, n = 32, 256
+    q, k, v, do, plane, mask = _att(B, n, n, 4, 4, 32, dtype, cuda_device, "shared", dtype, "pad")
+    o, saved = kernels.attention(q, k, v, plane, mask, save=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = kernels.attention_bwd(do, q, k, v, o, saved, plane.expand(B, -1, -1, -1), mask)
+    peak = torch.cuda.max_memory_allocated() - before
+    # the gradients, the row constants (16 bytes a row) and the allocator's rounding of a dozen blocks
+    assert peak <= sum(t.numel() * t.element_size() for t in got) + 16 * B * n * 4 + 12 * (2 << 20)
+    want = kernels.attention_bwd(do, q, k, v, o, saved, plane.repeat(B, 1, 1, 1), mask)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
