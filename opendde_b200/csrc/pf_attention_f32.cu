@@ -9,7 +9,9 @@
 // additions. Against the FFMA form of the same kernels, which the multiply-adds bound at 128 per clock
 // and SM (149 rows of 149 tokens, 12 heads of 32, forward plus backward: 1.9 ms), six products at 1024
 // per clock and SM are 1.3 times as many, with a quarter of the instructions (0.76 ms; 0.55 ms of products).
-// An infinity splits into an infinity and a NaN: at a visible place it gives NaN.
+// An infinity splits into an infinity and a NaN: at a visible place it gives NaN. The third value of an operand
+// below 2^-110 falls under bf16's least step, 2^-133 (which the products keep): half of that is its error, and a
+// gradient whose operands are all of 2^-116 is 1e-5 off.
 //
 // The layout is that of pf_attention_bf16.cu, with every tile in three planes. The streamed tiles are read
 // into registers a tile ahead, split, and stored to the other buffer after the products of the current

@@ -41,3 +41,18 @@ def test_fp32_outputs(B, nq, nk, H, KV, d, bias, bias_dtype, mask, cuda_device):
     far = {name: distance(got[name], val[name]) / (FP32_TOL if got[name].dtype == F32 else (2.0 ** -7 * FP32_TOL) ** 0.5)
            for name in val}
     assert all(x <= 1 for x in far.values()), far
+
+
+def test_fp32_outputs_of_small_operands(cuda_device):
+    """Operands keep their 24 bits down to 2^-110 and an absolute error of 2^-134 below, half of bf16's least step."""
+    q, k, v, do, bias, mask = _att(2, 70, 80, 2, 2, 32, F32, cuda_device, "batch", F32, "pad")
+    for args in ((q, k, v, do * 2.0 ** -108, bias, mask), (q, k, v * 2.0 ** -108, do, bias, mask),
+                 (q, k * 2.0 ** -108, v, do, bias, mask)):
+        val, _ = attention_ref(*args)
+        got = _run(*args)
+        # ds has the spread of p in it: its smaller values lie 2^-6 and more below do
+        assert all(distance(got[name], val[name]) <= FP32_TOL for name in val)
+    args = (q, k, v * 2.0 ** -118, do, bias, mask)
+    val, bound = attention_ref(*args)
+    # o is a mean of v; its own rounding to a subnormal number is below 2^-149
+    assert ((_run(*args)["o"].double() - val["o"]).abs() <= bound["o"] - 1e-30 + 2.0 ** -134 + 2.0 ** -149).all()
