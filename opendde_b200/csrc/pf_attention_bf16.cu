@@ -410,14 +410,14 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   F2 nmx[2], lg[2], nd[2];
   bool peaked = false;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t i = w0 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
-      bp[r] = BT ? bias_row<BT>(a, b, h, ic) + 4 * t * BS : nullptr;
-      dp[r] = (put && i < a.nq) ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs + 4 * t) * BS : nullptr;
-      const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
-      nmx[r] = F2(-c.x), lg[r] = F2(c.y), nd[r] = F2(c.w);
-      peaked |= c.z != 0.f;
-    }
+  for (int r = 0; r < 2; ++r) {
+    const int64_t i = w0 + r * 8 + g, ic = i < a.nq ? i : a.nq - 1;
+    bp[r] = BT ? bias_row<BT>(a, b, h, ic) + 4 * t * BS : nullptr;
+    dp[r] = (put && i < a.nq) ? (char*)a.dbias + (b * a.db_bs + (int64_t)h * a.db_hs + i * a.db_rs + 4 * t) * BS : nullptr;
+    const float4 c = ((const float4*)a.rows)[(b * a.H + h) * a.nq + ic];
+    nmx[r] = F2(-c.x), lg[r] = F2(c.y), nd[r] = F2(c.w);
+    peaked |= c.z != 0.f;
+  }
   peaked = __any_sync(0xffffffffu, peaked);
   // what the body without checks needs of the warp's rows
   const bool plain = !peaked && (BT == 0 || bvec) && (!put || (a.db_vec && w0 + 16 <= a.nq));
@@ -425,14 +425,14 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   auto fetch = [&](int slot, int q, int64_t j0, bool fast) {
     if (BT == 0) return;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) bias_get<BT>(ring[slot][r], bp[r] + q * 16 * BS, j0 + q * 16 + 4 * t, nk, fast);
+    for (int r = 0; r < 2; ++r) bias_get<BT>(ring[slot][r], bp[r] + q * 16 * BS, j0 + q * 16 + 4 * t, nk, fast);
   };
   const F2 scale(a.scale);
   float acc[NB][4];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+  for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
   uint32_t fq[KS][4], fg[KS][4];
   uint64_t bits = seen_ballot(seen_raw(a, b, 0));
   if (nt > 0) issue(0, bits);
@@ -444,15 +444,14 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
     for (int k = 0; k < KS; ++k) kc[k] = ka[k] + off, tc[k] = ta[k] + off;
 #pragma unroll 1
     for (int hb = 0; hb < 2; ++hb) {
-    unrolled<2>([&](auto Q) {  // 16 keys
-      constexpr int q = decltype(Q)::value;
-      float x[2][4], y[2][4];
+      unrolled<2>([&](auto Q) {  // 16 keys
+        constexpr int q = decltype(Q)::value;
+        float x[2][4], y[2][4];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        uint32_t r[4], u[4];
-        ldsm4i<q * 16 * RB>(r, kc[k]);
-        ldsm4i<q * 16 * RB + kV>(u, kc[k]);
-        {
+        for (int k = 0; k < KS; ++k) {
+          uint32_t r[4], u[4];
+          ldsm4i<q * 16 * RB>(r, kc[k]);
+          ldsm4i<q * 16 * RB + kV>(u, kc[k]);
           if (k == 0) {
             mma0(x[0], fq[k], r[0], r[1]);
             mma0(x[1], fq[k], r[2], r[3]);
@@ -465,21 +464,19 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
             mma(y[1], fg[k], u[2], u[3]);
           }
         }
-      }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, ring[q][r], n);
-      fetch(q, 2 * hb + q + 2, j0, hb == 0 ? FAST || (bvec && j0 + (q + 3) * 16 <= nk) : nf);
-      if (!FAST) {
-        const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
+        fetch(q, 2 * hb + q + 2, j0, hb == 0 ? FAST || (bvec && j0 + (q + 3) * 16 <= nk) : nf);
+        if (!FAST) {
+          const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!((mine >> (2 * n + e)) & 1))
-      x[n][e] = x[n][2 + e] = -INFINITY;
-      }
+            for (int e = 0; e < 2; ++e)
+              if (!((mine >> (2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
+        }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -488,44 +485,44 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
             if (!FAST) p.get(x[n][2 * r], x[n][2 * r + 1]);
             mul2(p, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(y[n][2 * r], y[n][2 * r + 1]);
           }
-      if (!FAST && peaked) {
+        if (!FAST && peaked) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (x[n][e] == 1.f) y[n][e] = 0.f;
-      }
-      if (!FAST) {  // a hidden key's ds is 0, whatever do holds
-        const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
+        }
+        if (!FAST) {  // a hidden key's ds is 0, whatever do holds
+          const uint32_t mine = (uint32_t)(bits >> (32 * hb + 16 * q + 4 * t));
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!((mine >> (2 * n + e)) & 1)) y[n][e] = y[n][2 + e] = 0.f;
-      }
-      if (put) {
-        const int64_t j = j0 + hb * 32 + q * 16 + 4 * t;
+            for (int e = 0; e < 2; ++e)
+              if (!((mine >> (2 * n + e)) & 1)) y[n][e] = y[n][2 + e] = 0.f;
+        }
+        if (put) {
+          const int64_t j = j0 + hb * 32 + q * 16 + 4 * t;
 #pragma unroll
           for (int r = 0; r < 2; ++r)
             if (FAST || dp[r])
               put_bias4<BT>(dp[r] + (hb * 32 + q * 16) * BS, j, nk, FAST || (a.db_vec && j0 + hb * 32 + q * 16 + 16 <= nk),
                             y[0][2 * r], y[0][2 * r + 1], y[1][2 * r], y[1][2 * r + 1]);
-      }
-      uint32_t da[kTerms][4];
-      split_terms(da, y);
-#pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        uint32_t f[4];
-        ldsm4_ti<q * 16 * RB>(f, tc[c]);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          mma(acc[2 * c], da[term], f[0], f[1]);
-          mma(acc[2 * c + 1], da[term], f[2], f[3]);
         }
-      }
-    });
+        uint32_t da[kTerms][4];
+        split_terms(da, y);
 #pragma unroll
-    for (int k = 0; k < KS; ++k) kc[k] += 32 * RB, tc[k] += 32 * RB;
+        for (int c = 0; c < KS; ++c) {
+          uint32_t f[4];
+          ldsm4_ti<q * 16 * RB>(f, tc[c]);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) {
+            mma(acc[2 * c], da[term], f[0], f[1]);
+            mma(acc[2 * c + 1], da[term], f[2], f[3]);
+          }
+        }
+      });
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kc[k] += 32 * RB, tc[k] += 32 * RB;
     }
   };
   if (work) {
@@ -540,10 +537,10 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
     if (kt == 0) {
       const LaneAddr<DP> la = lane_a<DP>();
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          ldsm4(fq[k], la.at(sq, warp, k));
-          ldsm4(fg[k], la.at(sg, warp, k));
-        }
+      for (int k = 0; k < KS; ++k) {
+        ldsm4(fq[k], la.at(sq, warp, k));
+        ldsm4(fg[k], la.at(sg, warp, k));
+      }
     }
     if (kt + 1 < nt) issue(kt + 1, next);
     rawm = seen_raw(a, b, j0 + 2 * kTile);
@@ -559,10 +556,10 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
         fetch(1, 5, j0, nf);
       }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          bp[r] += kTile * BS;
-          if (dp[r]) dp[r] += kTile * BS;
-        }
+      for (int r = 0; r < 2; ++r) {
+        bp[r] += kTile * BS;
+        if (dp[r]) dp[r] += kTile * BS;
+      }
     }
     bits = next;
   }
@@ -571,14 +568,14 @@ __device__ __forceinline__ void dq_block(const Args& a, unsigned id, int64_t til
   if (!a.dq) return;
   const bool vec = pair_ok(a.dq, a.o_bs, a.o_ns, a.o_hs, a.d);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t i = w0 + r * 8 + g;
-      if (i >= a.nq) continue;
-      bf16* o = (bf16*)a.dq + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
+  for (int r = 0; r < 2; ++r) {
+    const int64_t i = w0 + r * 8 + g;
+    if (i >= a.nq) continue;
+    bf16* o = (bf16*)a.dq + b * a.o_bs + (int64_t)h * a.o_hs + i * a.o_ns;
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-        store_pair(o, n * 8 + 2 * t, a.d, vec, acc[n][2 * r] * a.scale, acc[n][2 * r + 1] * a.scale);
-    }
+    for (int n = 0; n < NB; ++n)
+      store_pair(o, n * 8 + 2 * t, a.d, vec, acc[n][2 * r] * a.scale, acc[n][2 * r + 1] * a.scale);
+  }
 }
 
 // ---------------------------------------------------------------- dk, dv
@@ -618,9 +615,9 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
   const F2 scale(a.scale);
   float dk[NB][4], dv[NB][4];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+  for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
+    for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
   uint32_t fk[HOLD ? KS : 1][4], fv[HOLD ? KS : 1][4];
   Bias4<BT> ring[2][2];
   const char* bp[2] = {nullptr, nullptr};  // the lane's first key in rows g, g + 8 of the block that is read next
@@ -630,13 +627,11 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const bool row = fast || i0 + 8 * r + g < nq;
-      {
-        if (row) {
-          bias_get<BT>(ring[slot][r], bp[r], w0 + 4 * t, a.nk, fast || bfast);
-        } else {
+      if (row) {
+        bias_get<BT>(ring[slot][r], bp[r], w0 + 4 * t, a.nk, fast || bfast);
+      } else {
 #pragma unroll
-          for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][r].w[w] = 0;
-        }
+        for (int w = 0; w < (BT == 2 ? 4 : (BT == 1 ? 2 : 1)); ++w) ring[slot][r].w[w] = 0;
       }
       bp[r] += bstep;
     }
@@ -649,15 +644,14 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     for (int k = 0; k < KS; ++k) qc[k] = qa[k] + off, tc[k] = ta[k] + off;
 #pragma unroll 1
     for (int hb = 0; hb < 2; ++hb) {
-    unrolled<2>([&](auto B) {  // 16 queries
-      constexpr int blk = decltype(B)::value;
-      float x[2][4], y[2][4];
+      unrolled<2>([&](auto B) {  // 16 queries
+        constexpr int blk = decltype(B)::value;
+        float x[2][4], y[2][4];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        uint32_t fq[4], fg[4];
-        ldsm4i<blk * 16 * RB>(fq, qc[k]);
-        ldsm4i<blk * 16 * RB + kG>(fg, qc[k]);
-        {
+        for (int k = 0; k < KS; ++k) {
+          uint32_t fq[4], fg[4];
+          ldsm4i<blk * 16 * RB>(fq, qc[k]);
+          ldsm4i<blk * 16 * RB + kG>(fg, qc[k]);
           uint32_t rk[4], rv[4];
           if (HOLD) {
 #pragma unroll
@@ -678,62 +672,61 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
             mma(y[1], fg, rv[2], rv[3]);
           }
         }
-      }
-      const float4 c[2] = {cst[s * kTile + hb * 32 + blk * 16 + g], cst[s * kTile + hb * 32 + blk * 16 + 8 + g]};
-      const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)}, nd[2] = {F2(c[0].w), F2(c[1].w)};
+        const float4 c[2] = {cst[s * kTile + hb * 32 + blk * 16 + g], cst[s * kTile + hb * 32 + blk * 16 + 8 + g]};
+        const F2 nmx[2] = {F2(-c[0].x), F2(-c[1].x)}, lg[2] = {F2(c[0].y), F2(c[1].y)}, nd[2] = {F2(c[0].w), F2(c[1].w)};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) score2<BT>(&x[n][2 * r], scale, ring[blk][r], n);
-      fetch(blk, i0 + hb * 32 + blk * 16 + 32, hb == 0 ? FAST : nf);
-      if (!FAST) {
+        fetch(blk, i0 + hb * 32 + blk * 16 + 32, hb == 0 ? FAST : nf);
+        if (!FAST) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               if (!((mine >> (4 * t + 2 * n + e)) & 1)) x[n][e] = x[n][2 + e] = -INFINITY;
-      }
-      const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
-      uint32_t pa[kTerms][4], da[kTerms][4];
+        }
+        const bool peaked = __any_sync(0xffffffffu, c[0].z != 0.f || c[1].z != 0.f);
+        uint32_t pa[kTerms][4], da[kTerms][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float p[2], ds[2];
-          const F2 p2 = prob2(&x[n][2 * r], nmx[r], lg[r]);
-          p2.get(p[0], p[1]);
-          mul2(p2, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
-          if (peaked) {
-            if (p[0] == 1.f) ds[0] = 0.f;
-            if (p[1] == 1.f) ds[1] = 0.f;
-          }
+          for (int r = 0; r < 2; ++r) {
+            float p[2], ds[2];
+            const F2 p2 = prob2(&x[n][2 * r], nmx[r], lg[r]);
+            p2.get(p[0], p[1]);
+            mul2(p2, add2(F2(y[n][2 * r], y[n][2 * r + 1]), nd[r])).get(ds[0], ds[1]);
+            if (peaked) {
+              if (p[0] == 1.f) ds[0] = 0.f;
+              if (p[1] == 1.f) ds[1] = 0.f;
+            }
 #pragma unroll
-          for (int term = 0; term < kTerms; ++term) {
-            const uint32_t a = pack_bf16(p[0], p[1]), c = pack_bf16(ds[0], ds[1]);
-            pa[term][2 * r + n] = transpose8(a);
-            da[term][2 * r + n] = transpose8(c);
-            if (term + 1 < kTerms) {
-              fma2(F2(lo_f(a), hi_f(a)), F2(-1.f), F2(p[0], p[1])).get(p[0], p[1]);
-              fma2(F2(lo_f(c), hi_f(c)), F2(-1.f), F2(ds[0], ds[1])).get(ds[0], ds[1]);
+            for (int term = 0; term < kTerms; ++term) {
+              const uint32_t a = pack_bf16(p[0], p[1]), c = pack_bf16(ds[0], ds[1]);
+              pa[term][2 * r + n] = transpose8(a);
+              da[term][2 * r + n] = transpose8(c);
+              if (term + 1 < kTerms) {
+                fma2(F2(lo_f(a), hi_f(a)), F2(-1.f), F2(p[0], p[1])).get(p[0], p[1]);
+                fma2(F2(lo_f(c), hi_f(c)), F2(-1.f), F2(ds[0], ds[1])).get(ds[0], ds[1]);
+              }
             }
           }
+#pragma unroll
+        for (int n = 0; n < KS; ++n) {
+          uint32_t fg[4], fq[4];
+          ldsm4_ti<blk * 16 * RB + kG>(fg, tc[n]);
+          ldsm4_ti<blk * 16 * RB>(fq, tc[n]);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) {
+            mma(dv[2 * n], pa[term], fg[0], fg[1]);
+            mma(dv[2 * n + 1], pa[term], fg[2], fg[3]);
+            mma(dk[2 * n], da[term], fq[0], fq[1]);
+            mma(dk[2 * n + 1], da[term], fq[2], fq[3]);
+          }
         }
+      });
 #pragma unroll
-      for (int n = 0; n < KS; ++n) {
-        uint32_t fg[4], fq[4];
-        ldsm4_ti<blk * 16 * RB + kG>(fg, tc[n]);
-        ldsm4_ti<blk * 16 * RB>(fq, tc[n]);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          mma(dv[2 * n], pa[term], fg[0], fg[1]);
-          mma(dv[2 * n + 1], pa[term], fg[2], fg[3]);
-          mma(dk[2 * n], da[term], fq[0], fq[1]);
-          mma(dk[2 * n + 1], da[term], fq[2], fq[3]);
-        }
-      }
-    });
-#pragma unroll
-    for (int k = 0; k < KS; ++k) qc[k] += 32 * RB, tc[k] += 32 * RB;
+      for (int k = 0; k < KS; ++k) qc[k] += 32 * RB, tc[k] += 32 * RB;
     }
   };
   if (live != 0 && per > 0) {
@@ -767,10 +760,10 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
         __syncthreads();
         if (HOLD && it == 0) {
 #pragma unroll
-            for (int k = 0; k < (HOLD ? KS : 1); ++k) {
-              ldsm4(fk[k], lb.at(sk, warp, k));
-              ldsm4(fv[k], lb.at(sv, warp, k));
-            }
+          for (int k = 0; k < (HOLD ? KS : 1); ++k) {
+            ldsm4(fk[k], lb.at(sk, warp, k));
+            ldsm4(fv[k], lb.at(sv, warp, k));
+          }
         }
         if (qt + 1 < per) issue(qt + 1, s ^ 1);
         if (mine == 0) continue;  // none of the warp's keys is visible
@@ -799,17 +792,17 @@ __device__ __forceinline__ void dkv_block(const Args& a, unsigned id, int64_t ti
     return;
   }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t j = w0 + perm_row(g, r);  // row g + 8 r of the block holds this key
-      if (j >= a.nk) continue;
-      bf16* ok = (bf16*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j * a.dk_ns;
-      bf16* ov = (bf16*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j * a.dv_ns;
+  for (int r = 0; r < 2; ++r) {
+    const int64_t j = w0 + perm_row(g, r);  // row g + 8 r of the block holds this key
+    if (j >= a.nk) continue;
+    bf16* ok = (bf16*)a.dk + b * a.dk_bs + (int64_t)kh * a.dk_hs + j * a.dk_ns;
+    bf16* ov = (bf16*)a.dv + b * a.dv_bs + (int64_t)kh * a.dv_hs + j * a.dv_ns;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        store_pair(ok, n * 8 + 2 * t, a.d, vk, dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
-        store_pair(ov, n * 8 + 2 * t, a.d, vv, dv[n][2 * r], dv[n][2 * r + 1]);
-      }
+    for (int n = 0; n < NB; ++n) {
+      store_pair(ok, n * 8 + 2 * t, a.d, vk, dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
+      store_pair(ov, n * 8 + 2 * t, a.d, vv, dv[n][2 * r], dv[n][2 * r + 1]);
     }
+  }
 }
 
 // dk and dv in the first blocks, dq in the others (either may be none): where neither fills the machine they
