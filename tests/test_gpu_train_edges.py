@@ -2,9 +2,9 @@
 import pytest
 import torch
 
-from opendde_b200 import kernels
+from opendde_b200 import autograd, kernels
 from test_gpu_train_ops import _att, _rand, _run
-from train_ops_support import check, layernorm_ref
+from train_ops_support import check, layernorm_ref, token_ids
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -75,3 +75,32 @@ def test_attention_gradient_of_an_expanded_plane_needs_no_copies(dtype, cuda_dev
     assert peak <= sum(t.numel() * t.element_size() for t in got) + 16 * B * n * 4 + 12 * (2 << 20)
     want = kernels.attention_bwd(do, q, k, v, o, saved, plane.repeat(B, 1, 1, 1), mask)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_backward_of_an_eager_forward_is_refused_in_a_capture(cuda_device):
+    """A forward pass made before the capture: its backward is refused inside, and works afterwards."""
+    x = _rand((1, 8, 2, 32), F32, cuda_device, 1).requires_grad_()
+    table = _rand((2, 139), F32, cuda_device, 2).requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [autograd.layer_norm(x), autograd.attention(x, x, x),
+                autograd.relative_position_bias(table, token_ids(8, 2, cuda_device), 32, 2)]
+        grads = [torch.ones_like(y) for y in outs]
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        try:
+            for y, g in zip(outs, grads):
+                with pytest.raises(RuntimeError, match="not captured"):
+                    y.backward(g, retain_graph=True)
+            z = kernels.layernorm(x, None, None)
+        finally:
+            graph.capture_end()
+        graph.replay()
+        side.synchronize()
+        assert torch.equal(z, outs[0].detach()) and x.grad is None and table.grad is None
+        for y, g in zip(outs, grads):
+            y.backward(g)
+        side.synchronize()
+    assert torch.isfinite(x.grad).all() and table.grad.any()
