@@ -99,6 +99,12 @@ def test_no_tokens(cuda_device):
         out = mod.differentiable(x, mask, uniform_rows=True)
         out.sum().backward()
         assert out.shape == x.shape and not mod.mha.linear_q.weight.grad.any()
+    apb = AttentionPairBias(has_s=False, create_offset_ln_z=True, n_heads=4, c_a=96, c_z=64).to(cuda_device)
+    for dtype in (F32, BF16):
+        a, z = torch.zeros(0, 96, device=cuda_device, dtype=dtype), torch.zeros(0, 0, 64, device=cuda_device, dtype=dtype)
+        out = apb.differentiable(a, z)
+        out.sum().backward()
+        assert out.shape == a.shape and not apb.linear_nobias_z.weight.grad.any()
 
 
 def test_attention_pair_bias_is_fp32(cuda_device, monkeypatch):
