@@ -5,7 +5,7 @@
 //   out[h, i, j] = W[h, res] + W[h, tok] + W[h, sym] + [same entity] W[h, ent]
 //   dW[h, f]     = sum over the pairs (i, j) whose column f is set of dout[h, i, j]
 // Both passes move the [H, rows, cols] plane once and are bound by that. A lane owns one column j
-// and a warp walks down rows i, for kHeads heads at a time, so the indices of a pair are computed
+// and a warp walks down rows i, for up to eight heads at a time, so the indices of a pair are computed
 // once for all of them. Down a column the buckets change rarely: the residue offset inside the
 // window of 2 r_max + 1 rows around j, the others at chain ends. The forward keeps the current sums
 // in registers and reads the table (shared memory) only when a column index changes; the backward
